@@ -257,7 +257,7 @@ def _own(s):
     if kind == "scan_grad":
         ga, gb, gh0 = Fused.recurrence_grad(s["g"], s["a"], s["h"], s["h0"], axis=s["axis"])
         return {"ga": _tensor(ga), "gb": _tensor(gb), "gh0": _tensor(gh0)}
-    return {"token": _tensor(Fused.sample(s["x"], s["u"], s["temperature"], s["top_k"], s["top_p"], s["min_p"]))}
+    return _tensor(Fused.sample(s["x"], s["u"], s["temperature"], s["top_k"], s["top_p"], s["min_p"]))
 
 
 def run(s):
