@@ -92,7 +92,7 @@ class NdFunc(C.Structure):
 
 NDF_FLAT_REDUCE = 1 << 6
 NDF_KEEP_DIM = 1 << 3
-TYPE_CODE = {"sfloat": 0, "dfloat": 1, "int32": 2, "int64": 3, "uint64": 4, "bit": 5}
+TYPE_CODE = {"sfloat": 0, "dfloat": 1, "int32": 2, "int64": 3, "uint64": 4, "bit": 5, "int8": 6}
 
 
 class EwPlan(C.Structure):
@@ -185,6 +185,15 @@ _sig = {
     "cumo_hip_na_mask": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc)]),
     "cumo_hip_na_softmax": (C.c_int, [P(NArrayDesc), P(NArrayDesc)]),
     "cumo_hip_na_layernorm": (C.c_int, [P(NArrayDesc), C.c_double, P(NArrayDesc)]),
+    "cumo_hip_na_rmsnorm": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), C.c_double, P(NArrayDesc), P(NArrayDesc)]),
+    "cumo_hip_na_rmsnorm_q8": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), C.c_double, P(NArrayDesc), P(NArrayDesc), P(NArrayDesc)]),
+    "cumo_hip_na_dequantize": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc)]),
+    "cumo_hip_na_rmsnorm_grad": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), C.c_double, P(NArrayDesc), P(NArrayDesc)]),
+    "cumo_hip_na_recurrence": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), C.c_int, P(NArrayDesc)]),
+    "cumo_hip_na_recurrence_grad": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), C.c_int, P(NArrayDesc), P(NArrayDesc),
+                                              P(NArrayDesc)]),
+    "cumo_hip_na_sample": (C.c_int, [P(NArrayDesc), P(NArrayDesc), C.c_double, P(NArrayDesc), C.c_ssize_t, P(NArrayDesc), C.c_double,
+                                     P(NArrayDesc), C.c_double, P(NArrayDesc), P(NArrayDesc)]),
     "cumo_hip_na_ewcomp": (C.c_int, [C.c_char_p, P(NArrayDesc), P(NArrayDesc), C.c_int, P(NArrayDesc)]),
     "cumo_hip_na_clip": (C.c_int, [P(NArrayDesc), C.c_int, C.c_double, P(NArrayDesc), C.c_int, C.c_double, P(NArrayDesc),
                                    P(NArrayDesc)]),

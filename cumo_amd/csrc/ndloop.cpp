@@ -25,55 +25,16 @@
 #include <cstring>
 
 #include "common.h"
-#include "cumo_hip_ndloop.h"
+#include "ndloop_views.h"
+
+using namespace cumo_hip;
 
 namespace {
-
-using cumo_hip::report_error;
 
 typedef cumo_na_iarray_t IA;
 typedef cumo_na_bit_iarray_t BIA;
 typedef cumo_na_indexer_t IX;
-typedef cumo_hip_narray_t NA;
 typedef cumo_hip_loop_t LP;
-
-const int kElmsz[CUMO_HIP_N_TYPES] = {4, 8, 4, 8, 8, 0};
-const int kMaxDim = CUMO_NA_MAX_DIMENSION;
-
-int fail(int kind, const char* msg) {
-    report_error(kind, 0, msg);
-    return kind;
-}
-
-inline bool valid_type(int t) { return t >= 0 && t < CUMO_HIP_N_TYPES; }
-inline bool is_arith(int t) { return t == CUMO_HIP_SFLOAT || t == CUMO_HIP_DFLOAT || t == CUMO_HIP_INT32; }
-inline bool is_float(int t) { return t == CUMO_HIP_SFLOAT || t == CUMO_HIP_DFLOAT; }
-
-size_t total_of(const NA* a) {
-    size_t n = 1;
-    for (int d = 0; d < a->ndim; d++) n *= a->shape[d];
-    return n;
-}
-
-// a view whose elements sit in row-major order without gaps (any offset)
-bool is_contiguous(const NA* a) {
-    ssize_t unit = a->type == CUMO_HIP_BIT ? 1 : kElmsz[a->type];
-    ssize_t s = unit;
-    for (int d = a->ndim - 1; d >= 0; d--) {
-        if (a->shape[d] != 1 && a->stride[d] != s) return false;
-        s *= (ssize_t)a->shape[d];
-    }
-    return true;
-}
-
-int check_view(const NA* a, const char* what) {
-    if (!a) return fail(CUMO_HIP_ERROR_ARGUMENT, "ndloop: missing array argument");
-    if (!valid_type(a->type)) return fail(CUMO_HIP_ERROR_TYPE, "ndloop: unknown element type");
-    if (a->ndim < 0 || a->ndim > kMaxDim) return fail(CUMO_HIP_ERROR_DIMENSION, "ndloop: too many dimensions");
-    if (a->type == CUMO_HIP_BIT && a->offset < 0) return fail(CUMO_HIP_ERROR_ARGUMENT, "ndloop: negative bit offset");
-    (void)what;
-    return CUMO_HIP_OK;
-}
 
 // Merges and drops loop dimensions inside [lo, hi) and appends what is left at
 // position `at`; returns the new end. Two neighbours merge when every argument
@@ -504,13 +465,6 @@ int no_method(const char* op) {
 int upcast(int a, int b) {
     static const int rank[3] = {1, 2, 0};  // indexed by type: sfloat, dfloat, int32
     return rank[a] >= rank[b] ? a : b;
-}
-
-void free_tmp(NA* t) {
-    if (t->ptr) {
-        cumo_cuda_runtime_free(t->ptr);
-        t->ptr = NULL;
-    }
 }
 
 // ---- iterators ---------------------------------------------------------------
@@ -1762,6 +1716,7 @@ int cumo_hip_na_mask(const cumo_hip_narray_t* mask, const cumo_hip_narray_t* x, 
     if (rc) return rc;
     if (mask->type != CUMO_HIP_BIT) return no_method("mask");
     if (x->type == CUMO_HIP_BIT) return fail(CUMO_HIP_ERROR_TYPE, "mask: a Bit array cannot be the masked array here");
+    if (x->type == CUMO_HIP_INT8) return fail(CUMO_HIP_ERROR_TYPE, "mask: an Int8 array cannot be the masked array here");
     bool same = mask->ndim == x->ndim;
     for (int d = 0; same && d < x->ndim; ++d) same = mask->shape[d] == x->shape[d];
     if (!same) return fail(CUMO_HIP_ERROR_SHAPE, "mask and masked arrays must have the same shape");

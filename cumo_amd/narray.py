@@ -14,7 +14,8 @@ Nothing here computes on the CPU. Arrays live in device memory from the pool and
 come back to the host only through explicit copies (`to_numpy`, `extract_cpu`).
 
 Classes: SFloat, DFloat, Int32, Bit (and Int64/UInt64 as result holders, which is
-what Int32#sum and Bit#count_true answer). `NMath` carries the module functions.
+what Int32#sum and Bit#count_true answer, and Int8, which Fused.rmsnorm_q8
+answers). `NMath` carries the module functions, `Fused` the row composites.
 """
 import ctypes as C
 import numbers
@@ -898,6 +899,11 @@ class UInt64(NArray):
     type_name, type_code, np_dtype, elmsz = "uint64", 4, np.uint64, 8
 
 
+class Int8(NArray):
+    """Result holder (Fused.rmsnorm_q8; Fused.dequantize takes it back)."""
+    type_name, type_code, np_dtype, elmsz = "int8", 6, np.int8, 1
+
+
 class Int32(_Numeric):
     type_name, type_code, np_dtype, elmsz = "int32", 2, np.int32, 4
 
@@ -1062,7 +1068,7 @@ class Bit(NArray):
         return self._cast_to(cls)
 
 
-for _cls in (SFloat, DFloat, Int32, Int64, UInt64, Bit):
+for _cls in (SFloat, DFloat, Int32, Int64, UInt64, Bit, Int8):
     _CLASS_BY_CODE[_cls.type_code] = _cls
 
 
@@ -1123,21 +1129,103 @@ NMath = _NMath()
 _native.setup(_CLASS_BY_CODE, _lib.raise_latched, NMath)
 
 
+def _optional(x):
+    """An array's descriptor, or None for none."""
+    return None if x is None else C.byref(NMath._check(x)._desc())
+
+
+def _one_axis(ndim, axis):
+    axis = int(axis)
+    if not -ndim <= axis < ndim:
+        raise DimensionError("dimension is out of range")
+    return axis % ndim
+
+
 class _Fused:
-    """Row-wise composites along the last dimension in one launch (library additions;
-    the reference writes them as chains of array operations,
-    bench/transformer_bench.rb:110-124). Layouts the row kernels do not take fall
-    back to that chain inside the library."""
+    """Composites along rows or an axis in one call (library additions). softmax and layernorm the reference
+    writes as chains of array operations (bench/transformer_bench.rb:110-124); layouts that the row kernels do not
+    take fall back to that chain inside the library. The others (rmsnorm, recurrence, sample) are what stands between
+    the matrix products of a recurrent language model."""
 
     @staticmethod
     def softmax(x):
-        d, z = _NMath._check(x)._desc(), NArrayDesc()
+        d, z = NMath._check(x)._desc(), NArrayDesc()
         return _run(_L.cumo_hip_na_softmax, C.byref(d), C.byref(z), results=(z,))
 
     @staticmethod
     def layernorm(x, eps=1e-5):
-        d, z = _NMath._check(x)._desc(), NArrayDesc()
+        d, z = NMath._check(x)._desc(), NArrayDesc()
         return _run(_L.cumo_hip_na_layernorm, C.byref(d), float(eps), C.byref(z), results=(z,))
+
+    @staticmethod
+    def rmsnorm(x, weight=None, residual=None, eps=1e-6):
+        """s / sqrt(mean(s**2) + eps) * weight along the last dimension, s = x + residual. With a residual the
+        answer is [that, s]."""
+        y, s = NArrayDesc(), NArrayDesc()
+        results = (y,) if residual is None else (y, s)
+        return _run(_L.cumo_hip_na_rmsnorm, _optional(x), _optional(weight), _optional(residual), float(eps), C.byref(y),
+                    None if residual is None else C.byref(s), results=results)
+
+    @staticmethod
+    def rmsnorm_q8(x, weight=None, residual=None, eps=1e-6):
+        """rmsnorm in 8 bits: [q, scale], q Int8 = round(y / scale), scale = max|y| / 127 of each row (its last
+        dimension is 1); [q, scale, s] with a residual."""
+        q, scale, s = NArrayDesc(), NArrayDesc(), NArrayDesc()
+        results = (q, scale) if residual is None else (q, scale, s)
+        return _run(_L.cumo_hip_na_rmsnorm_q8, _optional(x), _optional(weight), _optional(residual), float(eps), C.byref(q), C.byref(scale),
+                    None if residual is None else C.byref(s), results=results)
+
+    @staticmethod
+    def dequantize(q, scale):
+        """q * scale for an Int8 array and its rows' scales, in the scales' type."""
+        if not isinstance(q, Int8):
+            raise TypeError("dequantize needs an Int8 array")
+        d, z = q._desc(), NArrayDesc()
+        return _run(_L.cumo_hip_na_dequantize, C.byref(d), _optional(scale), C.byref(z), results=(z,))
+
+    @staticmethod
+    def rmsnorm_grad(g, s, weight=None, gsum=None, eps=1e-6):
+        """The gradient of x (and of residual) from g, that of y: s is x + residual as rmsnorm answered it (x where
+        there was no residual), gsum the gradient of s itself, if it has one. With a weight the answer is [that,
+        the weight's]."""
+        gx, gw = NArrayDesc(), NArrayDesc()
+        results = (gx,) if weight is None else (gx, gw)
+        return _run(_L.cumo_hip_na_rmsnorm_grad, _optional(g), _optional(s), _optional(weight), _optional(gsum), float(eps), C.byref(gx),
+                    None if weight is None else C.byref(gw), results=results)
+
+    @staticmethod
+    def recurrence(a, b, h0=None, axis=-1):
+        """h[t] = a[t] * h[t-1] + b[t] along an axis, from h0 (the arrays' shape without the axis) or zeros."""
+        z = NArrayDesc()
+        da, db, d0 = _optional(a), _optional(b), _optional(h0)
+        return _run(_L.cumo_hip_na_recurrence, da, db, d0, _one_axis(a.ndim, axis), C.byref(z), results=(z,))
+
+    @staticmethod
+    def recurrence_grad(g, a, h, h0=None, axis=-1):
+        """The gradients of a and b, and of h0 where it is given, from g, that of h: [ga, gb] or [ga, gb, gh0]."""
+        ga, gb, g0 = NArrayDesc(), NArrayDesc(), NArrayDesc()
+        results = (ga, gb) if h0 is None else (ga, gb, g0)
+        dg, da, dh, d0 = _optional(g), _optional(a), _optional(h), _optional(h0)
+        return _run(_L.cumo_hip_na_recurrence_grad, dg, da, dh, d0, _one_axis(g.ndim, axis), C.byref(ga), C.byref(gb),
+                    None if h0 is None else C.byref(g0), results=results)
+
+    @staticmethod
+    def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """A position of each row of logits (Int32, x's shape without the last dimension), chosen by the numbers u in
+        [0, 1): w = exp((x - max) / temperature) in order of falling x, equal ones by index; of that order the first
+        top_k stay (0: all), of these the shortest run from the start whose weights are top_p of their sum or more,
+        of these the ones of weight min_p or more; the answer is the first of those left whose running sum of weights
+        exceeds u times theirs. temperature 0 takes the largest. -1 where a row holds a NaN or nothing but -inf. Every
+        setting is a number, or an array with one for each row."""
+        def setting(v, cast):
+            return (cast(0), _optional(v)) if isinstance(v, NArray) else (cast(v), None)
+
+        z = NArrayDesc()
+        k, ks = setting(top_k, int)
+        if k != top_k and ks is None:
+            raise ValueError("top_k must be a whole number")
+        (t, ts), (p, ps), (m, ms) = (setting(v, float) for v in (temperature, top_p, min_p))
+        return _run(_L.cumo_hip_na_sample, _optional(x), _optional(u), t, ts, k, ks, p, ps, m, ms, C.byref(z), results=(z,))
 
 
 Fused = _Fused()

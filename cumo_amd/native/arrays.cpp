@@ -282,7 +282,7 @@ PyObject* wrap(Desc* d) {
     v->shape = shape;
     v->strides = strides;
     // a contiguous array: the unit is an element's bytes, a bit for Bit
-    static const Py_ssize_t unit[8] = {4, 8, 4, 8, 8, 1, 0, 0};
+    static const Py_ssize_t unit[8] = {4, 8, 4, 8, 8, 1, 1, 0};
     Py_ssize_t st = unit[d->type];
     for (int k = d->ndim - 1; k >= 0; k--) {
         PyObject* len = PyLong_FromSize_t(d->shape[k]);

@@ -633,6 +633,105 @@ typedef struct {
 } cumo_hip_fused_rows_t;
 int cumo_hip_fused_rows_kernel_launch(int type, int mode, const cumo_hip_fused_rows_t* rows);
 
+/* Root-mean-square normalisation of rows (no counterpart in the reference):
+ *   s = x + residual;  r = 1 / sqrt(sum(s^2) / n + eps);  y = s * r * weight
+ * rows runs of n contiguous elements, row k of an array at its start + k * its step (bytes);
+ * type 0 SFloat, 1 DFloat. residual == NULL: s is x, and sum is not written. weight == NULL:
+ * ones. quantised: y is 8-bit integers, round(y / scale) between -127 and 127, and
+ * scale[k] = max|y| / 127 of row k (0 for a row of zeros, whose y are 0; a row with a NaN
+ * has the scale NaN and y of 0). y and sum may be x or residual, element on element, but
+ * overlap them in no other way. */
+typedef struct {
+    uint64_t rows, n;
+    ssize_t  x_step, residual_step, y_step, sum_step;
+    const char* x;
+    const char* residual;
+    const char* weight;
+    char*    y;
+    char*    sum;
+    char*    scale;
+    double   eps;
+} cumo_hip_rmsnorm_t;
+void cumo_hip_rmsnorm_kernel_launch(int type, int quantised, const cumo_hip_rmsnorm_t* d);
+/* y[k][i] = q[k][i] * scale[k]: the 8-bit rows back as numbers (type 0 SFloat, 1 DFloat). */
+typedef struct {
+    uint64_t rows, n;
+    ssize_t  q_step, y_step;
+    const char* q;
+    const char* scale;
+    char*    y;
+} cumo_hip_dequantize_t;
+void cumo_hip_dequantize_kernel_launch(int type, const cumo_hip_dequantize_t* d);
+/* The gradients of the normalisation from s (x + residual as the forward call left it), g (of
+ * y) and gsum (of s, by way of the residual stream; NULL: none):
+ *   gx = r * (g * weight - s * r^2 * sum(g * weight * s) / n) + gsum
+ *   gweight = the sum over rows of g * s * r   (NULL: not wanted; n contiguous elements)
+ * gx is the gradient of x and of residual alike; it may be g or gsum, element on element.
+ * Partial sums live in a block from the pool. CUMO_HIP_OK or the error reported. */
+typedef struct {
+    uint64_t rows, n;
+    ssize_t  g_step, s_step, gsum_step, gx_step;
+    const char* g;
+    const char* s;
+    const char* weight;
+    const char* gsum;
+    char*    gx;
+    char*    gweight;
+    double   eps;
+} cumo_hip_rmsnorm_grad_t;
+int cumo_hip_rmsnorm_grad_kernel_launch(int type, const cumo_hip_rmsnorm_grad_t* d);
+
+/* The gated linear recurrence h[t] = a[t] * h[t-1] + b[t] (no counterpart in the reference;
+ * cumsum is the case a = 1) over outer x time x inner elements, three byte steps an array in
+ * that order. h0: the state before the first step, outer x inner contiguous elements, NULL for
+ * zeros. type 0 SFloat, 1 DFloat. No array may overlap another. */
+typedef struct {
+    uint64_t outer, time, inner;
+    ssize_t  a_step[3], b_step[3], h_step[3];
+    const char* a;
+    const char* b;
+    const char* h0;
+    char*    h;
+} cumo_hip_recurrence_t;
+int cumo_hip_recurrence_kernel_launch(int type, const cumo_hip_recurrence_t* d);
+/* Its gradients from g (of h), a and h: from the last step to the first,
+ *   gb[t] = g[t] + a[t+1] * gb[t+1];  ga[t] = gb[t] * h[t-1];  gh0 = a[0] * gb[0]
+ * h[-1] is h0 (NULL: zeros). gh0 may be NULL. */
+typedef struct {
+    uint64_t outer, time, inner;
+    ssize_t  g_step[3], a_step[3], h_step[3], ga_step[3], gb_step[3];
+    const char* g;
+    const char* a;
+    const char* h;
+    const char* h0;
+    char*    ga;
+    char*    gb;
+    char*    gh0;
+} cumo_hip_recurrence_grad_t;
+int cumo_hip_recurrence_grad_kernel_launch(int type, const cumo_hip_recurrence_grad_t* d);
+
+/* One position of each row of n logits, chosen by a number u in [0, 1) (no counterpart in the
+ * reference). w = exp((x - max x) / temperature), in order of falling x, equal ones by index.
+ * Of that order the first top_k stay (0: all); of these the shortest run from the start whose
+ * weights are top_p of their sum or more (1: all); of these the ones of weight min_p or more
+ * (0: all; the first always stays). The answer is the first of those left whose running sum of
+ * weights exceeds u times theirs. temperature <= 0 takes the largest x. -1 where a row has
+ * nothing to choose (n = 0, every x -inf) or holds a NaN. A setting is one number, or one a row
+ * (at: contiguous, of type 0 SFloat, 1 DFloat, 2 Int32). type: of x. */
+typedef struct {
+    const char* each;  /* NULL: value for every row */
+    int      type;
+    double   value;
+} cumo_hip_row_number_t;
+typedef struct {
+    uint64_t rows, n;
+    ssize_t  x_step;
+    const char* x;
+    cumo_hip_row_number_t u, temperature, top_k, top_p, min_p;
+    int32_t* out;
+} cumo_hip_sample_t;
+int cumo_hip_sample_kernel_launch(int type, const cumo_hip_sample_t* d);
+
 /* Product sums of many rows in one launch (the reference launches
  * cumo_<type>_mulsum_reduce_kernel_launch once per row from a host loop,
  * gen/tmpl/accum_binary.c:20-45): out[r] += sum_i p1[r][i] * p2[r][i] for rows of n

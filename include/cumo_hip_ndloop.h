@@ -37,7 +37,8 @@ extern "C" {
 
 /* Element types on the path (reference: the classes of gen/def/{sfloat,dfloat,
  * int32,int64,uint64,bit}.rb). Int64/UInt64 only appear as results (Int32#sum,
- * arg reductions over more than 2^32-1 elements, Bit#count_true). */
+ * arg reductions over more than 2^32-1 elements, Bit#count_true), and so does Int8 (what
+ * cumo_hip_na_rmsnorm_q8 answers: copied, read back, taken by cumo_hip_na_dequantize). */
 enum {
     CUMO_HIP_SFLOAT = 0,
     CUMO_HIP_DFLOAT = 1,
@@ -45,7 +46,8 @@ enum {
     CUMO_HIP_INT64  = 3,
     CUMO_HIP_UINT64 = 4,
     CUMO_HIP_BIT    = 5,
-    CUMO_HIP_N_TYPES = 6
+    CUMO_HIP_INT8   = 6,
+    CUMO_HIP_N_TYPES = 7
 };
 
 /* A view of device memory: what cumo_narray_view_t and the data object under
@@ -274,6 +276,49 @@ int cumo_hip_na_mask(const cumo_hip_narray_t* mask, const cumo_hip_narray_t* x, 
  * elementwise step is the chain's own; only the order of the two row sums differs. */
 int cumo_hip_na_softmax(const cumo_hip_narray_t* x, cumo_hip_narray_t* z);
 int cumo_hip_na_layernorm(const cumo_hip_narray_t* x, double eps, cumo_hip_narray_t* z);
+
+/* Library additions for what stands between the matrix products of a recurrent language model.
+ * Operands are SFloat or DFloat, all of one type unless it says otherwise; any strides. An
+ * optional array is NULL. Results come in with ptr == NULL or as arrays of the right type and
+ * shape, which may overlap operands but not one another. Memory that a call needs beside its
+ * results comes from the pool and goes back to it; a call on a stream that is being captured
+ * keeps it instead, since the graph goes on using it.
+ *
+ * rmsnorm: along the last dimension, s = x + residual, r = 1 / sqrt(mean(s^2) + eps),
+ * y = s * r * weight. residual has x's shape; weight is one dimension of that length. sum
+ * receives s, and is NULL when residual is. Sums are in double; y is rounded once.
+ * rmsnorm_q8: q is Int8, round(y / scale); scale has x's shape with a last dimension of 1 and is
+ * max|y| / 127 of the row, from y that is not rounded before. A row of zeros has scale 0, one
+ * with a NaN scale NaN; q is 0 there. dequantize: y = q * scale, in scale's type.
+ * rmsnorm_grad: from g (of y), s and gsum (of s, or NULL): gx, of x and residual alike, and
+ * gweight (NULL when weight is). */
+int cumo_hip_na_rmsnorm(const cumo_hip_narray_t* x, const cumo_hip_narray_t* weight, const cumo_hip_narray_t* residual, double eps,
+                        cumo_hip_narray_t* y, cumo_hip_narray_t* sum);
+int cumo_hip_na_rmsnorm_q8(const cumo_hip_narray_t* x, const cumo_hip_narray_t* weight, const cumo_hip_narray_t* residual, double eps,
+                           cumo_hip_narray_t* q, cumo_hip_narray_t* scale, cumo_hip_narray_t* sum);
+int cumo_hip_na_dequantize(const cumo_hip_narray_t* q, const cumo_hip_narray_t* scale, cumo_hip_narray_t* y);
+int cumo_hip_na_rmsnorm_grad(const cumo_hip_narray_t* g, const cumo_hip_narray_t* s, const cumo_hip_narray_t* weight,
+                             const cumo_hip_narray_t* gsum, double eps, cumo_hip_narray_t* gx, cumo_hip_narray_t* gweight);
+/* recurrence: h[t] = a[t] * h[t-1] + b[t] along one axis; a, b and h have one shape, h0 (NULL:
+ * zeros) that shape without the axis. Long axes are cut where there are few runs side by side
+ * and the parts joined by the products of their a: the same bits on every call, not those of one
+ * step after the other. The products are carried in double, so a part whose |a| multiply up
+ * beyond 1.8e308 gives infinities where the states themselves would not.
+ * recurrence_grad: from g (of h): ga, gb and gh0 (NULL when h0 is). */
+int cumo_hip_na_recurrence(const cumo_hip_narray_t* a, const cumo_hip_narray_t* b, const cumo_hip_narray_t* h0, int axis, cumo_hip_narray_t* h);
+int cumo_hip_na_recurrence_grad(const cumo_hip_narray_t* g, const cumo_hip_narray_t* a, const cumo_hip_narray_t* h,
+                                const cumo_hip_narray_t* h0, int axis, cumo_hip_narray_t* ga, cumo_hip_narray_t* gb, cumo_hip_narray_t* gh0);
+/* sample: z (Int32, x's shape without the last dimension) = a position of each row of x chosen by u, as
+ * cumo_hip_sample_kernel_launch says. u: a number in [0, 1) for each row, SFloat or DFloat whatever
+ * x is, of z's shape. The settings are numbers, or (where the array is not NULL) arrays of z's
+ * shape: SFloat or DFloat, top_k Int32. Numbers that are NaN, temperature < 0, top_k < 0, or top_p or min_p
+ * outside [0, 1] are refused; in arrays, whose values the host does not see, temperature <= 0 or NaN
+ * takes the largest, top_k <= 0 and a top_p or min_p that is NaN change nothing, and others are
+ * brought into the range. The weights are whole multiples of 2^-44 for rows of up to 2^18 (finer for shorter
+ * rows, coarser for longer ones), so their sums, and with them the answer, do not depend on an order. */
+int cumo_hip_na_sample(const cumo_hip_narray_t* x, const cumo_hip_narray_t* u, double temperature, const cumo_hip_narray_t* temperatures,
+                       ssize_t top_k, const cumo_hip_narray_t* top_ks, double top_p, const cumo_hip_narray_t* top_ps,
+                       double min_p, const cumo_hip_narray_t* min_ps, cumo_hip_narray_t* z);
 
 /* Bit logic: and or xor eq / copy not (reference: gen/tmpl_bit/binary.c, unary.c). */
 int cumo_hip_na_bit_binary(const char* op, const cumo_hip_narray_t* x, const cumo_hip_narray_t* y, cumo_hip_narray_t* z);

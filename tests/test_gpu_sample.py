@@ -1,0 +1,231 @@
+"""Tokens chosen by given numbers, against the definition by sorting in 64 bits.
+
+A weight is within 2^-39 of itself and half a unit (2^-45 for rows of 2^18) of exp; the fixed inputs here lie further than
+that from every border, unless a border is meant, and then the weights are exact (equal logits)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [np.float32, np.float64]
+
+
+def cls_of(m, dt):
+    return m.SFloat if dt == np.float32 else m.DFloat
+
+
+def chosen(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The definition, a row at a time."""
+    rows, n = x.shape
+    each = lambda v: np.broadcast_to(np.asarray(v, np.float64), (rows,))  # noqa: E731
+    u, temperature, top_k, top_p, min_p = (each(v) for v in (u, temperature, top_k, top_p, min_p))
+    out = np.empty(rows, np.int32)
+    for r in range(rows):
+        row = x[r].astype(np.float64)
+        if n == 0 or np.isnan(row).any() or row.max() == -np.inf:
+            out[r] = -1
+            continue
+        order = np.argsort(-row, kind="stable")
+        row = row[order]
+        if not temperature[r] > 0:
+            out[r] = order[0]
+            continue
+        with np.errstate(invalid="ignore"):
+            w = np.exp(np.where(row == row[0], 0.0, (row - row[0]) / temperature[r]))
+        if 0 < top_k[r] < n:
+            w[int(top_k[r]):] = 0
+        if top_p[r] < 1:
+            before = np.cumsum(w) - w
+            keep = before < max(top_p[r], 0) * w.sum()
+            keep[0] = True
+            w = np.where(keep, w, 0)
+        if min_p[r] > 0:
+            w = np.where(w >= min(min_p[r], 1.0), w, 0)
+        run = np.cumsum(w)
+        at = int((run <= u[r] * run[-1]).sum())
+        out[r] = order[min(at, int((w > 0).sum()) - 1)]
+    return out
+
+
+def take(m, x, u, dt, **settings):
+    cls = cls_of(m, dt)
+    given = {}
+    for name, v in settings.items():
+        if isinstance(v, np.ndarray):
+            given[name] = m.Int32.cast(v) if name == "top_k" else cls.cast(v)
+        else:
+            given[name] = v
+    out = m.Fused.sample(cls.cast(x), cls.cast(u), **given)
+    assert type(out) is m.Int32
+    return out.to_numpy()
+
+
+SETTINGS = [{}, {"temperature": 0.7}, {"temperature": 30.0}, {"top_k": 1}, {"top_k": 5}, {"top_k": 40}, {"top_p": 0.9}, {"top_p": 0.1}, {"top_p": 0.0}, {"min_p": 0.05},
+            {"min_p": 1.0}, {"temperature": 1.5, "top_k": 300, "top_p": 0.97, "min_p": 0.01}, {"temperature": 0.0}, {"top_k": 1 << 20}]
+SHAPES = [(1, 1), (4, 2), (7, 3), (33, 64), (20, 65), (9, 1000), (5, 1024), (3, 1025), (6, 4099), (2, 20001), (3, 50001), (1, 131072), (300, 777)]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_matches_the_definition(dt, shape):
+    import cumo_amd as m
+    rng = np.random.default_rng(shape[1])
+    x = (rng.standard_normal(shape) * 3).astype(dt)
+    u = rng.random(shape[0]).astype(dt)
+    for settings in SETTINGS:
+        assert (take(m, x, u, dt, **settings) == chosen(x, u, **settings)).all(), settings
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", [(8, 50), (4, 3000), (3, 40000), (2, 131072)])
+def test_flat_rows_peaked_rows_and_many_equal_logits(dt, shape):
+    import cumo_amd as m
+    rng = np.random.default_rng(shape[0])
+    u = rng.random(shape[0]).astype(dt)
+    flat = (rng.standard_normal(shape) * 0.01).astype(dt)
+    peaked = (rng.standard_normal(shape) * 2).astype(dt)
+    peaked[:, 7] += 25
+    coarse = (np.round(rng.standard_normal(shape) * 3 * 8) / 8).astype(dt)   # steps of 1/8: many of a kind
+    two = np.where(rng.random(shape) < 0.5, 1.0, 0.0).astype(dt)
+    for x in (flat, peaked, coarse, two):
+        for settings in SETTINGS:
+            assert (take(m, x, u, dt, **settings) == chosen(x, u, **settings)).all(), settings
+    # settings that keep part of the equal ones
+    for k in (1, 2, shape[1] // 3, shape[1] - 1):
+        assert (take(m, two, u, dt, top_k=k) == chosen(two, u, top_k=k)).all(), k
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n", [4, 64, 4096, 65536])
+def test_equal_logits_are_taken_by_index_exactly(dt, n):
+    """n equal weights (a power of two): the answer is floor(u n), at every border."""
+    import cumo_amd as m
+    k = np.unique(np.concatenate([np.arange(4), np.arange(n - 4, n), np.linspace(0, n - 1, 9).astype(int)]))
+    at = np.concatenate([k / n, np.nextafter((k + 1) / n, 0)]).astype(np.float64)
+    x = np.full((len(at), n), -2.5, dt)
+    u = m.DFloat.cast(at)   # (u may be of the other type)
+    got = m.Fused.sample(cls_of(m, dt).cast(x), u).to_numpy()
+    assert (got == np.concatenate([k, k])).all()
+    # the first half by top_k, then by top_p: a half exactly
+    for settings in ({"top_k": n // 2}, {"top_p": 0.5}):
+        got = m.Fused.sample(cls_of(m, dt).cast(x), u, **settings).to_numpy()
+        assert (got == np.floor(at * (n // 2))).all(), settings
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n", [3, 100, 5000, 70000])
+def test_masked_infinite_and_nan_logits(dt, n):
+    import cumo_amd as m
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((10, n)).astype(dt)
+    x[0] = -np.inf                       # nothing to choose
+    x[1] = -np.inf
+    x[1, n // 2] = -1e30                 # one left
+    x[2, 0] = np.nan
+    x[3, n - 1] = np.inf                 # one that outweighs all
+    x[4, [0, n - 1]] = np.inf            # two of those
+    x[5, : n - 2] = -np.inf
+    x[6] = np.finfo(dt).min              # the type's lowest value, everywhere
+    x[7, 1:] = np.finfo(dt).min
+    x[8] = 0.0
+    x[8, ::2] = -0.0                     # the zeros are equal
+    for u in (0.0, 0.3, 0.75, 1 - 2.0 ** -24):
+        us = np.full(10, u, dt)
+        for settings in SETTINGS + [{"top_k": 2}, {"top_k": n - 1}]:
+            got = take(m, x, us, dt, **settings)
+            want = chosen(x, us, **settings)
+            assert (got == want).all(), (u, settings)
+        assert got[0] == -1 and got[2] == -1 and got[1] == n // 2 and got[3] == n - 1
+
+
+def test_u_outside_its_range_and_settings_at_their_limits():
+    import cumo_amd as m
+    x = np.log(np.array([[0.5, 0.25, 0.125, 0.125]], np.float64))
+    for u, want in ((-1.0, 0), (np.nan, 0), (1.0, 3), (7.0, 3), (np.inf, 3)):
+        assert take(m, x, np.array([u]), np.float64)[0] == want, u
+    one = np.array([0.999])
+    f = lambda **s: take(m, x, one, np.float64, **s)[0]  # noqa: E731
+    d = lambda v: np.array([v], np.float64)  # noqa: E731
+    # settings of rows are not refused but brought into their range
+    assert f(temperature=d(-1.0)) == 0 and f(temperature=d(np.nan)) == 0 and f(temperature=d(np.inf)) == 3
+    assert f(top_k=np.array([-3], np.int32)) == 3 and f(top_k=np.array([0], np.int32)) == 3 and f(top_k=np.array([2], np.int32)) == 1
+    assert f(top_p=d(-0.5)) == 0 and f(top_p=d(np.nan)) == 3 and f(top_p=d(2.0)) == 3
+    assert f(min_p=d(-1.0)) == 3 and f(min_p=d(np.nan)) == 3 and f(min_p=d(5.0)) == 0 and f(min_p=d(0.4)) == 1
+    assert f(temperature=1e-30) == 0 and f(temperature=1e300) == 3 and f(temperature=float("inf")) == 3
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", [(40, 300), (64, 9001), (5, 60000)])
+def test_a_row_of_its_own_settings_each(dt, shape):
+    import cumo_amd as m
+    rng = np.random.default_rng(12)
+    rows = shape[0]
+    x = (rng.standard_normal(shape) * 2).astype(dt)
+    settings = {"temperature": np.where(rng.random(rows) < 0.2, 0, rng.uniform(0.3, 2, rows)).astype(dt), "top_k": rng.integers(0, 100, rows).astype(np.int32),
+                "top_p": rng.uniform(0.2, 1, rows).astype(dt), "min_p": rng.uniform(0, 0.1, rows).astype(dt)}
+    u = rng.random(rows).astype(dt)
+    want = chosen(x, u, **settings)
+    assert (take(m, x, u, dt, **settings) == want).all()
+    # each row's answer does not depend on the rows beside it, nor on how many there are
+    for r in range(0, rows, 7):
+        one = {k: v[r:r + 1] for k, v in settings.items()}
+        assert take(m, x[r:r + 1], u[r:r + 1], dt, **one)[0] == want[r]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_views_dimensions_and_nothing(dt):
+    import cumo_amd as m
+    cls = cls_of(m, dt)
+    rng = np.random.default_rng(13)
+    h = (rng.standard_normal((4, 6, 210)) * 2).astype(dt)
+    u = rng.random((4, 6)).astype(dt)
+    x, du = cls.cast(h), cls.cast(u)
+    flat = lambda a: np.ascontiguousarray(a).reshape(-1, a.shape[-1])  # noqa: E731
+    for key in [slice(None), (slice(None), slice(None), slice(3, 200)), (slice(None), slice(None), slice(None, None, 2)), (slice(None, None, -1), slice(1, 5)),
+                (slice(None), slice(None), slice(None, None, -1))]:
+        want = chosen(flat(h[key]), u[key[:2] if isinstance(key, tuple) else key].reshape(-1), top_p=0.8)
+        got = m.Fused.sample(x[key], du[key[:2] if isinstance(key, tuple) else key], top_p=0.8)
+        assert got.shape == h[key].shape[:-1] and (got.to_numpy().reshape(-1) == want).all(), key
+    t = np.ascontiguousarray(h[0].T)   # [210, 6]
+    assert (m.Fused.sample(cls.cast(t).transpose(), du[0]).to_numpy() == chosen(h[0], u[0])).all()
+    one = m.Fused.sample(cls.cast(h[0, 0]), cls.cast(u[0, 0]))   # a row: no dimensions are left
+    assert one.shape == () and int(one) == chosen(h[0, :1], u[0, :1])[0]
+    assert (m.Fused.sample(cls(5, 0), cls.cast(np.zeros(5, dt))).to_numpy() == -1).all()
+    assert m.Fused.sample(cls(0, 5), cls(0)).shape == (0,)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_shares_are_those_of_the_weights(dt):
+    """Numbers evenly over [0, 1): every token has its share of them, within one."""
+    import cumo_amd as m
+    cls = cls_of(m, dt)
+    rng = np.random.default_rng(14)
+    n, rows = 12, 4000
+    row = rng.standard_normal(n).astype(dt)
+    x = np.broadcast_to(row, (rows, n))
+    u = (np.arange(rows) + 0.5) / rows
+    got = m.Fused.sample(cls.cast(x), m.DFloat.cast(u), 0.9).to_numpy()
+    p = np.exp(row.astype(np.float64) / 0.9)
+    p /= p.sum()
+    assert (np.abs(np.bincount(got, minlength=n) - p * rows) <= 1).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 131072), (3, 900), (200, 5000)])
+def test_captured_and_replayed(shape):
+    import cumo_amd as m
+    from cumo_amd import _lib
+    from test_gpu_rmsnorm import replayed
+    rng = np.random.default_rng(3)
+    x = m.SFloat.cast((rng.standard_normal(shape) * 2).astype(np.float32))
+    u = m.SFloat.cast(rng.random(shape[0]).astype(np.float32))
+    results = [m.Fused.sample(x, u, 0.8, 40, 0.95, 0.01), m.Fused.sample(x, u, 1.0, 0, 0.99)]
+    wants = [v.to_numpy() for v in results]
+    dx, du, o1, o2 = (C.byref(v._desc()) for v in (x, u, *results))
+
+    def call():
+        _lib.call(_lib.lib.cumo_hip_na_sample, dx, du, 0.8, None, 40, None, 0.95, None, 0.01, None, o1)
+        _lib.call(_lib.lib.cumo_hip_na_sample, dx, du, 1.0, None, 0, None, 0.99, None, 0.0, None, o2)
+
+    replayed(m, call, results, wants)
