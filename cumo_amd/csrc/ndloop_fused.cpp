@@ -249,8 +249,8 @@ int norm(const NA* x, const NA* weight, const NA* residual, double eps, NA* y, N
         }
         if (rscale) d.scale = rscale->at();
         d.eps = eps;
-        // (rows of no elements still have a scale, 0)
-        if (d.rows && (n || rscale)) cumo_hip_rmsnorm_kernel_launch(x->type, scale ? 1 : 0, &d);
+        if (d.rows && n) cumo_hip_rmsnorm_kernel_launch(x->type, scale ? 1 : 0, &d);
+        else if (d.rows && rscale) rc = cumo_hip_na_fill(rscale->use, 0.0);  // (rows of no elements still have a scale)
     }
     return finish(rc, r, nr, &s);
 }

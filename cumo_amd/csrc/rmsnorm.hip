@@ -3,122 +3,551 @@
 //   s = x + residual        r = 1 / sqrt(sum(s^2) / n + eps)        y = s r w
 //   c = r^2 sum(g w s) / n  gx = r (g w - s c) + gsum               gw = sum over rows of g s r
 // (gx: with u = s r the derivative of u_i by s_j is r (delta_ij - u_i u_j / n).)
+//
+// Memory bounds all of them: a row is read once into the registers of the lanes that share it, its sums meet across those
+// lanes, and what is computed from them is written once. The sums, and everything between them and the one rounding of a
+// result, are in double: a square of a float is exact there, and the vector units do a hundred such operations in the time
+// that an element's bytes take.
 #include "common.h"
 
 namespace cumo_hip {
 namespace {
 
-constexpr int kRnBlock = 256;
-
-__device__ __forceinline__ double rn_shfl_xor(double v, int m) { return __shfl_xor(v, m); }
-
-template <class F>
-__device__ __forceinline__ double rn_allreduce(double v, F f) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v = f(v, rn_shfl_xor(v, m));
-    __shared__ double slot[kRnBlock / 64];
-    __syncthreads();  // the slots may still be read from the previous use
-    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = slot[0];
-#pragma unroll
-    for (int w = 1; w < kRnBlock / 64; ++w) v = f(v, slot[w]);
-    return v;
-}
 __device__ __forceinline__ double rn_add(double a, double b) { return a + b; }
 __device__ __forceinline__ double rn_max_nan(double a, double b) { return (a != a) ? a : ((b != b) ? b : (a > b ? a : b)); }
 
+// Combines K values a lane over the TPR lanes that share a row, in a fixed order; every lane gets the results.
+template <int TPR, int BLOCK, int K, class F>
+__device__ __forceinline__ void rn_allreduce(double (&v)[K], F f) {
+    constexpr int SPAN = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (int m = SPAN >> 1; m > 0; m >>= 1) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = f(v[k], __shfl_xor(v[k], m));
+    }
+    if constexpr (TPR > 64) {
+        __shared__ double slot[BLOCK / 64][K];
+        __syncthreads();  // the slots may still be read from the previous use
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) slot[threadIdx.x >> 6][k] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = slot[0][k];
+#pragma unroll
+        for (int w = 1; w < BLOCK / 64; ++w) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] = f(v[k], slot[w][k]);
+        }
+    }
+}
+
+// A row in the registers of TPR lanes: whole 128-bit vectors, lane l holding vectors l, l + TPR, ..., and, one to a lane, the
+// elements behind the last whole one. What is not there is 0.
+template <class T, int TPR, int NV>
+struct RnRow {
+    static constexpr int V = 16 / (int)sizeof(T);
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    union Vec { u4 q; T t[V]; __device__ Vec() {} };
+    Vec x[NV];
+    T last;
+
+    // `whole` and `rest`: vectors, and elements behind them, of this lane's row, 0 where there is no such row. A lane without a
+    // vector reads the row's first one (`any`: there is one), so that no branch stands between the loads.
+    template <bool NT>
+    __device__ __forceinline__ void load(const char* row, uint32_t lane, uint32_t whole, uint32_t rest, bool any) {
+        if (any) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const uint32_t at = (uint32_t)k * TPR + lane;
+                const u4* from = reinterpret_cast<const u4*>(row + (at < whole ? at * 16u : 0u));
+                x[k].q = NT ? __builtin_nontemporal_load(from) : *from;
+            }
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const bool there = (uint32_t)k * TPR + lane < whole;
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[k].t[j] = there ? x[k].t[j] : (T)0;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[k].t[j] = (T)0;
+            }
+        }
+        last = lane < rest ? reinterpret_cast<const T*>(row)[whole * V + lane] : (T)0;
+    }
+    __device__ __forceinline__ void fill(T v) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[k].t[j] = v;
+        }
+        last = v;
+    }
+    template <bool NT>
+    __device__ __forceinline__ void store(char* row, uint32_t lane, uint32_t whole, uint32_t rest, bool pieces) const {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const uint32_t at = (uint32_t)k * TPR + lane;
+            if (at < whole) store_vector<NT>(reinterpret_cast<u4*>(row + at * 16u), x[k].q, pieces);
+            if constexpr (NV > 4) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (lane < rest) reinterpret_cast<T*>(row)[whole * V + lane] = last;
+    }
+    // 8-bit integers, V of them side by side a lane: on any boundary
+    template <class F>
+    __device__ __forceinline__ void store_bytes(char* row, uint32_t lane, uint32_t whole, uint32_t rest, F f) const {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const uint32_t at = (uint32_t)k * TPR + lane;
+            int8_t b[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) b[j] = f(k, j);
+            if (at < whole) __builtin_memcpy(row + at * (uint32_t)V, b, V);
+            if constexpr (NV > 4) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (lane < rest) row[whole * V + lane] = f(NV, 0);
+    }
+    // The numbers as if they came anew: what has been worked out from them, their conversions to double above all, is not kept in
+    // registers beside them until it is wanted again (232 registers a lane in the gradients' kernel, 1024 lanes spilled).
+    __device__ __forceinline__ void forget() {
+        each([](T& v, int, int) { asm("" : "+v"(v)); });
+    }
+    __device__ __forceinline__ T at(int k, int j) const { return k < NV ? x[k < NV ? k : 0].t[j] : last; }
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) f(x[k].t[j], k, j);
+            if constexpr (NV > 4) __builtin_amdgcn_sched_barrier(0);  // (else what all vectors need is worked out side by side, and spilled)
+        }
+        f(last, NV, 0);
+    }
+};
+
+struct RnParams : cumo_hip_rmsnorm_t {
+    bool y_through, sum_through;  // whether rows may be written through (StoreRows)
+};
+
+// y / scale as an 8-bit integer; inverse: 1 / scale, 0 where the scale is 0 or NaN (what is NaN then is 0 too)
+__device__ __forceinline__ int8_t rn_byte(double y, double inverse) {
+    const double z = rint(y * inverse);
+    return z == z ? (int8_t)(int)__builtin_fmin(__builtin_fmax(z, -127.0), 127.0) : (int8_t)0;
+}
+template <class T>
+__device__ __forceinline__ double rn_inverse(T scale) {
+    return scale > (T)0 && scale < (T)INFINITY ? 1.0 / (double)scale : 0.0;
+}
+
+template <class T, int TPR, int NV, int BLOCK, bool Q8, bool NT>
+__global__ __launch_bounds__(BLOCK) void rmsnorm_kernel(RnParams p) {
+    typedef RnRow<T, TPR, NV> Row;
+    constexpr int RPB = BLOCK / TPR;  // rows a block
+    const uint32_t lane = threadIdx.x % TPR;
+    const uint32_t vectors = (uint32_t)p.n / Row::V, behind = (uint32_t)p.n % Row::V;
+    // the weight stays in registers from row to row where there are enough; lanes with sixteen vectors read it again for each
+    constexpr bool HELD = NV <= 4;
+    Row w;
+    auto read_weight = [&] {
+        if (p.weight) w.template load<false>(p.weight, lane, vectors, behind, vectors != 0);
+        else w.fill((T)1);
+    };
+    if constexpr (HELD) read_weight();
+    const bool y_pieces = p.y_through && store_pieces(p.y, p.y_step), sum_pieces = p.sum_through && store_pieces(p.sum, p.sum_step);
+    for (uint64_t first = (uint64_t)blockIdx.x * RPB; first < p.rows; first += (uint64_t)gridDim.x * RPB) {
+        const uint64_t mine = first + threadIdx.x / TPR;
+        const bool there = mine < p.rows;
+        const int64_t row = there ? (int64_t)mine : 0;
+        const uint32_t whole = there ? vectors : 0, rest = there ? behind : 0;
+        Row s;
+        s.template load<NT>(p.x + row * p.x_step, lane, whole, rest, vectors != 0);
+        if (p.residual) {
+            Row add;
+            add.template load<NT>(p.residual + row * p.residual_step, lane, whole, rest, vectors != 0);
+            s.each([&](T& v, int k, int j) { v += add.at(k, j); });
+            s.template store<NT>(p.sum + row * p.sum_step, lane, whole, rest, sum_pieces);
+        }
+        double q[1] = {0.0};
+        s.each([&](T& v, int, int) { q[0] = __builtin_fma((double)v, (double)v, q[0]); });
+        rn_allreduce<TPR, BLOCK>(q, rn_add);
+        const double r = 1.0 / sqrt(q[0] / (double)p.n + p.eps);
+        if constexpr (!HELD) read_weight();
+        s.forget();
+        w.forget();
+        if constexpr (Q8) {
+            double most[1] = {0.0};
+            s.each([&](T& v, int k, int j) { most[0] = rn_max_nan(most[0], fabs((double)v * r * (double)w.at(k, j))); });
+            rn_allreduce<TPR, BLOCK>(most, rn_max_nan);
+            s.forget();
+            w.forget();
+            const T scale = (T)(most[0] / 127.0);
+            if (there && lane == 0) reinterpret_cast<T*>(p.scale)[row] = scale;
+            const double inverse = rn_inverse(scale);
+            s.store_bytes(p.y + row * p.y_step, lane, whole, rest, [&](int k, int j) { return rn_byte((double)s.at(k, j) * r * (double)w.at(k, j), inverse); });
+        } else {
+            s.each([&](T& v, int k, int j) { v = (T)((double)v * r * (double)w.at(k, j)); });
+            s.template store<NT>(p.y + row * p.y_step, lane, whole, rest, y_pieces);
+        }
+    }
+}
+
+// Rows that no block's registers hold: read again from the caches for each of their sums.
+constexpr int kRnWide = 1024;
 template <class T, bool Q8>
-__global__ __launch_bounds__(kRnBlock) void rmsnorm_kernel(cumo_hip_rmsnorm_t p) {
+__global__ __launch_bounds__(kRnWide) void rmsnorm_long_kernel(cumo_hip_rmsnorm_t p) {
     for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T* x = reinterpret_cast<const T*>(p.x + (int64_t)row * p.x_step);
         const T* res = p.residual ? reinterpret_cast<const T*>(p.residual + (int64_t)row * p.residual_step) : nullptr;
         const T* w = reinterpret_cast<const T*>(p.weight);
         T* sum = p.sum ? reinterpret_cast<T*>(p.sum + (int64_t)row * p.sum_step) : nullptr;
-        double q = 0.0;
-        for (uint64_t i = threadIdx.x; i < p.n; i += kRnBlock) {
+        double q[1] = {0.0};
+        for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) {
             const T s = res ? x[i] + res[i] : x[i];
             if (sum) sum[i] = s;
-            q = __builtin_fma((double)s, (double)s, q);
+            q[0] = __builtin_fma((double)s, (double)s, q[0]);
         }
-        const double r = 1.0 / sqrt(rn_allreduce(q, rn_add) / (double)p.n + p.eps);
+        rn_allreduce<kRnWide, kRnWide>(q, rn_add);
+        const double r = 1.0 / sqrt(q[0] / (double)p.n + p.eps);
         const T* from = sum ? sum : x;
         auto value = [&](uint64_t i) { return (double)from[i] * r * (w ? (double)w[i] : 1.0); };
         if constexpr (Q8) {
-            double most = 0.0;
-            for (uint64_t i = threadIdx.x; i < p.n; i += kRnBlock) most = rn_max_nan(most, fabs(value(i)));
-            most = rn_allreduce(most, rn_max_nan);
-            const T scale = (T)(most / 127.0);
+            double most[1] = {0.0};
+            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) most[0] = rn_max_nan(most[0], fabs(value(i)));
+            rn_allreduce<kRnWide, kRnWide>(most, rn_max_nan);
+            const T scale = (T)(most[0] / 127.0);
             if (threadIdx.x == 0) reinterpret_cast<T*>(p.scale)[row] = scale;
+            const double inverse = rn_inverse(scale);
             int8_t* y = reinterpret_cast<int8_t*>(p.y + (int64_t)row * p.y_step);
-            for (uint64_t i = threadIdx.x; i < p.n; i += kRnBlock) {
-                const double z = rint(value(i) / (double)scale);
-                y[i] = scale > (T)0 ? (int8_t)(z > 127.0 ? 127.0 : (z < -127.0 ? -127.0 : (z == z ? z : 0.0))) : (int8_t)0;
-            }
+            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) y[i] = rn_byte(value(i), inverse);
         } else {
             T* y = reinterpret_cast<T*>(p.y + (int64_t)row * p.y_step);
-            for (uint64_t i = threadIdx.x; i < p.n; i += kRnBlock) y[i] = (T)value(i);
+            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) y[i] = (T)value(i);
         }
     }
 }
 
-template <class T>
-__global__ __launch_bounds__(kRnBlock) void dequantize_kernel(cumo_hip_dequantize_t p) {
-    const uint64_t total = p.rows * p.n;
-    for (uint64_t at = (uint64_t)blockIdx.x * kRnBlock + threadIdx.x; at < total; at += (uint64_t)gridDim.x * kRnBlock) {
-        const uint64_t row = at / p.n, i = at - row * p.n;
-        reinterpret_cast<T*>(p.y + (int64_t)row * p.y_step)[i] =
-            (T)reinterpret_cast<const int8_t*>(p.q + (int64_t)row * p.q_step)[i] * reinterpret_cast<const T*>(p.scale)[row];
+// V numbers to a lane and turn: 4 (DFloat 2) bytes in, 16 bytes out
+constexpr int kDqBlock = 256;
+template <class T, int TPR, bool NT>
+__global__ __launch_bounds__(kDqBlock) void dequantize_kernel(cumo_hip_dequantize_t p, bool through) {
+    typedef RnRow<T, TPR, 1> Row;
+    constexpr int RPB = kDqBlock / TPR;
+    const uint32_t lane = threadIdx.x % TPR;
+    const uint64_t vectors = p.n / Row::V;
+    const bool pieces = through && store_pieces(p.y, p.y_step);
+    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (uint64_t)gridDim.x * RPB) {
+        const int8_t* q = reinterpret_cast<const int8_t*>(p.q + (int64_t)row * p.q_step);
+        char* y = p.y + (int64_t)row * p.y_step;
+        const T scale = reinterpret_cast<const T*>(p.scale)[row];
+        constexpr int U = 4;
+        for (uint64_t k = lane; k < vectors; k += (uint64_t)TPR * U) {
+            int8_t b[U][Row::V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint64_t at = k + (uint64_t)u * TPR;
+                __builtin_memcpy(b[u], q + (at < vectors ? at : k) * Row::V, Row::V);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint64_t at = k + (uint64_t)u * TPR;
+                typename Row::Vec v;
+#pragma unroll
+                for (int j = 0; j < Row::V; ++j) v.t[j] = (T)b[u][j] * scale;
+                if (at < vectors) store_vector<NT>(reinterpret_cast<typename Row::u4*>(y + at * 16), v.q, pieces);
+            }
+        }
+        if (lane < p.n % Row::V) reinterpret_cast<T*>(y)[vectors * Row::V + lane] = (T)q[vectors * Row::V + lane] * scale;
     }
 }
 
-// the rows' gradients; r of each row is left for the weight's
+// ---- gradients ------------------------------------------------------------------------
+// A block takes every gridDim-th group of rows, so that what its rows add to the weight's gradient stays in registers until its
+// end; the blocks' parts, one row of doubles each, are added up by a second launch (or are the gradient, where one block has
+// taken all rows). Which rows a block takes, and the order of both sums, go by the sizes alone.
+struct RnGradParams : cumo_hip_rmsnorm_grad_t {
+    double* parts;  // [gridDim.x][n]; NULL: the weight's gradient is written at once, or not wanted
+    bool through;
+};
+
+template <class T, int TPR, int NV, int BLOCK, bool NT>
+__global__ __launch_bounds__(BLOCK) void rmsnorm_grad_kernel(RnGradParams p) {
+    typedef RnRow<T, TPR, NV> Row;
+    constexpr int RPB = BLOCK / TPR, V = Row::V;
+    const uint32_t lane = threadIdx.x % TPR;
+    const uint32_t vectors = (uint32_t)p.n / V, behind = (uint32_t)p.n % V;
+    constexpr bool HELD = NV <= 4;  // (as in the forward kernel; here the weight's gradient takes registers too)
+    Row w;
+    auto read_weight = [&] {
+        if (p.weight) w.template load<false>(p.weight, lane, vectors, behind, vectors != 0);
+        else w.fill((T)1);
+    };
+    if constexpr (HELD) read_weight();
+    double sum[NV + 1][V];
+#pragma unroll
+    for (int k = 0; k <= NV; ++k) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[k][j] = 0.0;
+    }
+    const bool pieces = p.through && store_pieces(p.gx, p.gx_step);
+    for (uint64_t first = (uint64_t)blockIdx.x * RPB; first < p.rows; first += (uint64_t)gridDim.x * RPB) {
+        const uint64_t mine = first + threadIdx.x / TPR;
+        const bool there = mine < p.rows;
+        const int64_t row = there ? (int64_t)mine : 0;
+        const uint32_t whole = there ? vectors : 0, rest = there ? behind : 0;
+        Row s, g, gs;
+        s.template load<NT>(p.s + row * p.s_step, lane, whole, rest, vectors != 0);
+        g.template load<NT>(p.g + row * p.g_step, lane, whole, rest, vectors != 0);
+        auto read_gsum = [&] {
+            if (p.gsum) gs.template load<NT>(p.gsum + row * p.gsum_step, lane, whole, rest, vectors != 0);
+            else gs.fill((T)0);
+        };
+        if constexpr (HELD) read_gsum();
+        else read_weight();
+        w.forget();
+        double q[2] = {0.0, 0.0};
+        s.each([&](T& v, int k, int j) {
+            q[0] = __builtin_fma((double)v, (double)v, q[0]);
+            q[1] = __builtin_fma((double)g.at(k, j) * (double)w.at(k, j), (double)v, q[1]);
+        });
+        rn_allreduce<TPR, BLOCK>(q, rn_add);
+        // (a row that is not there has no s: its r may be infinite, and 0 * infinity is no 0)
+        const double r = there ? 1.0 / sqrt(q[0] / (double)p.n + p.eps) : 0.0;
+        const double c = r * r * q[1] / (double)p.n;
+        if constexpr (!HELD) read_gsum();
+        s.forget();
+        g.forget();
+        w.forget();
+        s.each([&](T& v, int k, int j) {
+            const double gv = (double)g.at(k, j), sv = (double)v;
+            sum[k][j] = __builtin_fma(gv * sv, r, sum[k][j]);
+            v = (T)__builtin_fma(r, gv * (double)w.at(k, j) - sv * c, (double)gs.at(k, j));
+        });
+        s.template store<NT>(p.gx + row * p.gx_step, lane, whole, rest, pieces);
+    }
+    if (!p.gweight) return;
+    // the rows that the block holds side by side
+    __shared__ double other[RPB > 1 ? BLOCK : 1];
+    const uint32_t slot = threadIdx.x / TPR;
+    double* part = p.parts ? p.parts + (uint64_t)blockIdx.x * p.n : nullptr;
+#pragma unroll
+    for (int k = 0; k <= NV; ++k) {
+#pragma unroll
+        for (int j = 0; j < (k < NV ? V : 1); ++j) {
+            double all = sum[k][j];
+            if constexpr (RPB > 1) {
+                __syncthreads();
+                other[threadIdx.x] = all;
+                __syncthreads();
+                if (slot == 0) {
+#pragma unroll
+                    for (int i = 1; i < RPB; ++i) all += other[i * TPR + lane];
+                }
+            }
+            const uint32_t at = k < NV ? ((uint32_t)k * TPR + lane) * V + j : vectors * V + lane;
+            const bool mine = slot == 0 && (k < NV ? (uint32_t)k * TPR + lane < vectors : lane < behind);
+            if (mine) {
+                if (part) part[at] = all;
+                else reinterpret_cast<T*>(p.gweight)[at] = (T)all;
+            }
+        }
+    }
+}
+
+// Rows that no block's registers hold; r of each row is left for the weight's gradient.
 template <class T>
-__global__ __launch_bounds__(kRnBlock) void rmsnorm_grad_kernel(cumo_hip_rmsnorm_grad_t p, double* rs) {
+__global__ __launch_bounds__(kRnWide) void rmsnorm_grad_long_kernel(cumo_hip_rmsnorm_grad_t p, double* rs) {
     for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T* g = reinterpret_cast<const T*>(p.g + (int64_t)row * p.g_step);
         const T* s = reinterpret_cast<const T*>(p.s + (int64_t)row * p.s_step);
         const T* gs = p.gsum ? reinterpret_cast<const T*>(p.gsum + (int64_t)row * p.gsum_step) : nullptr;
         const T* w = reinterpret_cast<const T*>(p.weight);
         T* gx = reinterpret_cast<T*>(p.gx + (int64_t)row * p.gx_step);
-        double q = 0.0, c = 0.0;
-        for (uint64_t i = threadIdx.x; i < p.n; i += kRnBlock) {
+        double q[2] = {0.0, 0.0};
+        for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) {
             const double si = (double)s[i], gw = (double)g[i] * (w ? (double)w[i] : 1.0);
-            q = __builtin_fma(si, si, q);
-            c = __builtin_fma(gw, si, c);
+            q[0] = __builtin_fma(si, si, q[0]);
+            q[1] = __builtin_fma(gw, si, q[1]);
         }
-        const double r = 1.0 / sqrt(rn_allreduce(q, rn_add) / (double)p.n + p.eps);
-        c = r * r * rn_allreduce(c, rn_add) / (double)p.n;
+        rn_allreduce<kRnWide, kRnWide>(q, rn_add);
+        const double r = 1.0 / sqrt(q[0] / (double)p.n + p.eps);
+        const double c = r * r * q[1] / (double)p.n;
         if (rs && threadIdx.x == 0) rs[row] = r;
-        for (uint64_t i = threadIdx.x; i < p.n; i += kRnBlock) {
+        for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) {
             const double gw = (double)g[i] * (w ? (double)w[i] : 1.0);
-            gx[i] = (T)(r * (gw - (double)s[i] * c) + (gs ? (double)gs[i] : 0.0));
+            gx[i] = (T)__builtin_fma(r, gw - (double)s[i] * c, gs ? (double)gs[i] : 0.0);
         }
     }
 }
 
+// the weight's part of every blockIdx.y-th run of rows, by columns
 template <class T>
-__global__ __launch_bounds__(kRnBlock) void rmsnorm_grad_weight_kernel(cumo_hip_rmsnorm_grad_t p, const double* rs) {
-    const uint64_t i = (uint64_t)blockIdx.x * kRnBlock + threadIdx.x;
+__global__ __launch_bounds__(256) void rmsnorm_grad_columns_kernel(RnGradParams p, const double* rs, uint64_t per) {
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= p.n) return;
+    const uint64_t from = blockIdx.y * per, to = from + per < p.rows ? from + per : p.rows;
     double sum = 0.0;
-    for (uint64_t row = 0; row < p.rows; ++row)
-        sum += (double)reinterpret_cast<const T*>(p.g + (int64_t)row * p.g_step)[i] * (double)reinterpret_cast<const T*>(p.s + (int64_t)row * p.s_step)[i] * rs[row];
-    reinterpret_cast<T*>(p.gweight)[i] = (T)sum;
+    for (uint64_t row = from; row < to; ++row) {
+        const double g = (double)reinterpret_cast<const T*>(p.g + (int64_t)row * p.g_step)[i], s = (double)reinterpret_cast<const T*>(p.s + (int64_t)row * p.s_step)[i];
+        sum = __builtin_fma(g * s, rs[row], sum);
+    }
+    p.parts[blockIdx.y * p.n + i] = sum;
 }
 
-unsigned rn_grid(uint64_t blocks) { return (unsigned)(blocks < (1u << 20) ? blocks : (1u << 20)); }
+// [parts][n] down its columns: 64 columns a block, sixteen waves taking every sixteenth part
+template <class T>
+__global__ __launch_bounds__(1024) void rmsnorm_grad_parts_kernel(const double* parts, uint32_t n_parts, uint64_t n, T* out) {
+    __shared__ double slot[16][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t i = (uint64_t)blockIdx.x * 64 + lane;
+    double sum = 0.0;
+    if (i < n) {
+        uint32_t k = wave;
+        for (; k + 48 < n_parts; k += 64) {
+            const double a = parts[k * n + i], b = parts[(k + 16) * n + i], c = parts[(k + 32) * n + i], d = parts[(k + 48) * n + i];
+            sum += (a + b) + (c + d);
+        }
+        for (; k < n_parts; k += 16) sum += parts[k * n + i];
+    }
+    slot[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && i < n) {
+#pragma unroll
+        for (int w = 1; w < 16; ++w) sum += slot[w][lane];
+        out[i] = (T)sum;
+    }
+}
+
+unsigned rn_grid(uint64_t blocks, uint64_t most) { return (unsigned)(blocks < most ? blocks : most); }
 
 template <class T>
-int rn_grad(const cumo_hip_rmsnorm_grad_t& p, hipStream_t stream) {
-    char* rs = nullptr;
-    if (p.gweight && p.rows && !(rs = cumo_cuda_runtime_malloc(p.rows * sizeof(double)))) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
-    if (p.rows) hipLaunchKernelGGL((rmsnorm_grad_kernel<T>), dim3(rn_grid(p.rows)), dim3(kRnBlock), 0, stream, p, reinterpret_cast<double*>(rs));
-    if (p.gweight)
-        hipLaunchKernelGGL((rmsnorm_grad_weight_kernel<T>), dim3((unsigned)((p.n + kRnBlock - 1) / kRnBlock)), dim3(kRnBlock), 0, stream, p, reinterpret_cast<double*>(rs));
+bool rn_through(const void* p, uint64_t rows, uint64_t n, int64_t step, bool nt) {
+    StoreRows at(p, n * sizeof(T));
+    at.dimension(rows, step);
+    return at.through(nt);
+}
+
+template <class T, int TPR, int NV, int BLOCK, bool Q8>
+void rn_launch_one(RnParams p, bool nt, hipStream_t stream) {
+    constexpr int RPB = BLOCK / TPR;
+    const dim3 grid(rn_grid((p.rows + RPB - 1) / RPB, 256u * 64u)), block(BLOCK);
+    if (nt) hipLaunchKernelGGL((rmsnorm_kernel<T, TPR, NV, BLOCK, Q8, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((rmsnorm_kernel<T, TPR, NV, BLOCK, Q8, false>), grid, block, 0, stream, p);
+}
+
+template <class T, bool Q8>
+void rn_launch(const cumo_hip_rmsnorm_t& d, hipStream_t stream) {
+    RnParams p;
+    static_cast<cumo_hip_rmsnorm_t&>(p) = d;
+    const bool nt = stream_past_caches(p.rows * p.n * (sizeof(T) * (p.residual ? 3 : 1) + (Q8 ? 1 : sizeof(T))));
+    p.y_through = !Q8 && rn_through<T>(p.y, p.rows, p.n, p.y_step, nt);
+    p.sum_through = p.sum && rn_through<T>(p.sum, p.rows, p.n, p.sum_step, nt);
+    const uint64_t nv = (p.n + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+    if (nv <= 8) rn_launch_one<T, 8, 1, 256, Q8>(p, nt, stream);
+    else if (nv <= 16) rn_launch_one<T, 8, 2, 256, Q8>(p, nt, stream);
+    else if (nv <= 32) rn_launch_one<T, 8, 4, 256, Q8>(p, nt, stream);
+    else if (nv <= 64) rn_launch_one<T, 16, 4, 256, Q8>(p, nt, stream);
+    else if (nv <= 128) rn_launch_one<T, 32, 4, 256, Q8>(p, nt, stream);
+    else if (nv <= 256) rn_launch_one<T, 64, 4, 256, Q8>(p, nt, stream);
+    else if (nv <= 512) rn_launch_one<T, 256, 2, 256, Q8>(p, nt, stream);
+    else if (nv <= 1024) rn_launch_one<T, 256, 4, 256, Q8>(p, nt, stream);
+    else if (nv <= 2048) rn_launch_one<T, 512, 4, 512, Q8>(p, nt, stream);
+    else if (nv <= 4096) rn_launch_one<T, 1024, 4, 1024, Q8>(p, nt, stream);
+    else if (nv <= 8192) rn_launch_one<T, 512, 16, 512, Q8>(p, nt, stream);
+    else hipLaunchKernelGGL((rmsnorm_long_kernel<T, Q8>), dim3(rn_grid(p.rows, 1u << 20)), dim3(kRnWide), 0, stream, d);
     cumo_cuda_runtime_check_kernel_launch();
-    if (rs && !stream_under_capture()) cumo_cuda_runtime_free(rs);
-    return CUMO_HIP_OK;
+}
+
+template <class T, int TPR>
+void dq_launch_one(const cumo_hip_dequantize_t& d, hipStream_t stream) {
+    constexpr int RPB = kDqBlock / TPR;
+    const bool nt = stream_past_caches(d.rows * d.n * (1 + sizeof(T)));
+    const bool through = rn_through<T>(d.y, d.rows, d.n, d.y_step, nt);
+    const dim3 grid(rn_grid((d.rows + RPB - 1) / RPB, 256u * 64u)), block(kDqBlock);
+    if (nt) hipLaunchKernelGGL((dequantize_kernel<T, TPR, true>), grid, block, 0, stream, d, through);
+    else hipLaunchKernelGGL((dequantize_kernel<T, TPR, false>), grid, block, 0, stream, d, through);
+    cumo_cuda_runtime_check_kernel_launch();
+}
+
+template <class T>
+void dq_launch(const cumo_hip_dequantize_t& d, hipStream_t stream) {
+    const uint64_t nv = d.n / (16 / sizeof(T));
+    if (nv <= 32) dq_launch_one<T, 8>(d, stream);
+    else if (nv <= 256) dq_launch_one<T, 64>(d, stream);
+    else dq_launch_one<T, 256>(d, stream);
+}
+
+// blocks that take the rows of a gradient: two to a compute unit hold enough loads on the way, and keep the parts few
+constexpr uint64_t kRnGradBlocks = 512;
+
+template <class T, int TPR, int NV, int BLOCK>
+bool rn_grad_one(RnGradParams p, hipStream_t stream) {
+    constexpr int RPB = BLOCK / TPR;
+    const unsigned blocks = rn_grid((p.rows + RPB - 1) / RPB, p.gweight ? kRnGradBlocks : 256u * 64u);
+    const bool nt = stream_past_caches(p.rows * p.n * sizeof(T) * (p.gsum ? 4 : 3));
+    p.through = rn_through<T>(p.gx, p.rows, p.n, p.gx_step, nt);
+    char* parts = nullptr;
+    if (p.gweight && blocks > 1 && !(parts = cumo_cuda_runtime_malloc(blocks * p.n * sizeof(double)))) return false;
+    p.parts = reinterpret_cast<double*>(parts);
+    const dim3 grid(blocks), block(BLOCK);
+    if (nt) hipLaunchKernelGGL((rmsnorm_grad_kernel<T, TPR, NV, BLOCK, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((rmsnorm_grad_kernel<T, TPR, NV, BLOCK, false>), grid, block, 0, stream, p);
+    if (parts) {
+        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, (uint32_t)blocks, p.n,
+                           reinterpret_cast<T*>(p.gweight));
+        // (the memory of a captured launch stays with its graph)
+        if (!stream_under_capture()) cumo_cuda_runtime_free(parts);
+    }
+    return true;
+}
+
+template <class T>
+bool rn_grad_long(RnGradParams p, hipStream_t stream) {
+    uint64_t runs = p.rows < 64 ? p.rows : 64;
+    const uint64_t per = (p.rows + runs - 1) / runs;
+    runs = (p.rows + per - 1) / per;
+    char* memory = nullptr;
+    if (p.gweight && !(memory = cumo_cuda_runtime_malloc((p.rows + runs * p.n) * sizeof(double)))) return false;
+    double* rs = reinterpret_cast<double*>(memory);
+    hipLaunchKernelGGL((rmsnorm_grad_long_kernel<T>), dim3(rn_grid(p.rows, 1u << 20)), dim3(kRnWide), 0, stream, p, rs);
+    if (memory) {
+        p.parts = rs + p.rows;
+        hipLaunchKernelGGL((rmsnorm_grad_columns_kernel<T>), dim3((unsigned)((p.n + 255) / 256), (unsigned)runs), dim3(256), 0, stream, p, rs, per);
+        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, (uint32_t)runs, p.n,
+                           reinterpret_cast<T*>(p.gweight));
+        if (!stream_under_capture()) cumo_cuda_runtime_free(memory);
+    }
+    return true;
+}
+
+template <class T>
+int rn_grad(const cumo_hip_rmsnorm_grad_t& d, hipStream_t stream) {
+    RnGradParams p;
+    static_cast<cumo_hip_rmsnorm_grad_t&>(p) = d;
+    p.parts = nullptr;
+    p.through = false;
+    const uint64_t nv = (p.n + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+    bool ok = true;
+    if (p.rows == 0) {
+        if (p.gweight)
+            hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 63) / 64)), dim3(1024), 0, stream, nullptr, 0u, p.n, reinterpret_cast<T*>(p.gweight));
+    }
+    else if (nv <= 8) ok = rn_grad_one<T, 8, 1, 256>(p, stream);
+    else if (nv <= 16) ok = rn_grad_one<T, 8, 2, 256>(p, stream);
+    else if (nv <= 32) ok = rn_grad_one<T, 8, 4, 256>(p, stream);
+    else if (nv <= 64) ok = rn_grad_one<T, 16, 4, 256>(p, stream);
+    else if (nv <= 128) ok = rn_grad_one<T, 32, 4, 256>(p, stream);
+    else if (nv <= 256) ok = rn_grad_one<T, 64, 4, 256>(p, stream);
+    else if (nv <= 512) ok = rn_grad_one<T, 256, 2, 256>(p, stream);
+    else if (nv <= 1024) ok = rn_grad_one<T, 256, 4, 256>(p, stream);
+    else if (nv <= 2048) ok = rn_grad_one<T, 512, 4, 512>(p, stream);
+    else if (nv <= 4096) ok = rn_grad_one<T, 512, 8, 512>(p, stream);
+    else ok = rn_grad_long<T>(p, stream);
+    cumo_cuda_runtime_check_kernel_launch();
+    return ok ? CUMO_HIP_OK : CUMO_HIP_ERROR_OUT_OF_MEMORY;
 }
 
 }  // namespace
@@ -128,19 +557,13 @@ using namespace cumo_hip;
 
 extern "C" void cumo_hip_rmsnorm_kernel_launch(int type, int quantised, const cumo_hip_rmsnorm_t* d) {
     hipStream_t stream = current_stream();
-    const dim3 grid(rn_grid(d->rows)), block(kRnBlock);
-    if (type == 0 && !quantised) hipLaunchKernelGGL((rmsnorm_kernel<float, false>), grid, block, 0, stream, *d);
-    else if (type == 0) hipLaunchKernelGGL((rmsnorm_kernel<float, true>), grid, block, 0, stream, *d);
-    else if (!quantised) hipLaunchKernelGGL((rmsnorm_kernel<double, false>), grid, block, 0, stream, *d);
-    else hipLaunchKernelGGL((rmsnorm_kernel<double, true>), grid, block, 0, stream, *d);
-    cumo_cuda_runtime_check_kernel_launch();
+    if (type == 0) quantised ? rn_launch<float, true>(*d, stream) : rn_launch<float, false>(*d, stream);
+    else quantised ? rn_launch<double, true>(*d, stream) : rn_launch<double, false>(*d, stream);
 }
 
 extern "C" void cumo_hip_dequantize_kernel_launch(int type, const cumo_hip_dequantize_t* d) {
-    const dim3 grid(rn_grid((d->rows * d->n + kRnBlock - 1) / kRnBlock)), block(kRnBlock);
-    if (type == 0) hipLaunchKernelGGL((dequantize_kernel<float>), grid, block, 0, current_stream(), *d);
-    else hipLaunchKernelGGL((dequantize_kernel<double>), grid, block, 0, current_stream(), *d);
-    cumo_cuda_runtime_check_kernel_launch();
+    if (type == 0) dq_launch<float>(*d, current_stream());
+    else dq_launch<double>(*d, current_stream());
 }
 
 extern "C" int cumo_hip_rmsnorm_grad_kernel_launch(int type, const cumo_hip_rmsnorm_grad_t* d) {
