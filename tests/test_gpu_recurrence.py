@@ -205,6 +205,15 @@ def test_nan_infinity_and_products_beyond_the_type(dt, shape, axis):
     h0 = np.full(f(a).shape[1:], 3.0, dt)
     got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(h0), axis=axis).to_numpy())
     assert (got[n - 1] == 3).all()
+    # products that vanish beyond any type and grow back as far: a state that is left, or none, but nothing larger than it
+    a[:] = 0.5
+    f(a)[n // 2:] = 2.0
+    got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(h0), axis=axis).to_numpy())
+    assert (got >= 0).all() and (got <= 3).all() and np.abs(got[0] - 1.5).max() == 0
+    # an infinite state stays so through such a product, with its sign
+    f(a)[:] = -0.5
+    got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(np.full(h0.shape, np.inf, dt)), axis=axis).to_numpy())
+    assert (got[0::2] == -np.inf).all() and (got[1::2] == np.inf).all()
 
 
 @pytest.mark.parametrize("dt", TYPES)
