@@ -1,13 +1,17 @@
 // One position of each row of logits, chosen by a given number (see cumo_hip_sample_kernel_launch in include/cumo_hip.h).
 //
 // Every limit (top_k, top_p, min_p) keeps a run from the start of the order "falling x, equal ones by index", and the answer is
-// itself the end of such a run, so nothing is sorted: what is asked of the order is always "the element at which the running
-// sum first exceeds t", with the sum a count or a sum of weights. That element is found by its key, an unsigned integer that
-// orders as the numbers do, digit by digit from the top: sums over the elements by digit, the digit where the running sum
-// passes t, then the next digit of the elements that share it. Elements of the same key have the same weight, so which of them
-// it is follows from a division.
+// itself the end of such a run, so rows are not sorted: what is asked of the order is always "the element at which the running
+// sum first exceeds t", with the sum a count or a sum of weights. A row's elements are counted into bins by their distance from
+// its maximum, the running sum over the bins says in which bin that element is, and the elements of that bin alone (or of all
+// bins up to it, where they are few, as for a small top_k) are put into a list and ordered.
 // Weights are whole numbers, exp((x - max) / temperature) in units of 2^-S with S such that the sum of a row fits 62 bits:
-// sums do not depend on their order, and neither does the answer, although the sums are taken by atomics.
+// sums do not depend on their order, and neither does the answer, although bins are added to by atomics.
+//
+// Three launches: the largest, the smallest and the first position of the largest of each row's parts; the bins of each row's parts, a
+// block to a part with its bins in shared memory; then a block to a row, which adds the parts' bins up, takes their running sums
+// and reads the row once more for its list. The rows come from memory once and from the last-level cache the other times; what
+// else bounds this is the weights' arithmetic in double (some twenty operations an element) and, for a few rows, the launches.
 #include "common.h"
 #include "ew_ops.h"
 
@@ -17,8 +21,11 @@ namespace cumo_hip {
 namespace {
 
 constexpr int kSaBlock = 1024;
-constexpr int kSaDigit = 8;
-constexpr int kSaBins = 1 << kSaDigit;
+constexpr int kSaBins = 2048;     // the last one: what has no weight
+constexpr int kSaList = 1024;
+constexpr uint32_t kSaFew = 256;  // elements that are ordered together rather than a bin at a time
+constexpr double kSaBinsPerNat = 48.0;   // the last bin then begins at exp(-42.6), less than half of the smallest unit
+constexpr uint64_t kSaSmallK = 512;
 
 // an unsigned integer that orders as the numbers do; both zeros have one
 template <class T> struct SaKey;
@@ -41,6 +48,24 @@ template <> struct SaKey<double> {
     }
 };
 
+// a value that every lane of the block holds, as one of the wave's: branches on it are the wave's too, and it takes no lane's registers
+template <class V>
+__device__ __forceinline__ V sa_same(V v) {
+    if constexpr (sizeof(V) <= 4) {
+        union { V v; int w; } u;
+        u.w = 0;
+        u.v = v;
+        u.w = __builtin_amdgcn_readfirstlane(u.w);
+        return u.v;
+    } else {
+        union { V v; int w[2]; } u;
+        u.v = v;
+        u.w[0] = __builtin_amdgcn_readfirstlane(u.w[0]);
+        u.w[1] = __builtin_amdgcn_readfirstlane(u.w[1]);
+        return u.v;
+    }
+}
+
 __device__ __forceinline__ double sa_number(const cumo_hip_row_number_t& a, uint64_t row) {
     if (!a.each) return a.value;
     if (a.type == 0) return (double)reinterpret_cast<const float*>(a.each)[row];
@@ -48,182 +73,561 @@ __device__ __forceinline__ double sa_number(const cumo_hip_row_number_t& a, uint
     return (double)reinterpret_cast<const int32_t*>(a.each)[row];
 }
 
-// weights of a row: 2^S for its maximum. The sum with 1.5 * 2^52 leaves the rounded product in the lower bits.
+// Weights of a row, 2^S for its maximum, and the bins. The sum with 1.5 * 2^52 leaves the rounded product in the lower bits.
+template <class T>
 struct SaWeight {
-    double max, rate, unit;  // rate: log2(e) / temperature; unit: 2^S, S <= 50
-    __device__ __forceinline__ double share(double x) const {
+    T max, bins_per;   // bins per unit of x
+    double rate, unit;  // rate: log2(e) / temperature; unit: 2^S, S <= 50
+    __device__ __forceinline__ double share(T x) const {
         if (x == max) return 1.0;
-        const double e = (x - max) * rate;
+        const double e = ((double)x - (double)max) * rate;
         return e > -70.0 ? exp2_by_table(e, float_tables()) : 0.0;  // (2^-70 and less is less than half of a unit; so is NaN, from -inf * 0)
     }
-    __device__ __forceinline__ uint64_t of(double x) const { return units(share(x)); }
     __device__ __forceinline__ uint64_t units(double share) const {
         return (uint64_t)__double_as_longlong(__builtin_fma(share, unit, 6755399441055744.0)) & 0x7ffffffffffffull;
     }
+    // falls with x, never out of order: a difference, a product and a cut, each rounded
+    __device__ __forceinline__ uint32_t bin(T x) const {
+        const T d = x == max ? (T)0 : (max - x) * bins_per;
+        return d < (T)(kSaBins - 1) ? (uint32_t)d : (uint32_t)(kSaBins - 1);   // (NaN, from inf * 0: the last)
+    }
 };
 
-// the element at which a running sum passes what was asked
-template <class T>
-struct SaPlace {
-    typename SaKey<T>::U key;
-    uint64_t before_weight;   // of the elements in front of the first of its key
-    uint64_t number;          // how many of its key stand in front of it
+struct SaPart {
+    double max, least;   // of what is finite the smallest
+    uint32_t first;      // position of the first of the largest
+    uint32_t nan;
 };
 
 struct SaParams : cumo_hip_sample_t {
     int unit_bits;
+    uint32_t looks, fills;   // parts of a row in the first two launches (64 and 16 at most)
+    SaPart* parts;           // [rows][looks]
+    uint64_t* masses;        // [rows][fills][bins]
+    uint32_t* counts;        // the same, where a row may have a top_k
 };
+
+// f of the elements [from, to) of a row, by whole waves: lanes without one bring -inf
+template <class T, int BLOCK, class F>
+__device__ __forceinline__ void sa_each(const T* row, uint32_t from, uint32_t to, F f) {
+    constexpr int V = 16 / (int)sizeof(T), U = 4;
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    union Vec { u4 q; T t[V]; __device__ Vec() {} };
+    const T* part = row + from;
+    const uint32_t n = to - from, whole = n / V;
+#pragma unroll 1
+    for (uint32_t first = 0; first < whole; first += BLOCK * U) {
+        Vec x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t at = first + (uint32_t)u * BLOCK + threadIdx.x;
+            x[u].q = reinterpret_cast<const u4*>(part)[at < whole ? at : 0];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t at = first + (uint32_t)u * BLOCK + threadIdx.x;
+#pragma unroll
+            for (int j = 0; j < V; ++j) f(at < whole ? x[u].t[j] : (T)-INFINITY, from + at * V + j);
+        }
+    }
+    f(threadIdx.x < n % V ? part[whole * V + threadIdx.x] : (T)-INFINITY, from + whole * V + threadIdx.x);
+}
+
+// a part's first and last element, whole vectors of it but for the row's end
+__device__ __forceinline__ void sa_part(uint32_t n, uint32_t parts, uint32_t part, uint32_t& from, uint32_t& to) {
+    const uint32_t per = ((n + parts - 1) / parts + 3) & ~3u;
+    from = part * per < n ? part * per : n;
+    to = n - from < per ? n : from + per;
+}
+
+template <class T>
+__device__ __forceinline__ void sa_larger(T& m, uint32_t& first, T other, uint32_t other_first) {
+    const bool take = other > m || (other == m && other_first < first);
+    first = take ? other_first : first;
+    m = take ? other : m;
+}
+
+constexpr int kSaLook = 256;
+template <class T>
+__global__ __launch_bounds__(kSaLook) void sample_look_kernel(SaParams p) {
+    __shared__ T wave_max[kSaLook / 64], wave_least[kSaLook / 64];
+    __shared__ uint32_t wave_first[kSaLook / 64], wave_nan[kSaLook / 64];
+    uint32_t from, to;
+    sa_part((uint32_t)p.n, p.looks, blockIdx.y, from, to);
+    T m = -INFINITY, least = INFINITY;
+    uint32_t first = 0xffffffffu;
+    bool nan = false;
+    if (from < to) {
+        sa_each<T, kSaLook>(reinterpret_cast<const T*>(p.x + (int64_t)blockIdx.x * p.x_step), from, to, [&](T v, uint32_t i) {
+            nan |= v != v;
+            first = v > m ? i : first;   // (a lane's positions rise)
+            m = v > m ? v : m;
+            least = v < least && v > (T)-INFINITY ? v : least;
+        });
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        sa_larger(m, first, __shfl_xor(m, d), __shfl_xor(first, d));
+        const T l = __shfl_xor(least, d);
+        least = l < least ? l : least;
+    }
+    const bool wave_has_nan = __ballot(nan) != 0;
+    const uint32_t wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+        wave_max[wave] = m;
+        wave_least[wave] = least;
+        wave_first[wave] = first;
+        wave_nan[wave] = wave_has_nan;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    nan = wave_has_nan;
+    for (int w = 1; w < kSaLook / 64; ++w) {
+        sa_larger(m, first, wave_max[w], wave_first[w]);
+        least = wave_least[w] < least ? wave_least[w] : least;
+        nan |= wave_nan[w] != 0;
+    }
+    p.parts[(uint64_t)blockIdx.x * p.looks + blockIdx.y] = {(double)m, (double)least, first, nan ? 1u : 0u};
+}
+
+// a row's settings, the same for every lane
+template <class T>
+struct SaSettings {
+    SaWeight<T> weight;
+    uint32_t first;            // of the largest
+    bool none, greedy;         // nothing to choose; the first of the largest
+    bool all, cut_p, cut_m, small;   // no top_k; top_p, min_p cut; a top_k small enough for a list
+    uint64_t top_k;
+    double top_p, likely;
+    __device__ __forceinline__ SaSettings(const SaParams& p, uint64_t row) {
+        const uint32_t lane = threadIdx.x & 63;
+        T m = -INFINITY, least = INFINITY;
+        first = 0xffffffffu;
+        uint32_t nan = 0;
+        if (lane < p.looks) {
+            const SaPart part = p.parts[row * p.looks + lane];
+            m = (T)part.max;
+            least = (T)part.least;
+            first = part.first;
+            nan = part.nan;
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            sa_larger(m, first, __shfl_xor(m, d), __shfl_xor(first, d));
+            const T l = __shfl_xor(least, d);
+            least = l < least ? l : least;
+        }
+        m = sa_same(m);
+        first = sa_same(first);
+        none = __ballot(nan != 0) != 0 || m == (T)-INFINITY;
+        const double temperature = sa_same(sa_number(p.temperature, row)), k = sa_same(sa_number(p.top_k, row)), min_p = sa_same(sa_number(p.min_p, row));
+        top_p = sa_same(sa_number(p.top_p, row));
+        all = !(k > 0.0 && k < (double)p.n);
+        greedy = !(temperature > 0.0) || (!all && k < 2.0) || top_p <= 0.0;
+        top_k = all ? p.n : (uint64_t)k;
+        cut_p = top_p < 1.0;
+        cut_m = min_p > 0.0;
+        likely = min_p < 1.0 ? min_p : 1.0;
+        small = !all && top_k <= kSaSmallK;
+        weight.max = m;
+        weight.rate = sa_same(1.44269504088896338700e+00 / temperature);
+        weight.unit = __longlong_as_double((long long)(1023 + p.unit_bits) << 52);
+        // bins of 1/48 of a factor e, or finer ones where the row's numbers span less than the bins then reach
+        const double per = kSaBinsPerNat / temperature, span = (double)m - (double)least, most = sizeof(T) == 4 ? 1e37 : 1e300;
+        weight.bins_per = sa_same((T)(span * per < (double)(kSaBins - 2) ? __builtin_fmin((double)(kSaBins - 2) / span, most) : per));   // (span 0: one number)
+    }
+};
+
+template <class T>
+__global__ __launch_bounds__(kSaBlock) void sample_fill_kernel(SaParams p) {
+    __shared__ uint64_t masses[kSaBins];
+    __shared__ uint32_t counts[kSaBins];
+    const SaSettings<T> s(p, blockIdx.x);
+    if (s.none || s.greedy) return;
+    float_tables_prepare();
+    for (uint32_t b = threadIdx.x; b < kSaBins; b += kSaBlock) {
+        masses[b] = 0;
+        counts[b] = 0;
+    }
+    __syncthreads();
+    uint32_t from, to;
+    sa_part((uint32_t)p.n, p.fills, blockIdx.y, from, to);
+    const T* x = reinterpret_cast<const T*>(p.x + (int64_t)blockIdx.x * p.x_step);
+    if (from < to) {
+        if (s.small) {
+            sa_each<T, kSaBlock>(x, from, to, [&](T v, uint32_t) {
+                if (v > (T)-INFINITY) atomicAdd(&counts[s.weight.bin(v)], 1u);
+            });
+        } else {
+            // (where min_p alone cuts, what it leaves out need not be summed)
+            const double least = s.cut_m && s.all && !s.cut_p ? s.likely : 0.0;
+            sa_each<T, kSaBlock>(x, from, to, [&](T v, uint32_t) {
+                const double share = s.weight.share(v);
+                const uint64_t units = share >= least ? s.weight.units(share) : 0;
+                const uint32_t b = s.weight.bin(v);
+                if (units) atomicAdd((unsigned long long*)&masses[b], (unsigned long long)units);
+                if (!s.all && v > (T)-INFINITY) atomicAdd(&counts[b], 1u);
+            });
+        }
+    }
+    __syncthreads();
+    const uint64_t at = ((uint64_t)blockIdx.x * p.fills + blockIdx.y) * kSaBins;
+    for (uint32_t b = threadIdx.x; b < kSaBins; b += kSaBlock) {
+        if (!s.small) p.masses[at + b] = masses[b];
+        if (!s.all) p.counts[at + b] = counts[b];
+    }
+}
+
+__device__ __forceinline__ uint64_t sa_up(uint64_t v, int d) { return (uint64_t)__shfl_up((unsigned long long)v, d); }
+
+// inclusive sums over the block's lanes, in the lanes' order; slots: one for each wave
+__device__ __forceinline__ uint64_t sa_scan(uint64_t v, uint64_t* slots) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t o = sa_up(v, d);
+        v += lane >= (uint32_t)d ? o : 0;
+    }
+    __syncthreads();
+    if (lane == 63) slots[wave] = v;
+    __syncthreads();
+    uint64_t before = lane < wave ? slots[lane & (kSaBlock / 64 - 1)] : 0;   // (sixteen waves: lanes 0 to 14 at most)
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) before += (uint64_t)__shfl_xor((unsigned long long)before, d);
+    return v + sa_same(before);
+}
 
 template <class T>
 __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
     typedef SaKey<T> Key;
     typedef typename Key::U U;
-    __shared__ uint64_t counts[kSaBins], weights[kSaBins];
-    __shared__ T wave_max[kSaBlock / 64];
-    __shared__ uint32_t wave_nan[kSaBlock / 64], wave_count[kSaBlock / 64];
-    __shared__ uint64_t shared_place[3], shared_sum;
-    float_tables_prepare();
+    constexpr int kWaves = kSaBlock / 64, KV = 16 / (int)sizeof(U);
+    typedef U UV __attribute__((ext_vector_type(KV)));
+    __shared__ uint64_t masses[kSaBins];   // running sums of the bins
+    __shared__ uint32_t counts[kSaBins];
+    __shared__ __attribute__((aligned(16))) U list_key[kSaList];
+    __shared__ U sorted_key[kSaList];
+    __shared__ uint32_t list_index[kSaList], sorted_index[kSaList];
+    __shared__ uint64_t list_sum[kSaList], slots[kWaves], found[3], digit_count[256], digit_mass[256];
+    __shared__ uint32_t list_size;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T* x = reinterpret_cast<const T*>(p.x + (int64_t)row * p.x_step);
-        T m = -INFINITY;
-        bool nan = false;
-        for (uint64_t i = tid; i < p.n; i += kSaBlock) {
-            const T v = x[i];
-            nan |= v != v;
-            m = v > m ? v : m;
-        }
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-            const T o = __shfl_xor(m, d);
-            m = o > m ? o : m;
-        }
-        const bool wave_has_nan = __ballot(nan) != 0;
-        __syncthreads();
-        if (lane == 0) {
-            wave_max[wave] = m;
-            wave_nan[wave] = wave_has_nan;
-        }
-        __syncthreads();
-        nan = false;
-        for (int w = 0; w < kSaBlock / 64; ++w) {
-            m = wave_max[w] > m ? wave_max[w] : m;
-            nan |= wave_nan[w] != 0;
-        }
-        if (nan || m == (T)-INFINITY) {   // (the same for the whole block)
-            if (tid == 0) p.out[row] = -1;
-            continue;
-        }
-        const double temperature = sa_number(p.temperature, row);
-        const bool greedy = !(temperature > 0.0);
-        SaWeight weight;
-        weight.max = (double)m;
-        weight.rate = 1.44269504088896338700e+00 / (greedy ? 1.0 : temperature);
-        weight.unit = __longlong_as_double((long long)(1023 + p.unit_bits) << 52);
-
-        // the element at which the running count (weight) first exceeds t, which the whole sum does
-        auto find = [&](bool by_weight, uint64_t t) {
-            SaPlace<T> at;
-            U prefix = 0;
-            uint64_t before = 0, before_weight = 0, number = 0;
-            for (int shift = (int)sizeof(U) * 8 - kSaDigit; shift >= 0; shift -= kSaDigit) {
-                if (tid < kSaBins) counts[tid] = weights[tid] = 0;
-                __syncthreads();
-                for (uint64_t i = tid; i < p.n; i += kSaBlock) {
-                    const U k = Key::of(x[i]);
-                    // (a shift by the whole width would not be one: the first digit compares nothing)
-                    if (shift + kSaDigit < (int)sizeof(U) * 8 && (k >> (shift + kSaDigit)) != prefix) continue;
-                    const uint32_t digit = (uint32_t)(k >> shift) & (kSaBins - 1);
-                    atomicAdd((unsigned long long*)&counts[digit], 1ull);
-                    atomicAdd((unsigned long long*)&weights[digit], (unsigned long long)weight.of((double)x[i]));
-                }
-                __syncthreads();
-                if (tid == 0) {
-                    uint64_t run = before, run_weight = before_weight;
-                    int digit = kSaBins - 1;
-                    for (; digit > 0; --digit) {
-                        const uint64_t next = run + (by_weight ? weights[digit] : counts[digit]);
-                        if (next > t) break;
-                        run = next;
-                        run_weight += weights[digit];
-                    }
-                    shared_place[0] = (uint64_t)digit;
-                    shared_place[1] = run;
-                    shared_place[2] = run_weight;
-                }
-                __syncthreads();
-                prefix = (U)((prefix << kSaDigit) | (U)shared_place[0]);
-                before = shared_place[1];
-                before_weight = shared_place[2];
-                if (shift == 0) {
-                    const uint64_t one = by_weight ? weights[shared_place[0]] / counts[shared_place[0]] : 1;
-                    number = (t - before) / (one ? one : 1);
-                }
-                __syncthreads();
+    const uint32_t n = (uint32_t)p.n;
+    const uint64_t row = blockIdx.x;
+    const T* x = reinterpret_cast<const T*>(p.x + (int64_t)row * p.x_step);
+    const SaSettings<T> s(p, row);
+    const SaWeight<T>& weight = s.weight;
+    if (s.none || s.greedy) {
+        if (tid == 0) p.out[row] = s.none ? -1 : (int32_t)s.first;
+        return;
+    }
+    float_tables_prepare();
+    const double u = sa_same(sa_number(p.u, row));
+    bool small = s.small;
+    {
+        const uint32_t b = 2 * tid;   // (two bins a lane)
+        uint64_t one = 0, two = 0;
+        uint32_t c_one = 0, c_two = 0;
+#pragma unroll 4
+        for (uint32_t part = 0; part < p.fills; ++part) {
+            const uint64_t at = (row * p.fills + part) * kSaBins + b;
+            if (!small) {
+                one += p.masses[at];
+                two += p.masses[at + 1];
             }
-            at.key = prefix;
-            at.before_weight = before_weight;
-            at.number = number;
-            return at;
-        };
-        auto sum_of = [&](double least) {   // of the weights whose share is `least` or more
-            uint64_t mine = 0;
-            for (uint64_t i = tid; i < p.n; i += kSaBlock) {
-                const double s = weight.share((double)x[i]);
-                mine += s >= least ? weight.units(s) : 0;
+            if (!s.all) {
+                c_one += p.counts[at];
+                c_two += p.counts[at + 1];
             }
-            if (tid == 0) shared_sum = 0;
-            __syncthreads();
-            atomicAdd((unsigned long long*)&shared_sum, (unsigned long long)mine);
-            __syncthreads();
-            const uint64_t all = shared_sum;
-            __syncthreads();
-            return all;
-        };
+        }
+        if (!small) {
+            const uint64_t run = sa_scan(one + two, slots);
+            masses[b] = run - two;
+            masses[b + 1] = run;
+        }
+        if (!s.all) {
+            const uint32_t run = (uint32_t)sa_scan(c_one + c_two, slots);
+            counts[b] = run - c_two;
+            counts[b + 1] = run;
+        }
+        __syncthreads();
+    }
 
-        const double k_given = sa_number(p.top_k, row), p_given = sa_number(p.top_p, row), m_given = sa_number(p.min_p, row);
-        const uint64_t top_k = greedy ? 1 : (k_given > 0.0 && k_given < (double)p.n ? (uint64_t)k_given : p.n);
-        uint64_t sum;
-        if (top_k < p.n) {
-            const SaPlace<T> at = find(false, top_k - 1);
-            sum = at.before_weight + (at.number + 1) * weight.of((double)Key::value(at.key));
-        } else {
-            sum = sum_of(0.0);
-        }
-        if (p_given < 1.0) {
-            double want = ceil((p_given > 0.0 ? p_given : 0.0) * (double)sum);
-            want = want < 1.0 ? 1.0 : want;
-            const uint64_t t = (uint64_t)want - 1;
-            const SaPlace<T> at = find(true, t < sum ? t : sum - 1);
-            sum = at.before_weight + (at.number + 1) * weight.of((double)Key::value(at.key));
-        }
-        if (m_given > 0.0) {
-            const uint64_t likely = sum_of(m_given < 1.0 ? m_given : 1.0);
-            sum = likely < sum ? likely : sum;
-        }
-        const double u = sa_number(p.u, row);
-        const double want = floor((u > 0.0 ? u : 0.0) * (double)sum);
-        const SaPlace<T> at = find(true, want < (double)sum ? (uint64_t)want < sum ? (uint64_t)want : sum - 1 : sum - 1);
-
-        // the element of that key with `number` before it, in order of the index
-        uint64_t left = at.number;
-        for (uint64_t first = 0; first < p.n; first += kSaBlock) {
-            const uint64_t i = first + tid;
-            const bool hit = i < p.n && Key::of(x[i]) == at.key;
+    // the list: of the elements in bins [lo, hi], in order, with their running sum of weights; false where they are too many
+    uint32_t lo = 1, hi = 0;
+    auto make_list = [&](uint32_t from, uint32_t to) {
+        __syncthreads();
+        if (tid == 0) list_size = 0;
+        list_key[tid] = 0;   // (below every number's key)
+        __syncthreads();
+        sa_each<T, kSaBlock>(x, 0, n, [&](T v, uint32_t i) {
+            const uint32_t b = weight.bin(v);
+            const bool hit = b >= from && b <= to && v > (T)-INFINITY;
             const uint64_t hits = __ballot(hit);
-            if (lane == 0) wave_count[wave] = (uint32_t)__popcll(hits);
-            __syncthreads();
-            uint32_t ahead = (uint32_t)__popcll(hits & ((1ull << lane) - 1)), all = 0;
-            for (uint32_t w = 0; w < kSaBlock / 64; ++w) {
-                ahead += w < wave ? wave_count[w] : 0;
-                all += wave_count[w];
+            if (hits) {
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(&list_size, (uint32_t)__popcll(hits));
+                at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(hits & ((1ull << lane) - 1));
+                if (hit && at < kSaList) {
+                    list_key[at] = Key::of(v);
+                    list_index[at] = i;
+                }
             }
-            if (hit && ahead == left) p.out[row] = (int32_t)i;
+        });
+        __syncthreads();
+        const uint32_t size = sa_same(list_size);
+        lo = 1;
+        hi = 0;
+        if (size > kSaList) return false;
+        // an element's place is the number of those before it
+        if (wave * 64 < size) {
+            const U key = list_key[tid];
+            const uint32_t index = list_index[tid];
+            uint32_t place = 0;
+#pragma unroll 2
+            for (uint32_t i = 0; i < size; i += KV) {
+                const UV other = *reinterpret_cast<const UV*>(&list_key[i]);
+#pragma unroll
+                for (int j = 0; j < KV; ++j) {
+                    place += other[j] > key ? 1 : 0;
+                    if (other[j] == key && i + j < size) place += list_index[i + j] < index ? 1 : 0;
+                }
+            }
+            if (tid < size) {
+                sorted_key[place] = key;
+                sorted_index[place] = index;
+            }
+        }
+        __syncthreads();
+        const uint64_t sum = sa_scan(tid < size ? weight.units(weight.share(Key::value(sorted_key[tid]))) : 0, slots);
+        if (tid < size) list_sum[tid] = sum;
+        __syncthreads();
+        lo = from;
+        hi = to;
+        return true;
+    };
+    // the position in the list at which its running sum passes t (which it does)
+    auto in_list = [&](uint64_t t) {
+        if (tid < list_size && list_sum[tid] > t && (tid == 0 || list_sum[tid - 1] <= t)) found[0] = tid;
+        __syncthreads();
+        const uint32_t at = sa_same((uint32_t)found[0]);
+        __syncthreads();
+        return at;
+    };
+    // the bin in which the running sum passes t; kSaBins where it does not
+    auto bin_of = [&](bool by_weight, uint64_t t) {
+        if (tid == 0) found[0] = kSaBins;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k) {
+            const uint32_t b = 2 * tid + k;
+            const uint64_t run = by_weight ? masses[b] : counts[b], before = b == 0 ? 0 : (by_weight ? masses[b - 1] : counts[b - 1]);
+            if (run > t && before <= t) found[0] = b;
+        }
+        __syncthreads();
+        const uint32_t b = sa_same((uint32_t)found[0]);
+        __syncthreads();
+        return b;
+    };
+    // the weights of the elements that share `least` of the largest or more
+    auto sum_of = [&](double least) {
+        uint64_t mine = 0;
+        sa_each<T, kSaBlock>(x, 0, n, [&](T v, uint32_t) {
+            const double share = weight.share(v);
+            mine += share >= least ? weight.units(share) : 0;
+        });
+        const uint64_t run = sa_scan(mine, slots);
+        __syncthreads();
+        if (tid == kSaBlock - 1) found[0] = run;
+        __syncthreads();
+        const uint64_t all = sa_same(found[0]);
+        __syncthreads();
+        return all;
+    };
+    // Digit by digit of the keys, over the whole row: for bins that hold more than a list does. Elements of one key have one weight,
+    // so which of them it is follows from a division.
+    U key = 0;
+    uint64_t number = 0;   // how many of that key stand before it
+    auto by_digits = [&](bool by_weight, uint64_t t) {
+        U prefix = 0;
+        uint64_t before = 0, before_weight = 0;
+#pragma unroll 1
+        for (int shift = (int)sizeof(U) * 8 - 8; shift >= 0; shift -= 8) {
+            if (tid < 256) digit_count[tid] = digit_mass[tid] = 0;
             __syncthreads();
-            if (left < all) break;
-            left -= all;
+#pragma unroll 1
+            for (uint32_t i = tid; i < n; i += kSaBlock) {
+                const T v = x[i];
+                const U k = Key::of(v);
+                // (a shift by the whole width would not be one: the first digit compares nothing)
+                if (shift + 8 < (int)sizeof(U) * 8 && (k >> (shift + 8)) != prefix) continue;
+                const uint32_t digit = (uint32_t)(k >> shift) & 255;
+                atomicAdd((unsigned long long*)&digit_count[digit], 1ull);
+                atomicAdd((unsigned long long*)&digit_mass[digit], (unsigned long long)weight.units(weight.share(v)));
+            }
+            __syncthreads();
+            if (tid == 0) {
+                uint64_t run = before, run_weight = before_weight;
+                int digit = 255;
+                for (; digit > 0; --digit) {
+                    const uint64_t next = run + (by_weight ? digit_mass[digit] : digit_count[digit]);
+                    if (next > t) break;
+                    run = next;
+                    run_weight += digit_mass[digit];
+                }
+                found[0] = (uint64_t)digit;
+                found[1] = run;
+                found[2] = run_weight;
+            }
+            __syncthreads();
+            prefix = (U)((prefix << 8) | (U)sa_same((uint32_t)found[0]));
+            before = sa_same(found[1]);
+            before_weight = sa_same(found[2]);
+            __syncthreads();
+        }
+        const uint64_t one = sa_same(weight.units(weight.share(Key::value(prefix))));
+        key = prefix;
+        number = by_weight && one ? (t - before) / one : t - before;
+        return before_weight + (number + 1) * one;
+    };
+
+    // top_k, top_p, then the answer itself: each the element at which a running sum first passes t. For a small top_k the elements
+    // of the bins that hold it are all that is needed: those alone have weights here. Where they do not fit the list, everything
+    // goes by digits.
+    bool digits = false, listed = false;
+    uint32_t index = 0;
+    uint64_t sum = small ? 0 : sa_same(masses[kSaBins - 1]);
+#pragma unroll 1
+    for (int stage = s.all ? 1 : 0; stage < 3; ++stage) {
+        const bool by_weight = stage > 0;
+        uint64_t t = s.top_k - 1;
+        if (stage == 0) {   // (of what is not -inf)
+            const uint32_t there = sa_same(counts[kSaBins - 1]);
+            t = t < there ? t : there - 1;
+        } else if (stage == 1) {
+            if (!s.cut_p) continue;
+            const double want = sa_same(ceil(s.top_p * (double)sum));
+            t = want > 1.0 ? (uint64_t)want - 1 : 0;
+            t = t < sum ? t : sum - 1;
+        } else if (stage == 2) {
+            if (s.cut_m && (!s.all || s.cut_p)) {
+                uint64_t likely;
+                if (small) {
+                    const bool mine = tid < list_size && weight.share(Key::value(sorted_key[tid])) >= s.likely;
+                    const uint64_t those = __ballot(mine);   // (the first ones of the list)
+                    if (lane == 0) slots[wave] = (uint64_t)__popcll(those);
+                    __syncthreads();
+                    uint64_t number_of = lane < kWaves ? slots[lane] : 0;
+#pragma unroll
+                    for (int d = 8; d > 0; d >>= 1) number_of += (uint64_t)__shfl_xor((unsigned long long)number_of, d);
+                    likely = sa_same(list_sum[sa_same((uint32_t)number_of) - 1]);
+                    __syncthreads();
+                } else {
+                    likely = sum_of(s.likely);
+                }
+                sum = likely < sum ? likely : sum;
+            }
+            const double want = sa_same(floor((u > 0.0 ? u : 0.0) * (double)sum));
+            t = want < (double)sum && (uint64_t)want < sum ? (uint64_t)want : sum - 1;
+        }
+        if (!digits && !(small && by_weight)) {
+            const uint32_t b = bin_of(by_weight, t);
+            if (b >= kSaBins - 1 && !small) continue;   // (a count that reaches what has no weight: everything that has is in front of it)
+            if (b < lo || b > hi) {
+                bool few;
+                if (s.all) {
+                    // few for sure: each element of the bins up to it weighs what the last one's end does, or more
+                    const double edge = weight.unit * exp2(-((double)(b + 1) / (double)weight.bins_per) * weight.rate);
+                    few = sa_same((uint32_t)((double)masses[b] < edge * (0.999 * kSaFew))) != 0;
+                } else {
+                    few = sa_same(counts[b]) <= (small ? (uint32_t)kSaList : kSaFew);
+                }
+                digits = small && !few;
+                if (!digits) digits = !make_list(few ? 0 : b, b);
+                small = small && !digits;
+            }
+        }
+        listed = !digits;
+        if (digits) {
+            sum = by_digits(by_weight, t);
+            // (a bin that is too full says nothing of the next one; without the bins' weights all goes by digits)
+            digits = s.small;
+        } else {
+            const uint64_t base = lo == 0 ? 0 : sa_same(masses[lo - 1]);
+            const uint32_t place = by_weight ? in_list(t - base) : (uint32_t)t - (lo == 0 ? 0 : sa_same(counts[lo - 1]));
+            index = sa_same(sorted_index[place]);
+            sum = base + sa_same(list_sum[place]);
         }
     }
+    if (listed) {
+        if (tid == 0) p.out[row] = (int32_t)index;
+        return;
+    }
+    // the element of that key with `number` before it, in order of the index
+    uint64_t left = number;
+#pragma unroll 1
+    for (uint32_t first = 0; first < n; first += kSaBlock) {
+        const uint32_t i = first + tid;
+        const bool hit = i < n && Key::of(x[i]) == key;
+        const uint64_t hits = __ballot(hit);
+        if (lane == 0) slots[wave] = (uint64_t)__popcll(hits);
+        __syncthreads();
+        uint64_t ahead = (uint64_t)__popcll(hits & ((1ull << lane) - 1)), here = 0;
+#pragma unroll 1
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            ahead += w < wave ? slots[w] : 0;
+            here += slots[w];
+        }
+        if (hit && ahead == left) p.out[row] = (int32_t)i;
+        __syncthreads();
+        here = sa_same(here);
+        if (left < here) break;
+        left -= here;
+    }
+}
+
+// rows of one round of launches: their bins take 12 to 24 KiB a part
+constexpr uint64_t kSaRows = 4096;
+
+template <class T>
+int sa_launch(const cumo_hip_sample_t& d, hipStream_t stream) {
+    SaParams p;
+    std::memset(&p, 0, sizeof(p));
+    static_cast<cumo_hip_sample_t&>(p) = d;
+    int bits = 0;
+    while ((1ull << bits) < d.n) ++bits;
+    p.unit_bits = 62 - bits < 50 ? 62 - bits : 50;
+    const uint64_t rows = d.rows < kSaRows ? d.rows : kSaRows;
+    // enough blocks for every compute unit, and enough elements for every block
+    auto parts = [&](uint64_t blocks, uint64_t elements, uint64_t most) {
+        uint64_t k = blocks / rows, fit = d.n / elements;
+        k = k < fit ? k : fit;
+        k = k < most ? k : most;
+        return (uint32_t)(k ? k : 1);
+    };
+    p.looks = parts(2048, 2048, 64);
+    p.fills = parts(512, 4096, 16);
+    const bool may_count = d.top_k.each || (d.top_k.value > 0.0 && d.top_k.value < (double)d.n);
+    const uint64_t part_bytes = rows * p.looks * sizeof(SaPart), bins = rows * p.fills * kSaBins;
+    char* memory = cumo_cuda_runtime_malloc(part_bytes + bins * (8 + (may_count ? 4 : 0)));
+    if (!memory) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
+    p.parts = reinterpret_cast<SaPart*>(memory);
+    p.masses = reinterpret_cast<uint64_t*>(memory + part_bytes);
+    p.counts = may_count ? reinterpret_cast<uint32_t*>(p.masses + bins) : nullptr;
+    cumo_hip_row_number_t* const settings[5] = {&p.u, &p.temperature, &p.top_k, &p.top_p, &p.min_p};
+    for (uint64_t done = 0; done < d.rows; done += rows) {
+        const unsigned now = (unsigned)(d.rows - done < rows ? d.rows - done : rows);
+        hipLaunchKernelGGL((sample_look_kernel<T>), dim3(now, p.looks), dim3(kSaLook), 0, stream, p);
+        hipLaunchKernelGGL((sample_fill_kernel<T>), dim3(now, p.fills), dim3(kSaBlock), 0, stream, p);
+        hipLaunchKernelGGL((sample_kernel<T>), dim3(now), dim3(kSaBlock), 0, stream, p);
+        p.x += (int64_t)now * p.x_step;
+        p.out += now;
+        for (cumo_hip_row_number_t* a : settings)
+            if (a->each) a->each += (uint64_t)now * (a->type == 1 ? 8 : 4);
+    }
+    cumo_cuda_runtime_check_kernel_launch();
+    // (the memory of a captured launch stays with its graph)
+    if (!stream_under_capture()) cumo_cuda_runtime_free(memory);
+    return CUMO_HIP_OK;
 }
 
 }  // namespace
@@ -233,15 +637,5 @@ using namespace cumo_hip;
 
 extern "C" int cumo_hip_sample_kernel_launch(int type, const cumo_hip_sample_t* d) {
     if (d->rows == 0) return CUMO_HIP_OK;
-    SaParams p;
-    std::memset(&p, 0, sizeof(p));
-    static_cast<cumo_hip_sample_t&>(p) = *d;
-    int bits = 0;
-    while ((1ull << bits) < d->n) ++bits;
-    p.unit_bits = 62 - bits < 50 ? 62 - bits : 50;
-    const dim3 grid((unsigned)(d->rows < 65536 ? d->rows : 65536)), block(kSaBlock);
-    if (type == 0) hipLaunchKernelGGL((sample_kernel<float>), grid, block, 0, current_stream(), p);
-    else hipLaunchKernelGGL((sample_kernel<double>), grid, block, 0, current_stream(), p);
-    cumo_cuda_runtime_check_kernel_launch();
-    return CUMO_HIP_OK;
+    return type == 0 ? sa_launch<float>(*d, current_stream()) : sa_launch<double>(*d, current_stream());
 }

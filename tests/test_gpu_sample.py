@@ -131,6 +131,7 @@ def test_masked_infinite_and_nan_logits(dt, n):
     x[7, 1:] = np.finfo(dt).min
     x[8] = 0.0
     x[8, ::2] = -0.0                     # the zeros are equal
+    x[9] = rng.integers(0, 3, n) * np.finfo(dt).smallest_subnormal   # three numbers next to each other
     for u in (0.0, 0.3, 0.75, 1 - 2.0 ** -24):
         us = np.full(10, u, dt)
         for settings in SETTINGS + [{"top_k": 2}, {"top_k": n - 1}]:
@@ -172,6 +173,34 @@ def test_a_row_of_its_own_settings_each(dt, shape):
     for r in range(0, rows, 7):
         one = {k: v[r:r + 1] for k, v in settings.items()}
         assert take(m, x[r:r + 1], u[r:r + 1], dt, **one)[0] == want[r]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n", [300, 9000, 140000])
+def test_few_tokens_left_by_a_mask_and_large_limits(dt, n):
+    """A top_k beyond what a mask leaves, and top_k of every size around what lists hold."""
+    import cumo_amd as m
+    rng = np.random.default_rng(n)
+    x = np.full((6, n), -np.inf, dt)
+    for r, left in enumerate((1, 2, 17, 120, 200, 250)):
+        x[r, rng.choice(n, left, replace=False)] = rng.standard_normal(left) * 2
+    u = rng.random(6).astype(dt)
+    full = (rng.standard_normal((6, n)) * 2).astype(dt)
+    coarse = np.round(full * 4) / 4
+    for k in (2, 17, 50, 255, 256, 257, 511, 512, 513, 1023, 1025, 5000, n - 1):
+        for rows in (x, full, coarse):
+            for more in ({}, {"top_p": 0.9}, {"min_p": 0.2, "temperature": 2.0}, {"top_p": 0.7, "min_p": 0.1}):
+                assert (take(m, rows, u, dt, top_k=k, **more) == chosen(rows, u, top_k=k, **more)).all(), (k, more)
+
+
+def test_more_rows_than_one_round_takes():
+    import cumo_amd as m
+    rng = np.random.default_rng(21)
+    x = (rng.standard_normal((9001, 40)) * 2).astype(np.float32)
+    u = rng.random(9001).astype(np.float32)
+    k = rng.integers(0, 20, 9001).astype(np.int32)
+    p = rng.uniform(0.3, 1, 9001).astype(np.float32)
+    assert (take(m, x, u, np.float32, top_k=k, top_p=p) == chosen(x, u, top_k=k, top_p=p)).all()
 
 
 @pytest.mark.parametrize("dt", TYPES)
