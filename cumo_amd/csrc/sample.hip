@@ -107,10 +107,10 @@ struct SaParams : cumo_hip_sample_t {
     uint32_t* counts;        // the same, where a row may have a top_k
 };
 
-// f of the elements [from, to) of a row, by whole waves: lanes without one bring -inf
-template <class T, int BLOCK, class F>
+// f of the elements [from, to) of a row, by whole waves: lanes without one bring -inf. U: vectors of a lane that are on their way at once.
+template <class T, int BLOCK, int U, class F>
 __device__ __forceinline__ void sa_each(const T* row, uint32_t from, uint32_t to, F f) {
-    constexpr int V = 16 / (int)sizeof(T), U = 4;
+    constexpr int V = 16 / (int)sizeof(T);
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     union Vec { u4 q; T t[V]; __device__ Vec() {} };
     const T* part = row + from;
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kSaLook) void sample_look_kernel(SaParams p) {
     uint32_t first = 0xffffffffu;
     bool nan = false;
     if (from < to) {
-        sa_each<T, kSaLook>(reinterpret_cast<const T*>(p.x + (int64_t)blockIdx.x * p.x_step), from, to, [&](T v, uint32_t i) {
+        sa_each<T, kSaLook, 4>(reinterpret_cast<const T*>(p.x + (int64_t)blockIdx.x * p.x_step), from, to, [&](T v, uint32_t i) {
             nan |= v != v;
             first = v > m ? i : first;   // (a lane's positions rise)
             m = v > m ? v : m;
@@ -255,13 +255,13 @@ __global__ __launch_bounds__(kSaBlock) void sample_fill_kernel(SaParams p) {
     const T* x = reinterpret_cast<const T*>(p.x + (int64_t)blockIdx.x * p.x_step);
     if (from < to) {
         if (s.small) {
-            sa_each<T, kSaBlock>(x, from, to, [&](T v, uint32_t) {
+            sa_each<T, kSaBlock, 4>(x, from, to, [&](T v, uint32_t) {
                 if (v > (T)-INFINITY) atomicAdd(&counts[s.weight.bin(v)], 1u);
             });
         } else {
             // (where min_p alone cuts, what it leaves out need not be summed)
             const double least = s.cut_m && s.all && !s.cut_p ? s.likely : 0.0;
-            sa_each<T, kSaBlock>(x, from, to, [&](T v, uint32_t) {
+            sa_each<T, kSaBlock, 4>(x, from, to, [&](T v, uint32_t) {
                 const double share = s.weight.share(v);
                 const uint64_t units = share >= least ? s.weight.units(share) : 0;
                 const uint32_t b = s.weight.bin(v);
@@ -327,16 +327,21 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         const uint32_t b = 2 * tid;   // (two bins a lane)
         uint64_t one = 0, two = 0;
         uint32_t c_one = 0, c_two = 0;
-#pragma unroll 4
-        for (uint32_t part = 0; part < p.fills; ++part) {
-            const uint64_t at = (row * p.fills + part) * kSaBins + b;
-            if (!small) {
-                one += p.masses[at];
-                two += p.masses[at + 1];
+        const uint64_t at = row * p.fills * kSaBins + b;
+        if (!small) {
+#pragma unroll 8
+            for (uint32_t part = 0; part < p.fills; ++part) {
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p.masses + at + (uint64_t)part * kSaBins);
+                one += v.x;
+                two += v.y;
             }
-            if (!s.all) {
-                c_one += p.counts[at];
-                c_two += p.counts[at + 1];
+        }
+        if (!s.all) {
+#pragma unroll 8
+            for (uint32_t part = 0; part < p.fills; ++part) {
+                const uint2 v = *reinterpret_cast<const uint2*>(p.counts + at + (uint64_t)part * kSaBins);
+                c_one += v.x;
+                c_two += v.y;
             }
         }
         if (!small) {
@@ -359,11 +364,16 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         if (tid == 0) list_size = 0;
         list_key[tid] = 0;   // (below every number's key)
         __syncthreads();
-        sa_each<T, kSaBlock>(x, 0, n, [&](T v, uint32_t i) {
-            const uint32_t b = weight.bin(v);
-            const bool hit = b >= from && b <= to && v > (T)-INFINITY;
-            const uint64_t hits = __ballot(hit);
-            if (hits) {
+        // What may be in those bins, half a bin more on either side: two comparisons for each number that is not. (The bins' rounding
+        // moves a number by less than a thousandth of a bin, and the bounds' keeps the order.)
+        const double above = from == 0 ? -INFINITY : ((double)from - 0.5) / (double)weight.bins_per;
+        const double lowest = (double)weight.max - ((double)to + 1.5) / (double)weight.bins_per;
+        const T most = (T)((double)weight.max - above), least = to < kSaBins - 1 && lowest == lowest ? (T)lowest : (T)-INFINITY;
+        sa_each<T, kSaBlock, 4>(x, 0, n, [&](T v, uint32_t i) {
+            if (__ballot(v >= least && v <= most)) {
+                const uint32_t b = weight.bin(v);
+                const bool hit = b >= from && b <= to && v > (T)-INFINITY;
+                const uint64_t hits = __ballot(hit);
                 uint32_t at = 0;
                 if (lane == 0) at = atomicAdd(&list_size, (uint32_t)__popcll(hits));
                 at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(hits & ((1ull << lane) - 1));
@@ -431,7 +441,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
     // the weights of the elements that share `least` of the largest or more
     auto sum_of = [&](double least) {
         uint64_t mine = 0;
-        sa_each<T, kSaBlock>(x, 0, n, [&](T v, uint32_t) {
+        sa_each<T, kSaBlock, 4>(x, 0, n, [&](T v, uint32_t) {
             const double share = weight.share(v);
             mine += share >= least ? weight.units(share) : 0;
         });
@@ -607,7 +617,7 @@ int sa_launch(const cumo_hip_sample_t& d, hipStream_t stream) {
     p.looks = parts(2048, 2048, 64);
     p.fills = parts(512, 4096, 16);
     const bool may_count = d.top_k.each || (d.top_k.value > 0.0 && d.top_k.value < (double)d.n);
-    const uint64_t part_bytes = rows * p.looks * sizeof(SaPart), bins = rows * p.fills * kSaBins;
+    const uint64_t part_bytes = (rows * p.looks * sizeof(SaPart) + 15) & ~15ull, bins = rows * p.fills * kSaBins;
     char* memory = cumo_cuda_runtime_malloc(part_bytes + bins * (8 + (may_count ? 4 : 0)));
     if (!memory) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
     p.parts = reinterpret_cast<SaPart*>(memory);

@@ -154,6 +154,15 @@ def test_u_outside_its_range_and_settings_at_their_limits():
     assert f(top_k=np.array([-3], np.int32)) == 3 and f(top_k=np.array([0], np.int32)) == 3 and f(top_k=np.array([2], np.int32)) == 1
     assert f(top_p=d(-0.5)) == 0 and f(top_p=d(np.nan)) == 3 and f(top_p=d(2.0)) == 3
     assert f(min_p=d(-1.0)) == 3 and f(min_p=d(np.nan)) == 3 and f(min_p=d(5.0)) == 0 and f(min_p=d(0.4)) == 1
+    # numbers far from zero, an infinite one, at any temperature
+    for shift in (1e6, -3e7, 1e30):
+        for dt in TYPES:
+            y = (np.array([[3.0, 2.0, 1.0, 0.0]]) * (1 if abs(shift) < 1e20 else 1e24) + shift).astype(dt)
+            for t in (0.5, 1.0, 1e24, float("inf")):
+                for u in (0.1, 0.6, 0.99):
+                    assert take(m, y, np.array([u], dt), dt, temperature=t)[0] == chosen(y, np.array([u], dt), temperature=t)[0], (shift, dt, t, u)
+    y = np.array([[1.0, np.inf, 2.0, np.inf]])
+    assert take(m, y, np.array([0.3]), np.float64, temperature=float("inf"))[0] == 1 and take(m, y, np.array([0.7]), np.float64, temperature=2.0)[0] == 3
     assert f(temperature=1e-30) == 0 and f(temperature=1e300) == 3 and f(temperature=float("inf")) == 3
 
 
