@@ -1161,6 +1161,9 @@ class _Fused:
     def rmsnorm(x, weight=None, residual=None, eps=1e-6):
         """s / sqrt(mean(s**2) + eps) * weight along the last dimension, s = x + residual. With a residual the
         answer is [that, s]."""
+        done = _native.rmsnorm(x, weight, residual, eps)  # None: the general way
+        if done is not None:
+            return done
         y, s = NArrayDesc(), NArrayDesc()
         results = (y,) if residual is None else (y, s)
         return _run(_L.cumo_hip_na_rmsnorm, _optional(x), _optional(weight), _optional(residual), float(eps), C.byref(y),
@@ -1170,6 +1173,9 @@ class _Fused:
     def rmsnorm_q8(x, weight=None, residual=None, eps=1e-6):
         """rmsnorm in 8 bits: [q, scale], q Int8 = round(y / scale), scale = max|y| / 127 of each row (its last
         dimension is 1); [q, scale, s] with a residual."""
+        done = _native.rmsnorm_q8(x, weight, residual, eps)  # None: the general way
+        if done is not None:
+            return done
         q, scale, s = NArrayDesc(), NArrayDesc(), NArrayDesc()
         results = (q, scale) if residual is None else (q, scale, s)
         return _run(_L.cumo_hip_na_rmsnorm_q8, _optional(x), _optional(weight), _optional(residual), float(eps), C.byref(q), C.byref(scale),
@@ -1178,6 +1184,9 @@ class _Fused:
     @staticmethod
     def dequantize(q, scale):
         """q * scale for an Int8 array and its rows' scales, in the scales' type."""
+        done = _native.dequantize(q, scale)  # None: the general way
+        if done is not None:
+            return done
         if not isinstance(q, Int8):
             raise TypeError("dequantize needs an Int8 array")
         d, z = q._desc(), NArrayDesc()
@@ -1188,6 +1197,9 @@ class _Fused:
         """The gradient of x (and of residual) from g, that of y: s is x + residual as rmsnorm answered it (x where
         there was no residual), gsum the gradient of s itself, if it has one. With a weight the answer is [that,
         the weight's]."""
+        done = _native.rmsnorm_grad(g, s, weight, gsum, eps)  # None: the general way
+        if done is not None:
+            return done
         gx, gw = NArrayDesc(), NArrayDesc()
         results = (gx,) if weight is None else (gx, gw)
         return _run(_L.cumo_hip_na_rmsnorm_grad, _optional(g), _optional(s), _optional(weight), _optional(gsum), float(eps), C.byref(gx),
@@ -1196,6 +1208,9 @@ class _Fused:
     @staticmethod
     def recurrence(a, b, h0=None, axis=-1):
         """h[t] = a[t] * h[t-1] + b[t] along an axis, from h0 (the arrays' shape without the axis) or zeros."""
+        done = _native.recurrence(a, b, h0, axis)  # None: the general way
+        if done is not None:
+            return done
         z = NArrayDesc()
         da, db, d0 = _optional(a), _optional(b), _optional(h0)
         return _run(_L.cumo_hip_na_recurrence, da, db, d0, _one_axis(a.ndim, axis), C.byref(z), results=(z,))
@@ -1203,6 +1218,9 @@ class _Fused:
     @staticmethod
     def recurrence_grad(g, a, h, h0=None, axis=-1):
         """The gradients of a and b, and of h0 where it is given, from g, that of h: [ga, gb] or [ga, gb, gh0]."""
+        done = _native.recurrence_grad(g, a, h, h0, axis)  # None: the general way
+        if done is not None:
+            return done
         ga, gb, g0 = NArrayDesc(), NArrayDesc(), NArrayDesc()
         results = (ga, gb) if h0 is None else (ga, gb, g0)
         dg, da, dh, d0 = _optional(g), _optional(a), _optional(h), _optional(h0)
@@ -1217,6 +1235,9 @@ class _Fused:
         of these the ones of weight min_p or more; the answer is the first of those left whose running sum of weights
         exceeds u times theirs. temperature 0 takes the largest. -1 where a row holds a NaN or nothing but -inf. Every
         setting is a number, or an array with one for each row."""
+        done = _native.sample(x, u, temperature, top_k, top_p, min_p)  # None: the general way
+        if done is not None:
+            return done
         def setting(v, cast):
             return (cast(0), _optional(v)) if isinstance(v, NArray) else (cast(v), None)
 
