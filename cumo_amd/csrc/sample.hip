@@ -66,12 +66,24 @@ __device__ __forceinline__ V sa_same(V v) {
     }
 }
 
-__device__ __forceinline__ double sa_number(const cumo_hip_row_number_t& a, uint64_t row) {
-    if (!a.each) return a.value;
-    if (a.type == 0) return (double)reinterpret_cast<const float*>(a.each)[row];
-    if (a.type == 1) return reinterpret_cast<const double*>(a.each)[row];
-    return (double)reinterpret_cast<const int32_t*>(a.each)[row];
-}
+// A row's number in two steps: its words, without a branch, so that several numbers are on their way together (from `any`, some
+// memory, where there is one number for all rows), then what they say.
+struct SaNumber {
+    uint32_t low, high;
+    __device__ __forceinline__ SaNumber(const cumo_hip_row_number_t& a, uint64_t row, const void* any) {
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(a.each ? a.each : static_cast<const char*>(any));
+        const uint64_t k = a.each ? (a.type == 1 ? 2 * row : row) : 0;
+        low = at[k];
+        high = at[a.each && a.type == 1 ? k + 1 : k];
+    }
+    __device__ __forceinline__ double value(const cumo_hip_row_number_t& a) const {
+        if (!a.each) return a.value;
+        const uint32_t l = sa_same(low);
+        if (a.type == 0) return (double)__uint_as_float(l);
+        if (a.type == 1) return __hiloint2double((int)sa_same(high), (int)l);
+        return (double)(int32_t)l;
+    }
+};
 
 // Weights of a row, 2^S for its maximum, and the bins. The sum with 1.5 * 2^52 leaves the rounded product in the lower bits.
 template <class T>
@@ -107,7 +119,8 @@ struct SaParams : cumo_hip_sample_t {
     uint32_t* counts;        // the same, where a row may have a top_k
 };
 
-// f of the elements [from, to) of a row, by whole waves: lanes without one bring -inf. U: vectors of a lane that are on their way at once.
+// f of the elements [from, to) of a row, by whole waves: lanes without one bring -inf. U: vectors of a lane that are on their way at
+// once (a second set behind them is no gain: 256 rows at once are bound by the last-level cache's rate).
 template <class T, int BLOCK, int U, class F>
 __device__ __forceinline__ void sa_each(const T* row, uint32_t from, uint32_t to, F f) {
     constexpr int V = 16 / (int)sizeof(T);
@@ -198,19 +211,16 @@ struct SaSettings {
     bool none, greedy;         // nothing to choose; the first of the largest
     bool all, cut_p, cut_m, small;   // no top_k; top_p, min_p cut; a top_k small enough for a list
     uint64_t top_k;
-    double top_p, likely;
+    double u, top_p, likely;
     __device__ __forceinline__ SaSettings(const SaParams& p, uint64_t row) {
         const uint32_t lane = threadIdx.x & 63;
-        T m = -INFINITY, least = INFINITY;
-        first = 0xffffffffu;
-        uint32_t nan = 0;
-        if (lane < p.looks) {
-            const SaPart part = p.parts[row * p.looks + lane];
-            m = (T)part.max;
-            least = (T)part.least;
-            first = part.first;
-            nan = part.nan;
-        }
+        const SaPart part = p.parts[row * p.looks + (lane < p.looks ? lane : 0)];   // (one of them more than once changes nothing)
+        const SaNumber u_at(p.u, row, p.parts), temperature_at(p.temperature, row, p.parts), k_at(p.top_k, row, p.parts), top_p_at(p.top_p, row, p.parts),
+            min_p_at(p.min_p, row, p.parts);
+        float_tables_prepare();
+        T m = (T)part.max, least = (T)part.least;
+        first = part.first;
+        const uint32_t nan = part.nan;
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) {
             sa_larger(m, first, __shfl_xor(m, d), __shfl_xor(first, d));
@@ -220,8 +230,9 @@ struct SaSettings {
         m = sa_same(m);
         first = sa_same(first);
         none = __ballot(nan != 0) != 0 || m == (T)-INFINITY;
-        const double temperature = sa_same(sa_number(p.temperature, row)), k = sa_same(sa_number(p.top_k, row)), min_p = sa_same(sa_number(p.min_p, row));
-        top_p = sa_same(sa_number(p.top_p, row));
+        const double temperature = temperature_at.value(p.temperature), k = k_at.value(p.top_k), min_p = min_p_at.value(p.min_p);
+        u = u_at.value(p.u);
+        top_p = top_p_at.value(p.top_p);
         all = !(k > 0.0 && k < (double)p.n);
         greedy = !(temperature > 0.0) || (!all && k < 2.0) || top_p <= 0.0;
         top_k = all ? p.n : (uint64_t)k;
@@ -244,7 +255,6 @@ __global__ __launch_bounds__(kSaBlock) void sample_fill_kernel(SaParams p) {
     __shared__ uint32_t counts[kSaBins];
     const SaSettings<T> s(p, blockIdx.x);
     if (s.none || s.greedy) return;
-    float_tables_prepare();
     for (uint32_t b = threadIdx.x; b < kSaBins; b += kSaBlock) {
         masses[b] = 0;
         counts[b] = 0;
@@ -303,11 +313,13 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
     typedef typename Key::U U;
     constexpr int kWaves = kSaBlock / 64, KV = 16 / (int)sizeof(U);
     typedef U UV __attribute__((ext_vector_type(KV)));
+    typedef uint32_t IV __attribute__((ext_vector_type(KV)));
     __shared__ uint64_t masses[kSaBins];   // running sums of the bins
     __shared__ uint32_t counts[kSaBins];
     __shared__ __attribute__((aligned(16))) U list_key[kSaList];
     __shared__ U sorted_key[kSaList];
-    __shared__ uint32_t list_index[kSaList], sorted_index[kSaList];
+    __shared__ __attribute__((aligned(16))) uint32_t list_index[kSaList];
+    __shared__ uint32_t sorted_index[kSaList];
     __shared__ uint64_t list_sum[kSaList], slots[kWaves], found[3], digit_count[256], digit_mass[256];
     __shared__ uint32_t list_size;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -320,8 +332,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         if (tid == 0) p.out[row] = s.none ? -1 : (int32_t)s.first;
         return;
     }
-    float_tables_prepare();
-    const double u = sa_same(sa_number(p.u, row));
+    const double u = s.u;
     bool small = s.small;
     {
         const uint32_t b = 2 * tid;   // (two bins a lane)
@@ -394,13 +405,11 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
             const uint32_t index = list_index[tid];
             uint32_t place = 0;
 #pragma unroll 2
-            for (uint32_t i = 0; i < size; i += KV) {
+            for (uint32_t i = 0; i < size; i += KV) {   // (behind the list's end are keys of 0, which no number has)
                 const UV other = *reinterpret_cast<const UV*>(&list_key[i]);
+                const IV other_index = *reinterpret_cast<const IV*>(&list_index[i]);
 #pragma unroll
-                for (int j = 0; j < KV; ++j) {
-                    place += other[j] > key ? 1 : 0;
-                    if (other[j] == key && i + j < size) place += list_index[i + j] < index ? 1 : 0;
-                }
+                for (int j = 0; j < KV; ++j) place += (other[j] > key) | ((other[j] == key) & (other_index[j] < index)) ? 1 : 0;
             }
             if (tid < size) {
                 sorted_key[place] = key;
