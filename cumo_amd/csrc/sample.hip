@@ -116,6 +116,7 @@ struct SaParams : cumo_hip_sample_t {
     uint32_t looks, fills;   // parts of a row in the first two launches (64 and 16 at most)
     SaPart* parts;           // [rows][looks]
     uint64_t* masses;        // [rows][fills][bins]
+    uint64_t* likely;        // [rows][fills]: the weights that min_p leaves of a part, where other limits come before it
     uint32_t* counts;        // the same, where a row may have a top_k
 };
 
@@ -251,10 +252,11 @@ struct SaSettings {
 
 template <class T>
 __global__ __launch_bounds__(kSaBlock) void sample_fill_kernel(SaParams p) {
-    __shared__ uint64_t masses[kSaBins];
+    __shared__ uint64_t masses[kSaBins], likely;
     __shared__ uint32_t counts[kSaBins];
     const SaSettings<T> s(p, blockIdx.x);
     if (s.none || s.greedy) return;
+    if (threadIdx.x == 0) likely = 0;
     for (uint32_t b = threadIdx.x; b < kSaBins; b += kSaBlock) {
         masses[b] = 0;
         counts[b] = 0;
@@ -271,16 +273,25 @@ __global__ __launch_bounds__(kSaBlock) void sample_fill_kernel(SaParams p) {
         } else {
             // (where min_p alone cuts, what it leaves out need not be summed)
             const double least = s.cut_m && s.all && !s.cut_p ? s.likely : 0.0;
+            uint64_t mine = 0;
             sa_each<T, kSaBlock, 4>(x, from, to, [&](T v, uint32_t) {
                 const double share = s.weight.share(v);
                 const uint64_t units = share >= least ? s.weight.units(share) : 0;
+                mine += share >= s.likely ? units : 0;
+                asm("" : "+v"(mine));   // (one after the other: sixteen numbers' weights side by side are twice the registers, and half the blocks)
                 const uint32_t b = s.weight.bin(v);
                 if (units) atomicAdd((unsigned long long*)&masses[b], (unsigned long long)units);
                 if (!s.all && v > (T)-INFINITY) atomicAdd(&counts[b], 1u);
             });
+            if (s.cut_m) {
+#pragma unroll
+                for (int d = 32; d > 0; d >>= 1) mine += (uint64_t)__shfl_xor((unsigned long long)mine, d);
+                if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long*)&likely, (unsigned long long)mine);
+            }
         }
     }
     __syncthreads();
+    if (threadIdx.x == 0) p.likely[(uint64_t)blockIdx.x * p.fills + blockIdx.y] = likely;
     const uint64_t at = ((uint64_t)blockIdx.x * p.fills + blockIdx.y) * kSaBins;
     for (uint32_t b = threadIdx.x; b < kSaBins; b += kSaBlock) {
         if (!s.small) p.masses[at + b] = masses[b];
@@ -333,6 +344,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         return;
     }
     const double u = s.u;
+    const uint64_t part_likely = lane < p.fills ? p.likely[row * p.fills + lane] : 0;
     bool small = s.small;
     {
         const uint32_t b = 2 * tid;   // (two bins a lane)
@@ -540,8 +552,13 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
                     for (int d = 8; d > 0; d >>= 1) number_of += (uint64_t)__shfl_xor((unsigned long long)number_of, d);
                     likely = sa_same(list_sum[sa_same((uint32_t)number_of) - 1]);
                     __syncthreads();
-                } else {
+                } else if (s.small) {   // (no part has taken weights)
                     likely = sum_of(s.likely);
+                } else {
+                    likely = part_likely;
+#pragma unroll
+                    for (int d = 32; d > 0; d >>= 1) likely += (uint64_t)__shfl_xor((unsigned long long)likely, d);
+                    likely = sa_same(likely);
                 }
                 sum = likely < sum ? likely : sum;
             }
@@ -627,11 +644,12 @@ int sa_launch(const cumo_hip_sample_t& d, hipStream_t stream) {
     p.fills = parts(512, 4096, 16);
     const bool may_count = d.top_k.each || (d.top_k.value > 0.0 && d.top_k.value < (double)d.n);
     const uint64_t part_bytes = (rows * p.looks * sizeof(SaPart) + 15) & ~15ull, bins = rows * p.fills * kSaBins;
-    char* memory = cumo_cuda_runtime_malloc(part_bytes + bins * (8 + (may_count ? 4 : 0)));
+    char* memory = cumo_cuda_runtime_malloc(part_bytes + (bins + rows * p.fills) * 8 + (may_count ? bins * 4 : 0));
     if (!memory) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
     p.parts = reinterpret_cast<SaPart*>(memory);
     p.masses = reinterpret_cast<uint64_t*>(memory + part_bytes);
-    p.counts = may_count ? reinterpret_cast<uint32_t*>(p.masses + bins) : nullptr;
+    p.likely = p.masses + bins;
+    p.counts = may_count ? reinterpret_cast<uint32_t*>(p.likely + rows * p.fills) : nullptr;
     cumo_hip_row_number_t* const settings[5] = {&p.u, &p.temperature, &p.top_k, &p.top_p, &p.min_p};
     for (uint64_t done = 0; done < d.rows; done += rows) {
         const unsigned now = (unsigned)(d.rows - done < rows ? d.rows - done : rows);
