@@ -103,7 +103,17 @@ struct ReLanes {
     __device__ __forceinline__ void put(int64_t offset, T v) const { *reinterpret_cast<T*>(const_cast<char*>(low) + offset + up) = v; }
     template <class T>
     __device__ __forceinline__ void put_away(int64_t offset, T v) const { __builtin_nontemporal_store(v, reinterpret_cast<T*>(const_cast<char*>(low) + offset + up)); }
+    template <class T>   // written through the second-level cache
+    __device__ __forceinline__ void put_through(int64_t offset, T v) const {
+        __hip_atomic_store(reinterpret_cast<T*>(const_cast<char*>(low) + offset + up), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
 };
+
+// Forms of a pass over arrays larger than the caches, us (with a sum of the result behind it) for SFloat [8,4096,2048] forwards,
+// backwards, and [1,65536,1000], in tiles:
+//   loads plain / nt, stores nt              161 (201) / 156 (197),  216 / 236,  184 (224) / 190 (231)
+//   loads nt, stores plain / written through 145 (182) / 140 (178),  272 / 244,  190 (220) / 195 (224)
+enum ReStore { RE_PLAIN, RE_AWAY, RE_THROUGH };
 
 // what a wave holds of a, b and h: R rows of 64 columns
 template <class T, bool GRAD>
@@ -111,9 +121,9 @@ struct ReTile {
     static constexpr int R = kReRows<T, GRAD>;
     T a[R], b[R], h[GRAD ? R : 1];
     // rows [t, t + R) that there are; the others leave a state as it is
-    template <bool ONCE>
+    template <bool NT>
     __device__ __forceinline__ void load(const ReArgs& p, const ReLanes& la, const ReLanes& lb, const ReLanes& lh, uint64_t t, T first) {
-        auto get = [](const ReLanes& x, int64_t offset) { return ONCE ? x.template get_once<T>(offset) : x.template get<T>(offset); };
+        auto get = [](const ReLanes& x, int64_t offset) { return NT ? x.template get_once<T>(offset) : x.template get<T>(offset); };
         const int64_t at = (int64_t)t;
         if (t + R <= p.time && (!GRAD || t + R < p.time)) {
 #pragma unroll
@@ -147,9 +157,13 @@ struct ReTile {
         }
         product = re_product(product, re_gates(own, least));
     }
-    template <bool ONCE>
+    template <ReStore FORM>
     __device__ __forceinline__ void take(const ReArgs& p, const ReLanes& lout, const ReLanes& lgb, uint64_t t, uint64_t to, bool there, T& state) {
-        auto put = [](const ReLanes& x, int64_t offset, T v) { ONCE ? x.put_away(offset, v) : x.put(offset, v); };
+        auto put = [](const ReLanes& x, int64_t offset, T v) {
+            if constexpr (FORM == RE_AWAY) x.put_away(offset, v);
+            else if constexpr (FORM == RE_THROUGH) x.put_through(offset, v);
+            else x.put(offset, v);
+        };
         const int64_t at = (int64_t)t;
 #pragma unroll
         for (int j = 0; j < R; ++j) re_step<T, GRAD>(a[j], b[j], h[GRAD ? j : 0], state);   // (rows that are not there change nothing)
@@ -198,20 +212,20 @@ __global__ __launch_bounds__(NW * 64) void recurrence_columns_kernel(ReArgs p) {
             }
             turn ^= 1;
         }
-        tile.template take<ONCE>(p, lout, lgb, t, p.time, there, own);
+        tile.template take<!ONCE ? RE_PLAIN : GRAD ? RE_AWAY : RE_THROUGH>(p, lout, lgb, t, p.time, there, own);
         if constexpr (NW == 1) state = own;
         if (GRAD && p.last && there && t < p.time && t + R >= p.time) reinterpret_cast<T*>(p.last)[c] = own;   // (carried past the last step)
     };
     // two tiles in turn: one is on its way while the other's steps are taken. Every wave of the block goes round equally often.
     Tile one, two;
     uint64_t t = (uint64_t)wave * R, at = 0;
-    one.template load<ONCE>(p, la, lb, lh, t, first);
+    one.template load<ONCE && !GRAD>(p, la, lb, lh, t, first);
     for (;;) {
-        two.template load<ONCE>(p, la, lb, lh, t + kTile, first);
+        two.template load<ONCE && !GRAD>(p, la, lb, lh, t + kTile, first);
         walk(one, t);
         t += kTile;
         if ((at += kTile) >= p.time) break;
-        one.template load<ONCE>(p, la, lb, lh, t + kTile, first);
+        one.template load<ONCE && !GRAD>(p, la, lb, lh, t + kTile, first);
         walk(two, t);
         t += kTile;
         if ((at += kTile) >= p.time) break;
@@ -375,7 +389,7 @@ __global__ __launch_bounds__(kReChainWaves * 64, sizeof(T) == 4 ? 8 : 4) void re
     if (wave == 0 && k + 1 < chain.tiles) slot(k).put_state(re_join(product, b, state));
     for (uint32_t w = 0; w < wave; ++w) state = re_join(products[w][lane], reached[w][lane], state);
     const ReLanes lout(p.out, o, i, p.out_step), lgb(GRAD ? p.gb : p.out, o, i, GRAD ? p.gb_step : p.out_step);
-    tile.template take<true>(p, lout, lgb, t, p.time, there, state);
+    tile.template take<RE_AWAY>(p, lout, lgb, t, p.time, there, state);
     if (GRAD && p.last && there && t < p.time && t + R >= p.time) reinterpret_cast<T*>(p.last)[c] = state;   // (carried past the last step)
 }
 
@@ -586,6 +600,16 @@ __global__ __launch_bounds__(kReBlock) void recurrence_rows_kernel(ReArgs p) {
     }
 }
 
+// a lane's value for the whole wave; `lane` is the same for all
+template <class V>
+__device__ __forceinline__ V re_lane(V v, int lane) {
+    union { V v; int w[sizeof(V) / 4]; } u;
+    u.v = v;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(V) / 4); ++i) u.w[i] = __builtin_amdgcn_readlane(u.w[i], lane);
+    return u.v;
+}
+
 // Few long rows: a block of sixteen waves to a tile, the 64 tiles before it looked at by a wave, a lane each.
 template <class T, bool GRAD>
 __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kernel(ReArgs p, ReChain chain) {
@@ -648,8 +672,9 @@ __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kern
                 __builtin_amdgcn_s_sleep(1);
             }
             // (a tile whose state came first and sum was never asked for: only the nearest such is used, as a state)
-            state = __shfl(found_state, near);
-            for (int l = near - 1; l >= 0; --l) state = re_join(__shfl(found_product, l), __shfl(found, l), state);
+            near = __builtin_amdgcn_readfirstlane(near);
+            state = re_lane(found_state, near);
+            for (int l = near - 1; l >= 0; --l) state = re_join(re_lane(found_product, l), re_lane(found, l), state);
         }
         if (lane == 0) {
             start = state;
@@ -670,7 +695,7 @@ __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kern
 // ---- launches -------------------------------------------------------------------------
 constexpr uint64_t kReWaves = 4096;   // sixteen to a compute unit
 // time is cut where there are fewer rows or strips of columns than these, and more than so many tiles of them
-constexpr uint64_t kReFewRows = 256, kReFewStrips = 128, kReFewTiles = 4;
+constexpr uint64_t kReFewRows = 256, kReFewStrips = 256, kReFewTiles = 2;
 constexpr uint64_t kReMostTiles = 1u << 22;   // (2^30 blocks)
 
 template <class T, bool GRAD, int NW>

@@ -480,13 +480,15 @@ void dq_launch(const cumo_hip_dequantize_t& d, hipStream_t stream) {
     else dq_launch_one<T, 256>(d, stream);
 }
 
-// blocks that take the rows of a gradient: two to a compute unit hold enough loads on the way, and keep the parts few
-constexpr uint64_t kRnGradBlocks = 512;
+// Blocks that take the rows of a gradient, as many as the compute units hold at once of 256 lanes (three) and of 512 (one): more of
+// them leave more parts and take turns. us at 256, 512, 768, 1024, 2048 blocks: SFloat [8192,4096] 150, 101, 99.8, 115, 120; DFloat
+// [131072,257] 479, 304, 242, 323, 275; SFloat [131072,64] 50, 36, 34, 35, 46; [1024,8192], 512 lanes, 42, 50, 54, 65, 65.
+template <int BLOCK> constexpr uint64_t kRnGradBlocks = BLOCK > 256 ? 256 : 768;
 
 template <class T, int TPR, int NV, int BLOCK>
 bool rn_grad_one(RnGradParams p, hipStream_t stream) {
     constexpr int RPB = BLOCK / TPR;
-    const unsigned blocks = rn_grid((p.rows + RPB - 1) / RPB, p.gweight ? kRnGradBlocks : 256u * 64u);
+    const unsigned blocks = rn_grid((p.rows + RPB - 1) / RPB, p.gweight ? kRnGradBlocks<BLOCK> : 256u * 64u);
     const bool nt = stream_past_caches(p.rows * p.n * sizeof(T) * (p.gsum ? 4 : 3));
     p.through = rn_through<T>(p.gx, p.rows, p.n, p.gx_step, nt);
     char* parts = nullptr;
