@@ -109,10 +109,10 @@ struct ReLanes {
     }
 };
 
-// Forms of a pass over arrays larger than the caches, us (with a sum of the result behind it) for SFloat [8,4096,2048] forwards,
-// backwards, and [1,65536,1000], in tiles:
-//   loads plain / nt, stores nt              161 (201) / 156 (197),  216 / 236,  184 (224) / 190 (231)
-//   loads nt, stores plain / written through 145 (182) / 140 (178),  272 / 244,  190 (220) / 195 (224)
+// Forms of a pass over arrays larger than the caches, us. SFloat [8,4096,2048] forwards (with a sum of the result behind it) and
+// [1,65536,1000] in tiles; gradients of [8,2048,2048]:
+//   loads plain / nt, stores nt              161 (201) / 156 (197),  184 (224) / 190 (231),  139 / 133
+//   loads nt, stores plain / written through 145 (182) / 140 (178),  190 (220) / 195 (224),  - / 143
 enum ReStore { RE_PLAIN, RE_AWAY, RE_THROUGH };
 
 // what a wave holds of a, b and h: R rows of 64 columns
@@ -219,13 +219,13 @@ __global__ __launch_bounds__(NW * 64) void recurrence_columns_kernel(ReArgs p) {
     // two tiles in turn: one is on its way while the other's steps are taken. Every wave of the block goes round equally often.
     Tile one, two;
     uint64_t t = (uint64_t)wave * R, at = 0;
-    one.template load<ONCE && !GRAD>(p, la, lb, lh, t, first);
+    one.template load<ONCE>(p, la, lb, lh, t, first);
     for (;;) {
-        two.template load<ONCE && !GRAD>(p, la, lb, lh, t + kTile, first);
+        two.template load<ONCE>(p, la, lb, lh, t + kTile, first);
         walk(one, t);
         t += kTile;
         if ((at += kTile) >= p.time) break;
-        one.template load<ONCE && !GRAD>(p, la, lb, lh, t + kTile, first);
+        one.template load<ONCE>(p, la, lb, lh, t + kTile, first);
         walk(two, t);
         t += kTile;
         if ((at += kTile) >= p.time) break;
