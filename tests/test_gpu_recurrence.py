@@ -304,3 +304,51 @@ def test_into_given_arrays(shape, axis):
     d = [v._desc() for v in (g, x, h)]
     _lib.call(_lib.lib.cumo_hip_na_recurrence_grad, C.byref(d[0]), C.byref(d[1]), C.byref(d[2]), None, axis, C.byref(d[1]), C.byref(d[0]), None)
     assert (x.to_numpy() == grads[0]).all() and (g.to_numpy() == grads[1]).all()
+
+
+def test_columns_further_apart_than_32_bits_reach():
+    """Every 2^19th element of rows of 2^25: 40 columns 128 MiB apart, 5 GiB in all, time in steps of 2 MiB."""
+    import cumo_amd as m
+    rng = np.random.default_rng(8)
+    a, b = make(rng, (64, 40), np.float32)
+    wide = [m.SFloat(40, 1 << 25) for _ in range(2)]
+    views = [w.transpose()[::1 << 19] for w in wide]
+    for view, h in zip(views, (a, b)):
+        view.store(m.SFloat.cast(h))
+    check(m, a, b, rng.standard_normal(40).astype(np.float32), 0, np.float32, views)
+
+
+GIVING_UP = """
+import ctypes as C
+import cumo_amd as m
+from cumo_amd import _lib
+L = _lib.lib
+L.cumo_hip_wait_give_ups.restype = C.c_int
+L.cumo_hip_wait_give_ups.argtypes = [C.POINTER(C.c_uint32 * 4)]
+for shape, axis in (((1, 60000, 64), 1), ((1, 1 << 22), 1)):
+    a, b = m.SFloat(*shape).fill(0.5), m.SFloat(*shape).fill(1.0)
+    m.synchronize()
+    said = None
+    try:
+        for _ in range(5):
+            h = m.Fused.recurrence(a, b, axis=axis)
+            g = m.Fused.recurrence_grad(b, a, b, axis=axis)
+        m.synchronize()
+    except m.RuntimeError as e:
+        said = str(e)
+    counts = (C.c_uint32 * 4)()
+    assert L.cumo_hip_wait_give_ups(C.byref(counts)) == 0
+    assert said and "gave up" in said and counts[1] > 0, (shape, said, list(counts))
+print("reported")
+"""
+
+
+def test_waits_that_give_up_are_reported():
+    """With no looks allowed (the knob of tests/test_gpu_wait_give_up.py) tiles do not wait for those before them; every
+    kernel ends, and the next wait for the device says so."""
+    import os
+    import subprocess
+    import sys
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), CUMO_HIP_WAIT_LIMIT="0")
+    p = subprocess.run([sys.executable, "-c", GIVING_UP], env=env, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=100)
+    assert p.returncode == 0 and "reported" in p.stdout, p.stdout[-2000:]
