@@ -639,8 +639,7 @@ int cumo_hip_fused_rows_kernel_launch(int type, int mode, const cumo_hip_fused_r
  * type 0 SFloat, 1 DFloat. residual == NULL: s is x, and sum is not written. weight == NULL:
  * ones. quantised: y is 8-bit integers, round(y / scale) between -127 and 127, and
  * scale[k] = max|y| / 127 of row k (0 for a row of zeros, whose y are 0; a row with a NaN
- * has the scale NaN and y of 0). y and sum may be x or residual, element on element, but
- * overlap them in no other way. */
+ * has the scale NaN and y of 0). No result may overlap an operand. */
 typedef struct {
     uint64_t rows, n;
     ssize_t  x_step, residual_step, y_step, sum_step;
@@ -666,8 +665,9 @@ void cumo_hip_dequantize_kernel_launch(int type, const cumo_hip_dequantize_t* d)
  * y) and gsum (of s, by way of the residual stream; NULL: none):
  *   gx = r * (g * weight - s * r^2 * sum(g * weight * s) / n) + gsum
  *   gweight = the sum over rows of g * s * r   (NULL: not wanted; n contiguous elements)
- * gx is the gradient of x and of residual alike; it may be g or gsum, element on element.
- * Partial sums live in a block from the pool. CUMO_HIP_OK or the error reported. */
+ * gx is the gradient of x and of residual alike. No result may overlap an operand. Partial
+ * sums live in a block from the pool (kept where the stream is being captured). CUMO_HIP_OK or
+ * the error reported. */
 typedef struct {
     uint64_t rows, n;
     ssize_t  g_step, s_step, gsum_step, gx_step;
