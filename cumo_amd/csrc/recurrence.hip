@@ -303,8 +303,8 @@ struct ReSlot {
     }
 };
 
-__global__ __launch_bounds__(256) void recurrence_clear_kernel(uint64_t* words, uint64_t n) {
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) words[i] = 0;
+__global__ __launch_bounds__(256) void recurrence_clear_kernel(ulonglong2* pairs, uint64_t n) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) pairs[i] = make_ulonglong2(0, 0);
 }
 
 // Down columns: a block of sixteen waves to a tile, and as many tiles before it looked at, a wave each.
@@ -715,13 +715,13 @@ int re_chain(const ReArgs& p, uint64_t lines, uint64_t tile, hipStream_t stream)
         return CUMO_HIP_ERROR_RUNTIME;
     }
     chain.tiles = (uint32_t)((p.time + tile - 1) / tile);
-    const uint64_t words = lines * chain.tiles * kReWords<T> * (ROWS ? 1 : 64) + 1;
+    const uint64_t words = lines * chain.tiles * kReWords<T> * (ROWS ? 1 : 64) + 2;   // (an even number, the ticket among the last two)
     char* memory = cumo_cuda_runtime_malloc(words * sizeof(uint64_t));
     if (!memory) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
     chain.words = reinterpret_cast<uint64_t*>(memory);
     chain.ticket = reinterpret_cast<uint32_t*>(chain.words + words - 1);
-    const uint64_t blocks = (words + 1023) / 1024;
-    hipLaunchKernelGGL(recurrence_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, stream, chain.words, words);
+    const uint64_t blocks = (words / 2 + 255) / 256;
+    hipLaunchKernelGGL(recurrence_clear_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, reinterpret_cast<ulonglong2*>(memory), words / 2);
     const dim3 grid((unsigned)(lines * chain.tiles)), block(kReChainWaves * 64);
     if constexpr (ROWS) hipLaunchKernelGGL((recurrence_rows_chain_kernel<T, GRAD>), grid, block, 0, stream, p, chain);
     else hipLaunchKernelGGL((recurrence_columns_chain_kernel<T, GRAD>), grid, block, 0, stream, p, chain);

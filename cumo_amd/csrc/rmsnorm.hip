@@ -397,26 +397,27 @@ __global__ __launch_bounds__(256) void rmsnorm_grad_columns_kernel(RnGradParams 
     p.parts[blockIdx.y * p.n + i] = sum;
 }
 
-// [parts][n] down its columns: 64 columns a block, sixteen waves taking every sixteenth part
+// [parts][n] down its columns: 16 columns a block, every lane of the 64 to a column taking every 64th part (64 columns a block
+// and sixteen lanes to a column took 7.5 us for 768 parts of 4096, and as long for 257)
 template <class T>
 __global__ __launch_bounds__(1024) void rmsnorm_grad_parts_kernel(const double* parts, uint32_t n_parts, uint64_t n, T* out) {
-    __shared__ double slot[16][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t i = (uint64_t)blockIdx.x * 64 + lane;
+    __shared__ double slot[16][16];
+    const uint32_t column = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const uint64_t i = (uint64_t)blockIdx.x * 16 + column;
     double sum = 0.0;
     if (i < n) {
-        uint32_t k = wave;
-        for (; k + 48 < n_parts; k += 64) {
-            const double a = parts[k * n + i], b = parts[(k + 16) * n + i], c = parts[(k + 32) * n + i], d = parts[(k + 48) * n + i];
-            sum += (a + b) + (c + d);
-        }
-        for (; k < n_parts; k += 16) sum += parts[k * n + i];
+#pragma unroll 4
+        for (uint32_t k = group; k < n_parts; k += 64) sum += parts[k * n + i];
     }
-    slot[wave][lane] = sum;
+    // the wave's four groups, then the waves
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if ((group & 3) == 0) slot[group >> 2][column] = sum;
     __syncthreads();
-    if (wave == 0 && i < n) {
+    if (threadIdx.x < 16 && i < n) {
+        sum = slot[0][column];
 #pragma unroll
-        for (int w = 1; w < 16; ++w) sum += slot[w][lane];
+        for (int w = 1; w < 16; ++w) sum += slot[w][column];
         out[i] = (T)sum;
     }
 }
@@ -445,7 +446,7 @@ void rn_launch(const cumo_hip_rmsnorm_t& d, hipStream_t stream) {
     const bool nt = stream_past_caches(p.rows * p.n * (sizeof(T) * (p.residual ? 3 : 1) + (Q8 ? 1 : sizeof(T))));
     p.y_through = !Q8 && rn_through<T>(p.y, p.rows, p.n, p.y_step, nt);
     p.sum_through = p.sum && rn_through<T>(p.sum, p.rows, p.n, p.sum_step, nt);
-    const uint64_t nv = (p.n + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+    const uint64_t nv = p.n / (16 / sizeof(T));   // (whole vectors: the elements behind them have registers of their own)
     if (nv <= 8) rn_launch_one<T, 8, 1, 256, Q8>(p, nt, stream);
     else if (nv <= 16) rn_launch_one<T, 8, 2, 256, Q8>(p, nt, stream);
     else if (nv <= 32) rn_launch_one<T, 8, 4, 256, Q8>(p, nt, stream);
@@ -498,7 +499,7 @@ bool rn_grad_one(RnGradParams p, hipStream_t stream) {
     if (nt) hipLaunchKernelGGL((rmsnorm_grad_kernel<T, TPR, NV, BLOCK, true>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((rmsnorm_grad_kernel<T, TPR, NV, BLOCK, false>), grid, block, 0, stream, p);
     if (parts) {
-        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, (uint32_t)blocks, p.n,
+        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 15) / 16)), dim3(1024), 0, stream, p.parts, (uint32_t)blocks, p.n,
                            reinterpret_cast<T*>(p.gweight));
         // (the memory of a captured launch stays with its graph)
         if (!stream_under_capture()) cumo_cuda_runtime_free(parts);
@@ -518,7 +519,7 @@ bool rn_grad_long(RnGradParams p, hipStream_t stream) {
     if (memory) {
         p.parts = rs + p.rows;
         hipLaunchKernelGGL((rmsnorm_grad_columns_kernel<T>), dim3((unsigned)((p.n + 255) / 256), (unsigned)runs), dim3(256), 0, stream, p, rs, per);
-        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, (uint32_t)runs, p.n,
+        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 15) / 16)), dim3(1024), 0, stream, p.parts, (uint32_t)runs, p.n,
                            reinterpret_cast<T*>(p.gweight));
         if (!stream_under_capture()) cumo_cuda_runtime_free(memory);
     }
@@ -531,11 +532,11 @@ int rn_grad(const cumo_hip_rmsnorm_grad_t& d, hipStream_t stream) {
     static_cast<cumo_hip_rmsnorm_grad_t&>(p) = d;
     p.parts = nullptr;
     p.through = false;
-    const uint64_t nv = (p.n + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+    const uint64_t nv = p.n / (16 / sizeof(T));   // (whole vectors: the elements behind them have registers of their own)
     bool ok = true;
     if (p.rows == 0) {
         if (p.gweight)
-            hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 63) / 64)), dim3(1024), 0, stream, nullptr, 0u, p.n, reinterpret_cast<T*>(p.gweight));
+            hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 15) / 16)), dim3(1024), 0, stream, nullptr, 0u, p.n, reinterpret_cast<T*>(p.gweight));
     }
     else if (nv <= 8) ok = rn_grad_one<T, 8, 1, 256>(p, stream);
     else if (nv <= 16) ok = rn_grad_one<T, 8, 2, 256>(p, stream);
