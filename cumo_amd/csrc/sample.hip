@@ -8,10 +8,14 @@
 // Weights are whole numbers, exp((x - max) / temperature) in units of 2^-S with S such that the sum of a row fits 62 bits:
 // sums do not depend on their order, and neither does the answer, although bins are added to by atomics.
 //
-// Three launches: the largest, the smallest and the first position of the largest of each row's parts; the bins of each row's parts, a
-// block to a part with its bins in shared memory; then a block to a row, which adds the parts' bins up, takes their running sums
-// and reads the row once more for its list. The rows come from memory once and from the last-level cache the other times; what
-// else bounds this is the weights' arithmetic in double (some twenty operations an element) and, for a few rows, the launches.
+// Three launches. The largest and the smallest number of each row's parts, and the largest of every chunk of 64 vectors; the bins of
+// each row's parts, a block to a part with its bins in shared memory; then a block to a row, which adds the parts' bins up, takes
+// their running sums and reads the chunks that reach the list's bins once more. The rows come from memory once and from the
+// last-level cache the other times. What bounds it for many rows is the weights' arithmetic in double (some twenty operations an
+// element) and the order of steps within a row, for a few rows the launches and those steps. SFloat, temperature 0.8, top_k 50,
+// top_p 0.95: one row of 131072 in 25 us (4.1, 5.6 and 16.4 in the three), 256 rows of 50001 in 41 us with one setting for all, and
+// in 65 us (13, 27 and 26; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
+// chunks' maxima the last launch reads whole rows: 20.4 and 27.8 us of it, where the first one takes 4.0 and 11.2.
 #include "common.h"
 #include "ew_ops.h"
 
@@ -107,14 +111,15 @@ struct SaWeight {
 
 struct SaPart {
     double max, least;   // of what is finite the smallest
-    uint32_t first;      // position of the first of the largest
-    uint32_t nan;
+    uint64_t nan;
 };
 
 struct SaParams : cumo_hip_sample_t {
     int unit_bits;
     uint32_t looks, fills;   // parts of a row in the first two launches (64 and 16 at most)
+    uint32_t chunks;         // of a row: what a wave reads at once
     SaPart* parts;           // [rows][looks]
+    char* chunk_max;         // [rows][chunks]
     uint64_t* masses;        // [rows][fills][bins]
     uint64_t* likely;        // [rows][fills]: the weights that min_p leaves of a part, where other limits come before it
     uint32_t* counts;        // the same, where a row may have a top_k
@@ -147,68 +152,109 @@ __device__ __forceinline__ void sa_each(const T* row, uint32_t from, uint32_t to
     f(threadIdx.x < n % V ? part[whole * V + threadIdx.x] : (T)-INFINITY, from + whole * V + threadIdx.x);
 }
 
-// a part's first and last element, whole vectors of it but for the row's end
+// a part's first and last element, whole chunks of it but for the row's end
+template <class T> constexpr uint32_t kSaChunk = 64 * 16 / sizeof(T);
 __device__ __forceinline__ void sa_part(uint32_t n, uint32_t parts, uint32_t part, uint32_t& from, uint32_t& to) {
-    const uint32_t per = ((n + parts - 1) / parts + 3) & ~3u;
+    const uint32_t per = ((n + parts - 1) / parts + 255) & ~255u;
     from = part * per < n ? part * per : n;
     to = n - from < per ? n : from + per;
 }
 
+// (a NaN is lost here; rows that hold one are told apart)
+__device__ __forceinline__ float sa_max(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double sa_max(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ float sa_min(float a, float b) { return __builtin_fminf(a, b); }
+__device__ __forceinline__ double sa_min(double a, double b) { return __builtin_fmin(a, b); }
+
+// the largest of a wave's values, in lane 63: shifts within 16 lanes, then the last lanes of those handed on
+template <class T, int CTRL, int ROWS>
+__device__ __forceinline__ T sa_larger_from(T v) {
+    union { T t; int w[sizeof(T) / 4]; } u, o;
+    u.t = v;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) o.w[i] = __builtin_amdgcn_update_dpp(u.w[i], u.w[i], CTRL, ROWS, 0xf, false);
+    return sa_max(o.t, v);
+}
 template <class T>
-__device__ __forceinline__ void sa_larger(T& m, uint32_t& first, T other, uint32_t other_first) {
-    const bool take = other > m || (other == m && other_first < first);
-    first = take ? other_first : first;
-    m = take ? other : m;
+__device__ __forceinline__ T sa_largest(T v) {
+    v = sa_larger_from<T, 0x111, 0xf>(v);
+    v = sa_larger_from<T, 0x112, 0xf>(v);
+    v = sa_larger_from<T, 0x114, 0xf>(v);
+    v = sa_larger_from<T, 0x118, 0xf>(v);
+    v = sa_larger_from<T, 0x142, 0xa>(v);
+    return sa_larger_from<T, 0x143, 0xc>(v);
 }
 
 constexpr int kSaLook = 256;
 template <class T>
 __global__ __launch_bounds__(kSaLook) void sample_look_kernel(SaParams p) {
+    constexpr int V = 16 / (int)sizeof(T), U = 4;
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    union Vec { u4 q; T t[V]; __device__ Vec() {} };
     __shared__ T wave_max[kSaLook / 64], wave_least[kSaLook / 64];
-    __shared__ uint32_t wave_first[kSaLook / 64], wave_nan[kSaLook / 64];
+    __shared__ uint32_t wave_nan[kSaLook / 64];
     uint32_t from, to;
     sa_part((uint32_t)p.n, p.looks, blockIdx.y, from, to);
     T m = -INFINITY, least = INFINITY;
-    uint32_t first = 0xffffffffu;
     bool nan = false;
-    if (from < to) {
-        sa_each<T, kSaLook, 4>(reinterpret_cast<const T*>(p.x + (int64_t)blockIdx.x * p.x_step), from, to, [&](T v, uint32_t i) {
-            nan |= v != v;
-            first = v > m ? i : first;   // (a lane's positions rise)
-            m = v > m ? v : m;
-            least = v < least && v > (T)-INFINITY ? v : least;
-        });
+    auto look = [&](T v) {
+        nan |= v != v;
+        m = sa_max(m, v);
+        least = sa_min(least, v > (T)-INFINITY ? v : (T)INFINITY);
+    };
+    const T* part = reinterpret_cast<const T*>(p.x + (int64_t)blockIdx.x * p.x_step) + from;
+    T* chunk_max = reinterpret_cast<T*>(p.chunk_max) + (uint64_t)blockIdx.x * p.chunks + from / kSaChunk<T>;
+    const uint32_t whole = (to - from) / V, tail = (to - from) % V;
+#pragma unroll 1
+    for (uint32_t begin = 0; begin < whole; begin += kSaLook * U) {
+        Vec x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t at = begin + (uint32_t)u * kSaLook + threadIdx.x;
+            x[u].q = reinterpret_cast<const u4*>(part)[at < whole ? at : 0];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t at = begin + (uint32_t)u * kSaLook + threadIdx.x;
+            T most = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const T v = at < whole ? x[u].t[j] : (T)-INFINITY;
+                look(v);
+                most = sa_max(most, v);
+            }
+            most = sa_largest(most);
+            if ((threadIdx.x & 63) == 63 && at - 63 < whole) chunk_max[at / 64] = most;
+        }
     }
+    if (threadIdx.x < tail) look(part[whole * V + threadIdx.x]);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
-        sa_larger(m, first, __shfl_xor(m, d), __shfl_xor(first, d));
-        const T l = __shfl_xor(least, d);
-        least = l < least ? l : least;
+        m = sa_max(m, __shfl_xor(m, d));
+        least = sa_min(least, __shfl_xor(least, d));
     }
     const bool wave_has_nan = __ballot(nan) != 0;
     const uint32_t wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) {
         wave_max[wave] = m;
         wave_least[wave] = least;
-        wave_first[wave] = first;
         wave_nan[wave] = wave_has_nan;
     }
     __syncthreads();
     if (threadIdx.x != 0) return;
     nan = wave_has_nan;
     for (int w = 1; w < kSaLook / 64; ++w) {
-        sa_larger(m, first, wave_max[w], wave_first[w]);
-        least = wave_least[w] < least ? wave_least[w] : least;
+        m = sa_max(m, wave_max[w]);
+        least = sa_min(least, wave_least[w]);
         nan |= wave_nan[w] != 0;
     }
-    p.parts[(uint64_t)blockIdx.x * p.looks + blockIdx.y] = {(double)m, (double)least, first, nan ? 1u : 0u};
+    p.parts[(uint64_t)blockIdx.x * p.looks + blockIdx.y] = {(double)m, (double)least, nan ? 1u : 0u};
 }
 
 // a row's settings, the same for every lane
 template <class T>
 struct SaSettings {
     SaWeight<T> weight;
-    uint32_t first;            // of the largest
     bool none, greedy;         // nothing to choose; the first of the largest
     bool all, cut_p, cut_m, small;   // no top_k; top_p, min_p cut; a top_k small enough for a list
     uint64_t top_k;
@@ -220,17 +266,13 @@ struct SaSettings {
             min_p_at(p.min_p, row, p.parts);
         float_tables_prepare();
         T m = (T)part.max, least = (T)part.least;
-        first = part.first;
-        const uint32_t nan = part.nan;
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) {
-            sa_larger(m, first, __shfl_xor(m, d), __shfl_xor(first, d));
-            const T l = __shfl_xor(least, d);
-            least = l < least ? l : least;
+            m = sa_max(m, __shfl_xor(m, d));
+            least = sa_min(least, __shfl_xor(least, d));
         }
         m = sa_same(m);
-        first = sa_same(first);
-        none = __ballot(nan != 0) != 0 || m == (T)-INFINITY;
+        none = __ballot(part.nan != 0) != 0 || m == (T)-INFINITY;
         const double temperature = temperature_at.value(p.temperature), k = k_at.value(p.top_k), min_p = min_p_at.value(p.min_p);
         u = u_at.value(p.u);
         top_p = top_p_at.value(p.top_p);
@@ -339,8 +381,29 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
     const T* x = reinterpret_cast<const T*>(p.x + (int64_t)row * p.x_step);
     const SaSettings<T> s(p, row);
     const SaWeight<T>& weight = s.weight;
-    if (s.none || s.greedy) {
-        if (tid == 0) p.out[row] = s.none ? -1 : (int32_t)s.first;
+    if (s.none) {
+        if (tid == 0) p.out[row] = -1;
+        return;
+    }
+    const T* chunk_max = reinterpret_cast<const T*>(p.chunk_max) + row * p.chunks;
+    constexpr int V = 16 / (int)sizeof(T);
+    const uint32_t whole = n / V;   // vectors; 64 of them are a chunk
+    if (s.greedy) {
+        // the first of the largest: the first chunk that has it, or one of the elements behind the chunks
+        if (tid == 0) list_size = p.chunks;
+        __syncthreads();
+        uint32_t chunk = p.chunks;
+        for (uint32_t c = tid; c < p.chunks && chunk == p.chunks; c += kSaBlock) chunk = chunk_max[c] == weight.max ? c : chunk;
+        if (chunk < p.chunks) atomicMin(&list_size, chunk);
+        __syncthreads();
+        if (wave != 0) return;
+        chunk = sa_same(list_size);
+        const uint32_t at = chunk < p.chunks ? (chunk * 64 + lane) * V : whole * V + lane;
+        const uint32_t here = chunk < p.chunks ? (chunk * 64 + lane < whole ? V : 0) : (lane < n % V ? 1 : 0);
+        uint32_t found_at = 0xffffffffu;
+        for (int j = V - 1; j >= 0; --j) found_at = (uint32_t)j < here && x[at + j] == weight.max ? at + j : found_at;
+        const uint64_t hits = __ballot(found_at != 0xffffffffu);
+        if (hits && lane == (uint32_t)__builtin_ctzll(hits)) p.out[row] = (int32_t)found_at;
         return;
     }
     const double u = s.u;
@@ -392,7 +455,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         const double above = from == 0 ? -INFINITY : ((double)from - 0.5) / (double)weight.bins_per;
         const double lowest = (double)weight.max - ((double)to + 1.5) / (double)weight.bins_per;
         const T most = (T)((double)weight.max - above), least = to < kSaBins - 1 && lowest == lowest ? (T)lowest : (T)-INFINITY;
-        sa_each<T, kSaBlock, 4>(x, 0, n, [&](T v, uint32_t i) {
+        auto enter = [&](T v, uint32_t i) {
             if (__ballot(v >= least && v <= most)) {
                 const uint32_t b = weight.bin(v);
                 const bool hit = b >= from && b <= to && v > (T)-INFINITY;
@@ -405,7 +468,33 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
                     list_index[at] = i;
                 }
             }
-        });
+        };
+        // Chunks whose largest number reaches the bins, four at a time; each wave has every sixteenth.
+        constexpr int G = 4;
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        union Vec { u4 q; T t[V]; __device__ Vec() {} };
+#pragma unroll 1
+        for (uint32_t first = wave; first < p.chunks; first += 64 * kWaves) {
+            const uint32_t mine = first + lane * kWaves;
+            uint64_t want = __ballot(mine < p.chunks && chunk_max[mine < p.chunks ? mine : 0] >= least);
+#pragma unroll 1
+            while (want) {
+                Vec held[G];
+                uint32_t at[G];
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    at[g] = want ? (first + (uint32_t)__builtin_ctzll(want) * kWaves) * 64 + lane : whole;
+                    want &= want - 1;
+                    held[g].q = reinterpret_cast<const u4*>(x)[at[g] < whole ? at[g] : 0];
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) enter(at[g] < whole ? held[g].t[j] : (T)-INFINITY, at[g] * V + j);
+                }
+            }
+        }
+        enter(tid < n % V ? x[whole * V + tid] : (T)-INFINITY, whole * V + tid);
         __syncthreads();
         const uint32_t size = sa_same(list_size);
         lo = 1;
@@ -642,14 +731,16 @@ int sa_launch(const cumo_hip_sample_t& d, hipStream_t stream) {
     };
     p.looks = parts(2048, 2048, 64);
     p.fills = parts(512, 4096, 16);
+    p.chunks = (uint32_t)((d.n / (16 / sizeof(T)) + 63) / 64);
     const bool may_count = d.top_k.each || (d.top_k.value > 0.0 && d.top_k.value < (double)d.n);
     const uint64_t part_bytes = (rows * p.looks * sizeof(SaPart) + 15) & ~15ull, bins = rows * p.fills * kSaBins;
-    char* memory = cumo_cuda_runtime_malloc(part_bytes + (bins + rows * p.fills) * 8 + (may_count ? bins * 4 : 0));
+    char* memory = cumo_cuda_runtime_malloc(part_bytes + (bins + rows * p.fills) * 8 + rows * p.chunks * sizeof(T) + (may_count ? bins * 4 : 0));
     if (!memory) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
     p.parts = reinterpret_cast<SaPart*>(memory);
     p.masses = reinterpret_cast<uint64_t*>(memory + part_bytes);
     p.likely = p.masses + bins;
     p.counts = may_count ? reinterpret_cast<uint32_t*>(p.likely + rows * p.fills) : nullptr;
+    p.chunk_max = reinterpret_cast<char*>(p.likely + rows * p.fills) + (may_count ? bins * 4 : 0);
     cumo_hip_row_number_t* const settings[5] = {&p.u, &p.temperature, &p.top_k, &p.top_p, &p.min_p};
     for (uint64_t done = 0; done < d.rows; done += rows) {
         const unsigned now = (unsigned)(d.rows - done < rows ? d.rows - done : rows);
