@@ -13,8 +13,8 @@
 // their running sums and reads the chunks that reach the list's bins once more. The rows come from memory once and from the
 // last-level cache the other times. What bounds it for many rows is the weights' arithmetic in double (some twenty operations an
 // element) and the order of steps within a row, for a few rows the launches and those steps. SFloat, temperature 0.8, top_k 50,
-// top_p 0.95: one row of 131072 in 25 us (4.1, 5.6 and 16.4 in the three), 256 rows of 50001 in 41 us with one setting for all, and
-// in 65 us (13, 27 and 26; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
+// top_p 0.95: one row of 131072 in 25 us (4.1, 5.5 and 16.6 in the three), 256 rows of 50001 in 41 us with one setting for all, and
+// in 64 us (13, 27 and 25.5; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
 // chunks' maxima the last launch reads whole rows: 20.4 and 27.8 us of it, where the first one takes 4.0 and 11.2.
 #include "common.h"
 #include "ew_ops.h"
@@ -449,6 +449,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         __syncthreads();
         if (tid == 0) list_size = 0;
         list_key[tid] = 0;   // (below every number's key)
+        list_sum[tid] = 0;
         __syncthreads();
         // What may be in those bins, half a bin more on either side: two comparisons for each number that is not. (The bins' rounding
         // moves a number by less than a thousandth of a bin, and the bounds' keeps the order.)
@@ -500,22 +501,27 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         lo = 1;
         hi = 0;
         if (size > kSaList) return false;
-        // an element's place is the number of those before it
-        if (wave * 64 < size) {
-            const U key = list_key[tid];
-            const uint32_t index = list_index[tid];
+        // An element's place is the number of those before it, counted in as many parts as the block has lanes for.
+        const uint32_t lanes = size <= kSaBlock / 4 ? kSaBlock / 4 : size <= kSaBlock / 2 ? kSaBlock / 2 : kSaBlock, groups = kSaBlock / lanes;
+        const uint32_t group = tid / lanes, mine = tid & (lanes - 1), per = ((size + groups - 1) / groups + KV - 1) & ~(uint32_t)(KV - 1);
+        if ((mine & ~63u) < size) {
+            const U key = list_key[mine];
+            const uint32_t index = list_index[mine], end = size < (group + 1) * per ? size : (group + 1) * per;
             uint32_t place = 0;
 #pragma unroll 2
-            for (uint32_t i = 0; i < size; i += KV) {   // (behind the list's end are keys of 0, which no number has)
+            for (uint32_t i = group * per; i < end; i += KV) {   // (behind the list's end are keys of 0, which no number has)
                 const UV other = *reinterpret_cast<const UV*>(&list_key[i]);
                 const IV other_index = *reinterpret_cast<const IV*>(&list_index[i]);
 #pragma unroll
                 for (int j = 0; j < KV; ++j) place += (other[j] > key) | ((other[j] == key) & (other_index[j] < index)) ? 1 : 0;
             }
-            if (tid < size) {
-                sorted_key[place] = key;
-                sorted_index[place] = index;
-            }
+            atomicAdd(reinterpret_cast<uint32_t*>(&list_sum[mine]), place);
+        }
+        __syncthreads();
+        if (tid < size) {
+            const uint32_t place = (uint32_t)list_sum[tid];
+            sorted_key[place] = list_key[tid];
+            sorted_index[place] = list_index[tid];
         }
         __syncthreads();
         const uint64_t sum = sa_scan(tid < size ? weight.units(weight.share(Key::value(sorted_key[tid]))) : 0, slots);
