@@ -13,13 +13,14 @@
 // their running sums and reads the chunks that reach the list's bins once more. The rows come from memory once and from the
 // last-level cache the other times. What bounds it for many rows is the weights' arithmetic in double (some twenty operations an
 // element) and the order of steps within a row, for a few rows the launches and those steps. SFloat, temperature 0.8, top_k 50,
-// top_p 0.95: one row of 131072 in 25 us (4.1, 5.5 and 16.6 in the three), 256 rows of 50001 in 41 us with one setting for all, and
-// in 64 us (13, 27 and 25.5; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
+// top_p 0.95: one row of 131072 in 25 us (4, 5.5 and 16.6 in the three), 256 rows of 50001 in 41 us with one setting for all, and
+// in 63 us (13, 26.5 and 25; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
 // chunks' maxima the last launch reads whole rows: 20.4 and 27.8 us of it, where the first one takes 4.0 and 11.2.
 #include "common.h"
 #include "ew_ops.h"
 
 #include <cstring>
+#include <type_traits>
 
 namespace cumo_hip {
 namespace {
@@ -443,35 +444,10 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         __syncthreads();
     }
 
-    // the list: of the elements in bins [lo, hi], in order, with their running sum of weights; false where they are too many
-    uint32_t lo = 1, hi = 0;
-    auto make_list = [&](uint32_t from, uint32_t to) {
-        __syncthreads();
-        if (tid == 0) list_size = 0;
-        list_key[tid] = 0;   // (below every number's key)
-        list_sum[tid] = 0;
-        __syncthreads();
-        // What may be in those bins, half a bin more on either side: two comparisons for each number that is not. (The bins' rounding
-        // moves a number by less than a thousandth of a bin, and the bounds' keeps the order.)
-        const double above = from == 0 ? -INFINITY : ((double)from - 0.5) / (double)weight.bins_per;
-        const double lowest = (double)weight.max - ((double)to + 1.5) / (double)weight.bins_per;
-        const T most = (T)((double)weight.max - above), least = to < kSaBins - 1 && lowest == lowest ? (T)lowest : (T)-INFINITY;
-        auto enter = [&](T v, uint32_t i) {
-            if (__ballot(v >= least && v <= most)) {
-                const uint32_t b = weight.bin(v);
-                const bool hit = b >= from && b <= to && v > (T)-INFINITY;
-                const uint64_t hits = __ballot(hit);
-                uint32_t at = 0;
-                if (lane == 0) at = atomicAdd(&list_size, (uint32_t)__popcll(hits));
-                at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(hits & ((1ull << lane) - 1));
-                if (hit && at < kSaList) {
-                    list_key[at] = Key::of(v);
-                    list_index[at] = i;
-                }
-            }
-        };
-        // Chunks whose largest number reaches the bins, four at a time; each wave has every sixteenth.
-        constexpr int G = 4;
+    // f of the elements that are `least` or more, and of others: of the chunks whose largest number is. Chunks four at a time; each
+    // wave has every sixteenth, and all of its lanes call f (those without an element with -inf).
+    auto gather = [&](auto held_at_once, T least, auto f) {
+        constexpr int G = decltype(held_at_once)::value;
         typedef uint32_t u4 __attribute__((ext_vector_type(4)));
         union Vec { u4 q; T t[V]; __device__ Vec() {} };
 #pragma unroll 1
@@ -491,11 +467,47 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) enter(at[g] < whole ? held[g].t[j] : (T)-INFINITY, at[g] * V + j);
+                    for (int j = 0; j < V; ++j) f(at[g] < whole ? held[g].t[j] : (T)-INFINITY, at[g] * V + j);
                 }
             }
         }
-        enter(tid < n % V ? x[whole * V + tid] : (T)-INFINITY, whole * V + tid);
+        f(tid < n % V ? x[whole * V + tid] : (T)-INFINITY, whole * V + tid);
+    };
+    // What may be in bins [from, to], half a bin more on either side. (The bins' rounding moves a number by less than a thousandth
+    // of a bin, and the bounds' keeps the order.)
+    auto most_of = [&](uint32_t from) {
+        const double above = from == 0 ? -INFINITY : ((double)from - 0.5) / (double)weight.bins_per;
+        return (T)((double)weight.max - above);
+    };
+    auto least_of = [&](uint32_t to) {
+        const double lowest = (double)weight.max - ((double)to + 1.5) / (double)weight.bins_per;
+        return to < kSaBins - 1 && lowest == lowest ? (T)lowest : (T)-INFINITY;
+    };
+
+    // the list: of the elements in bins [lo, hi], in order, with their running sum of weights; false where they are too many
+    uint32_t lo = 1, hi = 0;
+    auto make_list = [&](uint32_t from, uint32_t to) {
+        __syncthreads();
+        if (tid == 0) list_size = 0;
+        list_key[tid] = 0;   // (below every number's key)
+        list_sum[tid] = 0;
+        __syncthreads();
+        const T most = most_of(from), least = least_of(to);   // (two comparisons for each number that is not)
+        auto enter = [&](T v, uint32_t i) {
+            if (__ballot(v >= least && v <= most)) {
+                const uint32_t b = weight.bin(v);
+                const bool hit = b >= from && b <= to && v > (T)-INFINITY;
+                const uint64_t hits = __ballot(hit);
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(&list_size, (uint32_t)__popcll(hits));
+                at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(hits & ((1ull << lane) - 1));
+                if (hit && at < kSaList) {
+                    list_key[at] = Key::of(v);
+                    list_index[at] = i;
+                }
+            }
+        };
+        gather(std::integral_constant<int, 4>(), least, enter);
         __syncthreads();
         const uint32_t size = sa_same(list_size);
         lo = 1;
@@ -560,6 +572,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         sa_each<T, kSaBlock, 4>(x, 0, n, [&](T v, uint32_t) {
             const double share = weight.share(v);
             mine += share >= least ? weight.units(share) : 0;
+            asm("" : "+v"(mine));   // (one after the other)
         });
         const uint64_t run = sa_scan(mine, slots);
         __syncthreads();
@@ -569,49 +582,105 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         __syncthreads();
         return all;
     };
-    // Digit by digit of the keys, over the whole row: for bins that hold more than a list does. Elements of one key have one weight,
-    // so which of them it is follows from a division.
+    // For a bin that holds more than a list does: its smallest and its largest key, then the key in question by eight more bits of what
+    // lies between the two, and again. Elements of one key have one weight, so which of them it is follows from a division. (One row
+    // of 131072 in steps of 1/4, top_p 0.95: 144 us, all of a key's bits by 256s over the whole row 858; 256 rows of 50001 129, 490.)
     U key = 0;
     uint64_t number = 0;   // how many of that key stand before it
-    auto by_digits = [&](bool by_weight, uint64_t t) {
-        U prefix = 0;
+    // the least and the largest key of bin b, or (b: none) of those in [lowest, highest]; weights: those of the bins before b
+    auto narrow = [&](uint32_t b, U& lowest, U& highest, uint64_t& weights) {
+        const bool weigh = b < kSaBins && s.small;
+        const T least = b < kSaBins ? least_of(b) : Key::value(lowest);
+        U low = ~(U)0, high = 0;
+        uint64_t sum_before = 0;
+        gather(std::integral_constant<int, 2>(), least, [&](T v, uint32_t) {
+            if (!(v >= least && v > (T)-INFINITY)) return;
+            const U k = Key::of(v);
+            const uint32_t of = b < kSaBins ? weight.bin(v) : kSaBins;
+            const bool in = b < kSaBins ? of == b : k >= lowest && k <= highest;
+            low = in && k < low ? k : low;
+            high = in && k > high ? k : high;
+            if (weigh && of < b) sum_before += weight.units(weight.share(v));
+            asm("" : "+v"(sum_before));   // (one after the other)
+        });
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            const U l = __shfl_xor(low, d), h = __shfl_xor(high, d);
+            low = l < low ? l : low;
+            high = h > high ? h : high;
+        }
+        __syncthreads();
+        if (lane == 0) {
+            digit_count[wave] = low;
+            digit_mass[wave] = high;
+        }
+        weights = weigh ? sa_scan(sum_before, slots) : 0;
+        if (tid == kSaBlock - 1) found[0] = weights;
+        __syncthreads();
+        low = (U)digit_count[lane & (kWaves - 1)];
+        high = (U)digit_mass[lane & (kWaves - 1)];
+#pragma unroll
+        for (int d = kWaves / 2; d > 0; d >>= 1) {
+            const U l = __shfl_xor(low, d), h = __shfl_xor(high, d);
+            low = l < low ? l : low;
+            high = h > high ? h : high;
+        }
+        low = sa_same(low);
+        high = sa_same(high);
+        if (low <= high) {
+            lowest = low;
+            highest = high;
+        }
+        weights = sa_same(found[0]);
+        __syncthreads();
+    };
+    // b: the bin; none after a top_k that went this way with no weights of bins: its key and all above it
+    auto by_digits = [&](bool by_weight, uint64_t t, uint32_t b) {
+        U lowest = key, highest = Key::of(weight.max);
         uint64_t before = 0, before_weight = 0;
+        if (b < kSaBins) {
+            narrow(b, lowest, highest, before_weight);
+            if (!s.small) before_weight = b ? sa_same(masses[b - 1]) : 0;
+            before = by_weight ? before_weight : b ? sa_same(counts[b - 1]) : 0;
+        }
 #pragma unroll 1
-        for (int shift = (int)sizeof(U) * 8 - 8; shift >= 0; shift -= 8) {
+        while (lowest < highest) {   // (fewer bits each time)
+            const int bits = 64 - __builtin_clzll((uint64_t)(highest - lowest)), shift = bits > 8 ? bits - 8 : 0;
             if (tid < 256) digit_count[tid] = digit_mass[tid] = 0;
-            __syncthreads();
-#pragma unroll 1
-            for (uint32_t i = tid; i < n; i += kSaBlock) {
-                const T v = x[i];
-                const U k = Key::of(v);
-                // (a shift by the whole width would not be one: the first digit compares nothing)
-                if (shift + 8 < (int)sizeof(U) * 8 && (k >> (shift + 8)) != prefix) continue;
-                const uint32_t digit = (uint32_t)(k >> shift) & 255;
-                atomicAdd((unsigned long long*)&digit_count[digit], 1ull);
-                atomicAdd((unsigned long long*)&digit_mass[digit], (unsigned long long)weight.units(weight.share(v)));
-            }
-            __syncthreads();
             if (tid == 0) {
-                uint64_t run = before, run_weight = before_weight;
-                int digit = 255;
-                for (; digit > 0; --digit) {
-                    const uint64_t next = run + (by_weight ? digit_mass[digit] : digit_count[digit]);
-                    if (next > t) break;
-                    run = next;
-                    run_weight += digit_mass[digit];
-                }
-                found[0] = (uint64_t)digit;
-                found[1] = run;
-                found[2] = run_weight;
+                found[0] = 0;
+                found[1] = before;
+                found[2] = before_weight;
             }
             __syncthreads();
-            prefix = (U)((prefix << 8) | (U)sa_same((uint32_t)found[0]));
+            const T least = Key::value(lowest);
+            gather(std::integral_constant<int, 2>(), least, [&](T v, uint32_t) {
+                const U k = Key::of(v);
+                if (!(v >= least && k <= highest)) return;
+                const uint32_t digit = (uint32_t)((k - lowest) >> shift);
+                if (!by_weight) atomicAdd((unsigned long long*)&digit_count[digit], 1ull);
+                atomicAdd((unsigned long long*)&digit_mass[digit], (unsigned long long)weight.units(weight.share(v)));
+            });
+            __syncthreads();
+            const uint64_t mass = tid < 256 ? digit_mass[255 - tid] : 0, count = tid < 256 ? digit_count[255 - tid] : 0;
+            const uint64_t run_mass = sa_scan(mass, slots), run = by_weight ? run_mass : sa_scan(count, slots), one = by_weight ? mass : count;
+            if (before + run > t && before + run - one <= t && one) {
+                found[0] = 255 - tid;
+                found[1] = before + run - one;
+                found[2] = before_weight + run_mass - mass;
+            }
+            __syncthreads();
+            lowest += (U)sa_same(found[0]) << shift;
+            const U span = ((U)1 << shift) - 1;   // (at infinity's key there need not be room for it)
+            highest = highest - lowest < span ? highest : lowest + span;
             before = sa_same(found[1]);
             before_weight = sa_same(found[2]);
             __syncthreads();
+            uint64_t none;
+            if (shift) narrow(kSaBins, lowest, highest, none);
         }
-        const uint64_t one = sa_same(weight.units(weight.share(Key::value(prefix))));
-        key = prefix;
+        const uint64_t one = sa_same(weight.units(weight.share(Key::value(lowest))));
+        key = lowest;
         number = by_weight && one ? (t - before) / one : t - before;
         return before_weight + (number + 1) * one;
     };
@@ -660,8 +729,9 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
             const double want = sa_same(floor((u > 0.0 ? u : 0.0) * (double)sum));
             t = want < (double)sum && (uint64_t)want < sum ? (uint64_t)want : sum - 1;
         }
+        uint32_t b = kSaBins;
         if (!digits && !(small && by_weight)) {
-            const uint32_t b = bin_of(by_weight, t);
+            b = bin_of(by_weight, t);
             if (b >= kSaBins - 1 && !small) continue;   // (a count that reaches what has no weight: everything that has is in front of it)
             if (b < lo || b > hi) {
                 bool few;
@@ -679,7 +749,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         }
         listed = !digits;
         if (digits) {
-            sum = by_digits(by_weight, t);
+            sum = by_digits(by_weight, t, b);
             // (a bin that is too full says nothing of the next one; without the bins' weights all goes by digits)
             digits = s.small;
         } else {
@@ -693,27 +763,35 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         if (tid == 0) p.out[row] = (int32_t)index;
         return;
     }
-    // the element of that key with `number` before it, in order of the index
+    // the element of that key with `number` before it, in order of the index: a part of the row to each wave, then the part that has it
+    uint32_t from = 0, to = n;
     uint64_t left = number;
 #pragma unroll 1
-    for (uint32_t first = 0; first < n; first += kSaBlock) {
-        const uint32_t i = first + tid;
-        const bool hit = i < n && Key::of(x[i]) == key;
-        const uint64_t hits = __ballot(hit);
-        if (lane == 0) slots[wave] = (uint64_t)__popcll(hits);
-        __syncthreads();
-        uint64_t ahead = (uint64_t)__popcll(hits & ((1ull << lane) - 1)), here = 0;
+    while (to - from > 64) {
+        const uint32_t per = ((to - from + kWaves - 1) / kWaves + 63) & ~63u;
+        const uint32_t begin = from + wave * per < to ? from + wave * per : to, end = to - begin < per ? to : begin + per;
+        uint64_t here = 0;
 #pragma unroll 1
-        for (uint32_t w = 0; w < kWaves; ++w) {
-            ahead += w < wave ? slots[w] : 0;
-            here += slots[w];
+        for (uint32_t i = begin; i < end; i += 8 * 64) {
+            T held[8];
+#pragma unroll
+            for (uint32_t g = 0; g < 8; ++g) held[g] = x[i + g * 64 + lane < end ? i + g * 64 + lane : begin];
+#pragma unroll
+            for (uint32_t g = 0; g < 8; ++g) here += (uint64_t)__popcll(__ballot(i + g * 64 + lane < end && Key::of(held[g]) == key));
         }
-        if (hit && ahead == left) p.out[row] = (int32_t)i;
+        if (lane == 0) slots[wave] = here;
         __syncthreads();
-        here = sa_same(here);
-        if (left < here) break;
-        left -= here;
+        uint32_t w = 0;
+        for (; w + 1 < kWaves && left >= slots[w]; ++w) left -= slots[w];
+        __syncthreads();
+        w = sa_same(w);
+        left = sa_same(left);
+        from = from + w * per < to ? from + w * per : to;
+        to = to - from < per ? to : from + per;
     }
+    const bool hit = from + lane < to && Key::of(x[from + lane]) == key;
+    const uint64_t hits = __ballot(hit);
+    if (wave == 0 && hit && (uint64_t)__popcll(hits & ((1ull << lane) - 1)) == left) p.out[row] = (int32_t)(from + lane);
 }
 
 // rows of one round of launches: their bins take 12 to 24 KiB a part

@@ -267,3 +267,27 @@ def test_captured_and_replayed(shape):
         _lib.call(_lib.lib.cumo_hip_na_sample, dx, du, 1.0, None, 0, None, 0.99, None, 0.0, None, o2)
 
     replayed(m, call, results, wants)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n", [6000, 70001])
+def test_more_numbers_together_than_are_put_in_order(dt, n):
+    """A crowd far below its row's largest number: of many different numbers, of few, of two with infinities above."""
+    import cumo_amd as m
+    rng = np.random.default_rng(n)
+    x = np.empty((8, n), dt)
+    x[0] = rng.standard_normal(n) * 1e-3
+    x[1] = 100 + rng.standard_normal(n) * 1e-3
+    x[2] = np.round(rng.standard_normal(n) * 8) / 4096
+    x[3] = np.where(rng.random(n) < 0.5, 0.0, np.finfo(dt).eps)
+    x[4] = rng.standard_normal(n) * 3
+    x[5] = np.where(rng.random(n) < 0.7, -1e30, 1e30)
+    x[6] = -np.exp(rng.uniform(-80, 80, n))
+    x[7] = rng.standard_normal(n)
+    x[:4, n // 3] += 9                       # (70001 exp(-9): 8.6, next to the largest's 1)
+    x[7, : n // 2] = np.inf
+    for u in (0.02, 0.4, 0.999):
+        us = np.full(8, u, dt)
+        for settings in ({}, {"top_k": 5}, {"top_k": 300}, {"top_k": 300, "min_p": 1e-5}, {"top_k": n // 2}, {"top_p": 0.9}, {"top_k": n // 3, "top_p": 0.7},
+                         {"top_k": 400, "top_p": 0.8, "min_p": 1e-4}, {"min_p": 1e-5}, {"top_k": n // 2 + 40}):
+            assert (take(m, x, us, dt, **settings) == chosen(x, us, **settings)).all(), (u, settings)
