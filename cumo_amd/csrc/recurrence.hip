@@ -18,6 +18,9 @@
 // Where there are enough columns or rows to fill the machine each is walked from its first step to its last by one block. Where
 // there are not, time is cut into tiles, a block each, all in one launch: a tile leaves its A and B in memory for the ones after
 // it, folds those of the tiles before it from the nearest one whose state is there already, and leaves its own state.
+// Memory bounds all but the shortest: SFloat [8,4096,2048] 157 us (5.1 TB/s, a large copy's rate), gradients of [8,2048,2048] 133
+// us (5.0), DFloat [4096,4095] along rows 83 us (4.9); in tiles [1,65536,1000] 184 us and 6.5 for clearing the words (4.1: in each tile
+// loads, joins and stores follow one another, and 10% more bytes go through the words). One step of 64 x 4096: 5.6 us.
 #include "common.h"
 #include "wait_ctl.h"
 
@@ -693,8 +696,13 @@ __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kern
 }
 
 // ---- launches -------------------------------------------------------------------------
-constexpr uint64_t kReWaves = 4096;   // sixteen to a compute unit
-// time is cut where there are fewer rows or strips of columns than these, and more than so many tiles of them
+// Waves that a walk down columns is given, sixteen to a compute unit: SFloat [8,4096,2048], 256 strips, with 1, 2, 4, 8 and 16 waves
+// each 303, 195, 157, 165 and 158 us.
+constexpr uint64_t kReWaves = 4096;
+// Time is cut where there are fewer rows or strips of columns than these, and more than so many tiles of them. us walked / in tiles,
+// SFloat, down columns: [1,2048,1000] 36 / 15, [15,1024,1000] 58 / 45, [4,4096,2048] (128 strips) 106 / 85, [8,4096,2048] (256) 155 / 162;
+// [1,512,1000] (2 tiles) 10.8 / 12.3, [1,700,1000] (3) 14.2 / 12.5. Along rows: [64,40000] 28 / 15, [160,40000] 30 / 25, [200,40000] 31 / 33,
+// [200,131072] 104 / 78, [300,131072] 123 / 110, [400,40000] 45 / 52, [1000,20000] 53 / 70, [1,2^24] 10980 / 96.
 constexpr uint64_t kReFewRows = 256, kReFewStrips = 256, kReFewTiles = 2;
 constexpr uint64_t kReMostTiles = 1u << 22;   // (2^30 blocks)
 
