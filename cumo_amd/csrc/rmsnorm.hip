@@ -8,8 +8,9 @@
 // lanes, and what is computed from them is written once. The sums, and everything between them and the one rounding of a
 // result, are in double: a square of a float is exact there, and the vector units do a hundred such operations in the time
 // that an element's bytes take. SFloat [8192,4096], with a residual, a sum and a weight: 87 us (6.2 TB/s, what an addition of two
-// large arrays reaches); in 8 bits [8192,4095] 92 us (6.1), and 31 us back (5.4); gradients with gsum 95 + 5.5 us (5.7 and the
-// weight's parts); DFloat [131072,257] gradients 200 + 5 (5.4). One row of 4096: 3.5 us, the launch's.
+// large arrays reaches); in 8 bits [8192,4095] 84 us (5.2; the vector units are busy for more than half of it), and 30 us back
+// (5.5); gradients with gsum 95 + 5.5 us (5.7 and the weight's parts); DFloat [131072,257] gradients 200 + 5 (5.4). One row of
+// 4096: 3.5 us, the launch's.
 #include "common.h"
 
 namespace cumo_hip {
@@ -135,14 +136,25 @@ struct RnParams : cumo_hip_rmsnorm_t {
     bool y_through, sum_through;  // whether rows may be written through (StoreRows)
 };
 
-// y / scale as an 8-bit integer; inverse: 1 / scale, 0 where the scale is 0 or NaN (what is NaN then is 0 too)
-__device__ __forceinline__ int8_t rn_byte(double y, double inverse) {
-    const double z = rint(y * inverse);
-    return z == z ? (int8_t)(int)__builtin_fmin(__builtin_fmax(z, -127.0), 127.0) : (int8_t)0;
-}
+// A row in 8 bits: y = p a, of which p is an element's, exact for SFloat, and a the row's (DFloat: 1, as s w can overflow where y
+// does not). The nearest integer of p b is what the sum with 1.5 * 2^52 leaves in its lower 32 bits; b: a / scale, or 0 where the
+// row's bytes are all 0 (a scale of 0, of infinity, of NaN), and so is then `kept`. A scale below the normal numbers can be half its
+// row's largest / 127, rounded: then the bytes end at 127. SFloat [8192,4096] 47 us; 58 with y itself,
+// its quotient and its limits in double for each element.
 template <class T>
-__device__ __forceinline__ double rn_inverse(T scale) {
-    return scale > (T)0 && scale < (T)INFINITY ? 1.0 / (double)scale : 0.0;
+__device__ __forceinline__ double rn_product(T s, double r, T w) { return sizeof(T) == 4 ? (double)s * (double)w : (double)s * r * (double)w; }
+template <class T>
+__device__ __forceinline__ double rn_common(double r) { return sizeof(T) == 4 ? r : 1.0; }
+__device__ __forceinline__ int8_t rn_byte(double p, double b, int kept) {
+    const int z = (int)__double_as_longlong(__builtin_fma(p, b, 6755399441055744.0)) & kept;
+    return (int8_t)(z < -127 ? -127 : z > 127 ? 127 : z);
+}
+// 1 / scale, where there is something to divide; `lift` a power of two for p and scale, with which it is no infinity
+template <class T>
+__device__ __forceinline__ double rn_lift(T scale) { return sizeof(T) == 8 && (double)scale < 0x1p-1000 ? 0x1p200 : 1.0; }
+template <class T>
+__device__ __forceinline__ double rn_inverse(T scale, double lift) {
+    return scale > (T)0 && scale < (T)INFINITY ? 1.0 / ((double)scale * lift) : 0.0;
 }
 
 template <class T, int TPR, int NV, int BLOCK, bool Q8, bool NT>
@@ -182,14 +194,23 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_kernel(RnParams p) {
         w.forget();
         if constexpr (Q8) {
             double most[1] = {0.0};
-            s.each([&](T& v, int k, int j) { most[0] = rn_max_nan(most[0], fabs((double)v * r * (double)w.at(k, j))); });
+            bool nan = false;
+            s.each([&](T& v, int k, int j) {
+                const double product = rn_product(v, r, w.at(k, j));
+                nan |= product != product;
+                most[0] = __builtin_fmax(most[0], __builtin_fabs(product));
+            });
+            most[0] = nan ? __builtin_nan("") : most[0];
             rn_allreduce<TPR, BLOCK>(most, rn_max_nan);
-            s.forget();
-            w.forget();
-            const T scale = (T)(most[0] / 127.0);
+            if constexpr (NV > 4) {
+                s.forget();
+                w.forget();
+            }
+            const T scale = (T)(most[0] * rn_common<T>(r) / 127.0);
             if (there && lane == 0) reinterpret_cast<T*>(p.scale)[row] = scale;
-            const double inverse = rn_inverse(scale);
-            s.store_bytes(p.y + row * p.y_step, lane, whole, rest, [&](int k, int j) { return rn_byte((double)s.at(k, j) * r * (double)w.at(k, j), inverse); });
+            const double lift = rn_lift(scale), inverse = rn_inverse(scale, lift), b = rn_common<T>(r) * inverse, raised = r * lift;
+            const int kept = inverse > 0.0 ? -1 : 0;
+            s.store_bytes(p.y + row * p.y_step, lane, whole, rest, [&](int k, int j) { return rn_byte(rn_product(s.at(k, j), raised, w.at(k, j)), b, kept); });
         } else {
             s.each([&](T& v, int k, int j) { v = (T)((double)v * r * (double)w.at(k, j)); });
             s.template store<NT>(p.y + row * p.y_step, lane, whole, rest, y_pieces);
@@ -216,19 +237,20 @@ __global__ __launch_bounds__(kRnWide) void rmsnorm_long_kernel(cumo_hip_rmsnorm_
         rn_allreduce<kRnWide, kRnWide>(q, rn_add);
         const double r = 1.0 / sqrt(q[0] / (double)p.n + p.eps);
         const T* from = sum ? sum : x;
-        auto value = [&](uint64_t i) { return (double)from[i] * r * (w ? (double)w[i] : 1.0); };
+        auto product = [&](uint64_t i, double by) { return rn_product(from[i], by, w ? w[i] : (T)1); };
         if constexpr (Q8) {
             double most[1] = {0.0};
-            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) most[0] = rn_max_nan(most[0], fabs(value(i)));
+            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) most[0] = rn_max_nan(most[0], fabs(product(i, r)));
             rn_allreduce<kRnWide, kRnWide>(most, rn_max_nan);
-            const T scale = (T)(most[0] / 127.0);
+            const T scale = (T)(most[0] * rn_common<T>(r) / 127.0);
             if (threadIdx.x == 0) reinterpret_cast<T*>(p.scale)[row] = scale;
-            const double inverse = rn_inverse(scale);
+            const double lift = rn_lift(scale), inverse = rn_inverse(scale, lift), b = rn_common<T>(r) * inverse, raised = r * lift;
+            const int kept = inverse > 0.0 ? -1 : 0;
             int8_t* y = reinterpret_cast<int8_t*>(p.y + (int64_t)row * p.y_step);
-            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) y[i] = rn_byte(value(i), inverse);
+            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) y[i] = rn_byte(product(i, raised), b, kept);
         } else {
             T* y = reinterpret_cast<T*>(p.y + (int64_t)row * p.y_step);
-            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) y[i] = (T)value(i);
+            for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) y[i] = (T)((double)from[i] * r * (w ? (double)w[i] : 1.0));
         }
     }
 }

@@ -355,3 +355,23 @@ def test_int8_arrays_are_copied_viewed_and_read_back():
     assert (a.reshape(91)[4:60].to_numpy() == h.reshape(91)[4:60]).all()
     with pytest.raises(TypeError):
         (m.SFloat.cast(h.astype(np.float32)) > 0).mask(a)
+
+
+@pytest.mark.parametrize("dt,size", [(np.float32, 1e-43), (np.float32, 1e-39), (np.float32, 1e38), (np.float64, 1e-321), (np.float64, 1e-310), (np.float64, 1e307)])
+@pytest.mark.parametrize("n", [5, 700, 4099, 33001])
+def test_rmsnorm_q8_of_weights_at_the_ends_of_their_type(dt, size, n):
+    """A scale is off by half a step of its type, near 0 of the smallest number's (and a little: largest / 127 is rounded twice
+    there); what is above 127 of them is 127."""
+    import cumo_amd as m
+    cls = cls_of(m, dt)
+    rng = np.random.default_rng(n)
+    s = (rng.standard_normal((3, n)) * 7).astype(dt)
+    w = (np.sign(rng.standard_normal(n)) * rng.uniform(0.3, 1.7, n) * size).astype(dt)
+    want, _ = reference(s, w, 1e-6)
+    q, scale = (a.to_numpy() for a in m.Fused.rmsnorm_q8(cls.cast(s), cls.cast(w)))
+    hs = scale.astype(np.longdouble)
+    least = np.longdouble(np.finfo(dt).smallest_subnormal)
+    most = np.abs(want).max(axis=-1, keepdims=True)
+    assert (np.abs(hs - most / 127) <= 0.51 * least + (half_step(dt) + (n + 16) * U64) * most / 127).all()
+    quotient = np.where(hs > 0, want / np.where(hs > 0, hs, 1), 0)
+    assert (np.abs(q - np.clip(quotient, -127, 127)) <= 0.5 + 127 * 4 * (n + 16) * U64).all()
