@@ -46,6 +46,21 @@ __device__ __forceinline__ void rn_allreduce(double (&v)[K], F f) {
     }
 }
 
+// How rows are written: through the second-level cache where their pieces are whole (store_form.h); else past it, or, `meet`, plainly
+// where rows follow one another, so that a row's end and the next one's start meet in that cache: for y beside s. us past it / plainly,
+// with a residual: SFloat [8192,4095] 94 / 88, [8192,4092] 96 / 85, [32768,1001] 96 / 100, [131072,257] 134 / 100, DFloat [131072,257]
+// 223 / 209, [8192,2047] 97 / 86. Otherwise it does not pay: 8 bits [8192,4092] 77 / 84, dequantize [8192,4095] 30 / 35, y alone [8192,4095]
+// 49 / 53, gradients DFloat [131072,257] 200 / 218.
+struct RnStore {
+    bool pieces, meet;
+    __device__ __forceinline__ RnStore(const char* p, int64_t step, bool through, bool may_meet) : pieces(through && store_pieces(p, step)), meet(through && may_meet) {}
+    template <bool NT, class Q>
+    __device__ __forceinline__ void put(Q* at, Q v) const {
+        if (NT && !pieces && meet) *at = v;
+        else store_vector<NT>(at, v, pieces);
+    }
+};
+
 // A row in the registers of TPR lanes: whole 128-bit vectors, lane l holding vectors l, l + TPR, ..., and, one to a lane, the
 // elements behind the last whole one. What is not there is 0.
 template <class T, int TPR, int NV>
@@ -91,11 +106,11 @@ struct RnRow {
         last = v;
     }
     template <bool NT>
-    __device__ __forceinline__ void store(char* row, uint32_t lane, uint32_t whole, uint32_t rest, bool pieces) const {
+    __device__ __forceinline__ void store(char* row, uint32_t lane, uint32_t whole, uint32_t rest, RnStore to) const {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const uint32_t at = (uint32_t)k * TPR + lane;
-            if (at < whole) store_vector<NT>(reinterpret_cast<u4*>(row + at * 16u), x[k].q, pieces);
+            if (at < whole) to.put<NT>(reinterpret_cast<u4*>(row + at * 16u), x[k].q);
             if constexpr (NV > 4) __builtin_amdgcn_sched_barrier(0);
         }
         if (lane < rest) reinterpret_cast<T*>(row)[whole * V + lane] = last;
@@ -171,7 +186,7 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_kernel(RnParams p) {
         else w.fill((T)1);
     };
     if constexpr (HELD) read_weight();
-    const bool y_pieces = p.y_through && store_pieces(p.y, p.y_step), sum_pieces = p.sum_through && store_pieces(p.sum, p.sum_step);
+    const RnStore to_y(p.y, p.y_step, p.y_through, p.sum != nullptr), to_sum(p.sum, p.sum_step, p.sum_through, !Q8);
     for (uint64_t first = (uint64_t)blockIdx.x * RPB; first < p.rows; first += (uint64_t)gridDim.x * RPB) {
         const uint64_t mine = first + threadIdx.x / TPR;
         const bool there = mine < p.rows;
@@ -183,7 +198,7 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_kernel(RnParams p) {
             Row add;
             add.template load<NT>(p.residual + row * p.residual_step, lane, whole, rest, vectors != 0);
             s.each([&](T& v, int k, int j) { v += add.at(k, j); });
-            s.template store<NT>(p.sum + row * p.sum_step, lane, whole, rest, sum_pieces);
+            s.template store<NT>(p.sum + row * p.sum_step, lane, whole, rest, to_sum);
         }
         double q[1] = {0.0};
         s.each([&](T& v, int, int) { q[0] = __builtin_fma((double)v, (double)v, q[0]); });
@@ -213,7 +228,7 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_kernel(RnParams p) {
             s.store_bytes(p.y + row * p.y_step, lane, whole, rest, [&](int k, int j) { return rn_byte(rn_product(s.at(k, j), raised, w.at(k, j)), b, kept); });
         } else {
             s.each([&](T& v, int k, int j) { v = (T)((double)v * r * (double)w.at(k, j)); });
-            s.template store<NT>(p.y + row * p.y_step, lane, whole, rest, y_pieces);
+            s.template store<NT>(p.y + row * p.y_step, lane, whole, rest, to_y);
         }
     }
 }
@@ -263,7 +278,7 @@ __global__ __launch_bounds__(kDqBlock) void dequantize_kernel(cumo_hip_dequantiz
     constexpr int RPB = kDqBlock / TPR;
     const uint32_t lane = threadIdx.x % TPR;
     const uint64_t vectors = p.n / Row::V;
-    const bool pieces = through && store_pieces(p.y, p.y_step);
+    const RnStore to(p.y, p.y_step, through, false);
     for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (uint64_t)gridDim.x * RPB) {
         const int8_t* q = reinterpret_cast<const int8_t*>(p.q + (int64_t)row * p.q_step);
         char* y = p.y + (int64_t)row * p.y_step;
@@ -282,7 +297,7 @@ __global__ __launch_bounds__(kDqBlock) void dequantize_kernel(cumo_hip_dequantiz
                 typename Row::Vec v;
 #pragma unroll
                 for (int j = 0; j < Row::V; ++j) v.t[j] = (T)b[u][j] * scale;
-                if (at < vectors) store_vector<NT>(reinterpret_cast<typename Row::u4*>(y + at * 16), v.q, pieces);
+                if (at < vectors) to.template put<NT>(reinterpret_cast<typename Row::u4*>(y + at * 16), v.q);
             }
         }
         if (lane < p.n % Row::V) reinterpret_cast<T*>(y)[vectors * Row::V + lane] = (T)q[vectors * Row::V + lane] * scale;
@@ -317,7 +332,7 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_grad_kernel(RnGradParams p) {
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[k][j] = 0.0;
     }
-    const bool pieces = p.through && store_pieces(p.gx, p.gx_step);
+    const RnStore to(p.gx, p.gx_step, p.through, false);
     for (uint64_t first = (uint64_t)blockIdx.x * RPB; first < p.rows; first += (uint64_t)gridDim.x * RPB) {
         const uint64_t mine = first + threadIdx.x / TPR;
         const bool there = mine < p.rows;
@@ -351,7 +366,7 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_grad_kernel(RnGradParams p) {
             sum[k][j] = __builtin_fma(gv * sv, r, sum[k][j]);
             v = (T)__builtin_fma(r, gv * (double)w.at(k, j) - sv * c, (double)gs.at(k, j));
         });
-        s.template store<NT>(p.gx + row * p.gx_step, lane, whole, rest, pieces);
+        s.template store<NT>(p.gx + row * p.gx_step, lane, whole, rest, to);
     }
     if (!p.gweight) return;
     // the rows that the block holds side by side
