@@ -35,6 +35,7 @@ struct ReArgs {
     char *out, *gb, *last;                       // h, or ga; gradients: gb, gh0
     int64_t a_step[3], b_step[3], h_step[3], out_step[3], gb_step[3];   // outer, time, inner
     uint64_t columns, inner, time;
+    uint64_t before;   // columns of the launches in front of this one
 };
 
 constexpr double kTooSmall = 4.9406564584124654e-324;
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(NW * 64) void recurrence_columns_kernel(ReArgs p) {
     __shared__ double products[2][NW][64];
     __shared__ T reached[2][NW][64];
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint64_t mine = (uint64_t)blockIdx.x * 64 + lane;
+    const uint64_t mine = p.before + (uint64_t)blockIdx.x * 64 + lane;
     const bool there = mine < p.columns;
     const uint64_t c = there ? mine : p.columns - 1;   // (a lane without a column reads the last one's)
     const int64_t o = (int64_t)(c / p.inner), i = (int64_t)(c - (uint64_t)o * p.inner);
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(kReChainWaves * 64, sizeof(T) == 4 ? 8 : 4) void re
 // Columns that lie further apart than a lane's 32 bits reach: a lane each, one step after the other.
 template <class T, bool GRAD>
 __global__ __launch_bounds__(64) void recurrence_apart_kernel(ReArgs p) {
-    const uint64_t c = (uint64_t)blockIdx.x * 64 + threadIdx.x;
+    const uint64_t c = p.before + (uint64_t)blockIdx.x * 64 + threadIdx.x;
     if (c >= p.columns) return;
     const int64_t o = (int64_t)(c / p.inner), i = (int64_t)(c - (uint64_t)o * p.inner);
     auto at = [&](const char* x, const int64_t (&step)[3], uint64_t t) { return reinterpret_cast<T*>(const_cast<char*>(x) + o * step[0] + (int64_t)t * step[1] + i * step[2]); };
@@ -704,13 +705,25 @@ constexpr uint64_t kReWaves = 4096;
 // [1,512,1000] (2 tiles) 10.8 / 12.3, [1,700,1000] (3) 14.2 / 12.5. Along rows: [64,40000] 28 / 15, [160,40000] 30 / 25, [200,40000] 31 / 33,
 // [200,131072] 104 / 78, [300,131072] 123 / 110, [400,40000] 45 / 52, [1000,20000] 53 / 70, [1,2^24] 10980 / 96.
 constexpr uint64_t kReFewRows = 256, kReFewStrips = 256, kReFewTiles = 2;
-constexpr uint64_t kReMostTiles = 1u << 22;   // (2^30 blocks)
+constexpr uint64_t kReMostTiles = 1u << 21;   // (of all lines together: a launch holds fewer than 2^32 lanes)
+
+// strips of 64 columns, in as many launches as it takes: a launch holds fewer than 2^32 lanes
+template <class F>
+void re_strips(ReArgs p, unsigned lanes, F launch) {
+    const uint64_t most = (1ull << 31) / lanes;
+    for (p.before = 0; p.before < p.columns; p.before += most * 64) {
+        const uint64_t strips = (p.columns - p.before + 63) / 64;
+        launch(p, dim3((unsigned)(strips < most ? strips : most)), dim3(lanes));
+    }
+}
 
 template <class T, bool GRAD, int NW>
 void re_launch_columns(const ReArgs& p, hipStream_t stream) {
-    const dim3 grid((unsigned)((p.columns + 63) / 64)), block(NW * 64);
-    if (stream_past_caches(p.columns * p.time * sizeof(T) * (GRAD ? 5 : 3))) hipLaunchKernelGGL((recurrence_columns_kernel<T, GRAD, NW, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((recurrence_columns_kernel<T, GRAD, NW, false>), grid, block, 0, stream, p);
+    const bool once = stream_past_caches(p.columns * p.time * sizeof(T) * (GRAD ? 5 : 3));
+    re_strips(p, NW * 64, [&](const ReArgs& part, dim3 grid, dim3 block) {
+        if (once) hipLaunchKernelGGL((recurrence_columns_kernel<T, GRAD, NW, true>), grid, block, 0, stream, part);
+        else hipLaunchKernelGGL((recurrence_columns_kernel<T, GRAD, NW, false>), grid, block, 0, stream, part);
+    });
 }
 
 // `lines`: strips of columns (`lanes` 64), or rows (1); `tile`: steps of a block
@@ -773,7 +786,7 @@ int re_launch(ReArgs p, hipStream_t stream) {
             return CUMO_HIP_OK;
         }
         constexpr uint64_t kTile = kReChainWaves * 64 * E;
-        if (p.columns < kReFewRows && p.time > kTile && p.time / kTile < kReMostTiles) return re_chain<T, GRAD, true>(p, p.columns, kTile, stream);
+        if (p.columns < kReFewRows && p.time > kTile && p.columns * (p.time / kTile + 1) < kReMostTiles) return re_chain<T, GRAD, true>(p, p.columns, kTile, stream);
         hipLaunchKernelGGL((recurrence_rows_kernel<T, GRAD>), dim3((unsigned)(p.columns < (1u << 20) ? p.columns : (1u << 20))), dim3(kReBlock), 0, stream, p);
         cumo_cuda_runtime_check_kernel_launch();
         return CUMO_HIP_OK;
@@ -785,14 +798,14 @@ int re_launch(ReArgs p, hipStream_t stream) {
         return across < (1ull << 40) && beside < (1ull << 40) && rows_across * across + columns_beside * beside < (1ull << 32);
     };
     if (!near(p.a_step) || !near(p.b_step) || !near(p.out_step) || (GRAD && (!near(p.h_step) || !near(p.gb_step)))) {
-        hipLaunchKernelGGL((recurrence_apart_kernel<T, GRAD>), dim3((unsigned)strips), dim3(64), 0, stream, p);
+        re_strips(p, 64, [&](const ReArgs& part, dim3 grid, dim3 block) { hipLaunchKernelGGL((recurrence_apart_kernel<T, GRAD>), grid, block, 0, stream, part); });
         cumo_cuda_runtime_check_kernel_launch();
         return CUMO_HIP_OK;
     }
     int waves = 1;
     while (waves < 16 && strips * waves < kReWaves && (uint64_t)waves * kReRows<T, GRAD> < p.time) waves *= 2;
     constexpr uint64_t kTile = kReChainWaves * kReRows<T, GRAD>;
-    if (strips < kReFewStrips && p.time > kReFewTiles * kTile && p.time / kTile < kReMostTiles) return re_chain<T, GRAD, false>(p, strips, kTile, stream);
+    if (strips < kReFewStrips && p.time > kReFewTiles * kTile && strips * (p.time / kTile + 1) < kReMostTiles) return re_chain<T, GRAD, false>(p, strips, kTile, stream);
     if (waves >= 16) re_launch_columns<T, GRAD, 16>(p, stream);
     else if (waves >= 8) re_launch_columns<T, GRAD, 8>(p, stream);
     else if (waves >= 4) re_launch_columns<T, GRAD, 4>(p, stream);

@@ -426,15 +426,15 @@ __global__ __launch_bounds__(kRnWide) void rmsnorm_grad_long_kernel(cumo_hip_rms
 // the weight's part of every blockIdx.y-th run of rows, by columns
 template <class T>
 __global__ __launch_bounds__(256) void rmsnorm_grad_columns_kernel(RnGradParams p, const double* rs, uint64_t per) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= p.n) return;
     const uint64_t from = blockIdx.y * per, to = from + per < p.rows ? from + per : p.rows;
-    double sum = 0.0;
-    for (uint64_t row = from; row < to; ++row) {
-        const double g = (double)reinterpret_cast<const T*>(p.g + (int64_t)row * p.g_step)[i], s = (double)reinterpret_cast<const T*>(p.s + (int64_t)row * p.s_step)[i];
-        sum = __builtin_fma(g * s, rs[row], sum);
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < p.n; i += (uint64_t)gridDim.x * 256) {
+        double sum = 0.0;
+        for (uint64_t row = from; row < to; ++row) {
+            const double g = (double)reinterpret_cast<const T*>(p.g + (int64_t)row * p.g_step)[i], s = (double)reinterpret_cast<const T*>(p.s + (int64_t)row * p.s_step)[i];
+            sum = __builtin_fma(g * s, rs[row], sum);
+        }
+        p.parts[blockIdx.y * p.n + i] = sum;
     }
-    p.parts[blockIdx.y * p.n + i] = sum;
 }
 
 // [parts][n] down its columns: 16 columns a block, every lane of the 64 to a column taking every 64th part (64 columns a block
@@ -443,26 +443,30 @@ template <class T>
 __global__ __launch_bounds__(1024) void rmsnorm_grad_parts_kernel(const double* parts, uint32_t n_parts, uint64_t n, T* out) {
     __shared__ double slot[16][16];
     const uint32_t column = threadIdx.x & 15, group = threadIdx.x >> 4;
-    const uint64_t i = (uint64_t)blockIdx.x * 16 + column;
-    double sum = 0.0;
-    if (i < n) {
+    for (uint64_t first = (uint64_t)blockIdx.x * 16; first < n; first += (uint64_t)gridDim.x * 16) {
+        const uint64_t i = first + column;
+        double sum = 0.0;
+        if (i < n) {
 #pragma unroll 4
-        for (uint32_t k = group; k < n_parts; k += 64) sum += parts[k * n + i];
-    }
-    // the wave's four groups, then the waves
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    if ((group & 3) == 0) slot[group >> 2][column] = sum;
-    __syncthreads();
-    if (threadIdx.x < 16 && i < n) {
-        sum = slot[0][column];
+            for (uint32_t k = group; k < n_parts; k += 64) sum += parts[k * n + i];
+        }
+        // the wave's four groups, then the waves
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if ((group & 3) == 0) slot[group >> 2][column] = sum;
+        __syncthreads();
+        if (threadIdx.x < 16 && i < n) {
+            sum = slot[0][column];
 #pragma unroll
-        for (int w = 1; w < 16; ++w) sum += slot[w][column];
-        out[i] = (T)sum;
+            for (int w = 1; w < 16; ++w) sum += slot[w][column];
+            out[i] = (T)sum;
+        }
+        __syncthreads();
     }
 }
 
 unsigned rn_grid(uint64_t blocks, uint64_t most) { return (unsigned)(blocks < most ? blocks : most); }
+dim3 rn_columns(uint64_t n) { return dim3(rn_grid((n + 15) / 16, 1u << 20)); }   // of the parts (a launch holds fewer than 2^32 lanes)
 
 template <class T>
 bool rn_through(const void* p, uint64_t rows, uint64_t n, int64_t step, bool nt) {
@@ -543,7 +547,7 @@ bool rn_grad_one(RnGradParams p, hipStream_t stream) {
     if (nt) hipLaunchKernelGGL((rmsnorm_grad_kernel<T, TPR, NV, BLOCK, true>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((rmsnorm_grad_kernel<T, TPR, NV, BLOCK, false>), grid, block, 0, stream, p);
     if (parts) {
-        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 15) / 16)), dim3(1024), 0, stream, p.parts, (uint32_t)blocks, p.n,
+        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), rn_columns(p.n), dim3(1024), 0, stream, p.parts, (uint32_t)blocks, p.n,
                            reinterpret_cast<T*>(p.gweight));
         // (the memory of a captured launch stays with its graph)
         if (!stream_under_capture()) cumo_cuda_runtime_free(parts);
@@ -562,8 +566,8 @@ bool rn_grad_long(RnGradParams p, hipStream_t stream) {
     hipLaunchKernelGGL((rmsnorm_grad_long_kernel<T>), dim3(rn_grid(p.rows, 1u << 20)), dim3(kRnWide), 0, stream, p, rs);
     if (memory) {
         p.parts = rs + p.rows;
-        hipLaunchKernelGGL((rmsnorm_grad_columns_kernel<T>), dim3((unsigned)((p.n + 255) / 256), (unsigned)runs), dim3(256), 0, stream, p, rs, per);
-        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 15) / 16)), dim3(1024), 0, stream, p.parts, (uint32_t)runs, p.n,
+        hipLaunchKernelGGL((rmsnorm_grad_columns_kernel<T>), dim3(rn_grid((p.n + 255) / 256, 1u << 20), (unsigned)runs), dim3(256), 0, stream, p, rs, per);
+        hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), rn_columns(p.n), dim3(1024), 0, stream, p.parts, (uint32_t)runs, p.n,
                            reinterpret_cast<T*>(p.gweight));
         if (!stream_under_capture()) cumo_cuda_runtime_free(memory);
     }
@@ -580,7 +584,7 @@ int rn_grad(const cumo_hip_rmsnorm_grad_t& d, hipStream_t stream) {
     bool ok = true;
     if (p.rows == 0) {
         if (p.gweight)
-            hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), dim3((unsigned)((p.n + 15) / 16)), dim3(1024), 0, stream, nullptr, 0u, p.n, reinterpret_cast<T*>(p.gweight));
+            hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), rn_columns(p.n), dim3(1024), 0, stream, nullptr, 0u, p.n, reinterpret_cast<T*>(p.gweight));
     }
     else if (nv <= 8) ok = rn_grad_one<T, 8, 1, 256>(p, stream);
     else if (nv <= 16) ok = rn_grad_one<T, 8, 2, 256>(p, stream);

@@ -352,3 +352,30 @@ def test_waits_that_give_up_are_reported():
     env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), CUMO_HIP_WAIT_LIMIT="0")
     p = subprocess.run([sys.executable, "-c", GIVING_UP], env=env, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=100)
     assert p.returncode == 0 and "reported" in p.stdout, p.stdout[-2000:]
+
+
+def test_more_columns_than_a_launch_has_lanes():
+    """2^32 columns and some: operands of one number each, broadcast; results looked at around the launches' borders."""
+    import cumo_amd as m
+    from cumo_amd import _lib
+    n = (1 << 32) + 777
+    one = [m.SFloat.cast(np.full((1, 1), v, np.float32)) for v in (0.5, 3.0, -2.0)]
+    wide = [v._desc() for v in one]
+    for d in wide:
+        d.shape[0], d.shape[1] = 2, n
+        d.stride[0] = d.stride[1] = 0
+    a, b, h = wide
+    out = m.SFloat(2, n).fill(9)
+    do = out._desc()
+    _lib.call(_lib.lib.cumo_hip_na_recurrence, C.byref(a), C.byref(b), None, 0, C.byref(do))
+    ends = [slice(0, 100), slice((1 << 31) - 100, (1 << 31) + 100), slice((1 << 32) - 100, (1 << 32) + 100), slice(n - 100, n)]
+    for s in ends:
+        got = out[:, s].to_numpy()
+        assert (got[0] == 3.0).all() and (got[1] == 4.5).all()
+    ga = m.SFloat(2, n).fill(9)
+    dg = ga._desc()
+    _lib.call(_lib.lib.cumo_hip_na_recurrence_grad, C.byref(b), C.byref(a), C.byref(h), None, 0, C.byref(dg), C.byref(do), None)
+    for s in ends:
+        got, gb = ga[:, s].to_numpy(), out[:, s].to_numpy()
+        assert (gb[1] == 3.0).all() and (gb[0] == 4.5).all()
+        assert (got[1] == -6.0).all() and (got[0] == 0.0).all()

@@ -375,3 +375,13 @@ def test_rmsnorm_q8_of_weights_at_the_ends_of_their_type(dt, size, n):
     assert (np.abs(hs - most / 127) <= 0.51 * least + (half_step(dt) + (n + 16) * U64) * most / 127).all()
     quotient = np.where(hs > 0, want / np.where(hs > 0, hs, 1), 0)
     assert (np.abs(q - np.clip(quotient, -127, 127)) <= 0.5 + 127 * 4 * (n + 16) * U64).all()
+
+
+def test_gradient_of_a_weight_longer_than_one_launch_of_its_parts():
+    import cumo_amd as m
+    n = (1 << 26) + 37
+    s, g, w = m.SFloat(2, n).fill(1), m.SFloat(2, n).fill(0.5), m.SFloat(n).fill(2)
+    gx, gw = m.Fused.rmsnorm_grad(g, s, w, eps=0.0)
+    for k in (slice(0, 50), slice((1 << 24) - 50, (1 << 24) + 50), slice(n - 50, n)):
+        assert (gw[k].to_numpy() == 1.0).all()                   # r = 1: 2 rows of 0.5
+        assert (gx[:, k].to_numpy() == 0.0).all()                # along s nothing is left
