@@ -701,10 +701,12 @@ __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kern
 // each 303, 195, 157, 165 and 158 us.
 constexpr uint64_t kReWaves = 4096;
 // Time is cut where there are fewer rows or strips of columns than these, and more than so many tiles of them. us walked / in tiles,
-// SFloat, down columns: [1,2048,1000] 36 / 15, [15,1024,1000] 58 / 45, [4,4096,2048] (128 strips) 106 / 85, [8,4096,2048] (256) 155 / 162;
+// SFloat, down columns: [1,2048,1000] 36 / 15, [15,1024,1000] 58 / 45, of [n,4096,2048] 128 strips 106 / 85, 160 110 / 104, 192 117 / 122, 224 127 /
+// 142 (gradients 181 / 144, 190 / 174, 208 / 214, 229 / 260), DFloat 96 strips 180 / 145, 128 185 / 194 (319 / 272, 331 / 357); SFloat
 // [1,512,1000] (2 tiles) 10.8 / 12.3, [1,700,1000] (3) 14.2 / 12.5. Along rows: [64,40000] 28 / 15, [160,40000] 30 / 25, [200,40000] 31 / 33,
 // [200,131072] 104 / 78, [300,131072] 123 / 110, [400,40000] 45 / 52, [1000,20000] 53 / 70, [1,2^24] 10980 / 96.
-constexpr uint64_t kReFewRows = 256, kReFewStrips = 256, kReFewTiles = 2;
+constexpr uint64_t kReFewRows = 256, kReFewTiles = 2;
+template <class T> constexpr uint64_t kReFewStrips = sizeof(T) == 4 ? 192 : 128;
 constexpr uint64_t kReMostTiles = 1u << 21;   // (of all lines together: a launch holds fewer than 2^32 lanes)
 
 // strips of 64 columns, in as many launches as it takes: a launch holds fewer than 2^32 lanes
@@ -805,7 +807,7 @@ int re_launch(ReArgs p, hipStream_t stream) {
     int waves = 1;
     while (waves < 16 && strips * waves < kReWaves && (uint64_t)waves * kReRows<T, GRAD> < p.time) waves *= 2;
     constexpr uint64_t kTile = kReChainWaves * kReRows<T, GRAD>;
-    if (strips < kReFewStrips && p.time > kReFewTiles * kTile && strips * (p.time / kTile + 1) < kReMostTiles) return re_chain<T, GRAD, false>(p, strips, kTile, stream);
+    if (strips < kReFewStrips<T> && p.time > kReFewTiles * kTile && strips * (p.time / kTile + 1) < kReMostTiles) return re_chain<T, GRAD, false>(p, strips, kTile, stream);
     if (waves >= 16) re_launch_columns<T, GRAD, 16>(p, stream);
     else if (waves >= 8) re_launch_columns<T, GRAD, 8>(p, stream);
     else if (waves >= 4) re_launch_columns<T, GRAD, 4>(p, stream);
