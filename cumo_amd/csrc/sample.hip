@@ -13,8 +13,8 @@
 // their running sums and reads the chunks that reach the list's bins once more. The rows come from memory once and from the
 // last-level cache the other times. What bounds it for many rows is the weights' arithmetic in double (some twenty operations an
 // element) and the order of steps within a row, for a few rows the launches and those steps. SFloat, temperature 0.8, top_k 50,
-// top_p 0.95: one row of 131072 in 25 us (4, 5.5 and 16.6 in the three), 256 rows of 50001 in 41 us with one setting for all, and
-// in 63 us (13, 26.5 and 25; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
+// top_p 0.95: one row of 131072 in 24 us (4.6, 5 and 14.7 in the three), 256 rows of 50001 in 40 us with one setting for all, and
+// in 62 us (13, 27 and 23.4; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
 // chunks' maxima the last launch reads whole rows: 20.4 and 27.8 us of it, where the first one takes 4.0 and 11.2.
 #include "common.h"
 #include "ew_ops.h"
@@ -186,6 +186,16 @@ __device__ __forceinline__ T sa_largest(T v) {
     return sa_larger_from<T, 0x143, 0xc>(v);
 }
 
+// of all lanes, the same in each
+template <class T>
+__device__ __forceinline__ T sa_largest_of_all(T v) {
+    union { T t; int w[sizeof(T) / 4]; } u;
+    u.t = sa_largest(v);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) u.w[i] = __builtin_amdgcn_readlane(u.w[i], 63);
+    return u.t;
+}
+
 constexpr int kSaLook = 256;
 template <class T>
 __global__ __launch_bounds__(kSaLook) void sample_look_kernel(SaParams p) {
@@ -259,7 +269,7 @@ struct SaSettings {
     bool none, greedy;         // nothing to choose; the first of the largest
     bool all, cut_p, cut_m, small;   // no top_k; top_p, min_p cut; a top_k small enough for a list
     uint64_t top_k;
-    double u, top_p, likely;
+    double u, top_p, likely, bin_size;
     __device__ __forceinline__ SaSettings(const SaParams& p, uint64_t row) {
         const uint32_t lane = threadIdx.x & 63;
         const SaPart part = p.parts[row * p.looks + (lane < p.looks ? lane : 0)];   // (one of them more than once changes nothing)
@@ -267,12 +277,8 @@ struct SaSettings {
             min_p_at(p.min_p, row, p.parts);
         float_tables_prepare();
         T m = (T)part.max, least = (T)part.least;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-            m = sa_max(m, __shfl_xor(m, d));
-            least = sa_min(least, __shfl_xor(least, d));
-        }
-        m = sa_same(m);
+        m = sa_largest_of_all(m);
+        least = -sa_largest_of_all(-least);
         none = __ballot(part.nan != 0) != 0 || m == (T)-INFINITY;
         const double temperature = temperature_at.value(p.temperature), k = k_at.value(p.top_k), min_p = min_p_at.value(p.min_p);
         u = u_at.value(p.u);
@@ -290,6 +296,7 @@ struct SaSettings {
         // bins of 1/48 of a factor e, or finer ones where the row's numbers span less than the bins then reach
         const double per = kSaBinsPerNat / temperature, span = (double)m - (double)least, most = sizeof(T) == 4 ? 1e37 : 1e300;
         weight.bins_per = sa_same((T)(span * per < (double)(kSaBins - 2) ? __builtin_fmin((double)(kSaBins - 2) / span, most) : per));   // (span 0: one number)
+        bin_size = sa_same(1.0 / (double)weight.bins_per);
     }
 };
 
@@ -342,22 +349,29 @@ __global__ __launch_bounds__(kSaBlock) void sample_fill_kernel(SaParams p) {
     }
 }
 
-__device__ __forceinline__ uint64_t sa_up(uint64_t v, int d) { return (uint64_t)__shfl_up((unsigned long long)v, d); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t sa_from(uint64_t v) {   // 0 for lanes that none hands on to
+    const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return ((uint64_t)high << 32) | low;
+}
 
 // inclusive sums over the block's lanes, in the lanes' order; slots: one for each wave
 __device__ __forceinline__ uint64_t sa_scan(uint64_t v, uint64_t* slots) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = sa_up(v, d);
-        v += lane >= (uint32_t)d ? o : 0;
-    }
+    const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    // within 16 lanes by shifts, then the last lanes of those handed on
+    v += sa_from<0x111, 0xf>(v);
+    v += sa_from<0x112, 0xf>(v);
+    v += sa_from<0x114, 0xf>(v);
+    v += sa_from<0x118, 0xf>(v);
+    v += sa_from<0x142, 0xa>(v);
+    v += sa_from<0x143, 0xc>(v);
     __syncthreads();
     if (lane == 63) slots[wave] = v;
     __syncthreads();
-    uint64_t before = lane < wave ? slots[lane & (kSaBlock / 64 - 1)] : 0;   // (sixteen waves: lanes 0 to 14 at most)
-#pragma unroll
-    for (int d = 8; d > 0; d >>= 1) before += (uint64_t)__shfl_xor((unsigned long long)before, d);
+    uint64_t before = 0;
+#pragma unroll 5
+    for (uint32_t w = 0; w + 1 < kSaBlock / 64; ++w) before += w < wave ? slots[w] : 0;
     return v + sa_same(before);
 }
 
@@ -476,11 +490,11 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
     // What may be in bins [from, to], half a bin more on either side. (The bins' rounding moves a number by less than a thousandth
     // of a bin, and the bounds' keeps the order.)
     auto most_of = [&](uint32_t from) {
-        const double above = from == 0 ? -INFINITY : ((double)from - 0.5) / (double)weight.bins_per;
+        const double above = from == 0 ? -INFINITY : ((double)from - 0.5) * s.bin_size;
         return (T)((double)weight.max - above);
     };
     auto least_of = [&](uint32_t to) {
-        const double lowest = (double)weight.max - ((double)to + 1.5) / (double)weight.bins_per;
+        const double lowest = (double)weight.max - ((double)to + 1.5) * s.bin_size;
         return to < kSaBins - 1 && lowest == lowest ? (T)lowest : (T)-INFINITY;
     };
 
@@ -737,7 +751,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
                 bool few;
                 if (s.all) {
                     // few for sure: each element of the bins up to it weighs what the last one's end does, or more
-                    const double edge = weight.unit * exp2(-((double)(b + 1) / (double)weight.bins_per) * weight.rate);
+                    const double edge = weight.unit * exp2(-((double)(b + 1) * s.bin_size) * weight.rate);
                     few = sa_same((uint32_t)((double)masses[b] < edge * (0.999 * kSaFew))) != 0;
                 } else {
                     few = sa_same(counts[b]) <= (small ? (uint32_t)kSaList : kSaFew);
