@@ -8,8 +8,8 @@
 // lanes, and what is computed from them is written once. The sums, and everything between them and the one rounding of a
 // result, are in double: a square of a float is exact there, and the vector units do a hundred such operations in the time
 // that an element's bytes take. SFloat [8192,4096], with a residual, a sum and a weight: 87 us (6.2 TB/s, what an addition of two
-// large arrays reaches); in 8 bits [8192,4095] 84 us (5.2; the vector units are busy for more than half of it), and 30 us back
-// (5.5); gradients with gsum 95 + 5.5 us (5.7 and the weight's parts); DFloat [131072,257] gradients 200 + 5 (5.4). One row of
+// large arrays reaches); in 8 bits [8192,4095] 80 us (5.4; the vector units are busy for more than half of it), and 30 us back
+// (5.5); gradients with gsum 94 + 5 us (5.7 and the weight's parts); DFloat [131072,257] gradients 200 + 5 (5.4). One row of
 // 4096: 3.5 us, the launch's.
 #include "common.h"
 
@@ -73,6 +73,9 @@ struct RnRow {
 
     // `whole` and `rest`: vectors, and elements behind them, of this lane's row, 0 where there is no such row. A lane without a
     // vector reads the row's first one (`any`: there is one), so that no branch stands between the loads.
+    // It waits for them before it goes on (what is not there is made 0): a row's arrays come one after the other, a stretch of memory each
+    // time. That suits kernels bound by memory alone, SFloat [8192,4096] with a residual 88 us, on their way together 90, DFloat [131072,257]
+    // gradients 201, 213; 8 bits, with more to compute, 84 and 80.
     template <bool NT>
     __device__ __forceinline__ void load(const char* row, uint32_t lane, uint32_t whole, uint32_t rest, bool any) {
         if (any) {
@@ -96,6 +99,29 @@ struct RnRow {
             }
         }
         last = lane < rest ? reinterpret_cast<const T*>(row)[whole * V + lane] : (T)0;
+    }
+    // the same in two steps: what is not there is something else until it is cut off
+    template <bool NT>
+    __device__ __forceinline__ void send_for(const char* row, uint32_t lane, uint32_t whole, uint32_t rest, bool any) {
+        if (any) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const uint32_t at = (uint32_t)k * TPR + lane;
+                const u4* from = reinterpret_cast<const u4*>(row + (at < whole ? at * 16u : 0u));
+                x[k].q = NT ? __builtin_nontemporal_load(from) : *from;
+            }
+        } else {
+            fill((T)0);
+        }
+        last = lane < rest ? reinterpret_cast<const T*>(row)[whole * V + lane] : (T)0;
+    }
+    __device__ __forceinline__ void trim(uint32_t lane, uint32_t whole) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const bool there = (uint32_t)k * TPR + lane < whole;
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[k].t[j] = there ? x[k].t[j] : (T)0;
+        }
     }
     __device__ __forceinline__ void fill(T v) {
 #pragma unroll
@@ -193,13 +219,16 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_kernel(RnParams p) {
         const int64_t row = there ? (int64_t)mine : 0;
         const uint32_t whole = there ? vectors : 0, rest = there ? behind : 0;
         Row s;
-        s.template load<NT>(p.x + row * p.x_step, lane, whole, rest, vectors != 0);
+        if constexpr (Q8) s.template send_for<NT>(p.x + row * p.x_step, lane, whole, rest, vectors != 0);
+        else s.template load<NT>(p.x + row * p.x_step, lane, whole, rest, vectors != 0);
         if (p.residual) {
             Row add;
-            add.template load<NT>(p.residual + row * p.residual_step, lane, whole, rest, vectors != 0);
+            if constexpr (Q8) add.template send_for<NT>(p.residual + row * p.residual_step, lane, whole, rest, vectors != 0);
+            else add.template load<NT>(p.residual + row * p.residual_step, lane, whole, rest, vectors != 0);
             s.each([&](T& v, int k, int j) { v += add.at(k, j); });
             s.template store<NT>(p.sum + row * p.sum_step, lane, whole, rest, to_sum);
         }
+        if constexpr (Q8) s.trim(lane, whole);
         double q[1] = {0.0};
         s.each([&](T& v, int, int) { q[0] = __builtin_fma((double)v, (double)v, q[0]); });
         rn_allreduce<TPR, BLOCK>(q, rn_add);
@@ -313,6 +342,8 @@ struct RnGradParams : cumo_hip_rmsnorm_grad_t {
     bool through;
 };
 
+template <class T, int NV, int BLOCK> constexpr bool kRnAhead = NV == 4 && (sizeof(T) == 4 || BLOCK > 256);
+
 template <class T, int TPR, int NV, int BLOCK, bool NT>
 __global__ __launch_bounds__(BLOCK) void rmsnorm_grad_kernel(RnGradParams p) {
     typedef RnRow<T, TPR, NV> Row;
@@ -333,14 +364,35 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_grad_kernel(RnGradParams p) {
         for (int j = 0; j < V; ++j) sum[k][j] = 0.0;
     }
     const RnStore to(p.gx, p.gx_step, p.through, false);
+    // Where few blocks share a compute unit they read their next rows while they work on some: SFloat [4096,8192] 104 us without, 93
+    // with (gsum: 128, 109), [32768,4096] 301, 273 (394, 370), [131072,257] 105, 98 (130, 124); DFloat of 256 lanes, three blocks, not:
+    // [8192,2048] 69, 70, [131072,257] 170, 171.
+    constexpr bool AHEAD = kRnAhead<T, NV, BLOCK>;
+    Row next_s, next_g;
+    auto read = [&](Row& s, Row& g, uint64_t first) {
+        const uint64_t mine = first + threadIdx.x / TPR;
+        const bool there = mine < p.rows;
+        const int64_t row = there ? (int64_t)mine : 0;
+        s.template send_for<NT>(p.s + row * p.s_step, lane, there ? vectors : 0, there ? behind : 0, vectors != 0);
+        g.template send_for<NT>(p.g + row * p.g_step, lane, there ? vectors : 0, there ? behind : 0, vectors != 0);
+    };
+    if constexpr (AHEAD) read(next_s, next_g, (uint64_t)blockIdx.x * RPB);
     for (uint64_t first = (uint64_t)blockIdx.x * RPB; first < p.rows; first += (uint64_t)gridDim.x * RPB) {
         const uint64_t mine = first + threadIdx.x / TPR;
         const bool there = mine < p.rows;
         const int64_t row = there ? (int64_t)mine : 0;
         const uint32_t whole = there ? vectors : 0, rest = there ? behind : 0;
         Row s, g, gs;
-        s.template load<NT>(p.s + row * p.s_step, lane, whole, rest, vectors != 0);
-        g.template load<NT>(p.g + row * p.g_step, lane, whole, rest, vectors != 0);
+        if constexpr (AHEAD) {
+            s = next_s;
+            g = next_g;
+            read(next_s, next_g, first + (uint64_t)gridDim.x * RPB);
+            s.trim(lane, whole);
+            g.trim(lane, whole);
+        } else {
+            s.template load<NT>(p.s + row * p.s_step, lane, whole, rest, vectors != 0);
+            g.template load<NT>(p.g + row * p.g_step, lane, whole, rest, vectors != 0);
+        }
         auto read_gsum = [&] {
             if (p.gsum) gs.template load<NT>(p.gsum + row * p.gsum_step, lane, whole, rest, vectors != 0);
             else gs.fill((T)0);
@@ -529,15 +581,16 @@ void dq_launch(const cumo_hip_dequantize_t& d, hipStream_t stream) {
     else dq_launch_one<T, 256>(d, stream);
 }
 
-// Blocks that take the rows of a gradient, as many as the compute units hold at once of 256 lanes (three) and of 512 (one): more of
-// them leave more parts and take turns. us at 256, 512, 768, 1024, 2048 blocks: SFloat [8192,4096] 150, 101, 99.8, 115, 120; DFloat
-// [131072,257] 479, 304, 242, 323, 275; SFloat [131072,64] 50, 36, 34, 35, 46; [1024,8192], 512 lanes, 42, 50, 54, 65, 65.
-template <int BLOCK> constexpr uint64_t kRnGradBlocks = BLOCK > 256 ? 256 : 768;
+// Blocks that take the rows of a gradient, as many as the compute units hold at once: of 256 lanes three, two where they read ahead,
+// of 512 one. More of them leave more parts and take turns. us at 256, 512, 768, 1024, 2048 blocks: DFloat [131072,257] 479, 304, 242, 323, 275;
+// SFloat [131072,64] 50, 36, 34, 35, 46; reading ahead, [32768,4096] at 512 and 768 273, 325, [131072,257] 98, 109; [1024,8192], 512 lanes, at
+// 256, 512, 768 42, 50, 54.
+template <class T, int NV, int BLOCK> constexpr uint64_t kRnGradBlocks = BLOCK > 256 ? 256 : kRnAhead<T, NV, BLOCK> ? 512 : 768;
 
 template <class T, int TPR, int NV, int BLOCK>
 bool rn_grad_one(RnGradParams p, hipStream_t stream) {
     constexpr int RPB = BLOCK / TPR;
-    const unsigned blocks = rn_grid((p.rows + RPB - 1) / RPB, p.gweight ? kRnGradBlocks<BLOCK> : 256u * 64u);
+    const unsigned blocks = rn_grid((p.rows + RPB - 1) / RPB, p.gweight ? kRnGradBlocks<T, NV, BLOCK> : 256u * 64u);
     const bool nt = stream_past_caches(p.rows * p.n * sizeof(T) * (p.gsum ? 4 : 3));
     p.through = rn_through<T>(p.gx, p.rows, p.n, p.gx_step, nt);
     char* parts = nullptr;
