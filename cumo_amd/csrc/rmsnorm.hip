@@ -528,7 +528,7 @@ bool rn_through(const void* p, uint64_t rows, uint64_t n, int64_t step, bool nt)
 }
 
 // Lanes to a row: as many as hold it in four vectors each (the loads that a lane has on their way), two for 257 to 512 vectors, whose
-// sum then takes one block's lanes; behind 4096 vectors sixteen. us, norm / gradients, of 2^25 SFloat elements in rows of n, lanes x
+// sum then takes one block's lanes; behind 4096 vectors sixteen. us, norm / gradients (not reading ahead), of 2^25 SFloat elements in rows of n, lanes x
 // vectors as here and otherwise: n = 128, 8x4 44 / 72, 32x1 45 / 103; 1024, 64x4 47 / 68, 256x1 45 / 121; 2048, 256x2 39 / 81, 128x4
 // 48 / 74; 4096, 256x4 43 / 80, 512x2 41 / 112; 8192, 512x4 49 / 104, 1024x2 47 / -, 256x8 - / 115; 32768, 512x16 61, 1024x8 105.
 template <class T, int TPR, int NV, int BLOCK, bool Q8>
