@@ -91,13 +91,16 @@ struct SaNumber {
 };
 
 // Weights of a row, 2^S for its maximum, and the bins. The sum with 1.5 * 2^52 leaves the rounded product in the lower bits.
+// Differences are of h x, h being 1, or 1/2 in rows whose largest and smallest number are further apart than their type reaches: an
+// infinite difference would put a number that has weight (at temperatures of the type's largest numbers) among those that have none.
 template <class T>
 struct SaWeight {
-    T max, bins_per;   // bins per unit of x
-    double rate, unit;  // rate: log2(e) / temperature; unit: 2^S, S <= 50
+    T max, bins_per;   // bins per unit of h x
+    double h, per_h, far;      // 1 / h, h max
+    double rate, unit;  // rate: log2(e) / (h temperature); unit: 2^S, S <= 50
     __device__ __forceinline__ double share(T x) const {
         if (x == max) return 1.0;
-        const double e = ((double)x - (double)max) * rate;
+        const double e = __builtin_fma((double)x, h, -far) * rate;
         return e > -70.0 ? exp2_by_table(e, float_tables()) : 0.0;  // (2^-70 and less is less than half of a unit; so is NaN, from -inf * 0)
     }
     __device__ __forceinline__ uint64_t units(double share) const {
@@ -105,7 +108,7 @@ struct SaWeight {
     }
     // falls with x, never out of order: a difference, a product and a cut, each rounded
     __device__ __forceinline__ uint32_t bin(T x) const {
-        const T d = x == max ? (T)0 : (max - x) * bins_per;
+        const T d = x == max ? (T)0 : __builtin_elementwise_fma(x, -(T)h, (T)far) * bins_per;
         return d < (T)(kSaBins - 1) ? (uint32_t)d : (uint32_t)(kSaBins - 1);   // (NaN, from inf * 0: the last)
     }
 };
@@ -291,11 +294,16 @@ struct SaSettings {
         likely = min_p < 1.0 ? min_p : 1.0;
         small = !all && top_k <= kSaSmallK;
         weight.max = m;
-        weight.rate = sa_same(1.44269504088896338700e+00 / temperature);
+        const bool within = (double)m - (double)least <= (sizeof(T) == 4 ? (double)__FLT_MAX__ : __DBL_MAX__);
+        const double h = sa_same(within ? 1.0 : 0.5), per_h = sa_same(within ? 1.0 : 2.0);
+        weight.h = h;
+        weight.per_h = per_h;
+        weight.far = sa_same((double)m * h);
+        weight.rate = sa_same(1.44269504088896338700e+00 / temperature * per_h);
         weight.unit = __longlong_as_double((long long)(1023 + p.unit_bits) << 52);
         // bins of 1/48 of a factor e, or finer ones where the row's numbers span less than the bins then reach
-        const double per = kSaBinsPerNat / temperature, span = (double)m - (double)least, most = sizeof(T) == 4 ? 1e37 : 1e300;
-        weight.bins_per = sa_same((T)(span * per < (double)(kSaBins - 2) ? __builtin_fmin((double)(kSaBins - 2) / span, most) : per));   // (span 0: one number)
+        const double per = kSaBinsPerNat / temperature * per_h, span = (double)m * h - (double)least * h, most = sizeof(T) == 4 ? 1e37 : 1e300;
+        weight.bins_per = sa_same((T)__builtin_fmin(span * per < (double)(kSaBins - 2) ? (double)(kSaBins - 2) / span : per, most));   // (span 0: one number)
         bin_size = sa_same(1.0 / (double)weight.bins_per);
     }
 };
@@ -491,10 +499,10 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
     // of a bin, and the bounds' keeps the order.)
     auto most_of = [&](uint32_t from) {
         const double above = from == 0 ? -INFINITY : ((double)from - 0.5) * s.bin_size;
-        return (T)((double)weight.max - above);
+        return (T)((weight.far - above) * weight.per_h);
     };
     auto least_of = [&](uint32_t to) {
-        const double lowest = (double)weight.max - ((double)to + 1.5) * s.bin_size;
+        const double lowest = (weight.far - ((double)to + 1.5) * s.bin_size) * weight.per_h;
         return to < kSaBins - 1 && lowest == lowest ? (T)lowest : (T)-INFINITY;
     };
 
@@ -565,9 +573,9 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         __syncthreads();
         return at;
     };
-    // the bin in which the running sum passes t; kSaBins where it does not
+    // the bin in which the running sum passes t; the last one where it does not
     auto bin_of = [&](bool by_weight, uint64_t t) {
-        if (tid == 0) found[0] = kSaBins;
+        if (tid == 0) found[0] = kSaBins - 1;
         __syncthreads();
 #pragma unroll
         for (uint32_t k = 0; k < 2; ++k) {
@@ -746,7 +754,7 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
         uint32_t b = kSaBins;
         if (!digits && !(small && by_weight)) {
             b = bin_of(by_weight, t);
-            if (b >= kSaBins - 1 && !small) continue;   // (a count that reaches what has no weight: everything that has is in front of it)
+            if (stage == 0 && b == kSaBins - 1 && !small) continue;   // (a count that reaches what has no weight: everything that has is in front of it)
             if (b < lo || b > hi) {
                 bool few;
                 if (s.all) {

@@ -291,3 +291,44 @@ def test_more_numbers_together_than_are_put_in_order(dt, n):
         for settings in ({}, {"top_k": 5}, {"top_k": 300}, {"top_k": 300, "min_p": 1e-5}, {"top_k": n // 2}, {"top_p": 0.9}, {"top_k": n // 3, "top_p": 0.7},
                          {"top_k": 400, "top_p": 0.8, "min_p": 1e-4}, {"min_p": 1e-5}, {"top_k": n // 2 + 40}):
             assert (take(m, x, us, dt, **settings) == chosen(x, us, **settings)).all(), (u, settings)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n", [2, 70, 5000, 70001])
+def test_logits_further_apart_than_their_type_reaches(dt, n):
+    """Differences beyond the type's largest number, at temperatures at which such logits still have weights. Logits and
+    temperature are a quarter of themselves for the definition, which goes by their quotients alone."""
+    import cumo_amd as m
+    rng = np.random.default_rng(n)
+    top = float(np.finfo(dt).max)
+    x = np.empty((5, n), dt)
+    x[0] = np.where(np.arange(n) % 2, -0.9, 0.9) * top
+    x[1] = -top
+    x[1, n // 2] = 0.3 * top
+    x[2] = rng.uniform(-1, 1, n) * top
+    x[3] = -top
+    x[3, ::3] = top
+    x[4] = rng.standard_normal(n)
+    x[4, n // 3] = -top
+    x[4, n - 1] = top
+    for u in (0.02, 0.4, 0.75, 0.999):
+        us = np.full(5, u, dt)
+        for temperature in (float("inf"), top, top / 3, top / 60, 1.0):
+            for settings in ({}, {"top_k": 1 << 20}, {"top_k": 600}, {"top_k": 300}, {"top_p": 0.9}, {"top_p": 0.3}, {"min_p": 0.2}, {"top_k": n - 1, "top_p": 0.7, "min_p": 0.01}):
+                got = take(m, x, us, dt, temperature=temperature, **settings)
+                want = chosen(x.astype(np.float64) / 4, us, temperature=temperature / 4, **settings)
+                assert (got == want).all(), (u, temperature, settings, got, want)
+
+
+@pytest.mark.parametrize("n", [2, 900, 20001])
+def test_logits_of_the_size_of_the_smallest_normal_numbers(n):
+    """Temperatures so small that a bin for each 48th of one is more bins a unit than SFloat counts."""
+    import cumo_amd as m
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal((4, n)) * 1e-36).astype(np.float32)
+    x[3, 0] = 7.0
+    for u in (0.1, 0.6, 0.95):
+        us = np.full(4, u, np.float32)
+        for settings in ({}, {"top_k": 700}, {"top_k": 40}, {"top_p": 0.8}, {"min_p": 0.05}):
+            for temperature in (1e-37, 1e-36, 1e-38):
+                assert (take(m, x, us, np.float32, temperature=temperature, **settings) == chosen(x, us, temperature=temperature, **settings)).all(), (u, settings)
