@@ -8,10 +8,8 @@
 // and stretches join: (A1, B1) then (A2, B2) is (A1 A2, A2 B1 + B2). Lanes and waves hold stretches side by side in registers,
 // hand on A and B, and then take their own steps from the state that reaches them, each step the one fused multiply-add of the
 // definition: a lane's states are those of one step after the other from where its stretch begins, only what reaches it has
-// gone through joins. A is carried in double whatever the type: products of float gates leave float's range long before the
-// states do. From a state of zero a stretch leads to B whatever A is (infinite, say), so joins take B there. A product of
-// gates that are not 0 can still be too small for double; it is then held at double's smallest number, kTooSmall, whatever comes
-// after it: finite states have vanished by then, and infinite ones are infinite still, which 0 would make NaN.
+// gone through joins. Products of gates leave the type's range long before the states do: A is a double for SFloat and a double with an
+// exponent of its own for DFloat (ReGates).
 //
 // Two layouts. Down columns (time across memory): a lane a column, 64 columns a wave, a wave's rows in registers, the waves of
 // a block one behind the other in time. Along rows (time along memory): a lane a stretch of 64 bytes.
@@ -38,25 +36,132 @@ struct ReArgs {
     uint64_t before;   // columns of the launches in front of this one
 };
 
-constexpr double kTooSmall = 4.9406564584124654e-324;
-// A of a stretch whose gates multiply up to `product`, `least` being the smallest magnitude of them
-template <class T>
-__device__ __forceinline__ double re_gates(double product, T least) {
-    return product == 0.0 && least != (T)0 ? __builtin_copysign(kTooSmall, product) : product;
-}
-// A of two stretches, one after the other
-__device__ __forceinline__ double re_product(double earlier, double later) {
-    const double both = earlier * later;
-    const double held = __builtin_copysign(kTooSmall, both);
-    if (__builtin_fabs(earlier) == kTooSmall) return later == 0.0 || later != later ? both : held;
-    return both == 0.0 && earlier != 0.0 && later != 0.0 ? held : both;
-}
+// the smaller magnitude
+__device__ __forceinline__ float re_less(float least, float a) { return __builtin_fminf(least, __builtin_fabsf(a)); }
+__device__ __forceinline__ double re_less(double least, double a) { return __builtin_fmin(least, __builtin_fabs(a)); }
 
-template <class T>
-__device__ __forceinline__ T re_join(double product, T reached, T state) {
-    const bool gone = state == (T)0 || (__builtin_fabs(product) == kTooSmall && __builtin_fabs((double)state) < INFINITY);
-    return gone ? reached : (T)__builtin_fma(product, (double)state, (double)reached);
-}
+// A: the product of a stretch's gates, always a finite number: infinite and NaN gates show in B, which they reach from zero as well.
+template <class T> struct ReGates;
+
+// SFloat: in double. Beyond 2^+-300 nothing is left of a finite state, or it is infinite, and neither changes with the gates that come
+// after, but for one of 0, which forgets either. So a product out there stays as it is but for its sign, or becomes 0.
+template <> struct ReGates<float> {
+    static constexpr int W = 2;   // words
+    double product;
+    // (0 too)
+    __device__ __forceinline__ static bool out(double v, int reach) { return (((uint32_t)__double2hiint(v) >> 20) & 0x7ffu) - (uint32_t)(1023 - reach) > 2u * reach; }
+    __device__ __forceinline__ static ReGates none() { return {1.0}; }
+    template <bool BACK, int N>   // (BACK: in the order of falling j)
+    __device__ __forceinline__ static ReGates of(const float (&a)[N]) {
+        double own = 1.0;
+        float least = 1.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            own *= (double)a[BACK ? N - 1 - j : j];
+            least = re_less(least, a[j]);
+        }
+        if (out(own, 600) && !(own == 0.0 && least == 0.0f)) {   // (rare; it may have been out of double's range in between)
+            double m = 1.0;
+            int e = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                m *= (double)__builtin_amdgcn_frexp_mantf(a[j]);
+                e += __builtin_amdgcn_frexp_expf(a[j]);
+            }
+            own = __builtin_fabs(m) <= 1.0 ? ldexp(m, e < -600 ? -600 : e > 600 ? 600 : e) : 0x1p600;
+        }
+        return {own};
+    }
+    // of two stretches, one after the other
+    __device__ __forceinline__ ReGates then(ReGates after) const {
+        const bool far = out(product, 300), far_after = out(after.product, 300);
+        const double x = far_after && !far ? __builtin_copysign(1.0, product) : product;
+        const double y = far && after.product != 0.0 ? __builtin_copysign(1.0, after.product) : after.product;
+        return {x * y};
+    }
+    __device__ __forceinline__ float join(float reached, float state) const { return (float)__builtin_fma(product, (double)state, (double)reached); }
+    __device__ __forceinline__ ReGates whole() const { return *this; }
+    __device__ __forceinline__ ReGates of_lane_below(int d) const { return {__shfl_up(product, d)}; }
+    __device__ __forceinline__ void to(uint32_t* w) const {
+        const uint64_t bits = (uint64_t)__double_as_longlong(product);
+        w[0] = (uint32_t)bits;
+        w[1] = (uint32_t)(bits >> 32);
+    }
+    __device__ __forceinline__ static ReGates from(const uint32_t* w) { return {__longlong_as_double((long long)(((uint64_t)w[1] << 32) | w[0]))}; }
+};
+
+// DFloat: m 2^e, as a state may be small where a product is large, or large where it is small, and stay finite. m is 0, or
+// at least 1/2 and less than 1 where it is whole(), half as much for each stretch that has come behind it since.
+template <> struct ReGates<double> {
+    static constexpr int W = 3;
+    static constexpr int kFar = 1 << 28;   // (of no account beyond 2^12: numbers reach from 2^-1074 to 2^1024)
+    double m;
+    int e;
+    __device__ __forceinline__ static ReGates none() { return {1.0, 0}; }
+    __device__ __forceinline__ ReGates whole() const { return {__builtin_amdgcn_frexp_mant(m), e + __builtin_amdgcn_frexp_exp(m)}; }
+    template <bool BACK, int N>
+    __device__ __forceinline__ static ReGates of(const double (&a)[N]) {
+        double own = 1.0, least = 1.0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            own *= a[BACK ? N - 1 - j : j];
+            least = re_less(least, a[j]);
+        }
+        ReGates all = {own, 0};
+        const double size = __builtin_fabs(own);
+        if (!(size < 0x1p1000) || (size < 0x1p-1000 && !(own == 0.0 && least == 0.0))) {   // (rare)
+            all = none();
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                all.m *= __builtin_amdgcn_frexp_mant(a[BACK ? N - 1 - j : j]);
+                all.e += __builtin_amdgcn_frexp_exp(a[j]);
+            }
+            if (!(__builtin_fabs(all.m) <= 1.0)) all = {1.0, kFar};
+        }
+        return all.whole();
+    }
+    __device__ __forceinline__ ReGates then(ReGates after) const {
+        const int both = e + after.e;
+        return {m * after.m, both < -kFar ? -kFar : both > kFar ? kFar : both};
+    }
+    __device__ __forceinline__ double join(double reached, double state) const {
+        const int near = e < -900 ? -900 : e > 900 ? 900 : e;   // (m has up to 65 halves: the product below is a normal number)
+        double there = state;
+        if (e != near && m != 0.0) there = ldexp(state, e - near);   // (rare)
+        return __builtin_fma(ldexp(m, near), there, reached);
+    }
+    __device__ __forceinline__ ReGates of_lane_below(int d) const { return {__shfl_up(m, d), __shfl_up(e, d)}; }
+    __device__ __forceinline__ void to(uint32_t* w) const {
+        const uint64_t bits = (uint64_t)__double_as_longlong(m);
+        w[0] = (uint32_t)bits;
+        w[1] = (uint32_t)(bits >> 32);
+        w[2] = (uint32_t)e;
+    }
+    __device__ __forceinline__ static ReGates from(const uint32_t* w) {
+        return {__longlong_as_double((long long)(((uint64_t)w[1] << 32) | w[0])), (int)w[2]};
+    }
+};
+
+// Products of N stretches in shared memory, for joins alone. A DFloat one is held as a plain double where it is one, and looked up where
+// that is NaN: [4,4096,2048] walked 190 us, 204 with all of them as m and e (tiles, which multiply them too: [1,65536,1000] 381 and 368).
+template <class T, int N> struct ReShelf {
+    double plain[N];
+    __device__ __forceinline__ void put(int at, ReGates<T> g) { plain[at] = g.product; }
+    __device__ __forceinline__ T join(int at, T reached, T state) const { return ReGates<T>{plain[at]}.join(reached, state); }
+};
+template <int N> struct ReShelf<double, N> {
+    double plain[N];
+    ReGates<double> other[N];
+    __device__ __forceinline__ void put(int at, ReGates<double> g) {
+        const bool is = (g.e >= -900 && g.e <= 900) || g.m == 0.0;
+        plain[at] = is ? ldexp(g.m, g.e) : __builtin_nan("");
+        if (!is) other[at] = g;
+    }
+    __device__ __forceinline__ double join(int at, double reached, double state) const {
+        const double a = plain[at];
+        return a == a ? __builtin_fma(a, state, reached) : other[at].join(reached, state);
+    }
+};
 
 // one step, in place: (a, b) forwards makes b the state; backwards (a, g, h before) makes g the l and h the gate's gradient.
 // Both leave what is carried on in `state`.
@@ -70,9 +175,6 @@ __device__ __forceinline__ void re_step(T a, T& b, T& h, T& state) {
         b = state = __builtin_elementwise_fma(a, state, b);
     }
 }
-// the smaller magnitude
-__device__ __forceinline__ float re_less(float least, float a) { return __builtin_fminf(least, __builtin_fabsf(a)); }
-__device__ __forceinline__ double re_less(double least, double a) { return __builtin_fmin(least, __builtin_fabs(a)); }
 template <class T, bool GRAD>
 __device__ __forceinline__ T re_carry(T a, T b, T state) {
     if constexpr (GRAD) return a * (b + state);
@@ -150,16 +252,11 @@ struct ReTile {
             }
         }
     }
-    __device__ __forceinline__ void sum_up(double& product, T& reached) const {
-        double own = 1.0;
-        T least = (T)1;
+    __device__ __forceinline__ void sum_up(ReGates<T>& product, T& reached) const {
+        reached = (T)0;
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            own *= (double)a[j];
-            least = re_less(least, a[j]);
-            reached = re_carry<T, GRAD>(a[j], b[j], reached);
-        }
-        product = re_product(product, re_gates(own, least));
+        for (int j = 0; j < R; ++j) reached = re_carry<T, GRAD>(a[j], b[j], reached);
+        product = ReGates<T>::template of<false>(a);
     }
     template <ReStore FORM>
     __device__ __forceinline__ void take(const ReArgs& p, const ReLanes& lout, const ReLanes& lgb, uint64_t t, uint64_t to, bool there, T& state) {
@@ -188,7 +285,7 @@ __global__ __launch_bounds__(NW * 64) void recurrence_columns_kernel(ReArgs p) {
     typedef ReTile<T, GRAD> Tile;
     constexpr int R = Tile::R;
     constexpr uint64_t kTile = (uint64_t)NW * R;
-    __shared__ double products[2][NW][64];
+    __shared__ ReShelf<T, NW * 64> products[2];
     __shared__ T reached[2][NW][64];
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint64_t mine = p.before + (uint64_t)blockIdx.x * 64 + lane;
@@ -203,16 +300,16 @@ __global__ __launch_bounds__(NW * 64) void recurrence_columns_kernel(ReArgs p) {
     auto walk = [&](Tile& tile, uint64_t t) {   // t: of the wave's first row
         T own = state;
         if constexpr (NW > 1) {
-            double product = 1.0;
-            T b = (T)0;
+            ReGates<T> product;
+            T b;
             tile.sum_up(product, b);
-            products[turn][wave][lane] = product;
+            products[turn].put((int)threadIdx.x, product);
             reached[turn][wave][lane] = b;
             __syncthreads();   // (the other half of the slots is what a wave may still be reading)
 #pragma unroll
             for (uint32_t w = 0; w < NW; ++w) {
                 own = w == wave ? state : own;
-                state = re_join(products[turn][w][lane], reached[turn][w][lane], state);
+                state = products[turn].join((int)(w * 64 + lane), reached[turn][w][lane], state);
             }
             turn ^= 1;
         }
@@ -252,7 +349,7 @@ struct ReChain {
     uint32_t tiles;   // of a strip of columns, or of a row
 };
 
-template <class T> constexpr int kReWords = sizeof(T) == 4 ? 4 : 6;   // of a tile and column: its state, its B, its A
+template <class T> constexpr int kReWords = (int)(2 * sizeof(T) / 4) + ReGates<T>::W;   // of a tile and column: its state, its A, its B
 
 template <int W>
 __device__ __forceinline__ void re_publish(uint64_t* slot, uint32_t stride, const uint32_t (&v)[W]) {
@@ -276,33 +373,38 @@ __device__ __forceinline__ bool re_peek(const uint64_t* slot, uint32_t stride, u
 // the words of one tile and column (or row), `stride` words from one to the next
 template <class T>
 struct ReSlot {
-    static constexpr int W = (int)(sizeof(T) / 4);
-    union State { T t; uint32_t w[W]; };
-    union Sum { struct { double product; T reached; } t; uint32_t w[2 + W]; };
+    static constexpr int W = (int)(sizeof(T) / 4), G = ReGates<T>::W;
+    union Number { T t; uint32_t w[W]; };
     uint64_t* at;
     uint32_t stride;
     __device__ __forceinline__ void put_state(T v) const {
-        State s;
+        Number s;
         s.t = v;
         re_publish<W>(at, stride, s.w);
     }
-    __device__ __forceinline__ void put_sum(double product, T reached) const {
-        Sum s;
-        s.t.product = product;
-        s.t.reached = reached;
-        re_publish<2 + W>(at + (uint64_t)W * stride, stride, s.w);
+    __device__ __forceinline__ void put_sum(ReGates<T> product, T reached) const {
+        uint32_t w[G + W];
+        Number s;
+        s.t = reached;
+        product.whole().to(w);
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[G + i] = s.w[i];
+        re_publish<G + W>(at + (uint64_t)W * stride, stride, w);
     }
     __device__ __forceinline__ bool state(T& v) const {
-        State s;
+        Number s;
         const bool is = re_peek<W>(at, stride, s.w);
         v = s.t;
         return is;
     }
-    __device__ __forceinline__ bool sum(double& product, T& reached) const {
-        Sum s;
-        const bool is = re_peek<2 + W>(at + (uint64_t)W * stride, stride, s.w);
-        product = s.t.product;
-        reached = s.t.reached;
+    __device__ __forceinline__ bool sum(ReGates<T>& product, T& reached) const {
+        uint32_t w[G + W];
+        const bool is = re_peek<G + W>(at + (uint64_t)W * stride, stride, w);
+        Number s;
+#pragma unroll
+        for (int i = 0; i < W; ++i) s.w[i] = w[G + i];
+        product = ReGates<T>::from(w);
+        reached = s.t;
         return is;
     }
 };
@@ -317,7 +419,7 @@ template <class T, bool GRAD>
 __global__ __launch_bounds__(kReChainWaves * 64, sizeof(T) == 4 ? 8 : 4) void recurrence_columns_chain_kernel(ReArgs p, ReChain chain) {
     typedef ReTile<T, GRAD> Tile;
     constexpr int NW = kReChainWaves, R = Tile::R;
-    __shared__ double products[NW][64], before_product[NW][64];
+    __shared__ ReGates<T> products[NW][64], before_product[NW][64];
     __shared__ T reached[NW][64], before_reached[NW][64];   // (of a tile whose state is there: that)
     __shared__ uint32_t is_state[NW], ticket;
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -336,8 +438,8 @@ __global__ __launch_bounds__(kReChainWaves * 64, sizeof(T) == 4 ? 8 : 4) void re
         const ReLanes la(p.a, o, i, p.a_step), lb(p.b, o, i, p.b_step), lh(GRAD ? p.h : p.a, o, i, GRAD ? p.h_step : p.a_step);
         tile.template load<false>(p, la, lb, lh, t, first);
     }
-    double product = 1.0;
-    T b = (T)0;
+    ReGates<T> product;
+    T b;
     tile.sum_up(product, b);
     products[wave][lane] = product;
     reached[wave][lane] = b;
@@ -348,14 +450,14 @@ __global__ __launch_bounds__(kReChainWaves * 64, sizeof(T) == 4 ? 8 : 4) void re
     if (wave == 0) {
 #pragma unroll
         for (int w = 1; w < NW; ++w) {
-            b = re_join(products[w][lane], reached[w][lane], b);
-            product = re_product(product, products[w][lane]);
+            b = products[w][lane].join(reached[w][lane], b);
+            product = product.then(products[w][lane]);
         }
         if (k > 0) slot(k).put_sum(product, b);
     }
     // the tile `wave` + 1 before this one: its state, or what it makes of one
     auto look = [&](bool want_state) {
-        double found_product = 1.0;
+        ReGates<T> found_product = ReGates<T>::none();
         T found = GRAD ? (T)0 : first;   // (before the first tile)
         bool state = true;
         if (k >= wave + 1) {
@@ -389,9 +491,9 @@ __global__ __launch_bounds__(kReChainWaves * 64, sizeof(T) == 4 ? 8 : 4) void re
     }
     near = __builtin_amdgcn_readfirstlane(near);
     T state = before_reached[near][lane];
-    for (int w = near - 1; w >= 0; --w) state = re_join(before_product[w][lane], before_reached[w][lane], state);
-    if (wave == 0 && k + 1 < chain.tiles) slot(k).put_state(re_join(product, b, state));
-    for (uint32_t w = 0; w < wave; ++w) state = re_join(products[w][lane], reached[w][lane], state);
+    for (int w = near - 1; w >= 0; --w) state = before_product[w][lane].join(before_reached[w][lane], state);
+    if (wave == 0 && k + 1 < chain.tiles) slot(k).put_state(product.join(b, state));
+    for (uint32_t w = 0; w < wave; ++w) state = products[w][lane].join(reached[w][lane], state);
     const ReLanes lout(p.out, o, i, p.out_step), lgb(GRAD ? p.gb : p.out, o, i, GRAD ? p.gb_step : p.out_step);
     tile.template take<RE_AWAY>(p, lout, lgb, t, p.time, there, state);
     if (GRAD && p.last && there && t < p.time && t + R >= p.time) reinterpret_cast<T*>(p.last)[c] = state;   // (carried past the last step)
@@ -459,17 +561,14 @@ struct ReStretch {
             }
         }
     }
-    __device__ __forceinline__ void sum_up(double& product, T& reached) const {
-        double own = 1.0;
-        T least = (T)1;
+    __device__ __forceinline__ void sum_up(ReGates<T>& product, T& reached) const {
+        reached = (T)0;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const int j = GRAD ? E - 1 - i : i;
-            own *= (double)a.t[j];
-            least = re_less(least, a.t[j]);
             reached = re_carry<T, GRAD>(a.t[j], b.t[j], reached);
         }
-        product = re_product(product, re_gates(own, least));
+        product = ReGates<T>::template of<GRAD>(a.t);
     }
     __device__ __forceinline__ T take(T state) {   // the state that is carried past it
 #pragma unroll
@@ -495,17 +594,18 @@ struct ReStretch {
 
 // joins of L lanes' stretches in the lanes' order: what stands before a lane's (product, reached)
 template <class T, int L>
-__device__ __forceinline__ void re_scan_lanes(double& product, T& reached) {
+__device__ __forceinline__ void re_scan_lanes(ReGates<T>& product, T& reached) {
     const int lane = (int)(threadIdx.x & 63) & (L - 1);
 #pragma unroll
     for (int d = 1; d < L; d <<= 1) {
-        const double before = __shfl_up(product, d);
+        const ReGates<T> before = product.of_lane_below(d);
         const T b = __shfl_up(reached, d);
         if (lane >= d) {
-            reached = re_join(product, reached, b);
-            product = re_product(before, product);
+            reached = product.join(reached, b);
+            product = before.then(product);
         }
     }
+    product = product.whole();
 }
 
 template <class T>
@@ -541,14 +641,14 @@ __global__ __launch_bounds__(kReBlock) void recurrence_short_rows_kernel(ReArgs 
         Stretch s;
         s.load(p, row.a, row.b, row.h, t, to, first);
         T state = GRAD ? (T)0 : first;
-        double product = 1.0;
-        T reached = (T)0;
+        ReGates<T> product;
+        T reached;
         if constexpr (L > 1) {
             s.sum_up(product, reached);
             re_scan_lanes<T, L>(product, reached);
         }
-        const T end = L > 1 ? re_join(product, reached, state) : state;   // after this lane's stretch
         if constexpr (L > 1) {
+            const T end = product.join(reached, state);   // after this lane's stretch
             const T before = __shfl_up(end, 1);
             state = lane > 0 ? before : state;
         }
@@ -565,7 +665,7 @@ __global__ __launch_bounds__(kReBlock) void recurrence_rows_kernel(ReArgs p) {
     typedef ReStretch<T, GRAD> Stretch;
     constexpr uint64_t kTile = (uint64_t)kReBlock * Stretch::E;
     constexpr int NW = kReBlock / 64;
-    __shared__ double products[2][NW];
+    __shared__ ReGates<T> products[2][NW];
     __shared__ T reached[2][NW];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (uint64_t c = blockIdx.x; c < p.columns; c += gridDim.x) {
@@ -577,8 +677,8 @@ __global__ __launch_bounds__(kReBlock) void recurrence_rows_kernel(ReArgs p) {
             const uint64_t t = at + (uint64_t)threadIdx.x * Stretch::E;
             Stretch s;
             s.load(p, row.a, row.b, row.h, t, p.time, first);
-            double product = 1.0;
-            T b = (T)0;
+            ReGates<T> product;
+            T b;
             s.sum_up(product, b);
             re_scan_lanes<T, 64>(product, b);
             if (lane == 63) {
@@ -590,10 +690,10 @@ __global__ __launch_bounds__(kReBlock) void recurrence_rows_kernel(ReArgs p) {
 #pragma unroll
             for (uint32_t w = 0; w < NW; ++w) {
                 own = w == wave ? state : own;
-                state = re_join(products[turn][w], reached[turn][w], state);
+                state = products[turn][w].join(reached[turn][w], state);
             }
             turn ^= 1;
-            const T reach = re_join(product, b, own);   // after this lane's stretch
+            const T reach = product.join(b, own);   // after this lane's stretch
             const T before = __shfl_up(reach, 1);
             own = s.take(lane > 0 ? before : own);
             if (GRAD && p.last && t < p.time && t + Stretch::E >= p.time) reinterpret_cast<T*>(p.last)[c] = own;
@@ -619,7 +719,7 @@ template <class T, bool GRAD>
 __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kernel(ReArgs p, ReChain chain) {
     typedef ReStretch<T, GRAD> Stretch;
     constexpr int NW = kReChainWaves;
-    __shared__ double products[NW];
+    __shared__ ReGates<T> products[NW];
     __shared__ T reached[NW], start;
     __shared__ uint32_t ticket;
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -632,8 +732,8 @@ __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kern
     const uint64_t t = ((uint64_t)k * (NW * 64) + threadIdx.x) * Stretch::E;
     Stretch s;
     s.load(p, row.a, row.b, row.h, t, p.time, first);
-    double product = 1.0;
-    T b = (T)0;
+    ReGates<T> product;
+    T b;
     s.sum_up(product, b);
     re_scan_lanes<T, 64>(product, b);
     if (lane == 63) {
@@ -643,12 +743,12 @@ __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kern
     __syncthreads();
     auto slot = [&](uint32_t tile_number) { return ReSlot<T>{chain.words + (c * chain.tiles + tile_number) * kReWords<T>, 1}; };
     if (wave == 0) {
-        double all = products[0];
+        ReGates<T> all = products[0];
         T end = reached[0];
 #pragma unroll
         for (int w = 1; w < NW; ++w) {
-            end = re_join(products[w], reached[w], end);
-            all = re_product(all, products[w]);
+            end = products[w].join(reached[w], end);
+            all = all.then(products[w]);
         }
         if (lane == 0 && k > 0 && k + 1 < chain.tiles) slot(k).put_sum(all, end);
         T state = GRAD ? (T)0 : first;
@@ -659,7 +759,7 @@ __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kern
             const uint32_t limit = wait_limit(chain.wait, kReLooks);
             bool have_state = false, have_sum = false;
             T found_state = (T)0, found = (T)0;
-            double found_product = 1.0;
+            ReGates<T> found_product = ReGates<T>::none();
             int near;
             for (uint32_t looks = 0;; ++looks) {
                 if (asks && !have_state) have_state = from.state(found_state);
@@ -678,17 +778,17 @@ __global__ __launch_bounds__(kReChainWaves * 64) void recurrence_rows_chain_kern
             // (a tile whose state came first and sum was never asked for: only the nearest such is used, as a state)
             near = __builtin_amdgcn_readfirstlane(near);
             state = re_lane(found_state, near);
-            for (int l = near - 1; l >= 0; --l) state = re_join(re_lane(found_product, l), re_lane(found, l), state);
+            for (int l = near - 1; l >= 0; --l) state = re_lane(found_product, l).join(re_lane(found, l), state);
         }
         if (lane == 0) {
             start = state;
-            if (k + 1 < chain.tiles) slot(k).put_state(re_join(all, end, state));
+            if (k + 1 < chain.tiles) slot(k).put_state(all.join(end, state));
         }
     }
     __syncthreads();
     T state = start;
-    for (uint32_t w = 0; w < wave; ++w) state = re_join(products[w], reached[w], state);
-    const T reach = re_join(product, b, state);
+    for (uint32_t w = 0; w < wave; ++w) state = products[w].join(reached[w], state);
+    const T reach = product.join(b, state);
     const T before = __shfl_up(reach, 1);
     state = s.take(lane > 0 ? before : state);
     if (GRAD && p.last && t < p.time && t + Stretch::E >= p.time) reinterpret_cast<T*>(p.last)[c] = state;
@@ -738,7 +838,7 @@ int re_chain(const ReArgs& p, uint64_t lines, uint64_t tile, hipStream_t stream)
         return CUMO_HIP_ERROR_RUNTIME;
     }
     chain.tiles = (uint32_t)((p.time + tile - 1) / tile);
-    const uint64_t words = lines * chain.tiles * kReWords<T> * (ROWS ? 1 : 64) + 2;   // (an even number, the ticket among the last two)
+    const uint64_t words = (lines * chain.tiles * kReWords<T> * (ROWS ? 1 : 64) + 2) & ~1ull;   // (an even number, the ticket behind the tiles')
     char* memory = cumo_cuda_runtime_malloc(words * sizeof(uint64_t));
     if (!memory) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
     chain.words = reinterpret_cast<uint64_t*>(memory);

@@ -302,9 +302,11 @@ int cumo_hip_na_rmsnorm_grad(const cumo_hip_narray_t* g, const cumo_hip_narray_t
 /* recurrence: h[t] = a[t] * h[t-1] + b[t] along one axis; a, b and h have one shape, h0 (NULL:
  * zeros) that shape without the axis. Long axes are cut where there are few runs side by side
  * and the parts joined by the products of their a: the same bits on every call, not those of one
- * step after the other. The products are carried in double: a part whose |a| multiply up beyond
- * 1.8e308 gives infinities where a small state would not have become one, and from a part where they
- * fall below 5e-324 on nothing is left of a finite state, whatever comes after it.
+ * step after the other. The products reach further than the type does, so that states are finite
+ * where the steps of the operands' magnitudes are (those may cancel out of infinity; parts do not).
+ * A gate of 0 forgets what comes before it, a state within its
+ * part that had become infinite too (which step by step is NaN from there on); an infinite gate
+ * leaves infinities or NaN.
  * recurrence_grad: from g (of h): ga, gb and gh0 (NULL when h0 is). */
 int cumo_hip_na_recurrence(const cumo_hip_narray_t* a, const cumo_hip_narray_t* b, const cumo_hip_narray_t* h0, int axis, cumo_hip_narray_t* h);
 int cumo_hip_na_recurrence_grad(const cumo_hip_narray_t* g, const cumo_hip_narray_t* a, const cumo_hip_narray_t* h,

@@ -379,3 +379,91 @@ def test_more_columns_than_a_launch_has_lanes():
         got, gb = ga[:, s].to_numpy(), out[:, s].to_numpy()
         assert (gb[1] == 3.0).all() and (gb[0] == 4.5).all()
         assert (got[1] == -6.0).all() and (got[0] == 0.0).all()
+
+
+def one_by_one(a, b, h0):
+    """States along axis 0 in the arrays' own type."""
+    h, state = np.empty_like(b), h0
+    with np.errstate(over="ignore", invalid="ignore"):
+        for t in range(len(b)):
+            state = h[t] = a[t] * state + b[t]
+    return h
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape,axis", LONG + [((1, 1200, 12800), 1), ((300, 3000), 1)])
+def test_gates_of_zero_beside_products_beyond_double(dt, shape, axis):
+    """What a gate of 0 forgets does not come back, however large the products of the gates after it, or before it; steps'
+    own values are finite all along. They are exact, too: every product here is one of powers of two, or with 0."""
+    import cumo_amd as m
+    cls = cls_of(m, dt)
+    n = shape[axis]
+    f = lambda v: np.moveaxis(v, axis, 0)  # noqa: E731
+    h0 = np.ones(f(np.empty(shape, dt)).shape[1:], dt)
+    for gate in (4.0, 16.0, -16.0):
+        for at in (0, 5, 31):
+            a, b = np.full(shape, gate, dt), np.zeros(shape, dt)
+            f(a)[at] = 0
+            want = one_by_one(f(a), f(b), h0)
+            assert np.isfinite(want).all()
+            assert (f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(h0), axis=axis).to_numpy()) == want).all(), (gate, at)
+            # backwards: a gradient at the last step alone, and a gate of 0 a few steps before it
+            f(a)[at], f(a)[n - 1 - at] = gate, 0
+            f(b)[n - 1] = 1
+            h = np.ones(shape, dt)
+            ga, gb, g0 = m.Fused.recurrence_grad(cls.cast(b), cls.cast(a), cls.cast(h), cls.cast(h0), axis=axis)
+            after = np.concatenate([f(a)[1:], np.zeros_like(f(a)[:1])])
+            want = one_by_one(after[::-1], f(b)[::-1], np.zeros_like(h0))[::-1]
+            assert np.isfinite(want).all() and (f(gb.to_numpy()) == want).all() and (f(ga.to_numpy()) == want).all(), (gate, at)
+            assert (g0.to_numpy() == (0 if n > at + 1 else f(a)[0] * want[0])).all()
+    if dt == np.float64:
+        # a small state through gates whose product is beyond double, and forgotten after that
+        for first, second, last in ((1, 2, 3), (1, 40, 70), (40, 41, 90)):
+            a, b = np.ones(shape, dt), np.zeros(shape, dt)
+            f(a)[first] = f(a)[second] = 2.0 ** 660
+            f(a)[last] = 0
+            f(b)[n - 1] = 5
+            h0[...] = 2.0 ** -990
+            want = one_by_one(f(a), f(b), h0)
+            got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(h0), axis=axis).to_numpy())
+            assert np.isfinite(want).all() and (got[last:] == want[last:]).all() and (got[:first] == want[:first]).all(), (first, second, last)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape,axis", LONG)
+def test_largest_numbers_as_gates(dt, shape, axis):
+    """A gate of the type's largest number is a number like any other; an infinite one leaves nothing finite behind."""
+    import cumo_amd as m
+    cls = cls_of(m, dt)
+    n = shape[axis]
+    f = lambda v: np.moveaxis(v, axis, 0)  # noqa: E731
+    a, b = np.ones(shape, dt), np.zeros(shape, dt)
+    h0 = np.full(f(a).shape[1:], 2.0 ** -100, dt)
+    f(a)[n // 2] = np.finfo(dt).max
+    want = one_by_one(f(a), f(b), h0)
+    got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(h0), axis=axis).to_numpy())
+    assert (np.abs(got - want) <= 2 * np.finfo(dt).eps * want).all()
+    f(a)[n // 2] = np.inf
+    got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(h0), axis=axis).to_numpy())
+    assert (got[: n // 2] == h0).all() and not np.isfinite(got[n // 2:]).any()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape,axis", LONG + [((1, 2500, 12800), 1), ((300, 5000), 1)])
+def test_products_beyond_the_type_of_states_within_it(dt, shape, axis):
+    """A large state halved until it is nearly the smallest number and doubled again, a small one the other way, over and
+    over: exact steps, however far their products reach."""
+    import cumo_amd as m
+    cls = cls_of(m, dt)
+    n = shape[axis]
+    f = lambda v: np.moveaxis(v, axis, 0)  # noqa: E731
+    large, small, k = (2.0 ** 110, 2.0 ** -120, 240) if dt == np.float32 else (2.0 ** 1000, 2.0 ** -1010, 2030)
+    for h0, first, second in ((large, 0.5, 2.0), (small, 2.0, 0.5), (-large, -0.5, 2.0)):
+        a, b = np.ones(shape, dt), np.zeros(shape, dt)
+        for at in range(0, n, 2 * k):
+            f(a)[at:at + k], f(a)[at + k:at + 2 * k] = first, second
+        start = np.full(f(a).shape[1:], h0, dt)
+        want = one_by_one(f(a), f(b), start)
+        assert np.isfinite(want).all() and (want != 0).all()
+        got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(start), axis=axis).to_numpy())
+        assert (got == want).all(), (h0, first)
