@@ -332,3 +332,21 @@ def test_logits_of_the_size_of_the_smallest_normal_numbers(n):
         for settings in ({}, {"top_k": 700}, {"top_k": 40}, {"top_p": 0.8}, {"min_p": 0.05}):
             for temperature in (1e-37, 1e-36, 1e-38):
                 assert (take(m, x, us, np.float32, temperature=temperature, **settings) == chosen(x, us, temperature=temperature, **settings)).all(), (u, settings)
+
+
+@pytest.mark.parametrize("dt,margin", [(np.float32, 2.0 ** -37), (np.float64, 2.0 ** -46)])
+def test_weights_are_as_exact_as_the_type(dt, margin):
+    """Two tokens, numbers next to either side of their border. A weight is off by half a unit (2^-51), by what its exponent has been
+    rounded (|z| e^z 2^-52 for z = (x - max) / temperature: 2^-53 at most) and by its exponential: 2^-39 for SFloat, less
+    than 2^-51 for DFloat."""
+    import cumo_amd as m
+    rng = np.random.default_rng(31)
+    x = np.zeros((3000, 2), dt)
+    x[:, 1] = -rng.uniform(0.01, 6, 3000)
+    for temperature in (1.0, 0.37, 2.5):
+        w = np.exp(x[:, 1].astype(np.longdouble) / np.longdouble(temperature))
+        border = 1 / (1 + w)
+        for side, want in ((-1, 0), (1, 1)):
+            u = (border + side * np.longdouble(margin)).astype(np.float64)
+            got = m.Fused.sample(cls_of(m, dt).cast(x), m.DFloat.cast(u), temperature).to_numpy()
+            assert (got == want).all(), (temperature, side, int((got != want).sum()))
