@@ -6,7 +6,9 @@
 // its maximum, the running sum over the bins says in which bin that element is, and the elements of that bin alone (or of all
 // bins up to it, where they are few, as for a small top_k) are put into a list and ordered.
 // Weights are whole numbers, exp((x - max) / temperature) in units of 2^-S with S such that the sum of a row fits 62 bits:
-// sums do not depend on their order, and neither does the answer, although bins are added to by atomics.
+// sums do not depend on their order, and neither does the answer, although bins are added to by atomics. In rows of up to 2^18, S is that
+// of a row whose weights are all the largest; a sum is off by n 2^-(S+1) of that, 2^-27 at most. Longer rows each have an S to what their
+// weights can come to, by the chunks' maxima (256 times the sum at most): a sum is off by n 2^-51 of itself at most.
 //
 // Three launches. The largest and the smallest number of each row's parts, and the largest of every chunk of 64 vectors; the bins of
 // each row's parts, a block to a part with its bins in shared memory; then a block to a row, which adds the parts' bins up, takes
@@ -101,9 +103,9 @@ struct SaWeight {
     __device__ __forceinline__ double share(T x) const {
         if (x == max) return 1.0;
         const double e = __builtin_fma((double)x, h, -far) * rate;
-        if (!(e > -70.0)) return 0.0;  // (2^-70 and less is less than half of a unit; so is NaN, from -inf * 0)
-        if constexpr (sizeof(T) == 4) return exp2_by_table(e, float_tables());   // (to 2^-39; DFloat by it: [256,50001] 71 us, 76)
-        else return exp2(e);
+        // (2^-70 and less is less than half of a unit; so is NaN, from -inf * 0. The table's to 2^-39; DFloat by it: [256,50001] 71 us, 76.)
+        if constexpr (sizeof(T) == 4) return e > -70.0 ? exp2_by_table(e, float_tables()) : 0.0;
+        else return e > -70.0 ? exp2(e) : 0.0;
     }
     __device__ __forceinline__ uint64_t units(double share) const {
         return (uint64_t)__double_as_longlong(__builtin_fma(share, unit, 6755399441055744.0)) & 0x7ffffffffffffull;
@@ -122,6 +124,7 @@ struct SaPart {
 
 struct SaParams : cumo_hip_sample_t {
     int unit_bits;
+    double* units;           // [rows]: 2^S of each row instead, where rows are long; else NULL
     uint32_t looks, fills;   // parts of a row in the first two launches (64 and 16 at most)
     uint32_t chunks;         // of a row: what a wave reads at once
     SaPart* parts;           // [rows][looks]
@@ -302,13 +305,35 @@ struct SaSettings {
         weight.per_h = per_h;
         weight.far = sa_same((double)m * h);
         weight.rate = sa_same(1.44269504088896338700e+00 / temperature * per_h);
-        weight.unit = __longlong_as_double((long long)(1023 + p.unit_bits) << 52);
+        weight.unit = p.units ? sa_same(p.units[row]) : __longlong_as_double((long long)(1023 + p.unit_bits) << 52);
         // bins of 1/48 of a factor e, or finer ones where the row's numbers span less than the bins then reach
         const double per = kSaBinsPerNat / temperature * per_h, span = (double)m * h - (double)least * h, most = sizeof(T) == 4 ? 1e37 : 1e300;
         weight.bins_per = sa_same((T)__builtin_fmin(span * per < (double)(kSaBins - 2) ? (double)(kSaBins - 2) / span : per, most));   // (span 0: one number)
         bin_size = sa_same(1.0 / (double)weight.bins_per);
     }
 };
+
+// 2^S of long rows: a chunk's weights are 256 (DFloat 128) times its largest number's at most
+template <class T>
+__global__ __launch_bounds__(kSaBlock) void sample_unit_kernel(SaParams p, double* units) {
+    __shared__ double slots[kSaBlock / 64];
+    const SaSettings<T> s(p, blockIdx.x);
+    if (s.none || s.greedy) return;   // (nobody asks)
+    constexpr int V = 16 / (int)sizeof(T);
+    const T* chunk_max = reinterpret_cast<const T*>(p.chunk_max) + (uint64_t)blockIdx.x * p.chunks;
+    double most = 0.0;
+    for (uint32_t c = threadIdx.x; c < p.chunks; c += kSaBlock) most += s.weight.share(chunk_max[c]) * kSaChunk<T>;
+    if (threadIdx.x < p.n % V) most += s.weight.share(reinterpret_cast<const T*>(p.x + (int64_t)blockIdx.x * p.x_step)[p.n / V * V + threadIdx.x]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) most += __shfl_xor(most, d);
+    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = most;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < kSaBlock / 64; ++w) most += slots[w];
+    // less than 2^61 of units, and half a unit for each of fewer than 2^31 weights
+    const int bits = 61 - __builtin_amdgcn_frexp_exp(most);
+    units[blockIdx.x] = ldexp(1.0, bits < 50 ? bits : 50);
+}
 
 template <class T>   // (two blocks a compute unit: DFloat's exponential would take 66 registers, [256,50001] 81 us instead of 76)
 __global__ __launch_bounds__(kSaBlock, 8) void sample_fill_kernel(SaParams p) {
@@ -820,6 +845,8 @@ __global__ __launch_bounds__(kSaBlock) void sample_kernel(SaParams p) {
 
 // rows of one round of launches: their bins take 12 to 24 KiB a part
 constexpr uint64_t kSaRows = 4096;
+// rows that are longer have units of their own, for another launch
+constexpr uint64_t kSaLong = 1u << 18;
 
 template <class T>
 int sa_launch(const cumo_hip_sample_t& d, hipStream_t stream) {
@@ -841,18 +868,24 @@ int sa_launch(const cumo_hip_sample_t& d, hipStream_t stream) {
     p.fills = parts(512, 4096, 16);
     p.chunks = (uint32_t)((d.n / (16 / sizeof(T)) + 63) / 64);
     const bool may_count = d.top_k.each || (d.top_k.value > 0.0 && d.top_k.value < (double)d.n);
-    const uint64_t part_bytes = (rows * p.looks * sizeof(SaPart) + 15) & ~15ull, bins = rows * p.fills * kSaBins;
-    char* memory = cumo_cuda_runtime_malloc(part_bytes + (bins + rows * p.fills) * 8 + rows * p.chunks * sizeof(T) + (may_count ? bins * 4 : 0));
+    const uint64_t part_bytes = (rows * p.looks * sizeof(SaPart) + 15) & ~15ull, bins = rows * p.fills * kSaBins, own_units = d.n > kSaLong ? rows : 0;
+    char* memory = cumo_cuda_runtime_malloc(part_bytes + (bins + rows * p.fills + own_units) * 8 + rows * p.chunks * sizeof(T) + (may_count ? bins * 4 : 0));
     if (!memory) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
     p.parts = reinterpret_cast<SaPart*>(memory);
     p.masses = reinterpret_cast<uint64_t*>(memory + part_bytes);
     p.likely = p.masses + bins;
-    p.counts = may_count ? reinterpret_cast<uint32_t*>(p.likely + rows * p.fills) : nullptr;
-    p.chunk_max = reinterpret_cast<char*>(p.likely + rows * p.fills) + (may_count ? bins * 4 : 0);
+    double* const units = reinterpret_cast<double*>(p.likely + rows * p.fills);
+    p.counts = may_count ? reinterpret_cast<uint32_t*>(units + own_units) : nullptr;
+    p.chunk_max = reinterpret_cast<char*>(units + own_units) + (may_count ? bins * 4 : 0);
     cumo_hip_row_number_t* const settings[5] = {&p.u, &p.temperature, &p.top_k, &p.top_p, &p.min_p};
     for (uint64_t done = 0; done < d.rows; done += rows) {
         const unsigned now = (unsigned)(d.rows - done < rows ? d.rows - done : rows);
         hipLaunchKernelGGL((sample_look_kernel<T>), dim3(now, p.looks), dim3(kSaLook), 0, stream, p);
+        if (own_units) {
+            p.units = nullptr;
+            hipLaunchKernelGGL((sample_unit_kernel<T>), dim3(now), dim3(kSaBlock), 0, stream, p, units);
+            p.units = units;
+        }
         hipLaunchKernelGGL((sample_fill_kernel<T>), dim3(now, p.fills), dim3(kSaBlock), 0, stream, p);
         hipLaunchKernelGGL((sample_kernel<T>), dim3(now), dim3(kSaBlock), 0, stream, p);
         p.x += (int64_t)now * p.x_step;

@@ -1235,7 +1235,8 @@ class _Fused:
         of these the ones of weight min_p or more; the answer is the first of those left whose running sum of weights
         exceeds u times theirs. temperature 0 takes the largest. -1 where a row holds a NaN or nothing but -inf. Every
         setting is a number, or an array with one for each row. Weights are within 2^-39 of themselves (DFloat a few 2^-53)
-        and half of a unit, 2^-44 of the largest for rows of up to 2^18 and less for shorter ones."""
+        and half a unit, of 2^-44 of the largest or less in rows of up to 2^18; in longer rows of n, n / 2 units are at most n 2^-51 of
+        their sum."""
         done = _native.sample(x, u, temperature, top_k, top_p, min_p)  # None: the general way
         if done is not None:
             return done

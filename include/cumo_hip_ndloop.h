@@ -317,9 +317,11 @@ int cumo_hip_na_recurrence_grad(const cumo_hip_narray_t* g, const cumo_hip_narra
  * shape: SFloat or DFloat, top_k Int32. Numbers that are NaN, temperature < 0, top_k < 0, or top_p or min_p
  * outside [0, 1] are refused; in arrays, whose values the host does not see, temperature <= 0 or NaN
  * takes the largest, top_k <= 0 and a top_p or min_p that is NaN change nothing, and others are
- * brought into the range. The weights are whole multiples of 2^-44 for rows of up to 2^18 (finer for shorter
- * rows, coarser for longer ones), so their sums, and with them the answer, do not depend on an order. Before it is
- * rounded to that, a weight is within 2^-39 of itself for SFloat logits and a few 2^-53 for DFloat ones. */
+ * brought into the range. The weights are whole multiples of a unit, so their sums, and with them the answer, do not
+ * depend on an order. For rows of n <= 2^18 the unit is 2^-S of the largest weight, S = 62 - ceil(log2 n) and 50 at most: a sum is off by
+ * n 2^-(S+1) of the largest weight, 2^-27 of it at most. Longer rows have a unit to their weights, and a sum is off by
+ * n 2^-51 of itself at most. Before it is rounded to a unit, a weight is within 2^-39 of itself for SFloat logits and a few
+ * 2^-53 for DFloat ones. */
 int cumo_hip_na_sample(const cumo_hip_narray_t* x, const cumo_hip_narray_t* u, double temperature, const cumo_hip_narray_t* temperatures,
                        ssize_t top_k, const cumo_hip_narray_t* top_ks, double top_p, const cumo_hip_narray_t* top_ps,
                        double min_p, const cumo_hip_narray_t* min_ps, cumo_hip_narray_t* z);

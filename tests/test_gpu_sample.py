@@ -350,3 +350,67 @@ def test_weights_are_as_exact_as_the_type(dt, margin):
             u = (border + side * np.longdouble(margin)).astype(np.float64)
             got = m.Fused.sample(cls_of(m, dt).cast(x), m.DFloat.cast(u), temperature).to_numpy()
             assert (got == want).all(), (temperature, side, int((got != want).sum()))
+
+
+def broadcast_row(m, x, u, **settings):
+    """One row of logits for every number of u, without copies of it."""
+    from cumo_amd import _lib
+    x, u = cls_of(m, x.dtype).cast(x), m.DFloat.cast(u)
+    d, du = x._desc(), u._desc()
+    d.ndim = 2
+    d.shape[0], d.shape[1], d.stride[0], d.stride[1] = u.shape[0], x.shape[0], 0, d.stride[0]
+    z = m.Int32(u.shape[0]).fill(-9)
+    dz = z._desc()
+    _lib.call(_lib.lib.cumo_hip_na_sample, C.byref(d), C.byref(du), settings.get("temperature", 1.0), None, settings.get("top_k", 0), None, settings.get("top_p", 1.0), None,
+              settings.get("min_p", 0.0), None, C.byref(dz))
+    return z.to_numpy()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n,low", [((1 << 18) + 1, -32.0), (1 << 20, -30.0), ((1 << 24) + 5, -30.0)])
+def test_long_rows_keep_what_a_flat_tail_holds(dt, n, low):
+    """One token and a flat tail far below it. Either sum that an answer compares is off by n / 2 units at most, the unit being 2^-50 of the
+    largest weight where the row's sum allows it, and by 2^-39 of the tail: so answers are those of numbers that far from u."""
+    import cumo_amd as m
+    x = np.full(n, low, dt)
+    top = n // 3
+    x[top] = 0
+    w = np.exp(np.float64(low))
+    tail = w * (n - 1)
+    u = np.concatenate([[0.0, 0.5, 1 - 2 * tail], 1 - tail * np.array([0.9, 0.5, 0.25, 0.1, 1e-3])])
+    got = broadcast_row(m, x, u)
+    place = np.where(got == top, 0, np.where(got < top, got + 1, got)).astype(np.float64)   # in order of falling x
+    total = 1 + tail
+    begin, end = np.where(place == 0, 0, 1 + (place - 1) * w) / total, (1 + place * w) / total
+    off = 2 * n * 2.0 ** -51 + 2.0 ** -38 * tail
+    assert ((got >= 0) & (begin - off <= u) & (u <= end + off)).all(), (got, begin - u, end - u)
+    assert (got[:2] == top).all() and (got[3:] != top).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n", [(1 << 18) + 1, 1 << 20, (1 << 22) + 77])
+def test_long_rows(dt, n):
+    """Every answer's stretch of the running sum holds u, but for n 2^-51 of the sum and 2^-39 of the weights, either way."""
+    import cumo_amd as m
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal(n) * 3).astype(dt)
+    u = np.concatenate([rng.random(20), [0.0, 0.999999]])
+    order = np.argsort(-x, kind="stable")
+    rank = np.empty(n, np.int64)
+    rank[order] = np.arange(n)
+    every = np.exp(x[order].astype(np.float64) - np.float64(x[order[0]]))
+    for settings in ({}, {"top_k": n // 2}, {"top_p": 0.9}, {"min_p": 1e-4}, {"top_k": 700}, {"top_k": 40}):
+        w = every.copy()
+        w[settings.get("top_k") or n:] = 0
+        w[w < settings.get("min_p", 0.0)] = 0
+        run = np.cumsum(w)
+        off = 2.0 ** -37 + 2 * n * 2.0 ** -51
+        if "top_p" in settings:
+            w[1:][run[:-1] >= settings["top_p"] * run[-1]] = 0
+            off += off + w[w > 0].min() / w.sum()   # (the limit may be a token off)
+            run = np.cumsum(w)
+        at = rank[broadcast_row(m, x, u, **settings)]
+        assert ((run[at] - w[at]) / run[-1] - off <= u).all() and (u <= run[at] / run[-1] + off).all(), settings
+    flat = np.full(1 << 20, 2.0, dt)
+    at = np.arange(0, 1 << 20, 99991)
+    assert (broadcast_row(m, flat, at / 2.0 ** 20) == at).all() and (broadcast_row(m, flat, np.nextafter((at + 1) / 2.0 ** 20, 0)) == at).all()
