@@ -53,6 +53,54 @@ bool overlap(const NA* a, const NA* b) {
     return al < bh && bl < ah;
 }
 
+// the dimensions of a view that are in the mask: from its first byte to behind its last, counted from the element at no index
+void span(const NA* a, unsigned mask, ssize_t* low, ssize_t* high) {
+    *low = 0;
+    *high = kElmsz[a->type];
+    for (int d = 0; d < a->ndim; ++d) {
+        if (!(mask >> d & 1)) continue;
+        const ssize_t far = a->stride[d] * (ssize_t)(a->shape[d] - 1);
+        *(far < 0 ? low : high) += far;
+    }
+}
+
+// Whether two views can share a byte, b's element at no index lying `ahead` bytes behind a's. Windows of one array often reach across each
+// other and share none (its left and its right columns, its even and its odd ones): bytes are compared by what is left of their
+// places on division by a stride, to which dimensions of whole multiples of it add nothing. What that does not tell apart is taken to meet.
+bool can_meet(const NA* a, unsigned in_a, const NA* b, unsigned in_b, ssize_t ahead, int depth) {
+    ssize_t al, ah, bl, bh;
+    span(a, in_a, &al, &ah);
+    span(b, in_b, &bl, &bh);
+    if (ahead + bh <= al || ah <= ahead + bl) return false;
+    for (int k = 0; depth > 0 && k < 2 * kMaxDim; ++k) {
+        const NA* of = k < kMaxDim ? a : b;
+        const int d = k % kMaxDim;
+        if (!((k < kMaxDim ? in_a : in_b) >> d & 1)) continue;
+        const ssize_t m = of->stride[d] < 0 ? -of->stride[d] : of->stride[d];
+        unsigned rest_a = in_a, rest_b = in_b;
+        for (int e = 0; e < kMaxDim; ++e) {
+            if ((in_a >> e & 1) && a->stride[e] % m == 0) rest_a &= ~(1u << e);
+            if ((in_b >> e & 1) && b->stride[e] % m == 0) rest_b &= ~(1u << e);
+        }
+        span(a, rest_a, &al, &ah);
+        span(b, rest_b, &bl, &bh);
+        if (ah - al > m || bh - bl > m) continue;
+        const ssize_t behind = ((ahead + bl - al) % m + m) % m;   // of b's first byte, from a's, or m less
+        const bool here = behind < ah - al && can_meet(a, rest_a, b, rest_b, behind + al - bl, depth - 1);
+        const bool there = behind - m + (bh - bl) > 0 && can_meet(a, rest_a, b, rest_b, behind - m + al - bl, depth - 1);
+        if (!here && !there) return false;
+    }
+    return true;
+}
+
+bool share(const NA* a, const NA* b) {
+    if (!overlap(a, b)) return false;
+    unsigned in_a = 0, in_b = 0;   // (dimensions that have somewhere to go)
+    for (int d = 0; d < a->ndim; ++d) in_a |= a->shape[d] > 1 && a->stride[d] ? 1u << d : 0;
+    for (int d = 0; d < b->ndim; ++d) in_b |= b->shape[d] > 1 && b->stride[d] ? 1u << d : 0;
+    return can_meet(a, in_a, b, in_b, (ssize_t)((uintptr_t)b->ptr + (uintptr_t)b->offset - (uintptr_t)a->ptr - (uintptr_t)a->offset), 3);
+}
+
 bool aligned(const NA* a) {
     uintptr_t bits = (uintptr_t)a->ptr + (uintptr_t)a->offset;
     for (int d = 0; d < a->ndim; ++d)
@@ -168,7 +216,7 @@ int finish(int rc, Result* r, int n, Scratch* s) {
 int results_apart(const NA* const* z, int n) {
     for (int a = 0; a < n; ++a)
         for (int b = a + 1; b < n; ++b)
-            if (z[a] && z[b] && z[a]->ptr && z[b]->ptr && overlap(z[a], z[b])) return fail(CUMO_HIP_ERROR_ARGUMENT, "results overlap each other");
+            if (z[a] && z[b] && z[a]->ptr && z[b]->ptr && share(z[a], z[b])) return fail(CUMO_HIP_ERROR_ARGUMENT, "results overlap each other");
     return CUMO_HIP_OK;
 }
 

@@ -280,7 +280,8 @@ int cumo_hip_na_layernorm(const cumo_hip_narray_t* x, double eps, cumo_hip_narra
 /* Library additions for what stands between the matrix products of a recurrent language model.
  * Operands are SFloat or DFloat, all of one type unless it says otherwise; any strides. An
  * optional array is NULL. Results come in with ptr == NULL or as arrays of the right type and
- * shape, which may overlap operands but not one another. Memory that a call needs beside its
+ * shape, which may overlap operands but share no element with one another (windows of one
+ * array that only reach across each other are told apart). Memory that a call needs beside its
  * results comes from the pool and goes back to it; a call on a stream that is being captured
  * keeps it instead, since the graph goes on using it.
  *

@@ -170,3 +170,23 @@ def test_python_names():
     for bad in (lambda: m.Fused.rmsnorm([1.0]), lambda: m.Fused.sample(3, 4), lambda: m.Fused.recurrence(1, 2), lambda: m.Fused.dequantize(1, 2)):
         with pytest.raises(TypeError):
             bad()
+
+
+def window(type_, ptr, shape, stride, offset=0):
+    d = view(type_, *shape, ptr=ptr)
+    d.offset = offset
+    for k, s in enumerate(stride):
+        d.stride[k] = s
+    return d
+
+
+def test_windows_of_one_array_that_share_elements():
+    """Columns [0, 6) and [5, 11) of rows of 11; channels 0, 2, ... and 1, 2, 3, ...; a matrix and its transpose; one row of another."""
+    f = L.cumo_hip_na_recurrence_grad
+    at = 0x70000000
+    cases = [((4, 6), (44, 4), 0, (44, 4), 20), ((4, 5), (88, 8), 0, (88, 4), 4), ((5, 5), (20, 4), 0, (4, 20), 0), ((1, 6), (24, 4), 48, (24, 4), 52),
+             ((3, 4), (160, 40), 0, (40, 40), 80), ((3, 2, 3), (120, 40, 8), 4, (120, 20, 8), 24)]
+    for shape, one, at_one, two, at_two in cases:
+        g, a, h = (view(SF, *shape) for _ in range(3))
+        refused(ARGUMENT, f, g, a, h, None, 0, window(SF, at, shape, one, at_one), window(SF, at, shape, two, at_two), None)
+        refused(ARGUMENT, f, g, a, h, None, 0, window(SF, at, shape, two, at_two), window(SF, at, shape, one, at_one), None)

@@ -184,3 +184,34 @@ def test_a_generation_step_captured_and_replayed():
         if graph:
             hip.hipGraphDestroy(graph)
         L.cumo_hip_stream_destroy(stream)
+
+
+@pytest.mark.parametrize("dt", [np.float32, np.float64])
+def test_results_side_by_side_in_one_array(dt):
+    """Two results as the left and the right half of rows, as their even and odd elements, as every other row, row by row in
+    turn backwards: what calls answer by themselves, and nothing beside them changes."""
+    import cumo_amd as m
+    from cumo_amd import _lib
+    L = _lib.lib
+    cls = m.SFloat if dt == np.float32 else m.DFloat
+    rng = np.random.default_rng(5)
+    rows, d = 37, 21
+    x, r, g, a = (cls.cast(rng.uniform(0.1, 0.9, (rows, d)).astype(dt)) for _ in range(4))
+    y, s = m.Fused.rmsnorm(x, None, r)
+    ga, gb = m.Fused.recurrence_grad(g, a, x, axis=0)
+    ref = lambda z: C.byref(z._desc())  # noqa: E731
+    every = slice(None)
+    for wide, one, two in (((rows, 2 * d), (every, slice(0, d)), (every, slice(d, 2 * d))), ((rows, 2 * d + 1), (every, slice(0, 2 * d, 2)), (every, slice(1, 2 * d + 1, 2))),
+                           ((rows, 2 * d + 6), (every, slice(d + 5, 5, -1)), (every, slice(d + 6, 2 * d + 6))), ((2 * rows, d), (slice(0, None, 2), every), (slice(1, None, 2), every)),
+                           ((2 * rows, d + 3), (slice(None, None, -2), slice(0, d)), (slice(0, None, 2), slice(2, d + 2)))):
+        for call, want in ((lambda p, q: (L.cumo_hip_na_rmsnorm, ref(x), None, ref(r), 1e-6, ref(p), ref(q)), (y, s)),
+                           (lambda p, q: (L.cumo_hip_na_recurrence_grad, ref(g), ref(a), ref(x), None, 0, ref(p), ref(q), None), (ga, gb))):
+            for order in (1, -1):
+                buf = cls(*wide).fill(7)
+                both = (buf[one], buf[two])[::order]
+                _lib.call(*call(*both))
+                got = buf.to_numpy()
+                for at, w in zip((one, two)[::order], want):
+                    assert (got[at] == w.to_numpy()).all(), (wide, one, two)
+                    got[at] = 7
+                assert (got == 7).all()
