@@ -33,6 +33,18 @@ class MemoryPool:
         else:
             _lib.call(_lib.lib.cumo_hip_pool_free_all_blocks_stream, stream)
 
+    @staticmethod
+    def capture_id():
+        """The number of the capture that the calling thread's stream is in, 0 if none."""
+        return _lib.lib.cumo_hip_capture_id()
+
+    @staticmethod
+    def free_captured(capture=0):
+        """Gives back what calls of a capture (0: of every one) left to its graph, which must have run for the last
+        time; the number of pieces."""
+        return _lib.lib.cumo_hip_captured_free(capture)
+
+    captured_blocks = staticmethod(lambda capture=0: _lib.lib.cumo_hip_captured_blocks(capture))
     n_free_blocks = staticmethod(lambda: _lib.lib.cumo_hip_pool_n_free_blocks())
     used_bytes = staticmethod(lambda: _lib.lib.cumo_hip_pool_used_bytes())
     free_bytes = staticmethod(lambda: _lib.lib.cumo_hip_pool_free_bytes())

@@ -157,6 +157,9 @@ _sig = {
     "cumo_hip_pool_free_bytes": (C.c_size_t, []),
     "cumo_hip_pool_total_bytes": (C.c_size_t, []),
     "cumo_hip_pool_device_malloc_calls": (C.c_size_t, []),
+    "cumo_hip_capture_id": (C.c_uint64, []),
+    "cumo_hip_captured_blocks": (C.c_size_t, [C.c_uint64]),
+    "cumo_hip_captured_free": (C.c_size_t, [C.c_uint64]),
     "cumo_hip_pool_enable": (C.c_int, [C.c_int]),
     "cumo_hip_pool_set_limit": (None, [C.c_size_t]),
     "cumo_hip_pool_use_host_backend": (C.c_int, [C.c_int]),

@@ -22,6 +22,10 @@ hipStream_t current_stream();
 // to the pool by then
 bool stream_under_capture();
 
+// Memory that a launch held beside its operands and results, once its last kernel is queued: back to the pool. While the stream is being
+// captured it stays with the graph, whose replays write it again when the pool could have given it to somebody else, until cumo_hip_captured_free.
+void scratch_free(char* memory);
+
 // A number in [0, kStreamSlots) that belongs to this stream until it is destroyed
 // through cumo_hip_stream_destroy, or -1 when every number is taken. Kernels that
 // keep per-stream words in a fixed device array (tickets) index it with this.

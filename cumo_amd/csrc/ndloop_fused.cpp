@@ -122,15 +122,13 @@ bool one_step(const NA* a, int lo, int hi, ssize_t* step) {
     return true;
 }
 
-// What a call holds beside its operands and results, given up at its end. A captured call's memory stays with the graph: a replay
-// writes it again, when the pool could have given it to somebody else.
+// What a call holds beside its operands and results, given up at its end.
 struct Scratch {
     char* held[16];
     int n;
 };
 void let_go(Scratch* s) {
-    if (s->n && !stream_under_capture())
-        for (int k = 0; k < s->n; ++k) cumo_cuda_runtime_free(s->held[k]);
+    for (int k = 0; k < s->n; ++k) scratch_free(s->held[k]);
     s->n = 0;
 }
 

@@ -849,8 +849,7 @@ int re_chain(const ReArgs& p, uint64_t lines, uint64_t tile, hipStream_t stream)
     if constexpr (ROWS) hipLaunchKernelGGL((recurrence_rows_chain_kernel<T, GRAD>), grid, block, 0, stream, p, chain);
     else hipLaunchKernelGGL((recurrence_columns_chain_kernel<T, GRAD>), grid, block, 0, stream, p, chain);
     cumo_cuda_runtime_check_kernel_launch();
-    // (the memory of a captured launch stays with its graph)
-    if (!stream_under_capture()) cumo_cuda_runtime_free(memory);
+    scratch_free(memory);
     return CUMO_HIP_OK;
 }
 

@@ -602,8 +602,7 @@ bool rn_grad_one(RnGradParams p, hipStream_t stream) {
     if (parts) {
         hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), rn_columns(p.n), dim3(1024), 0, stream, p.parts, (uint32_t)blocks, p.n,
                            reinterpret_cast<T*>(p.gweight));
-        // (the memory of a captured launch stays with its graph)
-        if (!stream_under_capture()) cumo_cuda_runtime_free(parts);
+        scratch_free(parts);
     }
     return true;
 }
@@ -622,7 +621,7 @@ bool rn_grad_long(RnGradParams p, hipStream_t stream) {
         hipLaunchKernelGGL((rmsnorm_grad_columns_kernel<T>), dim3(rn_grid((p.n + 255) / 256, 1u << 20), (unsigned)runs), dim3(256), 0, stream, p, rs, per);
         hipLaunchKernelGGL((rmsnorm_grad_parts_kernel<T>), rn_columns(p.n), dim3(1024), 0, stream, p.parts, (uint32_t)runs, p.n,
                            reinterpret_cast<T*>(p.gweight));
-        if (!stream_under_capture()) cumo_cuda_runtime_free(memory);
+        scratch_free(memory);
     }
     return true;
 }

@@ -12,6 +12,7 @@
 #include <cstring>
 #include <atomic>
 #include <mutex>
+#include <vector>
 
 namespace cumo_hip {
 
@@ -54,6 +55,38 @@ bool stream_under_capture() {
         return true;
     }
     return capturing != hipStreamCaptureStatusNone;
+}
+
+// ---- memory that captured calls leave to their graphs -----------------------------------
+struct Captured {
+    uint64_t capture;
+    char* memory;
+};
+static std::mutex g_captured_lock;
+static std::vector<Captured> g_captured;
+
+static uint64_t capture_of_stream(hipStream_t stream) {
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(stream, &capturing, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    return capturing == hipStreamCaptureStatusNone ? 0 : (uint64_t)id;
+}
+
+void scratch_free(char* memory) {
+    if (!memory) return;
+    if (!stream_under_capture()) {
+        cumo_cuda_runtime_free(memory);
+        return;
+    }
+    const uint64_t capture = capture_of_stream(t_stream);
+    std::lock_guard<std::mutex> hold(g_captured_lock);
+    try {
+        g_captured.push_back({capture, memory});
+    } catch (...) {   // (nobody will give it back, but the graph has it)
+    }
 }
 
 bool force_wide_indices() {
@@ -257,6 +290,34 @@ void cumo_hip_stream_destroy(void* hip_stream) {
     if (t_stream == (hipStream_t)hip_stream) t_stream = nullptr;
     cumo_hip_stream_release(hip_stream);
     hip_ok(hipStreamDestroy((hipStream_t)hip_stream), "hipStreamDestroy");
+}
+
+uint64_t cumo_hip_capture_id(void) { return capture_of_stream(t_stream); }
+
+size_t cumo_hip_captured_blocks(uint64_t capture) {
+    std::lock_guard<std::mutex> hold(g_captured_lock);
+    size_t n = 0;
+    for (const Captured& c : g_captured) n += capture == 0 || c.capture == capture;
+    return n;
+}
+
+size_t cumo_hip_captured_free(uint64_t capture) {
+    size_t n = 0;
+    for (;;) {
+        char* memory = nullptr;
+        {
+            std::lock_guard<std::mutex> hold(g_captured_lock);
+            for (size_t k = g_captured.size(); k-- > 0 && !memory;) {
+                if (capture != 0 && g_captured[k].capture != capture) continue;
+                memory = g_captured[k].memory;
+                g_captured[k] = g_captured.back();
+                g_captured.pop_back();
+            }
+        }
+        if (!memory) return n;
+        cumo_cuda_runtime_free_no_raise(memory);
+        ++n;
+    }
 }
 
 int cumo_hip_device_count(void) {

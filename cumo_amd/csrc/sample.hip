@@ -894,8 +894,7 @@ int sa_launch(const cumo_hip_sample_t& d, hipStream_t stream) {
             if (a->each) a->each += (uint64_t)now * (a->type == 1 ? 8 : 4);
     }
     cumo_cuda_runtime_check_kernel_launch();
-    // (the memory of a captured launch stays with its graph)
-    if (!stream_under_capture()) cumo_cuda_runtime_free(memory);
+    scratch_free(memory);
     return CUMO_HIP_OK;
 }
 

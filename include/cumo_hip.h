@@ -666,8 +666,8 @@ void cumo_hip_dequantize_kernel_launch(int type, const cumo_hip_dequantize_t* d)
  *   gx = r * (g * weight - s * r^2 * sum(g * weight * s) / n) + gsum
  *   gweight = the sum over rows of g * s * r   (NULL: not wanted; n contiguous elements)
  * gx is the gradient of x and of residual alike. No result may overlap an operand. Partial
- * sums live in a block from the pool (kept where the stream is being captured). CUMO_HIP_OK or
- * the error reported. */
+ * sums live in a block from the pool (left to the graph where the stream is being captured:
+ * cumo_hip_captured_free). CUMO_HIP_OK or the error reported. */
 typedef struct {
     uint64_t rows, n;
     ssize_t  g_step, s_step, gsum_step, gx_step;
@@ -862,6 +862,14 @@ size_t cumo_hip_pool_free_bytes(void);
 size_t cumo_hip_pool_total_bytes(void);
 /* bytes and calls that went to hipMalloc since the process started */
 size_t cumo_hip_pool_device_malloc_calls(void);
+/* Memory of graphs. Calls of cumo_hip_na_rmsnorm to _sample, and the launchers behind them, that are captured
+ * leave what they hold beside their results to the graph, in use. capture_id: the number of the capture that the calling
+ * thread's stream is in, 0 if none. captured_blocks: how many pieces a capture has left so (0: all captures).
+ * captured_free gives them back to the pool and answers their number. The graph, and what has been
+ * instantiated from it, must have run for the last time. */
+uint64_t cumo_hip_capture_id(void);
+size_t cumo_hip_captured_blocks(uint64_t capture);
+size_t cumo_hip_captured_free(uint64_t capture);
 int    cumo_hip_pool_enable(int on);                        /* returns previous state; CUMO_MEMORY_POOL env sets the default */
 /* test hook: cap what the pool may hold from the device (0 = no cap), so that
  * the out-of-memory path can be driven from the host without exhausting HBM */

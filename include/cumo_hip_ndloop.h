@@ -283,7 +283,7 @@ int cumo_hip_na_layernorm(const cumo_hip_narray_t* x, double eps, cumo_hip_narra
  * shape, which may overlap operands but share no element with one another (windows of one
  * array that only reach across each other are told apart). Memory that a call needs beside its
  * results comes from the pool and goes back to it; a call on a stream that is being captured
- * keeps it instead, since the graph goes on using it.
+ * leaves it to the graph, which goes on using it, until cumo_hip_captured_free.
  *
  * rmsnorm: along the last dimension, s = x + residual, r = 1 / sqrt(mean(s^2) + eps),
  * y = s * r * weight. residual has x's shape; weight is one dimension of that length. sum

@@ -215,3 +215,64 @@ def test_results_side_by_side_in_one_array(dt):
                     assert (got[at] == w.to_numpy()).all(), (wide, one, two)
                     got[at] = 7
                 assert (got == 7).all()
+
+
+def test_what_captures_leave_to_their_graphs_can_be_given_back():
+    """Captured calls with scratch and with copies of operands: in use until it is given back, a capture's at a time, and the pool
+    is then as it was; the other capture's graph still runs."""
+    import cumo_amd as m
+    from cumo_amd import _lib
+    from test_gpu_index import hip_runtime
+    hip, L = hip_runtime(), _lib.lib
+    rng = np.random.default_rng(6)
+    draw = lambda *shape: m.SFloat.cast(rng.uniform(0.1, 0.9, shape).astype(np.float32))  # noqa: E731
+    a, b, wide, w, u = draw(1, 3000, 8), draw(1, 3000, 8), draw(700, 520), draw(260), draw(700)
+    x = wide[:, ::2]   # (rows whose elements are not neighbours are copied)
+    h, gx, gw, token = m.SFloat(1, 3000, 8), m.SFloat(700, 260), m.SFloat(260), m.Int32(700)
+    ref = lambda z: C.byref(z._desc())  # noqa: E731
+    args = [ref(z) for z in (a, b, h, x, w, gx, gw, u, token)]
+
+    def call():
+        ra, rb, rh, rx, rw, rgx, rgw, ru, rt = args
+        _lib.call(L.cumo_hip_na_recurrence, ra, rb, None, 1, rh)
+        _lib.call(L.cumo_hip_na_rmsnorm_grad, rx, rx, rw, None, 1e-6, rgx, rgw)
+        _lib.call(L.cumo_hip_na_sample, rx, ru, 1.0, None, 30, None, 0.9, None, 0.0, None, rt)
+
+    results = (h, gx, gw, token)
+    call()
+    wants = [z.to_numpy() for z in results]
+    assert m.MemoryPool.capture_id() == 0
+    start, used = m.MemoryPool.captured_blocks(), m.MemoryPool.used_bytes()
+    stream = C.c_void_p(L.cumo_hip_stream_create())
+    m.synchronize()
+    L.cumo_hip_set_stream(stream)
+    made = []
+    try:
+        for _ in range(2):
+            graph, ready = C.c_void_p(), C.c_void_p()
+            assert hip.hipStreamBeginCapture(stream, 2) == 0
+            capture = m.MemoryPool.capture_id()
+            call()
+            assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+            assert hip.hipGraphInstantiate(C.byref(ready), graph, None, None, C.c_size_t(0)) == 0
+            made.append((capture, graph, ready))
+            # recurrence's words, two copies and the parts of the gradient, a copy and the bins
+            assert m.MemoryPool.captured_blocks(capture) == 6
+        assert made[0][0] and made[1][0] and made[0][0] != made[1][0] and m.MemoryPool.captured_blocks() == start + 12
+        for k in range(2):
+            for _, _, ready in made[k:]:
+                for z in results:
+                    z.fill(0)
+                held = [m.Int32((512 << s) // 4).fill(77) for s in range(15) for _ in range(2)]
+                assert hip.hipGraphLaunch(ready, stream) == 0
+                m.synchronize()
+                assert all((z.to_numpy() == want).all() for z, want in zip(results, wants))
+                assert all(int(v.ne(77).count_true()) == 0 for v in held)
+                del held
+            capture, graph, ready = made[k]
+            assert hip.hipGraphExecDestroy(ready) == 0 and hip.hipGraphDestroy(graph) == 0
+            assert m.MemoryPool.free_captured(capture) == 6 and m.MemoryPool.captured_blocks(capture) == 0
+        assert m.MemoryPool.captured_blocks() == start and m.MemoryPool.used_bytes() == used
+    finally:
+        L.cumo_hip_set_stream(None)
+        L.cumo_hip_stream_destroy(stream)
