@@ -33,7 +33,7 @@ COMMON = [
     "-Wall", "-Wno-unused-function", "-Wno-deprecated-declarations",
 ]
 # device code: no packed FP32 forms
-# --offload-compress: the device code of every unit is stored compressed in the library (a third of
+# --offload-compress: the device code of every unit is stored compressed in the library (a sixth of
 # the size; the runtime unpacks it once when the library is loaded)
 DEVICE = ["--offload-arch=" + ARCH, "--offload-compress", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

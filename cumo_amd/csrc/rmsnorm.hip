@@ -9,8 +9,8 @@
 // result, are in double: a square of a float is exact there, and the vector units do a hundred such operations in the time
 // that an element's bytes take. SFloat [8192,4096], with a residual, a sum and a weight: 87 us (6.2 TB/s, what an addition of two
 // large arrays reaches); in 8 bits [8192,4095] 80 us (5.4; the vector units are busy for more than half of it), and 30 us back
-// (5.5); gradients with gsum 94 + 5 us (5.7 and the weight's parts); DFloat [131072,257] gradients 200 + 5 (5.4). One row of
-// 4096: 3.5 us, the launch's.
+// (5.5); gradients with gsum 94 + 5 us (5.7 and the weight's parts); DFloat [131072,257] gradients 200 + 5 (5.4), [8192,2047] in 8 bits 76
+// and 31 back. One row of 4096: 3.5 us, the launch's.
 #include "common.h"
 
 namespace cumo_hip {
@@ -449,7 +449,8 @@ __global__ __launch_bounds__(BLOCK) void rmsnorm_grad_kernel(RnGradParams p) {
     }
 }
 
-// Rows that no block's registers hold; r of each row is left for the weight's gradient.
+// Rows that no block's registers hold (more than 16387 SFloat, 8193 DFloat); r of each row is left for the weight's gradient. SFloat
+// [1024,32768] with gsum and weight 239 + 54 + 7 us, DFloat [2048,16384] 263 + 129 + 5, [2048,8192] in registers 101 + 5.
 template <class T>
 __global__ __launch_bounds__(kRnWide) void rmsnorm_grad_long_kernel(cumo_hip_rmsnorm_grad_t p, double* rs) {
     for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {

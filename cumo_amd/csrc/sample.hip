@@ -13,11 +13,12 @@
 // Three launches. The largest and the smallest number of each row's parts, and the largest of every chunk of 64 vectors; the bins of
 // each row's parts, a block to a part with its bins in shared memory; then a block to a row, which adds the parts' bins up, takes
 // their running sums and reads the chunks that reach the list's bins once more. The rows come from memory once and from the
-// last-level cache the other times. What bounds it for many rows is the weights' arithmetic in double (some twenty operations an
-// element) and the order of steps within a row, for a few rows the launches and those steps. SFloat, temperature 0.8, top_k 50,
-// top_p 0.95: one row of 131072 in 24 us (4.6, 5 and 14.7 in the three), 256 rows of 50001 in 40 us with one setting for all, and
-// in 62 us (13, 27 and 23.4; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
-// chunks' maxima the last launch reads whole rows: 20.4 and 27.8 us of it, where the first one takes 4.0 and 11.2.
+// last-level cache the other times. What bounds it is the order of steps within a row, and for many rows the weights' arithmetic as
+// well: forty instructions an element, which keep the vector units busy for half of the second launch (shared memory 15 % of it, its
+// conflicts 7 %); its blocks, all at work at once, clear, read, count and write their bins in step. SFloat, temperature 0.8, top_k 50,
+// top_p 0.95: one row of 131072 in 24 us (4.1, 5.7 and 15.8 in the three), 256 rows of 50001 in 39 us with one setting for all, and
+// in 63 us (13, 27.5 and 24; 0.8 TB/s of logits) with settings of their own, most of which need weights in every bin. Without the
+// chunks' maxima the last launch read whole rows: 20.4 and 27.8 us of it, where the first one took 4.0 and 11.2.
 #include "common.h"
 #include "ew_ops.h"
 

@@ -1145,7 +1145,8 @@ class _Fused:
     """Composites along rows or an axis in one call (library additions). softmax and layernorm the reference
     writes as chains of array operations (bench/transformer_bench.rb:110-124); layouts that the row kernels do not
     take fall back to that chain inside the library. The others (rmsnorm, recurrence, sample) are what stands between
-    the matrix products of a recurrent language model."""
+    the matrix products of a recurrent language model. Their operands are SFloat or DFloat, all of one type but for
+    sample's settings and u, and of the shapes that each says: nothing is converted or repeated."""
 
     @staticmethod
     def softmax(x):

@@ -717,7 +717,7 @@ int cumo_hip_recurrence_grad_kernel_launch(int type, const cumo_hip_recurrence_g
  * (0: all; the first always stays). The answer is the first of those left whose running sum of
  * weights exceeds u times theirs. temperature <= 0 takes the largest x. -1 where a row has
  * nothing to choose (n = 0, every x -inf) or holds a NaN. A setting is one number, or one a row
- * (at: contiguous, of type 0 SFloat, 1 DFloat, 2 Int32). type: of x. */
+ * (at: contiguous, of type 0 SFloat, 1 DFloat, 2 Int32). type: of x. n is less than 2^31. */
 typedef struct {
     const char* each;  /* NULL: value for every row */
     int      type;

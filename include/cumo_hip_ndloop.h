@@ -278,7 +278,8 @@ int cumo_hip_na_softmax(const cumo_hip_narray_t* x, cumo_hip_narray_t* z);
 int cumo_hip_na_layernorm(const cumo_hip_narray_t* x, double eps, cumo_hip_narray_t* z);
 
 /* Library additions for what stands between the matrix products of a recurrent language model.
- * Operands are SFloat or DFloat, all of one type unless it says otherwise; any strides. An
+ * Operands are SFloat or DFloat, all of one type unless it says otherwise, of the shapes it says
+ * (nothing is converted or repeated, other types and shapes are refused); any strides. An
  * optional array is NULL. Results come in with ptr == NULL or as arrays of the right type and
  * shape, which may overlap operands but share no element with one another (windows of one
  * array that only reach across each other are told apart). Memory that a call needs beside its
@@ -287,9 +288,10 @@ int cumo_hip_na_layernorm(const cumo_hip_narray_t* x, double eps, cumo_hip_narra
  *
  * rmsnorm: along the last dimension, s = x + residual, r = 1 / sqrt(mean(s^2) + eps),
  * y = s * r * weight. residual has x's shape; weight is one dimension of that length. sum
- * receives s, and is NULL when residual is. Sums are in double; y is rounded once.
+ * receives s, and is NULL when residual is. Sums are in double; y is rounded once. (DFloat rows
+ * whose squares pass 1.8e308 have r = 0; with eps 0 a row of zeros has r infinite and y NaN.)
  * rmsnorm_q8: q is Int8, round(y / scale); scale has x's shape with a last dimension of 1 and is
- * max|y| / 127 of the row, from y that is not rounded before. A row of zeros has scale 0, one
+ * max|y| / 127 of the row, from y that is not rounded before. A row whose y are 0 has scale 0, one
  * with a NaN scale NaN; q is 0 there. dequantize: y = q * scale, in scale's type.
  * rmsnorm_grad: from g (of y), s and gsum (of s, or NULL): gx, of x and residual alike, and
  * gweight (NULL when weight is). */
