@@ -17,8 +17,9 @@
 // there are not, time is cut into tiles, a block each, all in one launch: a tile leaves its A and B in memory for the ones after
 // it, folds those of the tiles before it from the nearest one whose state is there already, and leaves its own state.
 // Memory bounds all but the shortest: SFloat [8,4096,2048] 158 us (5.1 TB/s, a large copy's rate), gradients of [8,2048,2048] 140
-// us (4.8), DFloat [4096,4095] along rows 82 us (4.9), its gradients 141 (4.8; SFloat 87, 3.8); in tiles [1,65536,1000] 184 us with 6.5 for clearing the words (4.3: in each tile
-// loads, joins and stores follow one another, and 10% more bytes go through the words). One step of 64 x 4096: 5.5 us.
+// us (4.8), DFloat [4096,4095] along rows 82 us (4.9), its gradients 141 (4.8; SFloat 87, 3.8); in tiles [1,65536,1000] 184 us with
+// 6.5 for clearing the words (4.3: in each tile loads, joins and stores follow one another, and 10% more bytes go through the words).
+// One step of 64 x 4096: 5.5 us.
 #include "common.h"
 #include "wait_ctl.h"
 

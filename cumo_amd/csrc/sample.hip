@@ -10,7 +10,7 @@
 // of a row whose weights are all the largest; a sum is off by n 2^-(S+1) of that, 2^-27 at most. Longer rows each have an S to what their
 // weights can come to, by the chunks' maxima (256 times the sum at most): a sum is off by n 2^-51 of itself at most.
 //
-// Three launches. The largest and the smallest number of each row's parts, and the largest of every chunk of 64 vectors; the bins of
+// Three launches (and a small one for the units of long rows). The largest and the smallest number of each row's parts, and the largest of every chunk of 64 vectors; the bins of
 // each row's parts, a block to a part with its bins in shared memory; then a block to a row, which adds the parts' bins up, takes
 // their running sums and reads the chunks that reach the list's bins once more. The rows come from memory once and from the
 // last-level cache the other times. What bounds it is the order of steps within a row, and for many rows the weights' arithmetic as

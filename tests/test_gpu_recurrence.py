@@ -467,3 +467,45 @@ def test_products_beyond_the_type_of_states_within_it(dt, shape, axis):
         assert np.isfinite(want).all() and (want != 0).all()
         got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(start), axis=axis).to_numpy())
         assert (got == want).all(), (h0, first)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape,axis", LONG + [((1, 1200, 12800), 1), ((300, 3000), 1)])
+def test_gates_of_every_size(dt, shape, axis):
+    """Powers of two from the type's smallest to its largest, at random but for the states that they lead through: those stay
+    within the type, so every step is exact, and so are the products of any of them that a state goes through."""
+    import cumo_amd as m
+    cls = cls_of(m, dt)
+    rng = np.random.default_rng(9)
+    n = shape[axis]
+    f = lambda v: np.moveaxis(v, axis, 0)  # noqa: E731
+    reach, least, most = (120, -149, 127) if dt == np.float32 else (1000, -1074, 1023)
+    lead = f(np.empty(shape, bool)).shape[1:]
+    at = np.zeros(lead, np.int64)
+    a, b = np.empty(shape, dt), np.zeros(shape, dt)
+    # each column's states: a walk over the exponents, the same for all but for where it starts
+    to = rng.integers(-reach, reach + 1, n)
+    start = rng.integers(-reach, reach + 1, lead)
+    at = start
+    want = np.empty(f(a).shape, dt)
+    for t in range(n):
+        step = np.clip(to[t] - at, least, most)
+        at = at + step
+        f(a)[t] = np.ldexp(dt(1), step)
+        want[t] = np.ldexp(dt(1), at)
+    h0 = np.ldexp(dt(1), start).astype(dt)
+    got = f(m.Fused.recurrence(cls.cast(a), cls.cast(b), cls.cast(h0), axis=axis).to_numpy())
+    assert (got == want).all()
+    # backwards the gradient of the last step walks the other way: gb[t] = a[t+1] ... a[n-1] = want[n-1] / want[t], where that stays in the type
+    g = np.zeros(shape, dt)
+    f(g)[n - 1] = 1
+    back = np.empty_like(want)
+    back[n - 1] = 1
+    with np.errstate(over="ignore", under="ignore"):
+        for t in range(n - 2, -1, -1):
+            back[t] = f(a)[t + 1] * back[t + 1]
+    gb = f(m.Fused.recurrence_grad(cls.cast(g), cls.cast(a), cls.cast(b), axis=axis)[1].to_numpy())
+    # (exact until a first gradient leaves the normal numbers of the type)
+    tiny, big = np.finfo(dt).tiny, np.finfo(dt).max
+    fine = np.logical_and.accumulate(((back >= tiny) & (back <= big))[::-1], axis=0)[::-1]
+    assert (gb[fine] == back[fine]).all() and fine[-1].all()
