@@ -45,3 +45,13 @@ def no_kernel_gave_up_a_wait():
     f = _lib.fn("cumo_hip_wait_give_ups", C.c_int, [C.POINTER(C.c_uint32 * 4)])
     assert f(C.byref(counts)) == 0
     assert list(counts) == [0, 0, 0, 0], "kernels gave up bounded waits during this run: %s" % list(counts)
+
+
+@pytest.fixture(autouse=True)
+def nothing_left_to_graphs():
+    """Graphs that a test has captured are gone when it ends: what its calls left to them goes back to the pool, so that
+    tests of the pool's books see the same whatever ran before them."""
+    yield
+    if HAS_GPU:
+        import cumo_amd
+        cumo_amd.MemoryPool.free_captured()
