@@ -197,6 +197,11 @@ _sig = {
                                               P(NArrayDesc)]),
     "cumo_hip_na_sample": (C.c_int, [P(NArrayDesc), P(NArrayDesc), C.c_double, P(NArrayDesc), C.c_ssize_t, P(NArrayDesc), C.c_double,
                                      P(NArrayDesc), C.c_double, P(NArrayDesc), P(NArrayDesc)]),
+    "cumo_hip_na_quantize": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc)]),
+    "cumo_hip_na_matmul_q8": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), P(NArrayDesc)]),
+    "cumo_hip_na_rotary": (C.c_int, [P(NArrayDesc), P(NArrayDesc), P(NArrayDesc), C.c_int, C.c_int, C.c_double, P(NArrayDesc)]),
+    "cumo_hip_na_linear_attention": (C.c_int, [P(NArrayDesc)] * 6 + [C.c_double] + [P(NArrayDesc)] * 2),
+    "cumo_hip_na_linear_attention_grad": (C.c_int, [P(NArrayDesc)] * 8 + [C.c_double] + [P(NArrayDesc)] * 4),
     "cumo_hip_na_ewcomp": (C.c_int, [C.c_char_p, P(NArrayDesc), P(NArrayDesc), C.c_int, P(NArrayDesc)]),
     "cumo_hip_na_clip": (C.c_int, [P(NArrayDesc), C.c_int, C.c_double, P(NArrayDesc), C.c_int, C.c_double, P(NArrayDesc),
                                    P(NArrayDesc)]),

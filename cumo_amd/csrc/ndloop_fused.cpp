@@ -1,5 +1,5 @@
-// The host layer's row operators and the recurrence: checks, layouts, results; the kernels are in rmsnorm.hip,
-// recurrence.hip and sample.hip. (Library additions; the reference has no such methods.)
+// The host layer's row operators, the recurrence, and what a layer with a matrix state takes: checks, layouts, results; the kernels are
+// in rmsnorm.hip, recurrence.hip, sample.hip, matmul_q8.hip, rotary.hip and linear_attention.hip. (Library additions; the reference has no such methods.)
 //
 // No function here keeps a C++ object with a destructor alive across a call that may report an error: the installed
 // handler may leave with longjmp.
@@ -133,12 +133,18 @@ void let_go(Scratch* s) {
 }
 
 // Layouts: rows whose elements lie side by side, with one step from row to row; elements without gaps; outer x axis x inner
-// with a step each.
-enum Layout { ROWS, DENSE, AXIS };
+// with a step each; heads whose elements lie side by side, with a step from head to head, from step to step (the dimension in front of the
+// heads) and one for what is in front of that.
+enum Layout { ROWS, DENSE, AXIS, HEADS };
 bool laid_out(const NA* a, Layout l, int axis, ssize_t* step) {
     if (!aligned(a)) return false;
     if (l == DENSE) return is_contiguous(a);
     if (l == ROWS) return (a->shape[a->ndim - 1] == 1 || a->stride[a->ndim - 1] == kElmsz[a->type]) && one_step(a, 0, a->ndim - 1, step);
+    if (l == HEADS) {
+        const int nd = a->ndim;
+        for (int k = 0; k < 2; ++k) step[1 + k] = nd < 3 - k || a->shape[nd - 3 + k] == 1 ? 0 : a->stride[nd - 3 + k];
+        return (a->shape[nd - 1] == 1 || a->stride[nd - 1] == kElmsz[a->type]) && (nd < 4 || one_step(a, 0, nd - 3, step));
+    }
     step[1] = a->shape[axis] == 1 ? 0 : a->stride[axis];
     return one_step(a, 0, axis, step) && one_step(a, axis + 1, a->ndim, step + 2);
 }
@@ -568,6 +574,336 @@ int cumo_hip_na_sample(const cumo_hip_narray_t* x, const cumo_hip_narray_t* u, d
         if (d.rows) rc = cumo_hip_sample_kernel_launch(x->type, &d);
     }
     return finish(rc, &r, nr, &s);
+}
+
+}  // extern "C"
+
+extern "C" {
+
+int cumo_hip_na_quantize(const cumo_hip_narray_t* x, cumo_hip_narray_t* q, cumo_hip_narray_t* scale) {
+    int rc = check_float(x, "quantize: the array is not SFloat or DFloat");
+    if (rc) return rc;
+    if (x->ndim < 1) return fail(CUMO_HIP_ERROR_DIMENSION, "quantize needs at least one dimension");
+    const int nd = x->ndim;
+    size_t scale_shape[kMaxDim];
+    std::memcpy(scale_shape, x->shape, sizeof(size_t) * nd);
+    scale_shape[nd - 1] = 1;
+    rc = check_result(q, CUMO_HIP_INT8, nd, x->shape);
+    if (!rc) rc = check_result(scale, x->type, nd, scale_shape);
+    const NA* const z[2] = {q, scale};
+    if (!rc) rc = results_apart(z, 2);
+    if (rc) return rc;
+    Scratch s;
+    s.n = 0;
+    Operand o;
+    Result r[2];
+    int nr = 0;
+    rc = take(&o, x, ROWS, 0, &s);
+    if (!rc) rc = make(&r[nr++], q, CUMO_HIP_INT8, nd, x->shape, ROWS, 0, &o, 1, &s);
+    if (!rc) rc = make(&r[nr++], scale, x->type, nd, scale_shape, DENSE, 0, &o, 1, &s);
+    if (!rc) {
+        cumo_hip_quantize_t d;
+        d.n = x->shape[nd - 1];
+        d.rows = total_of(scale);
+        d.x = o.at();
+        d.x_step = o.step[0];
+        d.q = r[0].at();
+        d.q_step = r[0].step[0];
+        d.scale = r[1].at();
+        if (d.rows && d.n) cumo_hip_quantize_kernel_launch(x->type, &d);
+        else if (d.rows) rc = cumo_hip_na_fill(r[1].use, 0.0);  // (rows of no elements still have a scale)
+    }
+    return finish(rc, r, nr, &s);
+}
+
+int cumo_hip_na_matmul_q8(const cumo_hip_narray_t* x, const cumo_hip_narray_t* xscale, const cumo_hip_narray_t* w, const cumo_hip_narray_t* wscale,
+                          const cumo_hip_narray_t* bias, cumo_hip_narray_t* y) {
+    const char* const types = "matmul_q8: the scales and bias are SFloat or DFloat, all of one type";
+    int rc = check_view(x, "operand");
+    if (!rc) rc = check_view(w, "operand");
+    if (!rc) rc = check_float(xscale, types);
+    if (!rc) rc = check_float(wscale, types);
+    if (!rc && bias) rc = check_float(bias, types);
+    if (rc) return rc;
+    if (x->type != CUMO_HIP_INT8 || w->type != CUMO_HIP_INT8) return fail(CUMO_HIP_ERROR_TYPE, "matmul_q8: the arrays are not Int8");
+    if (wscale->type != xscale->type || (bias && bias->type != xscale->type)) return fail(CUMO_HIP_ERROR_TYPE, types);
+    const int nd = x->ndim;
+    if (nd < 1) return fail(CUMO_HIP_ERROR_DIMENSION, "matmul_q8 needs at least one dimension");
+    if (w->ndim != 2) return fail(CUMO_HIP_ERROR_DIMENSION, "matmul_q8: w must have two dimensions");
+    if (w->shape[1] != x->shape[nd - 1]) return fail(CUMO_HIP_ERROR_SHAPE, "matmul_q8: rows of w must be as long as rows of x");
+    size_t want[kMaxDim];
+    std::memcpy(want, x->shape, sizeof(size_t) * nd);
+    want[nd - 1] = 1;
+    if (!same_shape(xscale, nd, want)) return fail(CUMO_HIP_ERROR_SHAPE, "matmul_q8: xscale must have x's shape with a last dimension of 1");
+    const size_t w_scales[2] = {w->shape[0], 1};
+    if (!same_shape(wscale, 2, w_scales)) return fail(CUMO_HIP_ERROR_SHAPE, "matmul_q8: wscale must have w's shape with a last dimension of 1");
+    if (bias && !same_shape(bias, 1, w_scales)) return fail(CUMO_HIP_ERROR_SHAPE, "matmul_q8: bias must be one dimension, a number for each row of w");
+    if (w->shape[1] >= (size_t)1 << 17) return fail(CUMO_HIP_ERROR_ARGUMENT, "matmul_q8: rows are too long for sums of 32 bits");
+    want[nd - 1] = w->shape[0];
+    rc = check_result(y, xscale->type, nd, want);
+    if (rc) return rc;
+    Scratch s;
+    s.n = 0;
+    Operand o[5];
+    o[4].given = NULL;
+    Result r;
+    int nr = 0;
+    rc = take(&o[0], x, ROWS, 0, &s);
+    if (!rc) rc = take(&o[1], w, ROWS, 0, &s);
+    if (!rc) rc = take(&o[2], xscale, DENSE, 0, &s);
+    if (!rc) rc = take(&o[3], wscale, DENSE, 0, &s);
+    if (!rc && bias) rc = take(&o[4], bias, DENSE, 0, &s);
+    if (!rc) rc = make(&r, y, xscale->type, nd, want, ROWS, 0, o, 5, &s), nr = 1;
+    if (!rc && total_of(r.use)) {
+        cumo_hip_matmul_q8_t d;
+        d.rows = total_of(xscale);
+        d.inner = w->shape[1];
+        d.cols = w->shape[0];
+        d.x = o[0].at();
+        d.x_step = o[0].step[0];
+        d.w = o[1].at();
+        d.w_step = o[1].step[0];
+        d.xscale = o[2].at();
+        d.wscale = o[3].at();
+        d.bias = bias ? o[4].at() : NULL;
+        d.y = r.at();
+        d.y_step = r.step[0];
+        rc = cumo_hip_matmul_q8_kernel_launch(xscale->type, &d);
+    }
+    return finish(rc, &r, nr, &s);
+}
+
+int cumo_hip_na_rotary(const cumo_hip_narray_t* x, const cumo_hip_narray_t* positions, const cumo_hip_narray_t* frequencies, int interleaved, int inverse,
+                       double amplitude, cumo_hip_narray_t* y) {
+    int rc = check_float(x, "rotary: the array is not SFloat or DFloat");
+    if (!rc) rc = check_view(positions, "operand");
+    if (!rc) rc = check_view(frequencies, "operand");
+    if (rc) return rc;
+    if (positions->type != CUMO_HIP_INT32) return fail(CUMO_HIP_ERROR_TYPE, "rotary: positions are Int32");
+    if (frequencies->type != CUMO_HIP_DFLOAT) return fail(CUMO_HIP_ERROR_TYPE, "rotary: frequencies are DFloat");
+    const int nd = x->ndim;
+    if (nd < 2) return fail(CUMO_HIP_ERROR_DIMENSION, "rotary needs at least two dimensions, heads and their elements");
+    if (!same_rows(positions, nd - 2, x->shape)) return fail(CUMO_HIP_ERROR_SHAPE, "rotary: positions must have the array's shape without the last two dimensions");
+    if (frequencies->ndim != 1) return fail(CUMO_HIP_ERROR_DIMENSION, "rotary: frequencies must be one dimension");
+    if (frequencies->shape[0] > x->shape[nd - 1] / 2) return fail(CUMO_HIP_ERROR_SHAPE, "rotary: there are more frequencies than pairs of a head's elements");
+    if (!std::isfinite(amplitude)) return fail(CUMO_HIP_ERROR_ARGUMENT, "rotary: amplitude must be a finite number");
+    if (x->shape[nd - 1] >= (size_t)1 << 31 || x->shape[nd - 2] >= (size_t)1 << 31) return fail(CUMO_HIP_ERROR_ARGUMENT, "rotary: heads are too long or too many");
+    rc = check_result(y, x->type, nd, x->shape);
+    if (rc) return rc;
+    Scratch s;
+    s.n = 0;
+    Operand o[3];
+    Result r;
+    int nr = 0;
+    rc = take(&o[0], x, HEADS, 0, &s);
+    if (!rc) rc = take(&o[1], positions, DENSE, 0, &s);
+    if (!rc) rc = take(&o[2], frequencies, DENSE, 0, &s);
+    if (!rc) rc = make(&r, y, x->type, nd, x->shape, HEADS, 0, o, 3, &s), nr = 1;
+    if (!rc && total_of(x)) {
+        cumo_hip_rotary_t d;
+        d.batch = 1;
+        for (int k = 0; k < nd - 3; ++k) d.batch *= x->shape[k];
+        d.time = nd > 2 ? x->shape[nd - 3] : 1;
+        d.heads = x->shape[nd - 2];
+        d.dim = x->shape[nd - 1];
+        d.pairs = frequencies->shape[0];
+        std::memcpy(d.x_step, o[0].step, sizeof(d.x_step));
+        std::memcpy(d.y_step, r.step, sizeof(d.y_step));
+        d.x = o[0].at();
+        d.y = r.at();
+        d.positions = reinterpret_cast<const int32_t*>(o[1].at());
+        d.frequencies = reinterpret_cast<const double*>(o[2].at());
+        d.amplitude = amplitude;
+        d.interleaved = interleaved != 0;
+        d.inverse = inverse != 0;
+        cumo_hip_rotary_kernel_launch(x->type, &d);
+    }
+    return finish(rc, &r, nr, &s);
+}
+
+}  // extern "C"
+
+namespace {
+
+const char kAttentionType[] = "linear_attention: operands are SFloat or DFloat, all of one type, lengths Int32";
+
+// whether an array is batch x time x heads x n, of which n is given (0: whatever it is), as are the others where they are not NULL
+int attention_operand(const NA* a, int type, const NA* like, size_t n) {
+    const int rc = check_float(a, kAttentionType);
+    if (rc) return rc;
+    if (a->type != type) return fail(CUMO_HIP_ERROR_TYPE, kAttentionType);
+    if (a->ndim != 4) return fail(CUMO_HIP_ERROR_DIMENSION, "linear_attention: the arrays must have four dimensions");
+    if (a->shape[0] != like->shape[0] || a->shape[1] != like->shape[1]) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: the arrays must have the same sequences and steps");
+    if (a->shape[3] != n) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: heads of k must be as long as those of q, heads of g as those of v");
+    return CUMO_HIP_OK;
+}
+
+int attention_operands(const NA* q, const NA* k, const NA* v, const NA* decay, const NA* state, const NA* lengths, double scale, size_t* state_shape) {
+    int rc = check_float(q, kAttentionType);
+    if (!rc) rc = check_float(v, kAttentionType);
+    if (rc) return rc;
+    if (q->ndim != 4 || v->ndim != 4) return fail(CUMO_HIP_ERROR_DIMENSION, "linear_attention: the arrays must have four dimensions");
+    rc = attention_operand(k, q->type, q, q->shape[3]);
+    if (!rc) rc = attention_operand(v, q->type, q, v->shape[3]);
+    if (rc) return rc;
+    if (k->shape[2] != v->shape[2]) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: k and v must have the same heads");
+    if (k->shape[2] ? q->shape[2] % k->shape[2] != 0 : q->shape[2] != 0) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: heads of q must be a multiple of those of k");
+    if (q->shape[3] > 256 || v->shape[3] > 256) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: heads of more than 256 elements");
+    if (!std::isfinite(scale)) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: scale must be a finite number");
+    rc = check_float(decay, kAttentionType);
+    if (rc) return rc;
+    if (decay->type != q->type) return fail(CUMO_HIP_ERROR_TYPE, kAttentionType);
+    if (decay->ndim != 1 || decay->shape[0] != q->shape[2]) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: decay must be one dimension, a number for each head of q");
+    state_shape[0] = q->shape[0];
+    state_shape[1] = q->shape[2];
+    state_shape[2] = q->shape[3];
+    state_shape[3] = v->shape[3];
+    if (state) {
+        rc = check_float(state, kAttentionType);
+        if (rc) return rc;
+        if (state->type != q->type) return fail(CUMO_HIP_ERROR_TYPE, kAttentionType);
+        if (!same_shape(state, 4, state_shape)) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: a state must have the shape sequences, heads of q, elements of k, elements of v");
+    }
+    if (lengths) {
+        rc = check_view(lengths, "operand");
+        if (rc) return rc;
+        if (lengths->type != CUMO_HIP_INT32) return fail(CUMO_HIP_ERROR_TYPE, kAttentionType);
+        if (!same_shape(lengths, 1, q->shape)) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: lengths must be one dimension, a number for each sequence");
+    }
+    // blocks are counted in 32 bits, as are the steps
+    if (q->shape[1] >= (size_t)1 << 31 || q->shape[0] * q->shape[2] >= (size_t)1 << 21) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: too many steps or heads");
+    return CUMO_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cumo_hip_na_linear_attention(const cumo_hip_narray_t* q, const cumo_hip_narray_t* k, const cumo_hip_narray_t* v, const cumo_hip_narray_t* decay,
+                                 const cumo_hip_narray_t* state, const cumo_hip_narray_t* lengths, double scale, cumo_hip_narray_t* o,
+                                 cumo_hip_narray_t* last) {
+    size_t state_shape[4];
+    int rc = attention_operands(q, k, v, decay, state, lengths, scale, state_shape);
+    if (rc) return rc;
+    size_t o_shape[4] = {q->shape[0], q->shape[1], q->shape[2], v->shape[3]};
+    rc = check_result(o, q->type, 4, o_shape);
+    if (!rc && last) rc = check_result(last, q->type, 4, state_shape);
+    const NA* const z[2] = {o, last};
+    if (!rc) rc = results_apart(z, 2);
+    if (rc) return rc;
+    Scratch s;
+    s.n = 0;
+    Operand in[6];
+    in[4].given = in[5].given = NULL;
+    Result r[2];
+    int nr = 0;
+    rc = take(&in[0], q, HEADS, 0, &s);
+    if (!rc) rc = take(&in[1], k, HEADS, 0, &s);
+    if (!rc) rc = take(&in[2], v, HEADS, 0, &s);
+    if (!rc) rc = take(&in[3], decay, DENSE, 0, &s);
+    if (!rc && state) rc = take(&in[4], state, DENSE, 0, &s);
+    if (!rc && lengths) rc = take(&in[5], lengths, DENSE, 0, &s);
+    if (!rc) rc = make(&r[nr++], o, q->type, 4, o_shape, HEADS, 0, in, 6, &s);
+    if (!rc && last) rc = make(&r[nr++], last, q->type, 4, state_shape, DENSE, 0, in, 6, &s);
+    if (!rc) {
+        cumo_hip_linear_attention_t d;
+        d.batch = q->shape[0];
+        d.time = q->shape[1];
+        d.heads = q->shape[2];
+        d.shared = k->shape[2];
+        d.dim = q->shape[3];
+        d.wide = v->shape[3];
+        std::memcpy(d.q_step, in[0].step, sizeof(d.q_step));
+        std::memcpy(d.k_step, in[1].step, sizeof(d.k_step));
+        std::memcpy(d.v_step, in[2].step, sizeof(d.v_step));
+        std::memcpy(d.o_step, r[0].step, sizeof(d.o_step));
+        d.q = in[0].at();
+        d.k = in[1].at();
+        d.v = in[2].at();
+        d.decay = in[3].at();
+        d.state = state ? in[4].at() : NULL;
+        d.lengths = lengths ? reinterpret_cast<const int32_t*>(in[5].at()) : NULL;
+        d.scale = scale;
+        d.o = r[0].at();
+        d.last = last ? r[1].at() : NULL;
+        // (elements of neither: nothing to do. Of q and k alone: no state, and every o is 0)
+        if (d.batch && d.heads && d.wide && (d.time || d.last)) rc = cumo_hip_linear_attention_kernel_launch(q->type, &d);
+    }
+    return finish(rc, r, nr, &s);
+}
+
+int cumo_hip_na_linear_attention_grad(const cumo_hip_narray_t* g, const cumo_hip_narray_t* q, const cumo_hip_narray_t* k, const cumo_hip_narray_t* v,
+                                      const cumo_hip_narray_t* decay, const cumo_hip_narray_t* state, const cumo_hip_narray_t* glast,
+                                      const cumo_hip_narray_t* lengths, double scale, cumo_hip_narray_t* gq, cumo_hip_narray_t* gk,
+                                      cumo_hip_narray_t* gv, cumo_hip_narray_t* gstate) {
+    size_t state_shape[4];
+    int rc = attention_operands(q, k, v, decay, state, lengths, scale, state_shape);
+    if (!rc) rc = attention_operand(g, q->type, q, v->shape[3]);
+    if (rc) return rc;
+    if (g->shape[2] != q->shape[2]) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: g must have the heads of q");
+    if (glast) {
+        rc = check_float(glast, kAttentionType);
+        if (rc) return rc;
+        if (glast->type != q->type) return fail(CUMO_HIP_ERROR_TYPE, kAttentionType);
+        if (!same_shape(glast, 4, state_shape)) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: glast must have the shape of a state");
+    }
+    if ((state != NULL) != (gstate != NULL)) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention_grad: gstate is the gradient of state");
+    rc = check_result(gq, q->type, 4, q->shape);
+    if (!rc) rc = check_result(gk, q->type, 4, k->shape);
+    if (!rc) rc = check_result(gv, q->type, 4, v->shape);
+    if (!rc && gstate) rc = check_result(gstate, q->type, 4, state_shape);
+    const NA* const z[4] = {gq, gk, gv, gstate};
+    if (!rc) rc = results_apart(z, 4);
+    if (rc) return rc;
+    Scratch s;
+    s.n = 0;
+    Operand in[8];
+    in[5].given = in[6].given = in[7].given = NULL;
+    Result r[4];
+    int nr = 0;
+    rc = take(&in[0], g, HEADS, 0, &s);
+    if (!rc) rc = take(&in[1], q, HEADS, 0, &s);
+    if (!rc) rc = take(&in[2], k, HEADS, 0, &s);
+    if (!rc) rc = take(&in[3], v, HEADS, 0, &s);
+    if (!rc) rc = take(&in[4], decay, DENSE, 0, &s);
+    if (!rc && state) rc = take(&in[5], state, DENSE, 0, &s);
+    if (!rc && glast) rc = take(&in[6], glast, DENSE, 0, &s);
+    if (!rc && lengths) rc = take(&in[7], lengths, DENSE, 0, &s);
+    if (!rc) rc = make(&r[nr++], gq, q->type, 4, q->shape, HEADS, 0, in, 8, &s);
+    if (!rc) rc = make(&r[nr++], gk, q->type, 4, k->shape, HEADS, 0, in, 8, &s);
+    if (!rc) rc = make(&r[nr++], gv, q->type, 4, v->shape, HEADS, 0, in, 8, &s);
+    if (!rc && gstate) rc = make(&r[nr++], gstate, q->type, 4, state_shape, DENSE, 0, in, 8, &s);
+    if (!rc) {
+        cumo_hip_linear_attention_grad_t d;
+        d.batch = q->shape[0];
+        d.time = q->shape[1];
+        d.heads = q->shape[2];
+        d.shared = k->shape[2];
+        d.dim = q->shape[3];
+        d.wide = v->shape[3];
+        std::memcpy(d.g_step, in[0].step, sizeof(d.g_step));
+        std::memcpy(d.q_step, in[1].step, sizeof(d.q_step));
+        std::memcpy(d.k_step, in[2].step, sizeof(d.k_step));
+        std::memcpy(d.v_step, in[3].step, sizeof(d.v_step));
+        std::memcpy(d.gq_step, r[0].step, sizeof(d.gq_step));
+        std::memcpy(d.gk_step, r[1].step, sizeof(d.gk_step));
+        std::memcpy(d.gv_step, r[2].step, sizeof(d.gv_step));
+        d.g = in[0].at();
+        d.q = in[1].at();
+        d.k = in[2].at();
+        d.v = in[3].at();
+        d.decay = in[4].at();
+        d.state = state ? in[5].at() : NULL;
+        d.glast = glast ? in[6].at() : NULL;
+        d.lengths = lengths ? reinterpret_cast<const int32_t*>(in[7].at()) : NULL;
+        d.scale = scale;
+        d.gq = r[0].at();
+        d.gk = r[1].at();
+        d.gv = r[2].at();
+        d.gstate = gstate ? r[3].at() : NULL;
+        if (d.batch && d.heads && (d.time || d.gstate)) rc = cumo_hip_linear_attention_grad_kernel_launch(q->type, &d);
+    }
+    return finish(rc, r, nr, &s);
 }
 
 }  // extern "C"

@@ -299,6 +299,79 @@ __global__ __launch_bounds__(kRnWide) void rmsnorm_long_kernel(cumo_hip_rmsnorm_
     }
 }
 
+// Rows in 8 bits as they are: the nearest integer of x / scale, to even where two are as near. x times 1 / scale gives it or, next to the
+// middle of two, a neighbour; what it leaves of x, one fused multiply-add, is exact, and says which. `b`: 1 / scale, of numbers lifted
+// by a power of two where it would be infinite.
+template <class T>
+__device__ __forceinline__ T qz_lift(T scale) { return scale < (sizeof(T) == 4 ? (T)0x1p-100f : (T)0x1p-1000) ? (T)0x1p64f : (T)1; }
+template <class T>
+__device__ __forceinline__ int8_t qz_byte(T x, T scale, T b, bool kept) {
+    T q;
+    if constexpr (sizeof(T) == 4) q = __builtin_rintf(x * b);
+    else q = __builtin_rint(x * b);
+    T r;
+    if constexpr (sizeof(T) == 4) r = __builtin_fmaf(-q, scale, x);
+    else r = __builtin_fma(-q, scale, x);
+    const T two = r + r, far = two < (T)0 ? -two : two;
+    int z = (int)q;
+    if (far > scale || (far == scale && (z & 1))) z += two < (T)0 ? -1 : 1;
+    z = z < -127 ? -127 : z > 127 ? 127 : z;
+    return (int8_t)(kept ? z : 0);
+}
+template <class T>
+struct QzScale {
+    T scale, lifted, lift, b;
+    bool kept;
+    __device__ __forceinline__ QzScale(double most) : scale((T)(most / 127.0)), lift(qz_lift(scale)) {
+        kept = scale > (T)0 && scale < (T)INFINITY;
+        lifted = scale * lift;
+        b = kept ? (T)1 / lifted : (T)0;
+    }
+    __device__ __forceinline__ int8_t byte(T x) const { return qz_byte<T>(kept ? x * lift : (T)0, lifted, b, kept); }
+};
+
+template <class T, int TPR, int NV, int BLOCK, bool NT>
+__global__ __launch_bounds__(BLOCK) void quantize_kernel(cumo_hip_quantize_t p) {
+    typedef RnRow<T, TPR, NV> Row;
+    constexpr int RPB = BLOCK / TPR;
+    const uint32_t lane = threadIdx.x % TPR;
+    const uint32_t vectors = (uint32_t)p.n / Row::V, behind = (uint32_t)p.n % Row::V;
+    for (uint64_t first = (uint64_t)blockIdx.x * RPB; first < p.rows; first += (uint64_t)gridDim.x * RPB) {
+        const uint64_t mine = first + threadIdx.x / TPR;
+        const bool there = mine < p.rows;
+        const int64_t row = there ? (int64_t)mine : 0;
+        const uint32_t whole = there ? vectors : 0, rest = there ? behind : 0;
+        Row s;
+        s.template load<NT>(p.x + row * p.x_step, lane, whole, rest, vectors != 0);
+        T most = (T)0;
+        bool nan = false;
+        s.each([&](T& v, int, int) {
+            nan |= v != v;
+            const T size = v < (T)0 ? -v : v;
+            most = size > most ? size : most;
+        });
+        double all[1] = {nan ? __builtin_nan("") : (double)most};
+        rn_allreduce<TPR, BLOCK>(all, rn_max_nan);
+        const QzScale<T> to(all[0]);
+        if (there && lane == 0) reinterpret_cast<T*>(p.scale)[row] = to.scale;
+        s.store_bytes(p.q + row * p.q_step, lane, whole, rest, [&](int k, int j) { return to.byte(s.at(k, j)); });
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kRnWide) void quantize_long_kernel(cumo_hip_quantize_t p) {
+    for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* x = reinterpret_cast<const T*>(p.x + (int64_t)row * p.x_step);
+        double most[1] = {0.0};
+        for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) most[0] = rn_max_nan(most[0], fabs((double)x[i]));
+        rn_allreduce<kRnWide, kRnWide>(most, rn_max_nan);
+        const QzScale<T> to(most[0]);
+        if (threadIdx.x == 0) reinterpret_cast<T*>(p.scale)[row] = to.scale;
+        int8_t* q = reinterpret_cast<int8_t*>(p.q + (int64_t)row * p.q_step);
+        for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) q[i] = to.byte(x[i]);
+    }
+}
+
 // V numbers to a lane and turn: 4 (DFloat 2) bytes in, 16 bytes out
 constexpr int kDqBlock = 256;
 template <class T, int TPR, bool NT>
@@ -563,6 +636,32 @@ void rn_launch(const cumo_hip_rmsnorm_t& d, hipStream_t stream) {
     cumo_cuda_runtime_check_kernel_launch();
 }
 
+template <class T, int TPR, int NV, int BLOCK>
+void qz_launch_one(const cumo_hip_quantize_t& d, bool nt, hipStream_t stream) {
+    constexpr int RPB = BLOCK / TPR;
+    const dim3 grid(rn_grid((d.rows + RPB - 1) / RPB, 256u * 64u)), block(BLOCK);
+    if (nt) hipLaunchKernelGGL((quantize_kernel<T, TPR, NV, BLOCK, true>), grid, block, 0, stream, d);
+    else hipLaunchKernelGGL((quantize_kernel<T, TPR, NV, BLOCK, false>), grid, block, 0, stream, d);
+}
+
+template <class T>
+void qz_launch(const cumo_hip_quantize_t& d, hipStream_t stream) {
+    const bool nt = stream_past_caches(d.rows * d.n * (sizeof(T) + 1));
+    const uint64_t nv = d.n / (16 / sizeof(T));
+    if (nv <= 8) qz_launch_one<T, 8, 1, 256>(d, nt, stream);
+    else if (nv <= 32) qz_launch_one<T, 8, 4, 256>(d, nt, stream);
+    else if (nv <= 64) qz_launch_one<T, 16, 4, 256>(d, nt, stream);
+    else if (nv <= 128) qz_launch_one<T, 32, 4, 256>(d, nt, stream);
+    else if (nv <= 256) qz_launch_one<T, 64, 4, 256>(d, nt, stream);
+    else if (nv <= 512) qz_launch_one<T, 256, 2, 256>(d, nt, stream);
+    else if (nv <= 1024) qz_launch_one<T, 256, 4, 256>(d, nt, stream);
+    else if (nv <= 2048) qz_launch_one<T, 512, 4, 512>(d, nt, stream);
+    else if (nv <= 4096) qz_launch_one<T, 1024, 4, 1024>(d, nt, stream);
+    else if (nv <= 8192) qz_launch_one<T, 512, 16, 512>(d, nt, stream);
+    else hipLaunchKernelGGL((quantize_long_kernel<T>), dim3(rn_grid(d.rows, 1u << 20)), dim3(kRnWide), 0, stream, d);
+    cumo_cuda_runtime_check_kernel_launch();
+}
+
 template <class T, int TPR>
 void dq_launch_one(const cumo_hip_dequantize_t& d, hipStream_t stream) {
     constexpr int RPB = kDqBlock / TPR;
@@ -663,6 +762,11 @@ extern "C" void cumo_hip_rmsnorm_kernel_launch(int type, int quantised, const cu
     hipStream_t stream = current_stream();
     if (type == 0) quantised ? rn_launch<float, true>(*d, stream) : rn_launch<float, false>(*d, stream);
     else quantised ? rn_launch<double, true>(*d, stream) : rn_launch<double, false>(*d, stream);
+}
+
+extern "C" void cumo_hip_quantize_kernel_launch(int type, const cumo_hip_quantize_t* d) {
+    if (type == 0) qz_launch<float>(*d, current_stream());
+    else qz_launch<double>(*d, current_stream());
 }
 
 extern "C" void cumo_hip_dequantize_kernel_launch(int type, const cumo_hip_dequantize_t* d) {

@@ -18,6 +18,7 @@ what Int32#sum and Bit#count_true answer, and Int8, which Fused.rmsnorm_q8
 answers). `NMath` carries the module functions, `Fused` the row composites.
 """
 import ctypes as C
+import math
 import numbers
 
 import numpy as np
@@ -900,7 +901,7 @@ class UInt64(NArray):
 
 
 class Int8(NArray):
-    """Result holder (Fused.rmsnorm_q8; Fused.dequantize takes it back)."""
+    """Result holder (Fused.rmsnorm_q8, Fused.quantize; Fused.dequantize takes it back, Fused.matmul_q8 multiplies it)."""
     type_name, type_code, np_dtype, elmsz = "int8", 6, np.int8, 1
 
 
@@ -1144,9 +1145,9 @@ def _one_axis(ndim, axis):
 class _Fused:
     """Composites along rows or an axis in one call (library additions). softmax and layernorm the reference
     writes as chains of array operations (bench/transformer_bench.rb:110-124); layouts that the row kernels do not
-    take fall back to that chain inside the library. The others (rmsnorm, recurrence, sample) are what stands between
-    the matrix products of a recurrent language model. Their operands are SFloat or DFloat, all of one type but for
-    sample's settings and u, and of the shapes that each says: nothing is converted or repeated."""
+    take fall back to that chain inside the library. The others are what a recurrent language model is made of: rmsnorm, recurrence
+    and sample, and for layers whose state is a matrix matmul_q8, rotary and linear_attention. Their operands are SFloat or DFloat, all of
+    one type but for what each says, and of the shapes that each says: nothing is converted or repeated."""
 
     @staticmethod
     def softmax(x):
@@ -1250,6 +1251,107 @@ class _Fused:
             raise ValueError("top_k must be a whole number")
         (t, ts), (p, ps), (m, ms) = (setting(v, float) for v in (temperature, top_p, min_p))
         return _run(_L.cumo_hip_na_sample, _optional(x), _optional(u), t, ts, k, ks, p, ps, m, ms, C.byref(z), results=(z,))
+
+    @staticmethod
+    def quantize(x):
+        """Rows in 8 bits: [q, scale], scale = max|x| / 127 of each row (its last dimension is 1), q Int8 = round(x / scale),
+        to even where two are as near. The weights of matmul_q8; what comes back by dequantize."""
+        done = _native.quantize(x)  # None: the general way
+        if done is not None:
+            return done
+        q, scale = NArrayDesc(), NArrayDesc()
+        return _run(_L.cumo_hip_na_quantize, _optional(x), C.byref(q), C.byref(scale), results=(q, scale))
+
+    @staticmethod
+    def matmul_q8(x, xscale, w, wscale, bias=None):
+        """The rows of x by the rows of w, both Int8 with their scales as rmsnorm_q8 and quantize answer them:
+        y[..., j] = sum(x[...] * w[j]) * xscale * wscale[j] (+ bias[j]), in the scales' type. The sum of products is exact (rows
+        of up to 131071), y is rounded once."""
+        done = _native.matmul_q8(x, xscale, w, wscale, bias)  # None: the general way
+        if done is not None:
+            return done
+        if not isinstance(x, Int8) or not isinstance(w, Int8):
+            raise TypeError("matmul_q8 needs Int8 arrays")
+        dx, dw, y = x._desc(), w._desc(), NArrayDesc()
+        return _run(_L.cumo_hip_na_matmul_q8, C.byref(dx), _optional(xscale), C.byref(dw), _optional(wscale), _optional(bias), C.byref(y), results=(y,))
+
+    @staticmethod
+    def rotary_frequencies(dims, base=10000.0, scaling=None, factor=1.0, trained=0, fast=32.0, slow=1.0):
+        """[frequencies, amplitude] for rotary: base ** (-2 i / dims) for the dims / 2 pairs of a head (DFloat), and 1. For contexts
+        `factor` times longer than those (of `trained` positions) that a model has learnt from, scaling is "linear" (every frequency
+        divided by factor), "base" (the base raised so that the slowest pair turns factor times slower and the fastest as before) or
+        "yarn" (pairs that turn `fast` times or more within `trained` stay, those that turn `slow` times or less are divided by factor, on a line by the
+        pair's index between; amplitude is 1 + 0.1 log(factor))."""
+        if dims < 2 or dims % 2:
+            raise ValueError("dims must be an even number of 2 or more")
+        if not base > 1 or not factor >= 1:
+            raise ValueError("base must be more than 1, factor 1 or more")
+        if scaling not in (None, "linear", "base", "yarn"):
+            raise ValueError("scaling must be None, linear, base or yarn")
+        if scaling == "base":
+            base = base * factor ** (dims / max(dims - 2, 1))
+        f = float(base) ** (-2.0 * np.arange(dims // 2) / dims)
+        amplitude = 1.0
+        if scaling == "linear":
+            f = f / factor
+        if scaling == "yarn":
+            if not trained >= 1 or not fast > slow > 0:
+                raise ValueError("yarn needs the number of trained positions, and fast above slow above 0")
+            pair = lambda turns: dims * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+            low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dims - 1)
+            part = np.clip((np.arange(dims // 2) - low) / max(high - low, 0.001), 0.0, 1.0)
+            f = f * (1 - part) + f / factor * part
+            amplitude = 0.1 * math.log(factor) + 1.0
+        return [DFloat.cast(f), amplitude]
+
+    @staticmethod
+    def rotary(x, positions, frequencies, interleaved=False, inverse=False, amplitude=1.0):
+        """x [..., heads, dim] with the first 2 n elements of its heads turned in n = len(frequencies) pairs: (x[i], x[i + n]), or
+        (x[2 i], x[2 i + 1]) where interleaved, by the angle positions * frequencies[i] (the product in double; of 2^50 or more: NaN), and
+        times amplitude; others are as they were. positions: Int32, x's shape without its last two dimensions; frequencies:
+        DFloat, as rotary_frequencies answers them. inverse turns back: the gradient of x is rotary(that of y, ..., inverse=True)
+        with the same amplitude."""
+        done = _native.rotary(x, positions, frequencies, interleaved, inverse, amplitude)  # None: the general way
+        if done is not None:
+            return done
+        y = NArrayDesc()
+        return _run(_L.cumo_hip_na_rotary, _optional(x), _optional(positions), _optional(frequencies), int(bool(interleaved)), int(bool(inverse)),
+                    float(amplitude), C.byref(y), results=(y,))
+
+    @staticmethod
+    def _attention_scale(q, scale):
+        if scale is not None:
+            return float(scale)
+        shape = NMath._check(q).shape
+        return float(shape[-1]) ** -0.5 if shape and shape[-1] else 1.0
+
+    @staticmethod
+    def linear_attention(q, k, v, decay, state=None, lengths=None, scale=None):
+        """[o, last]: S[t] = decay * S[t-1] + k[t] (x) v[t] for each head, from state or zeros, o[t] = scale * (q[t] by S[t]), last the
+        state behind the last step. q and k are [batch, time, heads, dim], v [batch, time, heads, wide] (transpose(0, 2, 1, 3) of arrays with heads in
+        front), dim and wide 256 at most; k and v may have fewer heads, each for as many of q's in a row. decay has a number for each head of q, state is
+        [batch, heads, dim, wide], lengths (Int32) the steps of each sequence, o being 0 behind them. scale: dim ** -0.5. A prompt and
+        a single token are the same call, with last handed on as state."""
+        scale = _Fused._attention_scale(q, scale)
+        done = _native.linear_attention(q, k, v, decay, state, lengths, scale)  # None: the general way
+        if done is not None:
+            return done
+        o, last = NArrayDesc(), NArrayDesc()
+        return _run(_L.cumo_hip_na_linear_attention, _optional(q), _optional(k), _optional(v), _optional(decay), _optional(state), _optional(lengths),
+                    scale, C.byref(o), C.byref(last), results=(o, last))
+
+    @staticmethod
+    def linear_attention_grad(g, q, k, v, decay, state=None, glast=None, lengths=None, scale=None):
+        """The gradients of q, k and v, and of state where it is given, from g, that of o, and glast, that of last, if it has one: [gq, gk, gv]
+        or [gq, gk, gv, gstate]. Decay is taken for a constant of the model: it has none."""
+        scale = _Fused._attention_scale(q, scale)
+        done = _native.linear_attention_grad(g, q, k, v, decay, state, glast, lengths, scale)  # None: the general way
+        if done is not None:
+            return done
+        z = tuple(NArrayDesc() for _ in range(3 if state is None else 4))
+        return _run(_L.cumo_hip_na_linear_attention_grad, _optional(g), _optional(q), _optional(k), _optional(v), _optional(decay), _optional(state),
+                    _optional(glast), _optional(lengths), scale, C.byref(z[0]), C.byref(z[1]), C.byref(z[2]),
+                    None if state is None else C.byref(z[3]), results=z)
 
 
 Fused = _Fused()

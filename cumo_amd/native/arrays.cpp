@@ -671,6 +671,74 @@ PyObject* na_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// a number that a caller means as yes or no
+bool yes_or_no(PyObject* o, int* yes) {
+    if (!PyBool_Check(o)) return false;
+    *yes = o == Py_True;
+    return true;
+}
+
+// (x)
+PyObject* na_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 1)) return nullptr;
+    Optional in;
+    Desc z[2];
+    if (!take_all(&in, a, 1) || !in.given) GENERAL_FORM_ANSWERS();
+    return run_list(z, 2, [&] { cumo_hip_na_quantize(in.given, &z[0], &z[1]); });
+}
+
+// (x, xscale, w, wscale, bias)
+PyObject* na_matmul_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 5)) return nullptr;
+    const View *x = as_view(a[0]), *w = as_view(a[2]);
+    Optional xscale, wscale, bias;
+    Desc dx, dw, z;
+    if (!x || x->code != CUMO_HIP_INT8 || !w || w->code != CUMO_HIP_INT8 || !take_all(&xscale, a + 1, 1) || !xscale.given || !take_all(&wscale, a + 3, 1) ||
+        !wscale.given || !take_all(&bias, a + 4, 1))
+        GENERAL_FORM_ANSWERS();
+    if (describe(x, &dx) < 0 || describe(w, &dw) < 0) return nullptr;
+    return run_list(&z, 1, [&] { cumo_hip_na_matmul_q8(&dx, xscale.given, &dw, wscale.given, bias.given, &z); });
+}
+
+// (x, positions, frequencies, interleaved, inverse, amplitude)
+PyObject* na_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 6)) return nullptr;
+    Optional in[3];
+    int interleaved, inverse;
+    double amplitude;
+    Desc z;
+    if (!yes_or_no(a[3], &interleaved) || !yes_or_no(a[4], &inverse) || !plain_number(a[5], &amplitude) || !take_all(in, a, 3) || !in[0].given || !in[1].given ||
+        !in[2].given)
+        GENERAL_FORM_ANSWERS();
+    return run_list(&z, 1, [&] { cumo_hip_na_rotary(in[0].given, in[1].given, in[2].given, interleaved, inverse, amplitude, &z); });
+}
+
+// (q, k, v, decay, state, lengths, scale)
+PyObject* na_linear_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 7)) return nullptr;
+    Optional in[6];
+    double scale;
+    Desc z[2];
+    if (!plain_number(a[6], &scale) || !take_all(in, a, 6) || !in[0].given || !in[1].given || !in[2].given || !in[3].given) GENERAL_FORM_ANSWERS();
+    return run_list(z, 2, [&] {
+        cumo_hip_na_linear_attention(in[0].given, in[1].given, in[2].given, in[3].given, in[4].given, in[5].given, scale, &z[0], &z[1]);
+    });
+}
+
+// (g, q, k, v, decay, state, glast, lengths, scale)
+PyObject* na_linear_attention_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!arity(n, 9)) return nullptr;
+    Optional in[8];
+    double scale;
+    Desc z[4];
+    if (!plain_number(a[8], &scale) || !take_all(in, a, 8) || !in[0].given || !in[1].given || !in[2].given || !in[3].given || !in[4].given) GENERAL_FORM_ANSWERS();
+    const bool state = in[5].given != nullptr;
+    return run_list(z, state ? 4 : 3, [&] {
+        cumo_hip_na_linear_attention_grad(in[0].given, in[1].given, in[2].given, in[3].given, in[4].given, in[5].given, in[6].given, in[7].given, scale, &z[0], &z[1],
+                                          &z[2], state ? &z[3] : nullptr);
+    });
+}
+
 // (self, positions): self[positions] for a one-dimensional array of 64-bit positions in the first dimension; None where the general
 // form answers (other kinds of positions, positions out of range, empty results; arrays of a class derived from the registered
 // ones, whose selections are of that class). x[2048 rows] 27.4 -> 8.5 us of the caller's time.
@@ -860,7 +928,8 @@ PyObject* set_recording(PyObject*, PyObject* rec) {
 #define CALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(na_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CALL(binary), CALL(compare), CALL(unary), CALL(math), CALL(reduce), CALL(mulsum), CALL(cum), CALL(bit_binary),
                          CALL(bit_count), CALL(take), CALL(window), CALL(rmsnorm), CALL(rmsnorm_q8), CALL(dequantize), CALL(rmsnorm_grad),
-                         CALL(recurrence), CALL(recurrence_grad), CALL(sample), {"setup", setup, METH_VARARGS, nullptr}, {"set_recording", set_recording, METH_O, nullptr}, {}};
+                         CALL(recurrence), CALL(recurrence_grad), CALL(sample), CALL(quantize), CALL(matmul_q8), CALL(rotary), CALL(linear_attention), CALL(linear_attention_grad),
+                         {"setup", setup, METH_VARARGS, nullptr}, {"set_recording", set_recording, METH_O, nullptr}, {}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "cumo_amd._native", "Buffers, views and calls of the array classes.", -1, methods};
 

@@ -732,6 +732,102 @@ typedef struct {
 } cumo_hip_sample_t;
 int cumo_hip_sample_kernel_launch(int type, const cumo_hip_sample_t* d);
 
+/* Rows in 8 bits with a scale each (no counterpart in the reference): scale[k] = max|x| / 127 of
+ * row k, rounded to the type, and q = round(x / scale), between -127 and 127; ties go to even. A
+ * row of zeros has the scale 0, one with a NaN the scale NaN, one with an infinity that scale; q
+ * is 0 there. rows runs of n contiguous elements, row k of an array at its start + k * its step
+ * (bytes); type 0 SFloat, 1 DFloat. No result may overlap the operand. */
+typedef struct {
+    uint64_t rows, n;
+    ssize_t  x_step, q_step;
+    const char* x;
+    char*    q;
+    char*    scale;
+} cumo_hip_quantize_t;
+void cumo_hip_quantize_kernel_launch(int type, const cumo_hip_quantize_t* d);
+
+/* The product of 8-bit rows by 8-bit rows (no counterpart in the reference):
+ *   y[i][j] = (sum over k < inner of x[i][k] * w[j][k]) * xscale[i] * wscale[j] + bias[j]
+ * The sum is exact in 32 bits for inner < 2^17; what follows is in double, rounded once to type
+ * (0 SFloat, 1 DFloat), which the scales and bias (NULL: none) have as well, contiguous each.
+ * Steps from row to row in bytes. y may overlap no operand. CUMO_HIP_OK or the error reported. */
+typedef struct {
+    uint64_t rows, inner, cols;
+    ssize_t  x_step, w_step, y_step;
+    const char* x;
+    const char* w;
+    const char* xscale;
+    const char* wscale;
+    const char* bias;
+    char*    y;
+} cumo_hip_matmul_q8_t;
+int cumo_hip_matmul_q8_kernel_launch(int type, const cumo_hip_matmul_q8_t* d);
+
+/* Rotary positions (no counterpart in the reference): the first 2 * pairs elements of every head
+ * of dim elements are turned in pairs (u, v), which are x[i] and x[i + pairs], or where interleaved
+ * x[2 i] and x[2 i + 1], by the angle t = position * frequencies[i] (the product in double):
+ *   (u cos t - v sin t, v cos t + u sin t) * amplitude;   inverse: by -t
+ * The others are copied. batch x time x heads heads of contiguous elements, three byte steps in
+ * that order; positions: batch x time contiguous numbers. type 0 SFloat, 1 DFloat (of x and y).
+ * y is x or does not overlap it. */
+typedef struct {
+    uint64_t batch, time, heads, dim, pairs;
+    ssize_t  x_step[3], y_step[3];
+    const char* x;
+    char*    y;
+    const int32_t* positions;
+    const double* frequencies;
+    double   amplitude;
+    int      interleaved, inverse;
+} cumo_hip_rotary_t;
+void cumo_hip_rotary_kernel_launch(int type, const cumo_hip_rotary_t* d);
+
+/* Linear attention with a decay a for each head (no counterpart in the reference):
+ *   S[t] = a * S[t-1] + k[t] (x) v[t];   o[t] = scale * (S[t] by q[t])
+ * for q and k of dim and v and o of wide elements (256 at most each), contiguous; three byte steps
+ * an array, of sequence, step and head. q and o have heads, k and v shared heads, each used by
+ * heads / shared of q's in a row. decay: heads contiguous numbers. state: S[-1], batch x heads x dim x wide
+ * contiguous elements, NULL for zeros; last: S behind the last step, alike, NULL where it is
+ * not wanted. lengths: the steps of each sequence (between 0 and time; others are brought there),
+ * NULL: time; o is 0 behind them, and last is S[length - 1]. type 0 SFloat, 1 DFloat. No result may
+ * overlap an operand. CUMO_HIP_OK or the error reported. */
+typedef struct {
+    uint64_t batch, time, heads, shared, dim, wide;
+    ssize_t  q_step[3], k_step[3], v_step[3], o_step[3];
+    const char* q;
+    const char* k;
+    const char* v;
+    const char* decay;
+    const char* state;
+    const int32_t* lengths;
+    double   scale;
+    char*    o;
+    char*    last;
+} cumo_hip_linear_attention_t;
+int cumo_hip_linear_attention_kernel_launch(int type, const cumo_hip_linear_attention_t* d);
+/* Its gradients from g (of o) and glast (of last; NULL: zeros), with G[t] = a * G[t+1] +
+ * scale * (q[t] (x) g[t]), a * G behind the last step being glast:
+ *   gq[t] = scale * (S[t] by g[t]);  gk[t] = G[t] by v[t];  gv[t] = G[t] by k[t];  gstate = a * G[0]
+ * gk and gv are summed over the heads that share k and v. gstate: NULL where it is not wanted. */
+typedef struct {
+    uint64_t batch, time, heads, shared, dim, wide;
+    ssize_t  g_step[3], q_step[3], k_step[3], v_step[3], gq_step[3], gk_step[3], gv_step[3];
+    const char* g;
+    const char* q;
+    const char* k;
+    const char* v;
+    const char* decay;
+    const char* state;
+    const char* glast;
+    const int32_t* lengths;
+    double   scale;
+    char*    gq;
+    char*    gk;
+    char*    gv;
+    char*    gstate;
+} cumo_hip_linear_attention_grad_t;
+int cumo_hip_linear_attention_grad_kernel_launch(int type, const cumo_hip_linear_attention_grad_t* d);
+
 /* Product sums of many rows in one launch (the reference launches
  * cumo_<type>_mulsum_reduce_kernel_launch once per row from a host loop,
  * gen/tmpl/accum_binary.c:20-45): out[r] += sum_i p1[r][i] * p2[r][i] for rows of n
@@ -862,7 +958,7 @@ size_t cumo_hip_pool_free_bytes(void);
 size_t cumo_hip_pool_total_bytes(void);
 /* bytes and calls that went to hipMalloc since the process started */
 size_t cumo_hip_pool_device_malloc_calls(void);
-/* Memory of graphs. Calls of cumo_hip_na_rmsnorm to _sample, and the launchers behind them, that are captured
+/* Memory of graphs. Calls of cumo_hip_na_rmsnorm to _linear_attention_grad, and the launchers behind them, that are captured
  * leave what they hold beside their results to the graph, in use. capture_id: the number of the capture that the calling
  * thread's stream is in, 0 if none. captured_blocks: how many pieces a capture has left so (0: all captures).
  * captured_free gives them back to the pool and answers their number. The graph, and what has been

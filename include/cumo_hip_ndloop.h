@@ -38,7 +38,8 @@ extern "C" {
 /* Element types on the path (reference: the classes of gen/def/{sfloat,dfloat,
  * int32,int64,uint64,bit}.rb). Int64/UInt64 only appear as results (Int32#sum,
  * arg reductions over more than 2^32-1 elements, Bit#count_true), and so does Int8 (what
- * cumo_hip_na_rmsnorm_q8 answers: copied, read back, taken by cumo_hip_na_dequantize). */
+ * cumo_hip_na_rmsnorm_q8 and cumo_hip_na_quantize answer: copied, read back, taken by
+ * cumo_hip_na_dequantize and cumo_hip_na_matmul_q8). */
 enum {
     CUMO_HIP_SFLOAT = 0,
     CUMO_HIP_DFLOAT = 1,
@@ -328,6 +329,34 @@ int cumo_hip_na_recurrence_grad(const cumo_hip_narray_t* g, const cumo_hip_narra
 int cumo_hip_na_sample(const cumo_hip_narray_t* x, const cumo_hip_narray_t* u, double temperature, const cumo_hip_narray_t* temperatures,
                        ssize_t top_k, const cumo_hip_narray_t* top_ks, double top_p, const cumo_hip_narray_t* top_ps,
                        double min_p, const cumo_hip_narray_t* min_ps, cumo_hip_narray_t* z);
+/* quantize: q (Int8, x's shape) and scale (x's shape with a last dimension of 1) of x's rows, as
+ * cumo_hip_quantize_kernel_launch says: what the weights of matmul_q8 are made with.
+ * matmul_q8: y = the rows of x by the rows of w, as cumo_hip_matmul_q8_kernel_launch says. x: Int8, with xscale
+ * of its shape with a last dimension of 1 (what rmsnorm_q8 and quantize answer); w: Int8 of two
+ * dimensions, with wscale of one number a row (its shape with a last dimension of 1); rows are shorter than 2^17. bias: one dimension, a
+ * number for each row of w, or NULL. y has x's shape with a last dimension of w's rows, and the scales' type. */
+int cumo_hip_na_quantize(const cumo_hip_narray_t* x, cumo_hip_narray_t* q, cumo_hip_narray_t* scale);
+int cumo_hip_na_matmul_q8(const cumo_hip_narray_t* x, const cumo_hip_narray_t* xscale, const cumo_hip_narray_t* w, const cumo_hip_narray_t* wscale,
+                          const cumo_hip_narray_t* bias, cumo_hip_narray_t* y);
+/* rotary: y = x (time x heads x dim behind any other dimensions; heads x dim is one step) with the pairs of
+ * its heads turned, as cumo_hip_rotary_kernel_launch says. positions: Int32, x's shape without the
+ * last two dimensions; frequencies: DFloat of one dimension, half of dim or fewer. The gradient of
+ * x is the same call with inverse on that of y. */
+int cumo_hip_na_rotary(const cumo_hip_narray_t* x, const cumo_hip_narray_t* positions, const cumo_hip_narray_t* frequencies, int interleaved, int inverse,
+                       double amplitude, cumo_hip_narray_t* y);
+/* linear_attention: o and last (NULL: not wanted) as cumo_hip_linear_attention_kernel_launch says, for q and k of batch x time x
+ * heads x dim and v of batch x time x heads x wide, dim and wide 256 at most, in any strides (heads in front of time is a transposed
+ * view). k and v may have fewer heads, a divisor of q's. decay: one dimension, a number a head; state
+ * and last: batch x heads x dim x wide; lengths: Int32, one dimension, a number a sequence. Long sequences go in stretches of steps,
+ * whose products and sums are in the arrays' type; a step's output depends on no later step, whatever that holds.
+ * linear_attention_grad: gq, gk, gv and gstate (NULL when state is) from g (of o) and glast (of last, or NULL). */
+int cumo_hip_na_linear_attention(const cumo_hip_narray_t* q, const cumo_hip_narray_t* k, const cumo_hip_narray_t* v, const cumo_hip_narray_t* decay,
+                                 const cumo_hip_narray_t* state, const cumo_hip_narray_t* lengths, double scale, cumo_hip_narray_t* o,
+                                 cumo_hip_narray_t* last);
+int cumo_hip_na_linear_attention_grad(const cumo_hip_narray_t* g, const cumo_hip_narray_t* q, const cumo_hip_narray_t* k, const cumo_hip_narray_t* v,
+                                      const cumo_hip_narray_t* decay, const cumo_hip_narray_t* state, const cumo_hip_narray_t* glast,
+                                      const cumo_hip_narray_t* lengths, double scale, cumo_hip_narray_t* gq, cumo_hip_narray_t* gk,
+                                      cumo_hip_narray_t* gv, cumo_hip_narray_t* gstate);
 
 /* Bit logic: and or xor eq / copy not (reference: gen/tmpl_bit/binary.c, unary.c). */
 int cumo_hip_na_bit_binary(const char* op, const cumo_hip_narray_t* x, const cumo_hip_narray_t* y, cumo_hip_narray_t* z);
