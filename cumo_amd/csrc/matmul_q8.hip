@@ -1,35 +1,295 @@
-// The product of 8-bit rows by 8-bit rows, y[i][j] = (sum of x[i][k] w[j][k]) xscale[i] wscale[j] + bias[j].
+// The product of 8-bit rows by 8-bit rows, y[i][j] = (sum of x[i][k] w[j][k]) xscale[i] wscale[j] + bias[j], by matrix instructions of
+// 16 x 16 x 64 bytes whose sums are 32-bit integers: exact, in whatever order, so that how inner is cut changes no bit.
+//
+// w is the first operand and x the second: a lane has four neighbouring numbers of a row of y. What follows the sum is in double and
+// rounded once.
 #include "common.h"
 
 namespace cumo_hip {
 namespace {
 
-// what a sum stands for, in double and rounded once
-template <class T>
-__device__ __forceinline__ T mq_value(int sum, double xs, double ws, double bias) { return (T)__builtin_fma((double)sum * xs, ws, bias); }
+typedef int32_t mq_i4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ mq_i4 mq_mma(mq_i4 a, mq_i4 b, mq_i4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+
+// sixteen bytes on any boundary
+__device__ __forceinline__ mq_i4 mq_read(const char* p) {
+    mq_i4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+// the first n of them, zeros behind (n may be 0 or less: nothing is read)
+__device__ __forceinline__ mq_i4 mq_read_part(const char* p, int64_t n) {
+    if (n >= 16) return mq_read(p);
+    union { mq_i4 v; int8_t b[16]; } u;
+    u.v = mq_i4{0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 15; ++k) u.b[k] = k < n ? (int8_t)p[k] : (int8_t)0;
+    return u.v;
+}
+
+struct MqParams : cumo_hip_matmul_q8_t {
+    int32_t* parts;    // [splits][rows][cols], where inner is cut
+    uint32_t splits;
+    uint64_t per;      // bytes of a row that a split takes
+    uint32_t tiles_m, tiles_n;
+};
 
 template <class T>
-__global__ __launch_bounds__(256) void matmul_q8_kernel(cumo_hip_matmul_q8_t p) {
-    const uint64_t total = p.rows * p.cols;
-    for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (uint64_t)gridDim.x * 256) {
-        const uint64_t i = at / p.cols, j = at - i * p.cols;
-        const int8_t* x = reinterpret_cast<const int8_t*>(p.x + (int64_t)i * p.x_step);
-        const int8_t* w = reinterpret_cast<const int8_t*>(p.w + (int64_t)j * p.w_step);
-        int sum = 0;
-        for (uint64_t k = 0; k < p.inner; ++k) sum += (int)x[k] * (int)w[k];
-        const T* bias = reinterpret_cast<const T*>(p.bias);
-        reinterpret_cast<T*>(p.y + (int64_t)i * p.y_step)[j] =
-            mq_value<T>(sum, (double)reinterpret_cast<const T*>(p.xscale)[i], (double)reinterpret_cast<const T*>(p.wscale)[j], bias ? (double)bias[j] : 0.0);
+struct MqOut {
+    T t[4];
+};
+// four numbers of row i from column j on, from their sums
+template <class T>
+__device__ __forceinline__ void mq_put(const cumo_hip_matmul_q8_t& p, uint64_t i, uint64_t j, mq_i4 sum) {
+    const double xs = (double)reinterpret_cast<const T*>(p.xscale)[i];
+    T* y = reinterpret_cast<T*>(p.y + (int64_t)i * p.y_step) + j;
+    const T* ws = reinterpret_cast<const T*>(p.wscale) + j;
+    const T* bias = reinterpret_cast<const T*>(p.bias);
+    if (j + 4 <= p.cols) {
+        MqOut<T> s, b, out;
+        __builtin_memcpy(&s, ws, sizeof(s));
+        if (bias) __builtin_memcpy(&b, bias + j, sizeof(b));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const double v = (double)sum[r] * xs;
+            out.t[r] = (T)(bias ? __builtin_fma(v, (double)s.t[r], (double)b.t[r]) : v * (double)s.t[r]);
+        }
+        __builtin_memcpy(y, &out, sizeof(out));
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (j + r >= p.cols) continue;
+            const double v = (double)sum[r] * xs;
+            y[r] = (T)(bias ? __builtin_fma(v, (double)ws[r], (double)bias[j + r]) : v * (double)ws[r]);
+        }
     }
+}
+
+// ---- few rows: a block takes sixteen rows of w, its waves every WAVES-th piece of inner, TM sixteens of x's rows --------------------------------------
+template <class T, int TM, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void matmul_q8_rows_kernel(cumo_hip_matmul_q8_t p) {
+    constexpr int U = TM <= 2 ? 4 : 2;  // pieces of 64 on their way at a time
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const uint64_t j0 = (uint64_t)blockIdx.x * 16;
+    const uint64_t wrow = j0 + m < p.cols ? j0 + m : p.cols - 1;
+    const char* w = p.w + (int64_t)wrow * p.w_step + g * 16;
+    const char* x[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+        const uint64_t row = (uint64_t)t * 16 + m;
+        x[t] = p.x + (int64_t)(row < p.rows ? row : p.rows - 1) * p.x_step + g * 16;
+    }
+    mq_i4 sum[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) sum[t] = mq_i4{0, 0, 0, 0};
+    const uint64_t whole = p.inner / 64;
+    uint64_t piece = wave;
+    for (; piece + (U - 1) * WAVES < whole; piece += U * WAVES) {
+        mq_i4 a[U], b[U][TM];
+#pragma unroll
+        for (int u = 0; u < U; ++u) a[u] = mq_read(w + (piece + u * WAVES) * 64);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int t = 0; t < TM; ++t) b[u][t] = mq_read(x[t] + (piece + u * WAVES) * 64);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int t = 0; t < TM; ++t) sum[t] = mq_mma(a[u], b[u][t], sum[t]);
+        }
+    }
+    for (; piece * 64 < p.inner; piece += WAVES) {
+        const int64_t n = (int64_t)(p.inner - piece * 64) - g * 16;
+        const mq_i4 a = mq_read_part(w + piece * 64, n);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) sum[t] = mq_mma(a, mq_read_part(x[t] + piece * 64, n), sum[t]);
+    }
+    __shared__ mq_i4 slot[WAVES][TM][64];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) slot[wave][t][lane] = sum[t];
+    __syncthreads();
+    for (uint32_t t = wave; t < TM; t += WAVES) {
+        mq_i4 all = slot[0][t][lane];
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) all += slot[k][t][lane];
+        const uint64_t i = (uint64_t)t * 16 + m, j = j0 + 4 * g;
+        if (i < p.rows && j < p.cols) mq_put<T>(p, i, j, all);
+    }
+}
+
+// ---- tiles: BM rows of x by BN of w, 128 bytes of inner at a time through LDS -----------------------------------------------------------
+// A row's eight pieces of sixteen bytes lie in its 128 bytes of LDS in the order piece ^ (row % 8), so that lanes that read one piece of
+// neighbouring rows, and those that write a row, meet in no bank.
+constexpr uint32_t kMqDepth = 128;
+
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void matmul_q8_tiles_kernel(MqParams p) {
+    constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, PIECES = (BM + BN) * 8 / THREADS;
+    __shared__ __attribute__((aligned(16))) char tile[2][(BM + BN) * kMqDepth];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    const uint32_t tiles = p.tiles_m * p.tiles_n, part = blockIdx.x / tiles;
+    uint32_t at = blockIdx.x % tiles;
+    // blocks go to the eight dies in turn: each die takes a run of tiles, in strips of eight tiles of x
+    if (tiles % 8 == 0) at = (at % 8) * (tiles / 8) + at / 8;
+    const uint32_t strip = at / (8 * p.tiles_n), in = at % (8 * p.tiles_n);
+    const uint32_t high = p.tiles_m - strip * 8 < 8 ? p.tiles_m - strip * 8 : 8;
+    const uint64_t i0 = (uint64_t)(strip * 8 + in % high) * BM, j0 = (uint64_t)(in / high) * BN;
+    const uint64_t from = part * p.per, to = from + p.per < p.inner ? from + p.per : p.inner;
+
+    const char* src[PIECES];
+    uint32_t dst[PIECES];
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+        const uint32_t id = threadIdx.x + k * THREADS, row = id / 8, piece = id % 8;
+        dst[k] = row * kMqDepth + ((piece ^ (row & 7)) * 16);
+        if (row < BM) {
+            const uint64_t i = i0 + row < p.rows ? i0 + row : p.rows - 1;
+            src[k] = p.x + (int64_t)i * p.x_step + piece * 16;
+        } else {
+            const uint64_t j = j0 + row - BM < p.cols ? j0 + row - BM : p.cols - 1;
+            src[k] = p.w + (int64_t)j * p.w_step + piece * 16;
+        }
+    }
+    mq_i4 held[PIECES];
+    auto fetch = [&](uint64_t k0) {
+        if (k0 + kMqDepth <= to) {
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) held[k] = mq_read(src[k] + k0);
+        } else {
+            const int64_t n = (int64_t)(to - k0) - (threadIdx.x % 8) * 16;
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) held[k] = mq_read_part(src[k] + k0, n);
+        }
+    };
+    auto place = [&](uint32_t buffer) {
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) *reinterpret_cast<mq_i4*>(&tile[buffer][dst[k]]) = held[k];
+    };
+
+    mq_i4 sum[TN][TM];
+#pragma unroll
+    for (int n = 0; n < TN; ++n) {
+#pragma unroll
+        for (int t = 0; t < TM; ++t) sum[n][t] = mq_i4{0, 0, 0, 0};
+    }
+    const uint32_t x_row = (wave % WM) * (TM * 16) + m, w_row = BM + (wave / WM) * (TN * 16) + m;
+    if (from < to) {
+        fetch(from);
+        place(0);
+    }
+    __syncthreads();
+    uint32_t buffer = 0;
+    for (uint64_t k0 = from; k0 < to; k0 += kMqDepth) {
+        const bool more = k0 + kMqDepth < to;
+        if (more) fetch(k0 + kMqDepth);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t swizzled = ((half * 4 + g) ^ (m & 7)) * 16;
+            mq_i4 a[TN], b[TM];
+#pragma unroll
+            for (int n = 0; n < TN; ++n) a[n] = *reinterpret_cast<const mq_i4*>(&tile[buffer][(w_row + n * 16) * kMqDepth + swizzled]);
+#pragma unroll
+            for (int t = 0; t < TM; ++t) b[t] = *reinterpret_cast<const mq_i4*>(&tile[buffer][(x_row + t * 16) * kMqDepth + swizzled]);
+#pragma unroll
+            for (int n = 0; n < TN; ++n) {
+#pragma unroll
+                for (int t = 0; t < TM; ++t) sum[n][t] = mq_mma(a[n], b[t], sum[n][t]);
+            }
+        }
+        if (more) place(buffer ^ 1);
+        buffer ^= 1;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < TM; ++t) {
+        const uint64_t i = i0 + (wave % WM) * (TM * 16) + t * 16 + m;
+        if (i >= p.rows) continue;
+#pragma unroll
+        for (int n = 0; n < TN; ++n) {
+            const uint64_t j = j0 + (wave / WM) * (TN * 16) + n * 16 + 4 * g;
+            if (j >= p.cols) continue;
+            if (p.splits == 1) {
+                mq_put<T>(p, i, j, sum[n][t]);
+            } else {
+                int32_t* q = p.parts + ((uint64_t)part * p.rows + i) * p.cols + j;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (j + r < p.cols) q[r] = sum[n][t][r];
+            }
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void matmul_q8_parts_kernel(MqParams p) {
+    const uint64_t fours = (p.cols + 3) / 4, total = p.rows * fours;
+    for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (uint64_t)gridDim.x * 256) {
+        const uint64_t i = at / fours, j = (at - i * fours) * 4;
+        mq_i4 sum = {0, 0, 0, 0};
+        for (uint32_t k = 0; k < p.splits; ++k) {
+            const int32_t* q = p.parts + ((uint64_t)k * p.rows + i) * p.cols + j;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[r] += j + r < p.cols ? q[r] : 0;
+        }
+        mq_put<T>(p, i, j, sum);
+    }
+}
+
+template <class T, int BM, int BN, int WM, int WN>
+int mq_tiles(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
+    MqParams p;
+    static_cast<cumo_hip_matmul_q8_t&>(p) = d;
+    p.tiles_m = (uint32_t)((d.rows + BM - 1) / BM);
+    p.tiles_n = (uint32_t)((d.cols + BN - 1) / BN);
+    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
+    // inner is cut where there are fewer tiles than compute units, into parts of 512 bytes or more
+    p.splits = 1;
+    if (tiles < 192) {
+        uint64_t most = d.inner / 512, wanted = 256 / tiles;
+        p.splits = (uint32_t)(wanted < most ? wanted : most);
+        if (p.splits < 1) p.splits = 1;
+    }
+    p.per = ((d.inner + p.splits - 1) / p.splits + kMqDepth - 1) / kMqDepth * kMqDepth;
+    if (p.per == 0) p.per = kMqDepth;
+    char* scratch = nullptr;
+    if (p.splits > 1 && !(scratch = cumo_cuda_runtime_malloc((uint64_t)p.splits * d.rows * d.cols * 4))) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
+    p.parts = reinterpret_cast<int32_t*>(scratch);
+    hipLaunchKernelGGL((matmul_q8_tiles_kernel<T, BM, BN, WM, WN>), dim3((unsigned)(tiles * p.splits)), dim3(64 * WM * WN), 0, stream, p);
+    if (scratch) {
+        const uint64_t blocks = (d.rows * ((d.cols + 3) / 4) + 255) / 256;
+        hipLaunchKernelGGL((matmul_q8_parts_kernel<T>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, stream, p);
+    }
+    cumo_cuda_runtime_check_kernel_launch();
+    if (scratch) scratch_free(scratch);
+    return CUMO_HIP_OK;
+}
+
+template <class T, int TM>
+int mq_rows(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
+    constexpr int WAVES = 8;
+    hipLaunchKernelGGL((matmul_q8_rows_kernel<T, TM, WAVES>), dim3((unsigned)((d.cols + 15) / 16)), dim3(64 * WAVES), 0, stream, d);
+    cumo_cuda_runtime_check_kernel_launch();
+    return CUMO_HIP_OK;
 }
 
 template <class T>
 int mq_launch(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
     if (d.rows == 0 || d.cols == 0) return CUMO_HIP_OK;
-    const uint64_t blocks = (d.rows * d.cols + 255) / 256;
-    hipLaunchKernelGGL((matmul_q8_kernel<T>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, stream, d);
-    cumo_cuda_runtime_check_kernel_launch();
-    return CUMO_HIP_OK;
+    // (tiles are counted in 32 bits, and a launch holds fewer than 2^32 lanes)
+    if (d.rows >= (uint64_t)1 << 31 || d.cols >= (uint64_t)1 << 31 || ((d.rows + 255) / 256) * ((d.cols + 255) / 256) >= (uint64_t)1 << 22) {
+        report_error(CUMO_HIP_ERROR_ARGUMENT, 0, "matmul_q8: too many rows by columns");
+        return CUMO_HIP_ERROR_ARGUMENT;
+    }
+    if (d.rows <= 16) return mq_rows<T, 1>(d, stream);
+    if (d.rows <= 32) return mq_rows<T, 2>(d, stream);
+    if (d.rows <= 64) return mq_rows<T, 4>(d, stream);
+    const uint64_t large = ((d.rows + 255) / 256) * ((d.cols + 255) / 256);
+    if (large >= 192) return mq_tiles<T, 256, 256, 2, 4>(d, stream);
+    const uint64_t middle = ((d.rows + 127) / 128) * ((d.cols + 127) / 128);
+    if (middle >= 128) return mq_tiles<T, 128, 128, 2, 2>(d, stream);
+    return mq_tiles<T, 64, 64, 2, 2>(d, stream);
 }
 
 }  // namespace
