@@ -180,8 +180,9 @@ void la_step(const LaWalk& w, const LaCommon& c, char* memory, hipStream_t strea
 // stretch, as the instruction leaves them: lane (m, g) of 16 x 4 has rows 4 g to 4 g + 3 of its column m. So held, S is the first operand of the
 // next product as it is (S^T by q^T, o transposed), and so is what k by q^T leaves (the masked products, transposed: the second operand of v^T by
 // them); v by columns serves as the second operand of k^T by v and the first of v^T. Nothing is moved between lanes but the products k q^T, of
-// which each of the NW waves works out a share, over its part of dim: they meet in LDS, one barrier a stretch. Operands are read straight
-// from memory as the lanes want them, each as soon as its predecessor has been used, so that they are on their way for most of a stretch.
+// which each of the NW waves works out a share, over its part of dim: they meet in LDS. Rows of q, k and v go through LDS too, a stretch ahead, and
+// are on their way there for a stretch before: read from memory by every wave as its lanes want them, they kept the first-level cache at
+// work for four fifths of the time (SFloat 8 x 2048 x 16 heads of 128: 266 us).
 //
 // Double precision counts rows otherwise (lane (m, g) has rows g, g + 4, ...): operands are read by la_label, so that what
 // stands above holds for it too.
@@ -210,7 +211,8 @@ struct LaWalks {
     LaWalk walk[3];
 };
 
-// rows of an array as a stretch takes them, in its direction: from `low`, unsigned offsets
+// rows of an array as a turn takes them, in its direction: from `low`, unsigned offsets
+template <uint32_t TURN>
 struct LaRows {
     const char* low;
     int64_t advance;
@@ -220,29 +222,85 @@ struct LaRows {
         const int64_t one = backwards ? -steps[1] : steps[1];
         down = one < 0;
         step = (uint32_t)(down ? -one : one);
-        advance = one * (int64_t)kLaStretch;
-        low = p + (int64_t)b * steps[0] + (int64_t)h * steps[2] + (int64_t)first * steps[1] + (down ? one * (int64_t)(kLaStretch - 1) : 0);
+        advance = one * (int64_t)TURN;
+        low = p + (int64_t)b * steps[0] + (int64_t)h * steps[2] + (int64_t)first * steps[1] + (down ? one * (int64_t)(TURN - 1) : 0);
     }
-    __device__ __forceinline__ uint32_t row(uint32_t k) const { return (down ? kLaStretch - 1 - k : k) * step; }
+    __device__ __forceinline__ uint32_t row(uint32_t k) const { return (down ? TURN - 1 - k : k) * step; }
 };
-template <class T>
-__device__ __forceinline__ T la_at(const char* low, uint32_t offset) {
-    T v;
-    __builtin_memcpy(&v, low + offset, sizeof(T));
-    return v;
+
+// LANES lanes to a row of N elements (a multiple of 16) in LDS, of which `cols` are there; 16 bytes of them a lane and turn, or one
+template <class T, int N, int LANES, bool QUADS>
+struct LaStage {
+    static constexpr uint32_t W = QUADS ? 16 / sizeof(T) : 1;             // elements at a time
+    static constexpr int COUNT = (N / (int)W + LANES - 1) / LANES;
+    static constexpr uint32_t ROW = N + 16 / sizeof(T);                   // (lanes that read one column of neighbouring rows meet in no bank)
+    struct Piece { T t[W]; };
+    Piece held[COUNT];
+    __device__ __forceinline__ void fetch(const char* low, uint32_t row_offset, uint32_t lane, uint32_t cols) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const uint32_t c = (lane + (uint32_t)i * LANES) * W;
+            __builtin_memcpy(&held[i], low + (row_offset + (c < cols ? c : 0) * (uint32_t)sizeof(T)), sizeof(Piece));
+        }
+    }
+    // zeros for a row that is not there, and behind its end
+    __device__ __forceinline__ void place(T* rows, uint32_t row, uint32_t lane, uint32_t cols, bool there) const {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const uint32_t c = (lane + (uint32_t)i * LANES) * W;
+            Piece x = held[i];
+#pragma unroll
+            for (uint32_t j = 0; j < W; ++j) x.t[j] = there && c < cols ? x.t[j] : (T)0;
+            if (N % ((int)W * LANES) == 0 || c < N) __builtin_memcpy(__builtin_assume_aligned(rows + row * ROW + c, QUADS ? 16 : sizeof(T)), &x, sizeof(Piece));
+        }
+    }
+};
+
+// the block's waves meet, for what LDS holds alone: loads from memory stay on their way
+__device__ __forceinline__ void la_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// DT: tiles of 16 that hold dim, of which the first FULL are whole. QUADS: rows of dim and of wide are whole fours. ONLY: what a segment
-// leaves by itself. Tiles of q and of k's columns are held a ring of RING at a time, each read again as soon as it has been used.
-template <class T, int DT> constexpr int kLaRing = DT <= (sizeof(T) == 4 ? 8 : 4) ? DT : DT % 4 == 0 ? 4 : 3;
-template <class T, int DT> constexpr int kLaWavesPerSimd = sizeof(T) * DT <= 64 ? 2 : 1;
+// A turn takes two stretches, one behind the other (one, where their rows would fill LDS or the registers that bring them): its rows are in LDS,
+// in two buffers where they fit twice.
+template <class T, int DT> constexpr int kLaSubs = sizeof(T) * DT <= 64 ? 2 : 1;
+template <class T, int DT> constexpr uint32_t kLaTurn = kLaStretch * kLaSubs<T, DT>;
+// products k q^T on their way from wave to wave: those of the next turn may meet those of this one where a turn has one barrier
+template <class T, int DT, int NW> constexpr uint64_t kLaSlots = (kLaSubs<T, DT> == 1 ? 2 : 1) * NW * 256 * sizeof(T);
+template <class T, int DT, int NW> constexpr uint64_t kLaBuffer = kLaTurn<T, DT> * (2 * (DT * 16 * sizeof(T) + 16) + NW * 16 * sizeof(T) + 16);
+template <class T, int DT, int NW> constexpr int kLaBuffers = 2 * kLaBuffer<T, DT, NW> + kLaSlots<T, DT, NW> <= 160 * 1024 ? 2 : 1;
+template <class T, int DT, int NW, bool ONLY>
+constexpr uint64_t kLaShared = kLaBuffers<T, DT, NW> * (kLaBuffer<T, DT, NW> - (ONLY ? kLaTurn<T, DT> * (DT * 16 * sizeof(T) + 16) : 0)) + (ONLY ? 0 : kLaSlots<T, DT, NW>);
+// Waves to a SIMD that the registers are shared out for: two, so 256 of one kind, where a lane holds less (else the compiler spreads them over both
+// kinds, and moves them: also where it knows that LDS, hence told at the launch, holds one block alone).
+template <class T, int DT> constexpr int kLaWaves = sizeof(T) * DT <= 48 ? 2 : 1;
+extern __shared__ __attribute__((aligned(16))) char la_shared[];
 
-template <class T, int DT, int FULL, int NW, bool QUADS, bool ONLY>
-__global__ __launch_bounds__(64 * NW, (kLaWavesPerSimd<T, DT>)) void la_stretch_kernel(LaWalks walks, LaCommon c, LaPlan plan) {
+// DT: tiles of 16 that hold dim. NW: tiles of 16 columns to a block, a wave each. QUADS: rows of dim and of wide are whole fours. ONLY: what a
+// segment leaves by itself.
+template <class T, int DT, int NW, bool QUADS, bool ONLY>
+__global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(LaWalks walks, LaCommon c, LaPlan plan) {
     typedef LaQuad<T> Quad;
     constexpr uint32_t E = sizeof(T);
-    constexpr int PM = (DT + NW - 1) / NW, RING = kLaRing<T, DT>;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4, label = la_label<T>(m);
+    constexpr int SUBS = kLaSubs<T, DT>;
+    constexpr uint32_t TURN = kLaTurn<T, DT>;
+    constexpr int LANES = 4 * NW / SUBS < 4 ? 4 : 4 * NW / SUBS;   // to a row, of a part of the turn's rows at a time
+    constexpr int ROWS = 64 * NW / LANES, LOADS = (int)TURN / ROWS;   // rows that the block brings at a time, and how often
+    constexpr int PARTS = NW / SUBS < 1 ? 1 : NW / SUBS, EACH = NW < SUBS ? SUBS / NW : 1;   // waves to a product k q^T; products to a wave
+    constexpr int PM = DT / PARTS;
+    constexpr int BUFFERS = kLaBuffers<T, DT, NW>;
+    static_assert(DT % PARTS == 0 && DT % 2 == 0, "tiles of dim are shared out whole, and taken in pairs");
+    typedef LaStage<T, DT * 16, LANES, QUADS> Keys;
+    typedef LaStage<T, NW * 16, LANES, QUADS> Values;
+    constexpr uint32_t KEYS = TURN * Keys::ROW, VALUES = TURN * Values::ROW;
+    T* const k_rows = reinterpret_cast<T*>(la_shared);
+    T* const v_rows = k_rows + BUFFERS * KEYS;
+    T* const q_rows = v_rows + BUFFERS * VALUES;
+    Quad* const slot = reinterpret_cast<Quad*>(q_rows + BUFFERS * KEYS);
+    static_assert(sizeof(T) * (BUFFERS * (2 * KEYS + VALUES)) + kLaSlots<T, DT, NW> == kLaShared<T, DT, NW, false> && kLaShared<T, DT, NW, false> <= 160 * 1024, "LDS");
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4, label = la_label<T>(m);
     const uint64_t bh_all = c.batch * c.heads;
     uint64_t at = blockIdx.x;
     const uint64_t bh = at % bh_all;
@@ -255,9 +313,9 @@ __global__ __launch_bounds__(64 * NW, (kLaWavesPerSimd<T, DT>)) void la_stretch_
     const uint32_t D = w.dim, W = w.wide;
     const uint64_t length = la_length(c, b), begin = segment * plan.steps;
     const uint64_t end = begin + plan.steps < length ? begin + plan.steps : length;
-    const uint64_t total = end > begin ? end - begin : 0;
-    const uint32_t e0 = (slice * NW + wave) * 16;             // the wave's columns
-    const uint32_t e_in = e0 + label < W ? e0 + label : W - 1;  // (columns behind the last are computed as that one, and not written)
+    const uint32_t total = end > begin ? (uint32_t)(end - begin) : 0;
+    const uint32_t b0 = slice * NW * 16, e0 = b0 + wave * 16;     // the block's columns, and the wave's
+    const uint32_t cols = W - b0 < NW * 16 ? W - b0 : NW * 16;
     const bool column = e0 + label < W;
     const double a = (double)reinterpret_cast<const T*>(c.decay)[h];
     const bool late = w.backwards;
@@ -270,238 +328,275 @@ __global__ __launch_bounds__(64 * NW, (kLaWavesPerSimd<T, DT>)) void la_stretch_
         const T* s = reinterpret_cast<const T*>(from) + bh * D * W;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) S[dt] = Quad{(T)0, (T)0, (T)0, (T)0};
-        if (!ONLY && from) {
+        if (!ONLY && from && column) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const uint32_t d = dt * 16 + 4 * g + r;
-                    S[dt][r] = s[(d < D ? d : D - 1) * row + e_in * col];   // (rows behind the last meet zeros of q, and are not written)
+                    const T x = s[(d < D ? d : D - 1) * row + (e0 + label) * col];
+                    S[dt][r] = d < D ? x : (T)0;
                 }
             }
         }
     }
 
     const uint64_t first = w.backwards ? (length ? length - 1 - begin : 0) : begin;
-    LaRows q(w.q, w.q_step, b, h / w.q_share, first, w.backwards), k(w.k, w.k_step, b, h / w.k_share, first, w.backwards), v(w.v, w.v_step, b, h / w.v_share, first, w.backwards);
+    LaRows<TURN> q(w.q, w.q_step, b, h / w.q_share, first, w.backwards), k(w.k, w.k_step, b, h / w.k_share, first, w.backwards), v(w.v, w.v_step, b, h / w.v_share, first, w.backwards);
+    v.low += b0 * E;
     char* o = w.o + (int64_t)b * w.o_step[0] + (int64_t)h * w.o_step[2] + (int64_t)first * w.o_step[1];
     const int64_t o_one = w.backwards ? -w.o_step[1] : w.o_step[1];
 
-    // where the lanes read, for stretches of n steps (rows behind the last are read as that one)
-    uint32_t q_at, k_at, v_at[4], kc_at[4];
-    auto places = [&](uint32_t n) {
-        auto in = [&](uint32_t row) { return row < n ? row : n - 1; };
-        q_at = q.row(in(m));
-        k_at = k.row(in(label));
+    // Every lane brings parts of rows; rows behind the last are read as that one. One turn's rows are on their way while another's are worked
+    // on; behind the last, those again.
+    const uint32_t my_row = threadIdx.x / LANES, my_lane = threadIdx.x % LANES;
+    Keys q_held[LOADS], k_held[LOADS];
+    Values v_held[LOADS];
+    uint32_t sent = 0;   // steps sent for, up to the last turn
+    auto of_turn = [&](uint32_t done) { return total - done < TURN ? total - done : TURN; };
+    auto fetch = [&] {
+        const uint32_t n = of_turn(sent);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            kc_at[r] = k.row(in(4 * g + r));
-            v_at[r] = v.row(in(4 * g + r)) + e_in * E;
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t row = my_row + i * ROWS < n ? my_row + i * ROWS : n - 1;
+            if constexpr (!ONLY) q_held[i].fetch(q.low, q.row(row), my_lane, D);
+            k_held[i].fetch(k.low, k.row(row), my_lane, D);
+            v_held[i].fetch(v.low, v.row(row), my_lane, cols);
         }
+        const bool more = sent + TURN < total;
+        sent += more ? TURN : 0;
+        q.low += more ? q.advance : 0;
+        k.low += more ? k.advance : 0;
+        v.low += more ? v.advance : 0;
     };
-    // four neighbours of a row from d on; behind the end of dim anything that is there
-    auto quad = [&](const char* low, uint32_t row, uint32_t d) {
-        Quad x;
-        if constexpr (QUADS) {
-            __builtin_memcpy(&x, low + (row + (d < D ? d : D - 4) * E), sizeof(x));
-        } else {
+    auto place = [&](uint32_t buffer, uint32_t n) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = la_at<T>(low, row + (d + r < D ? d + r : D - 1) * E);
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t row = my_row + i * ROWS;
+            if constexpr (!ONLY) q_held[i].place(q_rows + buffer * KEYS, row, my_lane, D, row < n);
+            k_held[i].place(k_rows + buffer * KEYS, row, my_lane, D, row < n);
+            v_held[i].place(v_rows + buffer * VALUES, row, my_lane, cols, row < n);
         }
-        return x;
-    };
-    auto cut = [&](Quad x, uint32_t d) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = d + r < D ? x[r] : (T)0;
-        return x;
     };
 
-    Quad Q[RING], KC[RING], V, PQ[PM], PK[PM];
-    auto read_q = [&](int dt) {
-        if (QUADS && dt < FULL) __builtin_memcpy(&Q[dt % RING], q.low + (q_at + (dt * 16 + 4 * g) * E), sizeof(Quad));
-        else Q[dt % RING] = quad(q.low, q_at, dt * 16 + 4 * g);
-    };
-    auto read_p = [&] {
-#pragma unroll
-        for (int i = 0; i < PM; ++i) {
-            const uint32_t d = (wave + NW * i) * 16 + 4 * g;
-            PQ[i] = quad(q.low, q_at, d);
-            PK[i] = quad(k.low, k_at, d);
-        }
-    };
-    auto read_v = [&] {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) V[r] = la_at<T>(v.low, v_at[r]);
-    };
-    auto read_k = [&](int dt) {
-        const uint32_t d = dt * 16 + label, col = (dt < FULL || d < D ? d : D - 1) * E;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) KC[dt % RING][r] = la_at<T>(k.low, kc_at[r] + col);
-    };
-
-    // decays: of the products of step i = m with steps j = 4 g + r, of what S gives to step i, of what step j leaves
-    T decay_p[4], decay_k[4], decay_q, decay_s;
+    // decays: of the products of step i = m with steps j = 4 g + r, of what S gives to step i, of what step j of a stretch leaves
+    T decay_p[4], decay_k[SUBS][4], decay_q, decay_s[SUBS];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const uint32_t j = 4 * g + r;
         decay_p[r] = j <= m ? (T)(la_power(a, m - j) * w.k_scale) : (T)0;
     }
     decay_q = (T)la_power(a, m + (late ? 0 : 1));
-    auto ends = [&](uint32_t n) {
+    T o_scale = (T)w.o_scale;
+    asm("" : "+v"(o_scale));   // (held: read from the arguments in every turn, it would wait for all that LDS has been asked for)
+    auto ends = [&](uint32_t of_all) {   // a turn of so many steps
+#pragma unroll 1
+        for (int sub = 0; sub < SUBS; ++sub) {
+            const uint32_t n = of_all <= sub * kLaStretch ? 0 : of_all - sub * kLaStretch < kLaStretch ? of_all - sub * kLaStretch : kLaStretch;
+            T k4[4], s1 = (T)la_power(a, n);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t j = 4 * g + r;
-            decay_k[r] = j < n ? (T)(la_power(a, n - 1 - j + (late ? 1 : 0)) * w.k_scale) : (T)0;
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t j = 4 * g + r;
+                k4[r] = j < n ? (T)(la_power(a, n - 1 - j + (late ? 1 : 0)) * w.k_scale) : (T)0;
+            }
+#pragma unroll
+            for (int to = 0; to < SUBS; ++to) {
+                decay_s[to] = sub == to ? s1 : decay_s[to];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) decay_k[to][r] = sub == to ? k4[r] : decay_k[to][r];
+            }
         }
-        decay_s = (T)la_power(a, n);
     };
 
-    __shared__ Quad slot[NW > 1 && !ONLY ? 2 : 1][NW][64];
-    uint64_t left = total;
-    if (left) {
-    {
-        const uint32_t n = left < kLaStretch ? (uint32_t)left : kLaStretch;
-        places(n);
-        ends(n);
-        // (in the order of the loop below: what a turn waits for is counted from the last load)
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!ONLY) {
-            read_p();
-            __builtin_amdgcn_sched_barrier(0);
+    // A turn, in the order in which the wave goes through it. What LDS has of the tiles is asked for well ahead of the products that take it (left to
+    // itself the compiler asks in front of each pair of them), and the waves meet where products are left to be worked on:
+    //   k q^T of the turn, shared out; with S of the first stretch q S, and meanwhile columns of k asked for, S decayed, the next turn's rows put into LDS
+    //   meet: the shares of k q^T are there;  k^T v of the stretch, between them what k q^T gives, and rows of q asked for;  q S of the second stretch
+    //   meet: the next turn's rows are there;  k^T v, meanwhile the first rows of that turn asked for
+    if (total) {
+        ends(TURN);
+        fetch();
+        place(0, of_turn(0));
+        if constexpr (BUFFERS == 2) fetch();
+        la_meet();
+        uint32_t buffer = 0, done = 0;
+        const T *qr = q_rows, *kr = k_rows, *vr = v_rows;
+        Quad V, F[DT];   // (F: rows of q, and each, once used, columns of k, and then those of q again)
+        Quad PQ[ONLY ? 1 : EACH][ONLY ? 1 : PM], PK[ONLY ? 1 : EACH][ONLY ? 1 : PM];
+        auto read_v = [&](int sub) {
 #pragma unroll
-            for (int dt = 0; dt < RING; ++dt) {
-                read_q(dt);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        read_v();
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int dt = 0; dt < RING; ++dt) {
-            read_k(dt);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    uint32_t turn = 0;
-    do {
-        const uint32_t n = left < kLaStretch ? (uint32_t)left : kLaStretch;
-        left -= n;
-        const uint32_t next = left < kLaStretch ? (uint32_t)left : kLaStretch;
-        // What is read ahead is of the next stretch; behind the last, of that one again. (Tiles that the rings do not hold yet are of this one.)
-        const char *q_low = q.low, *k_low = k.low;
-        const uint32_t q_was = q_at;
-        uint32_t kc_was[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) kc_was[r] = kc_at[r];
-        if (next) {
-            q.low += q.advance;
-            k.low += k.advance;
-            v.low += v.advance;
-            if (next < kLaStretch) places(next);
-        }
-        auto tile_q = [&](int dt) {   // into the ring behind tile dt
-            if (dt + RING < DT) {
-                const char* low = q.low;
-                const uint32_t here = q_at;
-                q.low = q_low, q_at = q_was;
-                read_q(dt + RING);
-                q.low = low, q_at = here;
-            } else {
-                read_q(dt + RING - DT);
-            }
+            for (int r = 0; r < 4; ++r) V[r] = vr[(sub * 16 + 4 * g + r) * Values::ROW + wave * 16 + label];
         };
-        auto tile_k = [&](int dt) {
-            if (dt + RING < DT) {
-                const char* low = k.low;
-                uint32_t here[4];
+        auto read_k = [&](int sub, int dt) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) here[r] = kc_at[r], kc_at[r] = kc_was[r];
-                k.low = k_low;
-                read_k(dt + RING);
-                k.low = low;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) kc_at[r] = here[r];
-            } else {
-                read_k(dt + RING - DT);
-            }
+            for (int r = 0; r < 4; ++r) F[dt][r] = kr[(sub * 16 + 4 * g + r) * Keys::ROW + dt * 16 + label];
         };
-        if constexpr (!ONLY) {
-            Quad P = {(T)0, (T)0, (T)0, (T)0};
+        auto read_q = [&](int sub, int dt) { F[dt] = *reinterpret_cast<const Quad*>(qr + (sub * 16 + m) * Keys::ROW + dt * 16 + 4 * g); };
+        auto read_first = [&](int sub, int dt) {
+            if constexpr (ONLY) read_k(sub, dt);
+            else read_q(sub, dt);
+        };
+        auto read_p = [&] {
+            if constexpr (!ONLY) {
+                const int part = wave % PARTS;
 #pragma unroll
-            for (int i = 0; i < PM; ++i) {
-                const Quad x = cut(PQ[i], (wave + NW * i) * 16 + 4 * g);
+                for (int e = 0; e < EACH; ++e) {
+                    const int sub = EACH > 1 ? e : (int)(wave / PARTS);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) P = la_mma(PK[i][r], x[r], P);
-            }
-            read_p();
-            if constexpr (NW > 1) slot[turn & 1][wave][lane] = P;
-            Quad O = {(T)0, (T)0, (T)0, (T)0};
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const Quad x = dt < FULL ? Q[dt % RING] : cut(Q[dt % RING], dt * 16 + 4 * g);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) O = la_mma(S[dt][r], x[r], O);
-                tile_q(dt);
-            }
-            O *= decay_q;
-            if constexpr (NW > 1) {
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-                __builtin_amdgcn_s_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-                P = slot[turn & 1][0][lane];
-#pragma unroll
-                for (int i = 1; i < NW; ++i) P += slot[turn & 1][i][lane];
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) P[r] = 4 * g + r <= m ? P[r] * decay_p[r] : (T)0;
-            // A v that is no number would meet the zeros of the steps before its own: then one step at a time.
-            T odd = (T)0;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) odd = la_fma(V[r], (T)0, odd);
-            if (__builtin_expect(__ballot(odd != odd) == 0, 1)) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) O = la_mma(V[r], P[r], O);
-            } else {
-#pragma unroll 1
-                for (int j = 0; j < 16; ++j) {
-                    const bool mine = (int)g == j / 4;
-                    const Quad zero = {(T)0, (T)0, (T)0, (T)0};
-                    const T vj = j % 4 == 0 ? V[0] : j % 4 == 1 ? V[1] : j % 4 == 2 ? V[2] : V[3], pj = j % 4 == 0 ? P[0] : j % 4 == 1 ? P[1] : j % 4 == 2 ? P[2] : P[3];
-                    const Quad x = la_mma(mine ? vj : (T)0, mine ? pj : (T)0, zero);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) O[r] = (int)m >= j ? O[r] + x[r] : O[r];
+                    for (int i = 0; i < PM; ++i) {
+                        PQ[e][i] = *reinterpret_cast<const Quad*>(qr + (sub * 16 + m) * Keys::ROW + (part * PM + i) * 16 + 4 * g);
+                        PK[e][i] = *reinterpret_cast<const Quad*>(kr + (sub * 16 + label) * Keys::ROW + (part * PM + i) * 16 + 4 * g);
+                    }
                 }
             }
-            if (m < n) {
-                O *= (T)w.o_scale;
-                char* to = o + (int64_t)m * o_one + (uint64_t)(e0 + 4 * g) * E;
-                if constexpr (QUADS) {
-                    if (e0 + 4 * g < W) __builtin_memcpy(to, &O, sizeof(O));
+        };
+        read_p();
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) read_first(0, dt);
+        read_v(0);
+        uint32_t slots = 0;
+        do {
+            const uint32_t n = of_turn(done);
+            done += n;
+            if (n < TURN) ends(n);
+            Quad P[EACH], all[SUBS];
+            if constexpr (!ONLY) {
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) {
+                    Quad one = {(T)0, (T)0, (T)0, (T)0}, two = one;
+#pragma unroll
+                    for (int i = 0; i < PM; ++i) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) (i & 1 ? two : one) = la_mma(PK[e][i][r], PQ[e][i][r], i & 1 ? two : one);
+                    }
+                    P[e] = one + two;
+                }
+            }
+#pragma unroll
+            for (int sub = 0; sub < SUBS; ++sub) {
+                const bool last = sub + 1 == SUBS;
+                const uint32_t here = n <= sub * kLaStretch ? 0 : n - sub * kLaStretch < kLaStretch ? n - sub * kLaStretch : kLaStretch;
+                Quad O = {(T)0, (T)0, (T)0, (T)0}, O2 = O;
+                if constexpr (!ONLY) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt += 2) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            O = la_mma(S[dt][r], F[dt][r], O);
+                            O2 = la_mma(S[dt + 1][r], F[dt + 1][r], O2);
+                        }
+                        S[dt] *= decay_s[sub];
+                        S[dt + 1] *= decay_s[sub];
+                        read_k(sub, dt);
+                        read_k(sub, dt + 1);
+                        if (sub == 0 && dt == 0 && NW > 1) slot[slots + wave * 64 + lane] = P[0];
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (sub == 0 && dt == 0) {
+                            if constexpr (BUFFERS == 2) place(buffer ^ 1, done < total ? of_turn(done) : 0);   // (behind the last turn, for nobody)
+                            fetch();
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (e0 + 4 * g + r < W) {
-                            const T one = O[r];
-                            __builtin_memcpy(to + r * E, &one, E);
-                        }
+                    for (int dt = 0; dt < DT; ++dt) S[dt] *= decay_s[sub];
+                    if (sub == 0) {
+                        if constexpr (BUFFERS == 2) place(buffer ^ 1, done < total ? of_turn(done) : 0);
+                        fetch();
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
+                Quad VW, U = V;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) VW[r] = V[r] * decay_k[sub][r];
+                if (last || (sub == 0 && NW > 1 && !ONLY)) la_meet();
+                if constexpr (!ONLY) {
+                    if (sub == 0) {
+#pragma unroll
+                        for (int to = 0; to < SUBS; ++to) {
+                            if constexpr (NW > 1) {
+                                all[to] = slot[slots + to * PARTS * 64 + lane];
+#pragma unroll
+                                for (int i = 1; i < PARTS; ++i) all[to] += slot[slots + (to * PARTS + i) * 64 + lane];
+                            } else {
+                                all[to] = P[to];
+                            }
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) all[to][r] = 4 * g + r <= m ? all[to][r] * decay_p[r] : (T)0;
+                        }
+                        if (SUBS == 1) slots ^= NW * 64;
+                    }
+                }
+                if (last) {   // from here on what is read is the next turn's (behind the last, whatever is there)
+                    if constexpr (BUFFERS == 2) buffer ^= 1;
+                    qr = q_rows + buffer * KEYS, kr = k_rows + buffer * KEYS, vr = v_rows + buffer * VALUES;
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; dt += 2) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        S[dt] = la_mma(F[dt][r], VW[r], S[dt]);
+                        S[dt + 1] = la_mma(F[dt + 1][r], VW[r], S[dt + 1]);
+                    }
+                    if constexpr (BUFFERS == 2) {
+                        read_first(last ? 0 : sub + 1, dt);
+                        read_first(last ? 0 : sub + 1, dt + 1);
+                        if (dt == 0) read_v(last ? 0 : sub + 1);
+                        if (dt == (DT > 2 ? 2 : 0) && last) read_p();
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (!ONLY) {
+                        if (dt == 0) {
+                            O = (O + O2) * decay_q;
+                            // A v that is no number would meet the zeros of the steps before its own: then one step at a time.
+                            T odd = (T)0;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) odd = la_fma(U[r], (T)0, odd);
+                            if (__builtin_expect(__ballot(odd != odd) == 0, 1)) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) O = la_mma(U[r], all[sub][r], O);
+                            } else {
+#pragma unroll 1
+                                for (int j = 0; j < 16; ++j) {
+                                    const bool mine = (int)g == j / 4;
+                                    const Quad zero = {(T)0, (T)0, (T)0, (T)0}, p = all[sub];
+                                    const T vj = j % 4 == 0 ? U[0] : j % 4 == 1 ? U[1] : j % 4 == 2 ? U[2] : U[3], pj = j % 4 == 0 ? p[0] : j % 4 == 1 ? p[1] : j % 4 == 2 ? p[2] : p[3];
+                                    const Quad x = la_mma(mine ? vj : (T)0, mine ? pj : (T)0, zero);
+#pragma unroll
+                                    for (int r = 0; r < 4; ++r) O[r] = (int)m >= j ? O[r] + x[r] : O[r];
+                                }
+                            }
+                        }
+                    }
+                }
+                if constexpr (BUFFERS == 1) {
+                    if (last) {
+                        // (one buffer: every wave has read what it needs, its rows are on their way)
+                        place(0, done < total ? of_turn(done) : 0);
+                        la_meet();
+                        read_p();
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) read_first(last ? 0 : sub + 1, dt);
+                    read_v(last ? 0 : sub + 1);
+                }
+                if (!ONLY && m < here) {
+                    O *= o_scale;
+                    char* to = o + (int64_t)m * o_one + (uint64_t)(e0 + 4 * g) * E;
+                    if constexpr (QUADS) {
+                        if (e0 + 4 * g < W) __builtin_memcpy(to, &O, sizeof(O));
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (e0 + 4 * g + r < W) {
+                                const T one = O[r];
+                                __builtin_memcpy(to + r * E, &one, E);
+                            }
+                    }
+                }
+                if constexpr (!ONLY) o += o_one * (int64_t)kLaStretch;
             }
-            o += o_one * (int64_t)kLaStretch;
-        }
-        Quad VW;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) VW[r] = 4 * g + r < n ? V[r] * decay_k[r] : (T)0;
-        read_v();
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            S[dt] *= decay_s;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) S[dt] = la_mma(KC[dt % RING][r], VW[r], S[dt]);
-            tile_k(dt);
-        }
-        if (next < kLaStretch && next) ends(next);
-        ++turn;
-    } while (left);
+        } while (done < total);
     }
 
     // what is left behind, and what is not there
@@ -549,31 +644,39 @@ __global__ __launch_bounds__(256) void la_starts_kernel(LaWalks walks, LaCommon 
     }
 }
 
-template <class T, int DT, int FULL, int NW, bool QUADS, bool ONLY>
+template <class T, int DT, int NW, bool QUADS, bool ONLY>
 void la_stretch_launch(const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
     const uint64_t blocks = (uint64_t)p.walks * p.segments * p.slices * c.batch * c.heads;
-    hipLaunchKernelGGL((la_stretch_kernel<T, DT, FULL, NW, QUADS, ONLY>), dim3((unsigned)blocks), dim3(64 * NW), 0, stream, walks, c, p);
+    hipLaunchKernelGGL((la_stretch_kernel<T, DT, NW, QUADS, ONLY>), dim3((unsigned)blocks), dim3(64 * NW), (kLaShared<T, DT, NW, ONLY>), stream, walks, c, p);
 }
-template <class T, int DT, int FULL, int NW>
+template <class T, int DT, int NW>
 void la_stretch_quads(bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
-    if (only) la_stretch_launch<T, DT, FULL, NW, true, true>(walks, c, p, stream);
-    else if (walks.walk[0].dim % 4 == 0 && walks.walk[0].wide % 4 == 0) la_stretch_launch<T, DT, FULL, NW, true, false>(walks, c, p, stream);
-    else la_stretch_launch<T, DT, FULL, NW, false, false>(walks, c, p, stream);
+    const bool quads = walks.walk[0].dim % 4 == 0 && walks.walk[0].wide % 4 == 0;
+    if (only) quads ? la_stretch_launch<T, DT, NW, true, true>(walks, c, p, stream) : la_stretch_launch<T, DT, NW, false, true>(walks, c, p, stream);
+    else quads ? la_stretch_launch<T, DT, NW, true, false>(walks, c, p, stream) : la_stretch_launch<T, DT, NW, false, false>(walks, c, p, stream);
 }
-template <class T, int DT, int FULL>
-void la_stretch_waves(uint32_t waves, bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
-    if (waves == 1) la_stretch_quads<T, DT, FULL, 1>(only, walks, c, p, stream);
-    else if (waves == 2) la_stretch_quads<T, DT, FULL, 2>(only, walks, c, p, stream);
-    else la_stretch_quads<T, DT, FULL, 4>(only, walks, c, p, stream);
+// Tiles of columns to a block: as many as wide has, four at most; and four where rows of dim would be too many registers for fewer lanes.
+template <class T>
+uint32_t la_columns(uint32_t dim, uint32_t wide) {
+    const uint32_t bytes = (dim + 31) / 32 * 32 * (uint32_t)sizeof(T);
+    return wide <= 16 && bytes <= 256 ? 1 : wide <= 32 && bytes <= 384 ? 2 : 4;
+}
+template <class T, int DT>
+void la_stretch_columns(uint32_t columns, bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
+    if constexpr (DT * 16 * sizeof(T) <= 256)
+        if (columns == 1) return la_stretch_quads<T, DT, 1>(only, walks, c, p, stream);
+    if constexpr (DT * 16 * sizeof(T) <= 384)
+        if (columns == 2) return la_stretch_quads<T, DT, 2>(only, walks, c, p, stream);
+    la_stretch_quads<T, DT, 4>(only, walks, c, p, stream);
 }
 template <class T>
-void la_stretch(uint32_t dim, uint32_t waves, bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
-    if (dim <= 32) la_stretch_waves<T, 2, 0>(waves, only, walks, c, p, stream);
-    else if (dim <= 64) la_stretch_waves<T, 4, 2>(waves, only, walks, c, p, stream);
-    else if (dim <= 96) la_stretch_waves<T, 6, 4>(waves, only, walks, c, p, stream);
-    else if (dim <= 128) la_stretch_waves<T, 8, 6>(waves, only, walks, c, p, stream);
-    else if (dim <= 192) la_stretch_waves<T, 12, 8>(waves, only, walks, c, p, stream);
-    else la_stretch_waves<T, 16, 12>(waves, only, walks, c, p, stream);
+void la_stretch(uint32_t dim, uint32_t columns, bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
+    if (dim <= 32) la_stretch_columns<T, 2>(columns, only, walks, c, p, stream);
+    else if (dim <= 64) la_stretch_columns<T, 4>(columns, only, walks, c, p, stream);
+    else if (dim <= 96) la_stretch_columns<T, 6>(columns, only, walks, c, p, stream);
+    else if (dim <= 128) la_stretch_columns<T, 8>(columns, only, walks, c, p, stream);
+    else if (dim <= 192) la_stretch_columns<T, 12>(columns, only, walks, c, p, stream);
+    else la_stretch_columns<T, 16>(columns, only, walks, c, p, stream);
 }
 
 // whether a stretch's rows are within 32 bits of each other
@@ -604,12 +707,12 @@ int la_walk(const LaWalk* w, uint32_t n, const LaCommon& c, hipStream_t stream) 
     for (uint32_t k = 0; k < n; ++k) walks.walk[k] = w[k];
     LaPlan p;
     p.walks = n;
-    const uint32_t waves = w[0].wide <= 16 ? 1 : w[0].wide <= 32 ? 2 : 4;
+    const uint32_t waves = la_columns<T>(w[0].dim, w[0].wide);
     p.slices = (w[0].wide + 16 * waves - 1) / (16 * waves);
     p.segments = 1;
     p.steps = (c.time + kLaStretch - 1) / kLaStretch * kLaStretch;
     const uint64_t blocks = (uint64_t)n * p.slices * heads;
-    const uint64_t wanted = 1024 / waves;   // a wave to every SIMD
+    const uint64_t wanted = 1024 / waves;   // a wave to every SIMD, or two
     if (blocks * 2 <= wanted) {
         uint64_t cuts = wanted * 2 / blocks;
         const uint64_t most = (c.time + 255) / 256;
