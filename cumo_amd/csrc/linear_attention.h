@@ -243,8 +243,16 @@ struct LaStage {
             __builtin_memcpy(&held[i], low + (row_offset + (c < cols ? c : 0) * (uint32_t)sizeof(T)), sizeof(Piece));
         }
     }
-    // zeros for a row that is not there, and behind its end
-    __device__ __forceinline__ void place(T* rows, uint32_t row, uint32_t lane, uint32_t cols, bool there) const {
+    // zeros for a row that is not there, and behind its end; `whole`: there is neither
+    __device__ __forceinline__ void place(T* rows, uint32_t row, uint32_t lane, uint32_t cols, bool there, bool whole) const {
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) {
+                const uint32_t c = (lane + (uint32_t)i * LANES) * W;
+                if (N % ((int)W * LANES) == 0 || c < N) __builtin_memcpy(__builtin_assume_aligned(rows + row * ROW + c, QUADS ? 16 : sizeof(T)), &held[i], sizeof(Piece));
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
             const uint32_t c = (lane + (uint32_t)i * LANES) * W;
@@ -270,17 +278,17 @@ template <class T, int DT> constexpr uint32_t kLaTurn = kLaStretch * kLaSubs<T, 
 // products k q^T on their way from wave to wave: those of the next turn may meet those of this one where a turn has one barrier
 template <class T, int DT, int NW> constexpr uint64_t kLaSlots = (kLaSubs<T, DT> == 1 ? 2 : 1) * NW * 256 * sizeof(T);
 template <class T, int DT, int NW> constexpr uint64_t kLaBuffer = kLaTurn<T, DT> * (2 * (DT * 16 * sizeof(T) + 16) + NW * 16 * sizeof(T) + 16);
-template <class T, int DT, int NW> constexpr int kLaBuffers = 2 * kLaBuffer<T, DT, NW> + kLaSlots<T, DT, NW> <= 160 * 1024 ? 2 : 1;
-template <class T, int DT, int NW, bool ONLY>
-constexpr uint64_t kLaShared = kLaBuffers<T, DT, NW> * (kLaBuffer<T, DT, NW> - (ONLY ? kLaTurn<T, DT> * (DT * 16 * sizeof(T) + 16) : 0)) + (ONLY ? 0 : kLaSlots<T, DT, NW>);
+template <class T, int DT, int NW> constexpr bool kLaTwice = 2 * kLaBuffer<T, DT, NW> + kLaSlots<T, DT, NW> <= 160 * 1024;
+template <class T, int DT, int NW, int BUFFERS, bool ONLY>
+constexpr uint64_t kLaShared = BUFFERS * (kLaBuffer<T, DT, NW> - (ONLY ? kLaTurn<T, DT> * (DT * 16 * sizeof(T) + 16) : 0)) + (ONLY ? 0 : kLaSlots<T, DT, NW>);
 // Waves to a SIMD that the registers are shared out for: two, so 256 of one kind, where a lane holds less (else the compiler spreads them over both
 // kinds, and moves them: also where it knows that LDS, hence told at the launch, holds one block alone).
-template <class T, int DT> constexpr int kLaWaves = sizeof(T) * DT <= 48 ? 2 : 1;
+template <class T, int DT> constexpr int kLaWaves = DT <= (sizeof(T) == 4 ? 8 : 2) ? 2 : 1;
 extern __shared__ __attribute__((aligned(16))) char la_shared[];
 
 // DT: tiles of 16 that hold dim. NW: tiles of 16 columns to a block, a wave each. QUADS: rows of dim and of wide are whole fours. ONLY: what a
 // segment leaves by itself.
-template <class T, int DT, int NW, bool QUADS, bool ONLY>
+template <class T, int DT, int NW, int BUFFERS, bool QUADS, bool ONLY>
 __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(LaWalks walks, LaCommon c, LaPlan plan) {
     typedef LaQuad<T> Quad;
     constexpr uint32_t E = sizeof(T);
@@ -290,7 +298,6 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(
     constexpr int ROWS = 64 * NW / LANES, LOADS = (int)TURN / ROWS;   // rows that the block brings at a time, and how often
     constexpr int PARTS = NW / SUBS < 1 ? 1 : NW / SUBS, EACH = NW < SUBS ? SUBS / NW : 1;   // waves to a product k q^T; products to a wave
     constexpr int PM = DT / PARTS;
-    constexpr int BUFFERS = kLaBuffers<T, DT, NW>;
     static_assert(DT % PARTS == 0 && DT % 2 == 0, "tiles of dim are shared out whole, and taken in pairs");
     typedef LaStage<T, DT * 16, LANES, QUADS> Keys;
     typedef LaStage<T, NW * 16, LANES, QUADS> Values;
@@ -299,7 +306,7 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(
     T* const v_rows = k_rows + BUFFERS * KEYS;
     T* const q_rows = v_rows + BUFFERS * VALUES;
     Quad* const slot = reinterpret_cast<Quad*>(q_rows + BUFFERS * KEYS);
-    static_assert(sizeof(T) * (BUFFERS * (2 * KEYS + VALUES)) + kLaSlots<T, DT, NW> == kLaShared<T, DT, NW, false> && kLaShared<T, DT, NW, false> <= 160 * 1024, "LDS");
+    static_assert(sizeof(T) * (BUFFERS * (2 * KEYS + VALUES)) + kLaSlots<T, DT, NW> == kLaShared<T, DT, NW, BUFFERS, false> && kLaShared<T, DT, NW, BUFFERS, false> <= 160 * 1024, "LDS");
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4, label = la_label<T>(m);
     const uint64_t bh_all = c.batch * c.heads;
     uint64_t at = blockIdx.x;
@@ -370,12 +377,13 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(
         v.low += more ? v.advance : 0;
     };
     auto place = [&](uint32_t buffer, uint32_t n) {
+        const bool whole_keys = n == TURN && D == DT * 16, whole_values = n == TURN && cols == NW * 16;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const uint32_t row = my_row + i * ROWS;
-            if constexpr (!ONLY) q_held[i].place(q_rows + buffer * KEYS, row, my_lane, D, row < n);
-            k_held[i].place(k_rows + buffer * KEYS, row, my_lane, D, row < n);
-            v_held[i].place(v_rows + buffer * VALUES, row, my_lane, cols, row < n);
+            if constexpr (!ONLY) q_held[i].place(q_rows + buffer * KEYS, row, my_lane, D, row < n, whole_keys);
+            k_held[i].place(k_rows + buffer * KEYS, row, my_lane, D, row < n, whole_keys);
+            v_held[i].place(v_rows + buffer * VALUES, row, my_lane, cols, row < n, whole_values);
         }
     };
 
@@ -644,16 +652,28 @@ __global__ __launch_bounds__(256) void la_starts_kernel(LaWalks walks, LaCommon 
     }
 }
 
-template <class T, int DT, int NW, bool QUADS, bool ONLY>
-void la_stretch_launch(const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
-    const uint64_t blocks = (uint64_t)p.walks * p.segments * p.slices * c.batch * c.heads;
-    hipLaunchKernelGGL((la_stretch_kernel<T, DT, NW, QUADS, ONLY>), dim3((unsigned)blocks), dim3(64 * NW), (kLaShared<T, DT, NW, ONLY>), stream, walks, c, p);
+template <class T, int DT, int NW, int BUFFERS, bool QUADS, bool ONLY>
+void la_stretch_launch(unsigned blocks, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
+    hipLaunchKernelGGL((la_stretch_kernel<T, DT, NW, BUFFERS, QUADS, ONLY>), dim3(blocks), dim3(64 * NW), (kLaShared<T, DT, NW, BUFFERS, ONLY>), stream, walks, c, p);
 }
-template <class T, int DT, int NW>
-void la_stretch_quads(bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
+template <class T, int DT, int NW, int BUFFERS>
+void la_stretch_quads(unsigned blocks, bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
     const bool quads = walks.walk[0].dim % 4 == 0 && walks.walk[0].wide % 4 == 0;
-    if (only) quads ? la_stretch_launch<T, DT, NW, true, true>(walks, c, p, stream) : la_stretch_launch<T, DT, NW, false, true>(walks, c, p, stream);
-    else quads ? la_stretch_launch<T, DT, NW, true, false>(walks, c, p, stream) : la_stretch_launch<T, DT, NW, false, false>(walks, c, p, stream);
+    if (only) quads ? la_stretch_launch<T, DT, NW, BUFFERS, true, true>(blocks, walks, c, p, stream) : la_stretch_launch<T, DT, NW, BUFFERS, false, true>(blocks, walks, c, p, stream);
+    else quads ? la_stretch_launch<T, DT, NW, BUFFERS, true, false>(blocks, walks, c, p, stream) : la_stretch_launch<T, DT, NW, BUFFERS, false, false>(blocks, walks, c, p, stream);
+}
+// Two buffers where a compute unit still holds two blocks, or gets no more than one. SFloat, heads of 128, one buffer / two: 8 x 2048 x 16 (256 blocks)
+// 235 / 225 us, 32 x 2048 x 16 (1024) 823 / 898; gradients 4 x 2048 x 16 (384) 382 / 444.
+template <class T, int DT, int NW>
+void la_stretch_buffers(bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
+    const unsigned blocks = (unsigned)((uint64_t)p.walks * p.segments * p.slices * c.batch * c.heads);
+    if constexpr (2 * kLaShared<T, DT, NW, 2, false> <= 160 * 1024) {
+        la_stretch_quads<T, DT, NW, 2>(blocks, only, walks, c, p, stream);
+    } else {
+        if constexpr (kLaTwice<T, DT, NW>)
+            if (blocks <= (unsigned)device_compute_units()) return la_stretch_quads<T, DT, NW, 2>(blocks, only, walks, c, p, stream);
+        la_stretch_quads<T, DT, NW, 1>(blocks, only, walks, c, p, stream);
+    }
 }
 // Tiles of columns to a block: as many as wide has, four at most; and four where rows of dim would be too many registers for fewer lanes.
 template <class T>
@@ -664,10 +684,10 @@ uint32_t la_columns(uint32_t dim, uint32_t wide) {
 template <class T, int DT>
 void la_stretch_columns(uint32_t columns, bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
     if constexpr (DT * 16 * sizeof(T) <= 256)
-        if (columns == 1) return la_stretch_quads<T, DT, 1>(only, walks, c, p, stream);
+        if (columns == 1) return la_stretch_buffers<T, DT, 1>(only, walks, c, p, stream);
     if constexpr (DT * 16 * sizeof(T) <= 384)
-        if (columns == 2) return la_stretch_quads<T, DT, 2>(only, walks, c, p, stream);
-    la_stretch_quads<T, DT, 4>(only, walks, c, p, stream);
+        if (columns == 2) return la_stretch_buffers<T, DT, 2>(only, walks, c, p, stream);
+    la_stretch_buffers<T, DT, 4>(only, walks, c, p, stream);
 }
 template <class T>
 void la_stretch(uint32_t dim, uint32_t columns, bool only, const LaWalks& walks, const LaCommon& c, const LaPlan& p, hipStream_t stream) {
@@ -712,7 +732,7 @@ int la_walk(const LaWalk* w, uint32_t n, const LaCommon& c, hipStream_t stream) 
     p.segments = 1;
     p.steps = (c.time + kLaStretch - 1) / kLaStretch * kLaStretch;
     const uint64_t blocks = (uint64_t)n * p.slices * heads;
-    const uint64_t wanted = 1024 / waves;   // a wave to every SIMD, or two
+    const uint64_t wanted = 1024 / waves;   // a wave to every SIMD
     if (blocks * 2 <= wanted) {
         uint64_t cuts = wanted * 2 / blocks;
         const uint64_t most = (c.time + 255) / 256;
