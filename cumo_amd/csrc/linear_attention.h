@@ -202,6 +202,22 @@ __device__ __forceinline__ double la_power(double a, uint64_t n) {
 }
 
 constexpr uint32_t kLaStretch = 16;
+
+// a^n of n up to 16 for many n
+struct LaPowers {
+    double a[5];
+    __device__ __forceinline__ explicit LaPowers(double x) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k, x *= x) a[k] = x;
+    }
+    __device__ __forceinline__ double operator()(uint32_t n) const {
+        double p = n & 1 ? a[0] : 1.0;
+#pragma unroll
+        for (int k = 1; k < 5; ++k) p *= n >> k & 1 ? a[k] : 1.0;
+        return p;
+    }
+};
+
 struct LaPlan {
     uint32_t walks, segments, slices;
     uint64_t steps;         // of a segment, a multiple of kLaStretch
@@ -324,7 +340,7 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(
     const uint32_t b0 = slice * NW * 16, e0 = b0 + wave * 16;     // the block's columns, and the wave's
     const uint32_t cols = W - b0 < NW * 16 ? W - b0 : NW * 16;
     const bool column = e0 + label < W;
-    const double a = (double)reinterpret_cast<const T*>(c.decay)[h];
+    const LaPowers power((double)reinterpret_cast<const T*>(c.decay)[h]);
     const bool late = w.backwards;
 
     // the state
@@ -392,20 +408,20 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const uint32_t j = 4 * g + r;
-        decay_p[r] = j <= m ? (T)(la_power(a, m - j) * w.k_scale) : (T)0;
+        decay_p[r] = j <= m ? (T)(power(m - j) * w.k_scale) : (T)0;
     }
-    decay_q = (T)la_power(a, m + (late ? 0 : 1));
+    decay_q = (T)power(m + (late ? 0 : 1));
     T o_scale = (T)w.o_scale;
     asm("" : "+v"(o_scale));   // (held: read from the arguments in every turn, it would wait for all that LDS has been asked for)
     auto ends = [&](uint32_t of_all) {   // a turn of so many steps
 #pragma unroll 1
         for (int sub = 0; sub < SUBS; ++sub) {
             const uint32_t n = of_all <= sub * kLaStretch ? 0 : of_all - sub * kLaStretch < kLaStretch ? of_all - sub * kLaStretch : kLaStretch;
-            T k4[4], s1 = (T)la_power(a, n);
+            T k4[4], s1 = (T)power(n);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const uint32_t j = 4 * g + r;
-                k4[r] = j < n ? (T)(la_power(a, n - 1 - j + (late ? 1 : 0)) * w.k_scale) : (T)0;
+                k4[r] = j < n ? (T)(power(n - 1 - j + (late ? 1 : 0)) * w.k_scale) : (T)0;
             }
 #pragma unroll
             for (int to = 0; to < SUBS; ++to) {
@@ -631,23 +647,35 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(
     }
 }
 
-// starts[s] from what segment s leaves by itself to what is left behind it: decay^steps times the start of s, and that
+// starts[s] from what segment s leaves by itself to what is left behind it: decay^steps times the start of s, and that. Segments are read eight
+// at a time, as none waits for another (one at a time SFloat 1 x 65536 x 8 heads of 64, 63 of them, took 24 us).
 template <class T>
 __global__ __launch_bounds__(256) void la_starts_kernel(LaWalks walks, LaCommon c, LaPlan plan) {
+    constexpr uint32_t U = 8;
     const LaWalk& w = walks.walk[blockIdx.y];
-    const uint64_t size = (uint64_t)w.dim * w.wide, all = c.batch * c.heads * size;
+    const uint32_t size = w.dim * w.wide;
+    const uint64_t all = c.batch * c.heads * size;
     for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (uint64_t)gridDim.x * 256) {
-        const uint64_t bh = at / size, in = at - bh * size, b = bh / c.heads, h = bh - b * c.heads, d = in / w.wide, e = in - d * w.wide;
+        const uint64_t bh = at / size, b = bh / c.heads;
+        const uint32_t in = (uint32_t)(at - bh * size), d = in / w.wide, e = in - d * w.wide;
         const uint64_t length = la_length(c, b);
-        const double a = (double)reinterpret_cast<const T*>(c.decay)[h];
+        const double a = (double)reinterpret_cast<const T*>(c.decay)[bh - b * c.heads];
         T s = w.state ? reinterpret_cast<const T*>(w.state)[bh * size + d * w.state_row + e * w.state_col] : (T)0;
         T* p = reinterpret_cast<T*>(plan.starts[blockIdx.y]) + at;
         const T whole = (T)la_power(a, plan.steps);
-        for (uint32_t k = 0; k + 1 < plan.segments; ++k) {
-            const uint64_t begin = k * plan.steps;
-            const uint64_t n = begin >= length ? 0 : length - begin < plan.steps ? length - begin : plan.steps;
-            s = la_fma(n == plan.steps ? whole : (T)la_power(a, n), s, p[k * all]);
-            p[k * all] = s;
+        const uint32_t n_starts = plan.segments - 1;
+        for (uint32_t k = 0; k < n_starts; k += U) {
+            T own[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) own[u] = p[(uint64_t)(k + u < n_starts ? k + u : k) * all];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                if (k + u >= n_starts) continue;
+                const uint64_t begin = (k + u) * plan.steps;
+                const uint64_t n = begin >= length ? 0 : length - begin < plan.steps ? length - begin : plan.steps;
+                s = la_fma(n == plan.steps ? whole : n == 0 ? (T)1 : (T)la_power(a, n), s, own[u]);
+                p[(uint64_t)(k + u) * all] = s;
+            }
         }
     }
 }
@@ -731,11 +759,12 @@ int la_walk(const LaWalk* w, uint32_t n, const LaCommon& c, hipStream_t stream) 
     p.slices = (w[0].wide + 16 * waves - 1) / (16 * waves);
     p.segments = 1;
     p.steps = (c.time + kLaStretch - 1) / kLaStretch * kLaStretch;
-    const uint64_t blocks = (uint64_t)n * p.slices * heads;
-    const uint64_t wanted = 1024 / waves;   // a wave to every SIMD
-    if (blocks * 2 <= wanted) {
-        uint64_t cuts = wanted * 2 / blocks;
-        const uint64_t most = (c.time + 255) / 256;
+    // A sequence is cut where that leaves a block or two, as the registers allow, to each compute unit, and no segment short of 64 steps: all but
+    // the last are then walked twice, the first time for half of the products.
+    const uint64_t blocks = (uint64_t)n * p.slices * heads, units = (uint64_t)device_compute_units();
+    if (blocks * 2 <= units) {
+        uint64_t cuts = units * (w[0].dim <= (sizeof(T) == 4 ? 128 : 32) ? 2 : 1) / blocks;
+        const uint64_t most = (c.time + 63) / 64;
         if (cuts > most) cuts = most;
         if (cuts > 1) {
             p.steps = ((c.time + cuts - 1) / cuts + kLaStretch - 1) / kLaStretch * kLaStretch;
