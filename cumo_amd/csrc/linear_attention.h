@@ -38,14 +38,22 @@ __device__ __forceinline__ uint64_t la_length(const LaCommon& c, uint64_t b) {
     return n < 0 ? 0 : (uint64_t)n < c.time ? (uint64_t)n : c.time;
 }
 
+// the block's waves meet, for what LDS holds alone: loads from memory stay on their way
+__device__ __forceinline__ void la_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // One step, or one after the other where a walk is not one for stretches. LPR lanes hold VE columns each of a row of S, the block's other
 // lanes other rows, each a run of them; S goes through memory from step to step (`memory`: last, or scratch), which every lane reads as it
-// wrote it. A step is bound by the state's bytes: a lane has U vectors of it on their way at a time.
+// wrote it. A step is bound by the state's bytes: a lane has U vectors of it on their way at a time, past the caches where they are many: SFloat
+// 64 x 16 heads of 128 25 us (5.4 TB/s), eight at a time 28, through the caches 40.
 constexpr int kLaStepBlock = 256;
-template <class T, int VE> struct LaColumns { T t[VE]; };
-template <class T, int VE, int LPR, bool LATE>
+template <class T, int VE> struct __attribute__((aligned(sizeof(T) * VE))) LaColumns { T t[VE]; };
+template <class T, int VE, int LPR, bool LATE, bool NT>
 __global__ __launch_bounds__(kLaStepBlock) void la_step_kernel(LaWalk w, LaCommon c, char* memory, uint32_t slices) {
-    constexpr int RG = kLaStepBlock / LPR, U = 8;
+    constexpr int RG = kLaStepBlock / LPR, U = 16;
     typedef LaColumns<T, VE> Columns;
     __shared__ T part[kLaStepBlock * VE];
     __shared__ T qs[256], ks[256];
@@ -63,7 +71,8 @@ __global__ __launch_bounds__(kLaStepBlock) void la_step_kernel(LaWalk w, LaCommo
         Columns x;
         const T* p = from + (uint64_t)d * w.state_row + (uint64_t)e * w.state_col;
         if (near) {
-            __builtin_memcpy(&x, p, sizeof(x));
+            if constexpr (NT && VE * sizeof(T) == 16) *reinterpret_cast<store_u4*>(&x) = __builtin_nontemporal_load(reinterpret_cast<const store_u4*>(p));
+            else __builtin_memcpy(&x, p, sizeof(x));
         } else {
 #pragma unroll
             for (int j = 0; j < VE; ++j) x.t[j] = p[(uint64_t)j * w.state_col];
@@ -73,7 +82,8 @@ __global__ __launch_bounds__(kLaStepBlock) void la_step_kernel(LaWalk w, LaCommo
     auto write = [&](uint32_t d, const Columns& x) {
         T* p = to + (uint64_t)d * w.state_row + (uint64_t)e * w.state_col;
         if (near) {
-            __builtin_memcpy(p, &x, sizeof(x));
+            if constexpr (NT && VE * sizeof(T) == 16) __builtin_nontemporal_store(*reinterpret_cast<const store_u4*>(&x), reinterpret_cast<store_u4*>(p));
+            else __builtin_memcpy(p, &x, sizeof(x));
         } else {
 #pragma unroll
             for (int j = 0; j < VE; ++j) p[(uint64_t)j * w.state_col] = x.t[j];
@@ -85,7 +95,7 @@ __global__ __launch_bounds__(kLaStepBlock) void la_step_kernel(LaWalk w, LaCommo
     char* o = w.o + (int64_t)b * w.o_step[0] + (int64_t)h * w.o_step[2];
     for (uint64_t n = 0; n < length; ++n) {
         const uint64_t t = LATE ? length - 1 - n : n;
-        __syncthreads();
+        la_meet();
         if (threadIdx.x < w.dim) {
             qs[threadIdx.x] = reinterpret_cast<const T*>(q + (int64_t)t * w.q_step[1])[threadIdx.x];
             ks[threadIdx.x] = reinterpret_cast<const T*>(k + (int64_t)t * w.k_step[1])[threadIdx.x] * (T)w.k_scale;
@@ -109,7 +119,7 @@ __global__ __launch_bounds__(kLaStepBlock) void la_step_kernel(LaWalk w, LaCommo
                     for (int j = 0; j < VE; ++j) s[u].t[j] = (T)0;
                 }
             }
-            if (d == d0) __syncthreads();
+            if (d == d0) la_meet();
             if (!there) continue;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -127,7 +137,7 @@ __global__ __launch_bounds__(kLaStepBlock) void la_step_kernel(LaWalk w, LaCommo
         from = to;
 #pragma unroll
         for (int j = 0; j < VE; ++j) part[threadIdx.x * VE + j] = sum[j];
-        __syncthreads();
+        la_meet();
         if (group == 0 && there) {
             Columns all;
 #pragma unroll
@@ -156,15 +166,19 @@ template <class T, int VE, int LPR>
 void la_step_one(const LaWalk& w, const LaCommon& c, char* memory, hipStream_t stream) {
     const uint32_t slices = (w.wide + LPR * VE - 1) / (LPR * VE);
     const dim3 grid((unsigned)(c.batch * c.heads * slices)), block(kLaStepBlock);
-    if (w.backwards) hipLaunchKernelGGL((la_step_kernel<T, VE, LPR, true>), grid, block, 0, stream, w, c, memory, slices);
-    else hipLaunchKernelGGL((la_step_kernel<T, VE, LPR, false>), grid, block, 0, stream, w, c, memory, slices);
+    const bool nt = stream_past_caches(c.batch * c.heads * w.dim * w.wide * sizeof(T) * 2) && c.time == 1;
+    if (w.backwards) hipLaunchKernelGGL((la_step_kernel<T, VE, LPR, true, false>), grid, block, 0, stream, w, c, memory, slices);
+    else if (nt) hipLaunchKernelGGL((la_step_kernel<T, VE, LPR, false, true>), grid, block, 0, stream, w, c, memory, slices);
+    else hipLaunchKernelGGL((la_step_kernel<T, VE, LPR, false, false>), grid, block, 0, stream, w, c, memory, slices);
 }
 
 template <class T>
 void la_step(const LaWalk& w, const LaCommon& c, char* memory, hipStream_t stream) {
     constexpr int V = 16 / (int)sizeof(T);
+    // (few heads: eight lanes to a row, so that more blocks share a head)
     if (w.wide % V == 0) {
-        if (w.wide <= 16 * V) la_step_one<T, V, 16>(w, c, memory, stream);
+        if (w.wide <= 8 * V || c.batch * c.heads * ((w.wide + 32 * V - 1) / (32 * V)) < (uint64_t)device_compute_units()) la_step_one<T, V, 8>(w, c, memory, stream);
+        else if (w.wide <= 16 * V) la_step_one<T, V, 16>(w, c, memory, stream);
         else if (w.wide <= 32 * V) la_step_one<T, V, 32>(w, c, memory, stream);
         else la_step_one<T, V, 64>(w, c, memory, stream);
     } else {
@@ -279,13 +293,6 @@ struct LaStage {
         }
     }
 };
-
-// the block's waves meet, for what LDS holds alone: loads from memory stay on their way
-__device__ __forceinline__ void la_meet() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
 
 // A turn takes two stretches, one behind the other (one, where their rows would fill LDS or the registers that bring them): its rows are in LDS,
 // in two buffers where they fit twice.
