@@ -35,34 +35,45 @@ struct MqParams : cumo_hip_matmul_q8_t {
     uint32_t tiles_m, tiles_n;
 };
 
+template <class T> struct __attribute__((aligned(16))) MqFour { T t[4]; };
+// what stands beside four numbers of a row of y: scales of w, and the bias
 template <class T>
-struct MqOut {
-    T t[4];
-};
-// four numbers of row i from column j on, from their sums
-template <class T>
-__device__ __forceinline__ void mq_put(const cumo_hip_matmul_q8_t& p, uint64_t i, uint64_t j, mq_i4 sum) {
-    const double xs = (double)reinterpret_cast<const T*>(p.xscale)[i];
-    T* y = reinterpret_cast<T*>(p.y + (int64_t)i * p.y_step) + j;
-    const T* ws = reinterpret_cast<const T*>(p.wscale) + j;
-    const T* bias = reinterpret_cast<const T*>(p.bias);
-    if (j + 4 <= p.cols) {
-        MqOut<T> s, b, out;
-        __builtin_memcpy(&s, ws, sizeof(s));
-        if (bias) __builtin_memcpy(&b, bias + j, sizeof(b));
+struct MqBeside {
+    double scale[4], bias[4];
+    __device__ __forceinline__ void read(const cumo_hip_matmul_q8_t& p, uint64_t j) {
+        const T* ws = reinterpret_cast<const T*>(p.wscale);
+        const T* bs = reinterpret_cast<const T*>(p.bias);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const double v = (double)sum[r] * xs;
-            out.t[r] = (T)(bias ? __builtin_fma(v, (double)s.t[r], (double)b.t[r]) : v * (double)s.t[r]);
+            const uint64_t at = j + r < p.cols ? j + r : p.cols - 1;
+            scale[r] = (double)ws[at];
+            bias[r] = bs ? (double)bs[at] : 0.0;
         }
-        __builtin_memcpy(y, &out, sizeof(out));
+    }
+};
+// Four numbers of a row of y from column j on, from their sums; `row`: where the row starts. NT: past the caches. (What is beside them is read before the
+// first is written: y may be any memory for all that the compiler knows, and each would wait for the one before.)
+template <class T, bool NT>
+__device__ __forceinline__ void mq_put(char* row, uint64_t j, uint64_t cols, bool biased, double xs, const MqBeside<T>& beside, mq_i4 sum) {
+    MqFour<T> out;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const double v = (double)sum[r] * xs;
+        out.t[r] = (T)(biased ? __builtin_fma(v, beside.scale[r], beside.bias[r]) : v * beside.scale[r]);
+    }
+    T* y = reinterpret_cast<T*>(row) + j;
+    if (j + 4 <= cols) {
+        if constexpr (NT) {
+            const store_u4* from = reinterpret_cast<const store_u4*>(&out);
+#pragma unroll
+            for (int k = 0; k < (int)(sizeof(out) / 16); ++k) __builtin_nontemporal_store(from[k], reinterpret_cast<store_u4*>(y) + k);
+        } else {
+            __builtin_memcpy(y, &out, sizeof(out));
+        }
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (j + r >= p.cols) continue;
-            const double v = (double)sum[r] * xs;
-            y[r] = (T)(bias ? __builtin_fma(v, (double)ws[r], (double)bias[j + r]) : v * (double)ws[r]);
-        }
+        for (int r = 0; r < 4; ++r)
+            if (j + r < cols) y[r] = out.t[r];
     }
 }
 
@@ -115,7 +126,11 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_q8_rows_kernel(cumo_hip_mat
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) all += slot[k][t][lane];
         const uint64_t i = (uint64_t)t * 16 + m, j = j0 + 4 * g;
-        if (i < p.rows && j < p.cols) mq_put<T>(p, i, j, all);
+        if (i < p.rows && j < p.cols) {
+            MqBeside<T> beside;
+            beside.read(p, j);
+            mq_put<T, false>(p.y + (int64_t)i * p.y_step, j, p.cols, p.bias != nullptr, (double)reinterpret_cast<const T*>(p.xscale)[i], beside, all);
+        }
     }
 }
 
@@ -124,7 +139,7 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_q8_rows_kernel(cumo_hip_mat
 // neighbouring rows, and those that write a row, meet in no bank.
 constexpr uint32_t kMqDepth = 128;
 
-template <class T, int BM, int BN, int WM, int WN>
+template <class T, int BM, int BN, int WM, int WN, bool NT>
 __global__ __launch_bounds__(64 * WM * WN) void matmul_q8_tiles_kernel(MqParams p) {
     constexpr int THREADS = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, PIECES = (BM + BN) * 8 / THREADS;
     __shared__ __attribute__((aligned(16))) char tile[2][(BM + BN) * kMqDepth];
@@ -202,22 +217,35 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_q8_tiles_kernel(MqParams 
         buffer ^= 1;
         __syncthreads();
     }
+    const uint64_t i_first = i0 + (wave % WM) * (TM * 16) + m, j_first = j0 + (wave / WM) * (TN * 16) + 4 * g;
+    if (p.splits == 1) {
+        double xs[TM];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) xs[t] = (double)reinterpret_cast<const T*>(p.xscale)[i_first + t * 16 < p.rows ? i_first + t * 16 : p.rows - 1];
+#pragma unroll
+        for (int n = 0; n < TN; ++n) {
+            const uint64_t j = j_first + n * 16;
+            MqBeside<T> beside;
+            beside.read(p, j);
+#pragma unroll
+            for (int t = 0; t < TM; ++t) {
+                const uint64_t i = i_first + t * 16;
+                if (i < p.rows && j < p.cols) mq_put<T, NT>(p.y + (int64_t)i * p.y_step, j, p.cols, p.bias != nullptr, xs[t], beside, sum[n][t]);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
-        const uint64_t i = i0 + (wave % WM) * (TM * 16) + t * 16 + m;
+        const uint64_t i = i_first + t * 16;
         if (i >= p.rows) continue;
 #pragma unroll
         for (int n = 0; n < TN; ++n) {
-            const uint64_t j = j0 + (wave / WM) * (TN * 16) + n * 16 + 4 * g;
-            if (j >= p.cols) continue;
-            if (p.splits == 1) {
-                mq_put<T>(p, i, j, sum[n][t]);
-            } else {
-                int32_t* q = p.parts + ((uint64_t)part * p.rows + i) * p.cols + j;
+            const uint64_t j = j_first + n * 16;
+            int32_t* q = p.parts + ((uint64_t)part * p.rows + i) * p.cols + j;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (j + r < p.cols) q[r] = sum[n][t][r];
-            }
+            for (int r = 0; r < 4; ++r)
+                if (j + r < p.cols) q[r] = sum[n][t][r];
         }
     }
 }
@@ -233,7 +261,9 @@ __global__ __launch_bounds__(256) void matmul_q8_parts_kernel(MqParams p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) sum[r] += j + r < p.cols ? q[r] : 0;
         }
-        mq_put<T>(p, i, j, sum);
+        MqBeside<T> beside;
+        beside.read(p, j);
+        mq_put<T, false>(p.y + (int64_t)i * p.y_step, j, p.cols, p.bias != nullptr, (double)reinterpret_cast<const T*>(p.xscale)[i], beside, sum);
     }
 }
 
@@ -256,7 +286,9 @@ int mq_tiles(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
     char* scratch = nullptr;
     if (p.splits > 1 && !(scratch = cumo_cuda_runtime_malloc((uint64_t)p.splits * d.rows * d.cols * 4))) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
     p.parts = reinterpret_cast<int32_t*>(scratch);
-    hipLaunchKernelGGL((matmul_q8_tiles_kernel<T, BM, BN, WM, WN>), dim3((unsigned)(tiles * p.splits)), dim3(64 * WM * WN), 0, stream, p);
+    const dim3 grid((unsigned)(tiles * p.splits)), block(64 * WM * WN);
+    if (stream_past_caches(d.rows * d.cols * sizeof(T))) hipLaunchKernelGGL((matmul_q8_tiles_kernel<T, BM, BN, WM, WN, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((matmul_q8_tiles_kernel<T, BM, BN, WM, WN, false>), grid, block, 0, stream, p);
     if (scratch) {
         const uint64_t blocks = (d.rows * ((d.cols + 3) / 4) + 255) / 256;
         hipLaunchKernelGGL((matmul_q8_parts_kernel<T>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, stream, p);
