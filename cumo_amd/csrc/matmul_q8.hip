@@ -80,7 +80,7 @@ __device__ __forceinline__ void mq_put(char* row, uint64_t j, uint64_t cols, boo
 // ---- few rows: a block takes sixteen rows of w, its waves every WAVES-th piece of inner, TM sixteens of x's rows --------------------------------------
 template <class T, int TM, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void matmul_q8_rows_kernel(cumo_hip_matmul_q8_t p) {
-    constexpr int U = TM <= 2 ? 4 : 2;  // pieces of 64 on their way at a time
+    constexpr int U = TM <= 2 ? 4 : TM <= 4 ? 2 : 1;  // pieces of 64 on their way at a time
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     const uint64_t j0 = (uint64_t)blockIdx.x * 16;
     const uint64_t wrow = j0 + m < p.cols ? j0 + m : p.cols - 1;
@@ -243,9 +243,13 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_q8_tiles_kernel(MqParams 
         for (int n = 0; n < TN; ++n) {
             const uint64_t j = j_first + n * 16;
             int32_t* q = p.parts + ((uint64_t)part * p.rows + i) * p.cols + j;
+            if (j + 4 <= p.cols) {
+                __builtin_memcpy(q, &sum[n][t], 16);
+            } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (j + r < p.cols) q[r] = sum[n][t][r];
+                for (int r = 0; r < 4; ++r)
+                    if (j + r < p.cols) q[r] = sum[n][t][r];
+            }
         }
     }
 }
@@ -256,10 +260,16 @@ __global__ __launch_bounds__(256) void matmul_q8_parts_kernel(MqParams p) {
     for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (uint64_t)gridDim.x * 256) {
         const uint64_t i = at / fours, j = (at - i * fours) * 4;
         mq_i4 sum = {0, 0, 0, 0};
-        for (uint32_t k = 0; k < p.splits; ++k) {
-            const int32_t* q = p.parts + ((uint64_t)k * p.rows + i) * p.cols + j;
+        const int32_t* q = p.parts + i * p.cols + j;
+        const uint64_t one = p.rows * p.cols;
+        if (j + 4 <= p.cols) {
+#pragma unroll 8
+            for (uint32_t k = 0; k < p.splits; ++k) sum += mq_read(reinterpret_cast<const char*>(q + k * one));
+        } else {
+            for (uint32_t k = 0; k < p.splits; ++k) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum[r] += j + r < p.cols ? q[r] : 0;
+                for (int r = 0; r < 4; ++r) sum[r] += j + r < p.cols ? q[k * one + r] : 0;
+            }
         }
         MqBeside<T> beside;
         beside.read(p, j);
@@ -274,10 +284,11 @@ int mq_tiles(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
     p.tiles_m = (uint32_t)((d.rows + BM - 1) / BM);
     p.tiles_n = (uint32_t)((d.cols + BN - 1) / BN);
     const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
-    // inner is cut where there are fewer tiles than compute units, into parts of 512 bytes or more
+    // Inner is cut where tiles are few, into parts of 512 bytes or more: small tiles to two blocks a compute unit, others to one. 128 x 4096 by 4096 rows
+    // in 64 x 64: 256, 512, 1024 blocks 16.9, 15.7, 17.5 us; 256 x 4096: 21.7, 18.3, 20.6.
     p.splits = 1;
-    if (tiles < 192) {
-        uint64_t most = d.inner / 512, wanted = 256 / tiles;
+    if (tiles < (BM == 64 ? 300 : 192)) {
+        uint64_t most = d.inner / 512, wanted = (BM == 64 ? 512 : 256) / tiles;
         p.splits = (uint32_t)(wanted < most ? wanted : most);
         if (p.splits < 1) p.splits = 1;
     }
@@ -314,13 +325,16 @@ int mq_launch(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
         report_error(CUMO_HIP_ERROR_ARGUMENT, 0, "matmul_q8: too many rows by columns");
         return CUMO_HIP_ERROR_ARGUMENT;
     }
-    if (d.rows <= 16) return mq_rows<T, 1>(d, stream);
-    if (d.rows <= 32) return mq_rows<T, 2>(d, stream);
-    if (d.rows <= 64) return mq_rows<T, 4>(d, stream);
+    // Few rows: straight from memory, unless inner is so long, or columns so few, that parts of it are better shared out. us so / in tiles, cut:
+    // 1 x 4096 by 256 5.4 / 8.0; 16 x 4096 by 2048 6.0 / 7.8; 16 x 16384 by 1024 16.2 / 10.5; 64 x 1024 by 512 5.6 / 7.8; 64 x 4096 by 1024 11.1 / 8.3.
+    const bool reach = d.inner <= 8192 || d.cols >= 4096;
+    if (d.rows <= 16 && reach) return mq_rows<T, 1>(d, stream);
+    if (d.rows <= 32 && reach) return mq_rows<T, 2>(d, stream);
+    if (d.rows <= 64 && d.inner <= 1024) return mq_rows<T, 4>(d, stream);
     const uint64_t large = ((d.rows + 255) / 256) * ((d.cols + 255) / 256);
     if (large >= 192) return mq_tiles<T, 256, 256, 2, 4>(d, stream);
     const uint64_t middle = ((d.rows + 127) / 128) * ((d.cols + 127) / 128);
-    if (middle >= 128) return mq_tiles<T, 128, 128, 2, 2>(d, stream);
+    if (middle >= 200) return mq_tiles<T, 128, 128, 2, 2>(d, stream);
     return mq_tiles<T, 64, 64, 2, 2>(d, stream);
 }
 
