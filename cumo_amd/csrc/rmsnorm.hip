@@ -299,35 +299,52 @@ __global__ __launch_bounds__(kRnWide) void rmsnorm_long_kernel(cumo_hip_rmsnorm_
     }
 }
 
-// Rows in 8 bits as they are: the nearest integer of x / scale, to even where two are as near. x times 1 / scale gives it or, next to the
-// middle of two, a neighbour; what it leaves of x, one fused multiply-add, is exact, and says which. `b`: 1 / scale, of numbers lifted
-// by a power of two where it would be infinite.
-template <class T>
-__device__ __forceinline__ T qz_lift(T scale) { return scale < (sizeof(T) == 4 ? (T)0x1p-100f : (T)0x1p-1000) ? (T)0x1p64f : (T)1; }
-template <class T>
-__device__ __forceinline__ int8_t qz_byte(T x, T scale, T b, bool kept) {
-    T q;
-    if constexpr (sizeof(T) == 4) q = __builtin_rintf(x * b);
-    else q = __builtin_rint(x * b);
-    T r;
-    if constexpr (sizeof(T) == 4) r = __builtin_fmaf(-q, scale, x);
-    else r = __builtin_fma(-q, scale, x);
-    const T two = r + r, far = two < (T)0 ? -two : two;
-    int z = (int)q;
-    if (far > scale || (far == scale && (z & 1))) z += two < (T)0 ? -1 : 1;
-    z = z < -127 ? -127 : z > 127 ? 127 : z;
-    return (int8_t)(kept ? z : 0);
-}
+// Rows in 8 bits as they are: the nearest integer of x / scale, to even where two are as near. x times 1 / scale, off by 128 steps of the type at
+// most, gives it but next to the middle of two (`near`), where what an integer leaves of x, one fused multiply-add, is exact and says which.
+// Rows of scales so small that 1 / scale is infinite, or that they have fewer digits, are lifted by a power of two and always go that way, ending
+// at 127.
 template <class T>
 struct QzScale {
     T scale, lifted, lift, b;
-    bool kept;
-    __device__ __forceinline__ QzScale(double most) : scale((T)(most / 127.0)), lift(qz_lift(scale)) {
+    bool kept, plain;
+    __device__ __forceinline__ QzScale(double most) : scale((T)(most / 127.0)) {
+        lift = scale < (sizeof(T) == 4 ? (T)0x1p-100f : (T)0x1p-1000) ? (T)0x1p64f : (T)1;
         kept = scale > (T)0 && scale < (T)INFINITY;
+        plain = kept && lift == (T)1;
         lifted = scale * lift;
         b = kept ? (T)1 / lifted : (T)0;
     }
-    __device__ __forceinline__ int8_t byte(T x) const { return qz_byte<T>(kept ? x * lift : (T)0, lifted, b, kept); }
+    static __device__ __forceinline__ T rint(T x) { return sizeof(T) == 4 ? (T)__builtin_rintf((float)x) : (T)__builtin_rint((double)x); }
+    static __device__ __forceinline__ T size(T x) { return sizeof(T) == 4 ? (T)__builtin_fabsf((float)x) : (T)__builtin_fabs((double)x); }
+    __device__ __forceinline__ int8_t exact(T given) const {
+        const T x = kept ? given * lift : (T)0, q = rint(x * b);
+        const T r = sizeof(T) == 4 ? (T)__builtin_fmaf(-(float)q, (float)lifted, (float)x) : (T)__builtin_fma(-(double)q, (double)lifted, (double)x);
+        const T two = r + r;
+        int z = (int)q;
+        if (size(two) > lifted || (size(two) == lifted && (z & 1))) z += two < (T)0 ? -1 : 1;
+        z = z < -127 ? -127 : z > 127 ? 127 : z;
+        return (int8_t)(kept ? z : 0);
+    }
+    // N of them
+    template <int N>
+    __device__ __forceinline__ void bytes(const T* x, int8_t* to) const {
+        constexpr T kNear = (T)0.5 - (sizeof(T) == 4 ? (T)0x1p-15f : (T)0x1p-44);
+        T q[N], off = (T)0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const T t = x[j] * b;
+            q[j] = rint(t);
+            const T d = size(t - q[j]);
+            off = d > off ? d : off;
+        }
+        if (plain && off < kNear) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) to[j] = (int8_t)(int)q[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) to[j] = exact(x[j]);
+        }
+    }
 };
 
 template <class T, int TPR, int NV, int BLOCK, bool NT>
@@ -354,7 +371,15 @@ __global__ __launch_bounds__(BLOCK) void quantize_kernel(cumo_hip_quantize_t p) 
         rn_allreduce<TPR, BLOCK>(all, rn_max_nan);
         const QzScale<T> to(all[0]);
         if (there && lane == 0) reinterpret_cast<T*>(p.scale)[row] = to.scale;
-        s.store_bytes(p.q + row * p.q_step, lane, whole, rest, [&](int k, int j) { return to.byte(s.at(k, j)); });
+        char* q = p.q + row * p.q_step;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const uint32_t at = (uint32_t)k * TPR + lane;
+            int8_t bytes[Row::V];
+            to.template bytes<Row::V>(s.x[k].t, bytes);
+            if (at < whole) __builtin_memcpy(q + at * (uint32_t)Row::V, bytes, Row::V);
+        }
+        if (lane < rest) q[whole * Row::V + lane] = to.exact(s.last);
     }
 }
 
@@ -368,7 +393,7 @@ __global__ __launch_bounds__(kRnWide) void quantize_long_kernel(cumo_hip_quantiz
         const QzScale<T> to(most[0]);
         if (threadIdx.x == 0) reinterpret_cast<T*>(p.scale)[row] = to.scale;
         int8_t* q = reinterpret_cast<int8_t*>(p.q + (int64_t)row * p.q_step);
-        for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) q[i] = to.byte(x[i]);
+        for (uint64_t i = threadIdx.x; i < p.n; i += kRnWide) q[i] = to.exact(x[i]);
     }
 }
 

@@ -55,20 +55,29 @@ struct RtParams : cumo_hip_rotary_t {
     uint32_t per;     // heads that a lane takes
     uint32_t chunks;  // such groups of heads
     uint32_t turns;   // pieces of W pairs
-    uint32_t copies;  // pieces of up to 2 W elements behind the pairs
+    uint32_t copies;  // pieces of C elements behind the pairs
 };
 
-// W numbers on any boundary of their type
-template <class T, int W>
-struct RtVec {
-    T t[W];
-    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(t, p, sizeof(t)); }
-    __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, t, sizeof(t)); }
+// N numbers on any boundary of their type
+template <class T, int N>
+struct __attribute__((aligned(sizeof(T) * N))) RtVec {
+    T t[N];
+    template <bool NT>
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (NT && sizeof(t) == 16) *reinterpret_cast<store_u4*>(t) = __builtin_nontemporal_load(reinterpret_cast<const store_u4*>(p));
+        else __builtin_memcpy(t, p, sizeof(t));
+    }
+    template <bool NT>
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (NT && sizeof(t) == 16) __builtin_nontemporal_store(*reinterpret_cast<const store_u4*>(t), reinterpret_cast<store_u4*>(p));
+        else __builtin_memcpy(p, t, sizeof(t));
+    }
 };
 
-template <class T, int W, bool NEIGHBOURS>
+// A lane takes W pairs, two vectors of W (neighbours: one of 2 W), or C elements behind the pairs, of `per` heads in a row: U of them are read
+// before the first is written. Lanes beside each other take pieces beside each other.
+template <class T, int W, int C, bool NEIGHBOURS, int U, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(RtParams p) {
-    typedef RtVec<T, W> Vec;
     const uint32_t pieces = p.turns + p.copies;
     const uint64_t total = p.batch * p.time * p.chunks * pieces;
     for (uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x; item < total; item += (uint64_t)gridDim.x * 256) {
@@ -80,6 +89,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RtParams p) {
         const char* x = p.x + (int64_t)b * p.x_step[0] + (int64_t)t * p.x_step[1] + (int64_t)first * p.x_step[2];
         char* y = p.y + (int64_t)b * p.y_step[0] + (int64_t)t * p.y_step[1] + (int64_t)first * p.y_step[2];
         const uint32_t n = p.heads - first < p.per ? (uint32_t)(p.heads - first) : p.per;
+        auto from = [&](uint32_t h) { return reinterpret_cast<const T*>(x + (int64_t)(h < n ? h : n - 1) * p.x_step[2]); };
+        auto to = [&](uint32_t h) { return reinterpret_cast<T*>(y + (int64_t)h * p.y_step[2]); };
         if (piece < p.turns) {
             const double at = (double)p.positions[token];
             double sn[W], cs[W];
@@ -89,61 +100,88 @@ __global__ __launch_bounds__(256) void rotary_kernel(RtParams p) {
                 sn[j] *= p.inverse ? -p.amplitude : p.amplitude;
                 cs[j] *= p.amplitude;
             }
-            const uint64_t one = (uint64_t)piece * W * (NEIGHBOURS ? 2 : 1), two = NEIGHBOURS ? one + W : one + p.pairs;
-#pragma unroll 4
-            for (uint32_t h = 0; h < n; ++h) {
-                const T* from = reinterpret_cast<const T*>(x + (int64_t)h * p.x_step[2]);
-                T* to = reinterpret_cast<T*>(y + (int64_t)h * p.y_step[2]);
-                Vec u, v;
-                u.load(from + one);
-                v.load(from + two);
-                Vec a = u, d = v;
+            auto turn = [&](T& u, T& v, int j) {
+                const double l = (double)u, r = (double)v;
+                u = (T)__builtin_fma(l, cs[j], -(r * sn[j]));
+                v = (T)__builtin_fma(r, cs[j], l * sn[j]);
+            };
+            for (uint32_t h = 0; h < n; h += U) {
+                if constexpr (NEIGHBOURS) {
+                    const uint64_t one = (uint64_t)piece * W * 2;
+                    RtVec<T, 2 * W> a[U];
 #pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    // neighbours: pair j is elements 2 j and 2 j + 1 of u and v, one behind the other
-                    T& first_of = NEIGHBOURS ? (2 * j < W ? a.t[2 * j < W ? 2 * j : 0] : d.t[2 * j < W ? 0 : 2 * j - W]) : a.t[j];
-                    T& second_of = NEIGHBOURS ? (2 * j + 1 < W ? a.t[2 * j + 1 < W ? 2 * j + 1 : 0] : d.t[2 * j + 1 < W ? 0 : 2 * j + 1 - W]) : d.t[j];
-                    const double l = (double)first_of, r = (double)second_of;
-                    first_of = (T)__builtin_fma(l, cs[j], -(r * sn[j]));
-                    second_of = (T)__builtin_fma(r, cs[j], l * sn[j]);
+                    for (int u = 0; u < U; ++u) a[u].template load<NT>(from(h + u) + one);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) turn(a[u].t[2 * j], a[u].t[2 * j + 1], j);
+                        if (h + u < n) a[u].template store<NT>(to(h + u) + one);
+                    }
+                } else {
+                    const uint64_t one = (uint64_t)piece * W, two = one + p.pairs;
+                    RtVec<T, W> a[U], d[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        a[u].template load<NT>(from(h + u) + one);
+                        d[u].template load<NT>(from(h + u) + two);
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) turn(a[u].t[j], d[u].t[j], j);
+                        if (h + u < n) {
+                            a[u].template store<NT>(to(h + u) + one);
+                            d[u].template store<NT>(to(h + u) + two);
+                        }
+                    }
                 }
-                a.store(to + one);
-                d.store(to + two);
             }
         } else {
-            const uint64_t one = p.pairs * 2 + (uint64_t)(piece - p.turns) * 2 * W;
-            for (uint32_t h = 0; h < n; ++h) {
-                const T* from = reinterpret_cast<const T*>(x + (int64_t)h * p.x_step[2]);
-                T* to = reinterpret_cast<T*>(y + (int64_t)h * p.y_step[2]);
-                for (uint64_t i = one; i < one + 2 * W && i < p.dim; ++i) to[i] = from[i];
+            const uint64_t one = p.pairs * 2 + (uint64_t)(piece - p.turns) * C;
+            for (uint32_t h = 0; h < n; h += U) {
+                RtVec<T, C> a[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) a[u].template load<NT>(from(h + u) + one);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (h + u < n) a[u].template store<NT>(to(h + u) + one);
             }
         }
     }
 }
 
-template <class T, int W>
+template <class T, int W, int C, bool NEIGHBOURS>
 void rt_launch_one(RtParams p, hipStream_t stream) {
     p.turns = (uint32_t)(p.pairs / W);
-    p.copies = (uint32_t)((p.dim - 2 * p.pairs + 2 * W - 1) / (2 * W));
+    p.copies = (uint32_t)((p.dim - 2 * p.pairs) / C);
     const uint64_t items = p.batch * p.time * (p.turns + p.copies);
     // a lane takes so many heads that the machine is full, eight at most
-    uint64_t per = items * p.heads >> 18;
+    const uint64_t per = items * p.heads >> 18;
     p.per = (uint32_t)(per < 1 ? 1 : per > 8 ? 8 : per);
     p.chunks = (uint32_t)((p.heads + p.per - 1) / p.per);
     const uint64_t blocks = (items * p.chunks + 255) / 256;
     const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536)), block(256);
-    if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<T, W, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((rotary_kernel<T, W, false>), grid, block, 0, stream, p);
+    // (heads read four at a time where a lane has as many: for one, 64 x 1 x 32 of 128, the others' reading took 5.7 us)
+    if (p.per < 4) hipLaunchKernelGGL((rotary_kernel<T, W, C, NEIGHBOURS, 1, false>), grid, block, 0, stream, p);
+    else if (stream_past_caches(p.batch * p.time * p.heads * p.dim * sizeof(T) * 2)) hipLaunchKernelGGL((rotary_kernel<T, W, C, NEIGHBOURS, 4, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((rotary_kernel<T, W, C, NEIGHBOURS, 4, false>), grid, block, 0, stream, p);
     cumo_cuda_runtime_check_kernel_launch();
 }
 
+// whole vectors where the pairs, and what is behind them, are some number of those; else one by one
 template <class T>
 void rt_launch(const cumo_hip_rotary_t& d, hipStream_t stream) {
     constexpr int V = 16 / (int)sizeof(T);
     RtParams p;
     static_cast<cumo_hip_rotary_t&>(p) = d;
-    if (d.pairs % V == 0) rt_launch_one<T, V>(p, stream);
-    else rt_launch_one<T, 1>(p, stream);
+    const bool copies = (d.dim - 2 * d.pairs) % V == 0;
+    if (d.interleaved) {
+        if (d.pairs % (V / 2) == 0) copies ? rt_launch_one<T, V / 2, V, true>(p, stream) : rt_launch_one<T, V / 2, 1, true>(p, stream);
+        else rt_launch_one<T, 1, 1, true>(p, stream);
+    } else {
+        if (d.pairs % V == 0) copies ? rt_launch_one<T, V, V, false>(p, stream) : rt_launch_one<T, V, 1, false>(p, stream);
+        else rt_launch_one<T, 1, 1, false>(p, stream);
+    }
 }
 
 }  // namespace
