@@ -420,11 +420,23 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(
     decay_q = (T)power(m + (late ? 0 : 1));
     T o_scale = (T)w.o_scale;
     asm("" : "+v"(o_scale));   // (held: read from the arguments in every turn, it would wait for all that LDS has been asked for)
-    auto ends = [&](uint32_t of_all) {   // a turn of so many steps
+    // S is multiplied by a^16 in every stretch. Rounded to a float, that would be off by as much each time, on one side: 1.4e-6 of a state that forgets
+    // over 2000 steps. So each factor is rounded from what makes the product of all so far the power that it stands for (5.7e-7: what the
+    // additions round). `behind`: that power by the product.
+    double behind = 1.0;
+    const double a16 = power(kLaStretch), inverse16 = 1.0 / a16;
+    const bool tracked = sizeof(T) == 4 && a16 > 0x1p-100 && a16 < 0x1p100;
+    auto next_decay = [&](double exact) {
+        const T s = (T)(exact * behind);
+        if (tracked) behind *= 2.0 - (double)s * inverse16;
+        return s;
+    };
+    auto ends = [&](uint32_t of_all) {   // a turn of so many steps, fewer than it can have: the last
 #pragma unroll 1
         for (int sub = 0; sub < SUBS; ++sub) {
             const uint32_t n = of_all <= sub * kLaStretch ? 0 : of_all - sub * kLaStretch < kLaStretch ? of_all - sub * kLaStretch : kLaStretch;
-            T k4[4], s1 = (T)power(n);
+            T k4[4], s1 = n ? (T)(power(n) * behind) : (T)1;
+            behind = 1.0;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const uint32_t j = 4 * g + r;
@@ -489,7 +501,12 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(
         do {
             const uint32_t n = of_turn(done);
             done += n;
-            if (n < TURN) ends(n);
+            if (n < TURN) {
+                ends(n);
+            } else {
+#pragma unroll
+                for (int sub = 0; sub < SUBS; ++sub) decay_s[sub] = next_decay(a16);
+            }
             Quad P[EACH], all[SUBS];
             if constexpr (!ONLY) {
 #pragma unroll
@@ -667,9 +684,9 @@ __global__ __launch_bounds__(256) void la_starts_kernel(LaWalks walks, LaCommon 
         const uint32_t in = (uint32_t)(at - bh * size), d = in / w.wide, e = in - d * w.wide;
         const uint64_t length = la_length(c, b);
         const double a = (double)reinterpret_cast<const T*>(c.decay)[bh - b * c.heads];
-        T s = w.state ? reinterpret_cast<const T*>(w.state)[bh * size + d * w.state_row + e * w.state_col] : (T)0;
+        double s = w.state ? (double)reinterpret_cast<const T*>(w.state)[bh * size + d * w.state_row + e * w.state_col] : 0.0;
         T* p = reinterpret_cast<T*>(plan.starts[blockIdx.y]) + at;
-        const T whole = (T)la_power(a, plan.steps);
+        const double whole = la_power(a, plan.steps);
         const uint32_t n_starts = plan.segments - 1;
         for (uint32_t k = 0; k < n_starts; k += U) {
             T own[U];
@@ -680,8 +697,8 @@ __global__ __launch_bounds__(256) void la_starts_kernel(LaWalks walks, LaCommon 
                 if (k + u >= n_starts) continue;
                 const uint64_t begin = (k + u) * plan.steps;
                 const uint64_t n = begin >= length ? 0 : length - begin < plan.steps ? length - begin : plan.steps;
-                s = la_fma(n == plan.steps ? whole : n == 0 ? (T)1 : (T)la_power(a, n), s, own[u]);
-                p[(uint64_t)(k + u) * all] = s;
+                s = __builtin_fma(n == plan.steps ? whole : n == 0 ? 1.0 : la_power(a, n), s, (double)own[u]);
+                p[(uint64_t)(k + u) * all] = (T)s;
             }
         }
     }
