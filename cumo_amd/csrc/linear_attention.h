@@ -294,9 +294,10 @@ struct LaStage {
     }
 };
 
-// A turn takes two stretches, one behind the other (one, where their rows would fill LDS or the registers that bring them): its rows are in LDS,
-// in two buffers where they fit twice.
-template <class T, int DT> constexpr int kLaSubs = sizeof(T) * DT <= 64 ? 2 : 1;
+// A turn takes two stretches, one behind the other; one, where their rows would fill LDS or the registers that bring them, and in double precision
+// where dim's tiles are shared out by fours (DFloat 4 x 2048 x 16 heads of 128 401 and 353 us, gradients 3 x 500 x 8 of 64 63 and 56). Its rows are in
+// LDS, in two buffers where they fit twice.
+template <class T, int DT> constexpr int kLaSubs = sizeof(T) == 8 && DT % 4 == 0 ? 1 : sizeof(T) * DT <= 64 ? 2 : 1;
 template <class T, int DT> constexpr uint32_t kLaTurn = kLaStretch * kLaSubs<T, DT>;
 // products k q^T on their way from wave to wave: those of the next turn may meet those of this one where a turn has one barrier
 template <class T, int DT, int NW> constexpr uint64_t kLaSlots = (kLaSubs<T, DT> == 1 ? 2 : 1) * NW * 256 * sizeof(T);
@@ -306,13 +307,13 @@ template <class T, int DT, int NW, int BUFFERS, bool ONLY>
 constexpr uint64_t kLaShared = BUFFERS * (kLaBuffer<T, DT, NW> - (ONLY ? kLaTurn<T, DT> * (DT * 16 * sizeof(T) + 16) : 0)) + (ONLY ? 0 : kLaSlots<T, DT, NW>);
 // Waves to a SIMD that the registers are shared out for: two, so 256 of one kind, where a lane holds less (else the compiler spreads them over both
 // kinds, and moves them: also where it knows that LDS, hence told at the launch, holds one block alone).
-template <class T, int DT> constexpr int kLaWaves = DT <= (sizeof(T) == 4 ? 8 : 2) ? 2 : 1;
+template <class T, int DT, int NW> constexpr int kLaWaves = sizeof(T) == 4 ? (DT <= 8 ? 2 : 1) : DT <= 4 && NW == 4 ? 2 : 1;
 extern __shared__ __attribute__((aligned(16))) char la_shared[];
 
 // DT: tiles of 16 that hold dim. NW: tiles of 16 columns to a block, a wave each. QUADS: rows of dim and of wide are whole fours. ONLY: what a
 // segment leaves by itself.
 template <class T, int DT, int NW, int BUFFERS, bool QUADS, bool ONLY>
-__global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT>)) void la_stretch_kernel(LaWalks walks, LaCommon c, LaPlan plan) {
+__global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_kernel(LaWalks walks, LaCommon c, LaPlan plan) {
     typedef LaQuad<T> Quad;
     constexpr uint32_t E = sizeof(T);
     constexpr int SUBS = kLaSubs<T, DT>;
@@ -787,7 +788,7 @@ int la_walk(const LaWalk* w, uint32_t n, const LaCommon& c, hipStream_t stream) 
     // the last are then walked twice, the first time for half of the products.
     const uint64_t blocks = (uint64_t)n * p.slices * heads, units = (uint64_t)device_compute_units();
     if (blocks * 2 <= units) {
-        uint64_t cuts = units * (w[0].dim <= (sizeof(T) == 4 ? 128 : 32) ? 2 : 1) / blocks;
+        uint64_t cuts = units * (w[0].dim <= (sizeof(T) == 4 ? 128 : 64) ? 2 : 1) / blocks;
         const uint64_t most = (c.time + 63) / 64;
         if (cuts > most) cuts = most;
         if (cuts > 1) {
