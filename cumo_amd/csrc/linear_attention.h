@@ -664,10 +664,10 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
             }
         }
         const uint64_t behind = begin + plan.steps < c.time && segment + 1 < plan.segments ? begin + plan.steps : c.time;
-        if (!ONLY && g == 0 && column) {
+        if (!ONLY && column) {
             char* z = w.o + (int64_t)b * w.o_step[0] + (int64_t)h * w.o_step[2] + (uint64_t)(e0 + label) * E;
             const T none = (T)0;
-            for (uint64_t t = begin > length ? begin : length; t < behind; ++t) __builtin_memcpy(z + (int64_t)t * w.o_step[1], &none, E);
+            for (uint64_t t = (begin > length ? begin : length) + g; t < behind; t += 4) __builtin_memcpy(z + (int64_t)t * w.o_step[1], &none, E);
         }
     }
 }
@@ -834,6 +834,7 @@ void la_steps(int64_t* to, const ssize_t* from) {
 
 template <class T>
 int la_forward(const cumo_hip_linear_attention_t& d, hipStream_t stream) {
+    if (!d.batch || !d.heads || !d.wide) return CUMO_HIP_OK;
     LaCommon c = {d.batch, d.time, d.heads, d.decay, d.lengths};
     LaWalk w;
     const uint32_t share = (uint32_t)(d.heads / d.shared);
@@ -849,6 +850,7 @@ int la_forward(const cumo_hip_linear_attention_t& d, hipStream_t stream) {
 
 template <class T>
 int la_backward(const cumo_hip_linear_attention_grad_t& d, hipStream_t stream) {
+    if (!d.batch || !d.heads) return CUMO_HIP_OK;
     LaCommon c = {d.batch, d.time, d.heads, d.decay, d.lengths};
     const uint32_t share = (uint32_t)(d.heads / d.shared), dim = (uint32_t)d.dim, wide = (uint32_t)d.wide;
     const uint64_t rows = d.batch * d.time * d.heads;

@@ -770,8 +770,8 @@ int attention_operands(const NA* q, const NA* k, const NA* v, const NA* decay, c
         if (lengths->type != CUMO_HIP_INT32) return fail(CUMO_HIP_ERROR_TYPE, kAttentionType);
         if (!same_shape(lengths, 1, q->shape)) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: lengths must be one dimension, a number for each sequence");
     }
-    // blocks are counted in 32 bits, as are the steps
-    if (q->shape[1] >= (size_t)1 << 31 || q->shape[0] * q->shape[2] >= (size_t)1 << 21) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: too many steps or heads");
+    // (a launch holds fewer than 2^32 lanes: 256 to a block, twelve blocks to a head at most)
+    if (q->shape[1] >= (size_t)1 << 31 || q->shape[0] * q->shape[2] >= (size_t)1 << 20) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: too many steps or heads");
     return CUMO_HIP_OK;
 }
 
@@ -804,7 +804,12 @@ int cumo_hip_na_linear_attention(const cumo_hip_narray_t* q, const cumo_hip_narr
     if (!rc && state) rc = take(&in[4], state, DENSE, 0, &s);
     if (!rc && lengths) rc = take(&in[5], lengths, DENSE, 0, &s);
     if (!rc) rc = make(&r[nr++], o, q->type, 4, o_shape, HEADS, 0, in, 6, &s);
-    if (!rc && last) rc = make(&r[nr++], last, q->type, 4, state_shape, DENSE, 0, in, 6, &s);
+    if (!rc && last) {
+        // a single step's state may be written where it was: a lane reads what it writes
+        const bool in_place = state && q->shape[1] == 1 && last->ptr && last->ptr + last->offset == in[4].at();
+        if (in_place) in[4].given = NULL;
+        rc = make(&r[nr++], last, q->type, 4, state_shape, DENSE, 0, in, 6, &s);
+    }
     if (!rc) {
         cumo_hip_linear_attention_t d;
         d.batch = q->shape[0];

@@ -750,7 +750,9 @@ void cumo_hip_quantize_kernel_launch(int type, const cumo_hip_quantize_t* d);
  *   y[i][j] = (sum over k < inner of x[i][k] * w[j][k]) * xscale[i] * wscale[j] + bias[j]
  * The sum is exact in 32 bits for inner < 2^17; what follows is in double, rounded once to type
  * (0 SFloat, 1 DFloat), which the scales and bias (NULL: none) have as well, contiguous each.
- * Steps from row to row in bytes. y may overlap no operand. CUMO_HIP_OK or the error reported. */
+ * Steps from row to row in bytes. y may overlap no operand. Fewer than 2^31 rows and columns, and
+ * fewer than 2^22 tiles of 256 by 256 of them. Scratch comes from the pool (left to the graph of a
+ * captured call: cumo_hip_captured_free). CUMO_HIP_OK or the error reported. */
 typedef struct {
     uint64_t rows, inner, cols;
     ssize_t  x_step, w_step, y_step;
@@ -790,7 +792,9 @@ void cumo_hip_rotary_kernel_launch(int type, const cumo_hip_rotary_t* d);
  * contiguous elements, NULL for zeros; last: S behind the last step, alike, NULL where it is
  * not wanted. lengths: the steps of each sequence (between 0 and time; others are brought there),
  * NULL: time; o is 0 behind them, and last is S[length - 1]. type 0 SFloat, 1 DFloat. No result may
- * overlap an operand. CUMO_HIP_OK or the error reported. */
+ * overlap an operand, but for last, which may be state where time is 1. batch x heads is less than
+ * 2^20, time than 2^31. Scratch comes from the pool (left to the graph of a captured call:
+ * cumo_hip_captured_free). CUMO_HIP_OK or the error reported. */
 typedef struct {
     uint64_t batch, time, heads, shared, dim, wide;
     ssize_t  q_step[3], k_step[3], v_step[3], o_step[3];

@@ -15,7 +15,8 @@ TYPES = [np.float32, np.float64]
 # batch, time, heads, shared heads, dim, wide: one step, a few, stretches of 16 and their ends, odd heads, the widest ones, long sequences
 SHAPES = [(1, 1, 1, 1, 1, 1), (2, 1, 3, 3, 16, 16), (3, 1, 4, 2, 128, 128), (2, 1, 2, 1, 100, 72), (1, 1, 1, 1, 256, 250), (3, 2, 2, 1, 5, 7), (2, 3, 2, 2, 64, 36), (2, 15, 2, 2, 16, 16),
           (1, 16, 4, 2, 32, 64), (2, 17, 2, 2, 33, 20), (1, 31, 2, 2, 48, 17), (1, 33, 2, 2, 64, 128), (2, 100, 3, 1, 72, 100), (1, 257, 2, 2, 128, 128), (1, 130, 2, 1, 256, 256),
-          (2, 64, 1, 1, 16, 256), (1, 300, 1, 1, 256, 16), (1, 47, 1, 1, 255, 1), (1, 47, 1, 1, 1, 255), (1, 2000, 1, 1, 8, 8), (1, 3001, 2, 2, 24, 40), (40, 70, 8, 8, 20, 30)]
+          (2, 64, 1, 1, 16, 256), (1, 300, 1, 1, 256, 16), (1, 47, 1, 1, 255, 1), (1, 47, 1, 1, 1, 255), (1, 2000, 1, 1, 8, 8), (1, 3001, 2, 2, 24, 40), (40, 70, 8, 8, 20, 30),
+          (70, 40, 4, 4, 256, 16), (70, 40, 4, 2, 150, 20), (70, 40, 4, 4, 128, 20), (1, 1500, 2, 1, 128, 80), (1, 700, 1, 1, 256, 40), (1, 1111, 2, 2, 80, 12)]
 
 
 def cls_of(m, dt):
@@ -281,9 +282,18 @@ def test_results_in_given_arrays(dt, time):
     got = buf.to_numpy()
     got[:, :, :, 4:28] = 7
     assert (got == 7).all()
-    # o over q, the state over itself
+    # o over q, the state over itself (a single step's where it is: nothing is held for it)
     _lib.call(L.cumo_hip_na_linear_attention, ref(q), ref(k), ref(v), ref(a), ref(s), None, 24 ** -0.5, ref(q), ref(s))
     assert (q.to_numpy() == want).all() and (s.to_numpy() == last).all()
+    # the state of two of its sequences in the middle of a wider array, in place
+    x = made(np.random.default_rng(7), shape, dt)
+    wide = np.concatenate([x["state"], 5 * np.ones_like(x["state"])], axis=0)
+    q, k, v, a = on_device(m, x, ("q", "k", "v", "decay"))
+    held = cls.cast(wide)
+    want, last = (z.to_numpy() for z in m.Fused.linear_attention(q, k, v, a, cls.cast(x["state"])))
+    o = cls(2, time, 4, 24)
+    _lib.call(L.cumo_hip_na_linear_attention, ref(q), ref(k), ref(v), ref(a), ref(held[0:2]), None, 24 ** -0.5, ref(o), ref(held[0:2]))
+    assert (o.to_numpy() == want).all() and (held.to_numpy()[:2] == last).all() and (held.to_numpy()[2:] == 5).all()
 
 
 @pytest.mark.parametrize("dt", TYPES)
@@ -383,3 +393,23 @@ def test_captured_on_another_stream(time):
         if graph:
             hip.hipGraphDestroy(graph)
         L.cumo_hip_stream_destroy(stream)
+
+
+@pytest.mark.parametrize("time", [3000, 40000])
+def test_slow_decays_stay_powers(time):
+    """States that forget over hundreds to thousands of steps pass a multiplication and five roundings or so a stretch of sixteen. Those fall on either
+    side: a window of 4000 steps, 250 stretches, 1250 roundings, is off by sqrt(1250) half steps in norm, 2.1e-6; three times that is
+    allowed. A decay that is off on one side would add up to 250 of its own roundings over the window, and more over longer ones."""
+    import cumo_amd as m
+    rng = np.random.default_rng(time)
+    a = (1 - 10.0 ** -np.linspace(2.0, 3.6, 12)).astype(np.float32)
+    shape = (1, time, 12, 12, 16, 16)
+    x = made(rng, shape, np.float32)
+    x["decay"] = a
+    _, last = m.Fused.linear_attention(*on_device(m, x, ("q", "k", "v", "decay", "state")))
+    steps = np.arange(time - 1, -1, -1)
+    for h in range(12):
+        by = a[h].astype(np.float64) ** steps
+        want = a[h].astype(np.float64) ** time * x["state"][0, h] + (x["k"][0, :, h].astype(np.float64) * by[:, None]).T @ x["v"][0, :, h].astype(np.float64)
+        got = last.to_numpy()[0, h]
+        assert np.linalg.norm(got - want) <= 3 * 35 * 2.0 ** -24 * np.linalg.norm(want), (h, np.linalg.norm(got - want) / np.linalg.norm(want))
