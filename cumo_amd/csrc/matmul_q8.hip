@@ -327,10 +327,11 @@ int mq_launch(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
     }
     // Few rows: straight from memory, unless inner is so long, or columns so few, that parts of it are better shared out. us so / in tiles, cut:
     // 1 x 4096 by 256 5.4 / 8.0; 16 x 4096 by 2048 6.0 / 7.8; 16 x 16384 by 1024 16.2 / 10.5; 64 x 1024 by 512 5.6 / 7.8; 64 x 4096 by 1024 11.1 / 8.3.
-    const bool reach = d.inner <= 8192 || d.cols >= 4096;
+    // (A block of 512 lanes to sixteen columns: as many columns as a launch's 2^32 lanes are enough for.)
+    const bool reach = (d.inner <= 8192 || d.cols >= 4096) && d.cols <= (uint64_t)1 << 26;
     if (d.rows <= 16 && reach) return mq_rows<T, 1>(d, stream);
     if (d.rows <= 32 && reach) return mq_rows<T, 2>(d, stream);
-    if (d.rows <= 64 && d.inner <= 1024) return mq_rows<T, 4>(d, stream);
+    if (d.rows <= 64 && d.inner <= 1024 && reach) return mq_rows<T, 4>(d, stream);
     const uint64_t large = ((d.rows + 255) / 256) * ((d.cols + 255) / 256);
     if (large >= 192) return mq_tiles<T, 256, 256, 2, 4>(d, stream);
     const uint64_t middle = ((d.rows + 127) / 128) * ((d.cols + 127) / 128);

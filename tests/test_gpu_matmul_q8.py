@@ -193,6 +193,16 @@ def test_matmul_of_nothing_and_of_no_numbers(dt):
     assert ((y == want) | (np.isnan(y) & np.isnan(want))).all()
 
 
+def test_matmul_of_more_columns_than_blocks_of_sixteen_reach():
+    """2^27 columns and some, two rows: more than 2^32 lanes if every sixteen columns were a block's."""
+    import cumo_amd as m
+    cols = (1 << 27) + 37
+    w = (np.arange(cols, dtype=np.uint32) * np.uint32(2654435761) >> np.uint32(24)).astype(np.uint8).view(np.int8).reshape(cols, 1)
+    y = m.Fused.matmul_q8(m.Int8.cast(np.array([[3], [-5]], np.int8)), m.SFloat.cast(np.ones((2, 1), np.float32)), m.Int8.cast(w), m.SFloat(cols, 1).fill(1)).to_numpy()
+    for r, x in enumerate((3, -5)):
+        assert (y[r] == np.int16(x) * w[:, 0].astype(np.int16)).all()
+
+
 @pytest.mark.parametrize("rows", [4, 200])
 def test_captured_on_another_stream(rows):
     import cumo_amd as m
