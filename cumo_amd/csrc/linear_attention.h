@@ -856,7 +856,7 @@ int la_backward(const cumo_hip_linear_attention_grad_t& d, hipStream_t stream) {
     const uint64_t rows = d.batch * d.time * d.heads;
     // gradients of heads that are shared, before their sum
     char* parts = nullptr;
-    if (share > 1 && !(parts = cumo_cuda_runtime_malloc(rows * (dim + wide) * sizeof(T)))) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
+    if (share > 1 && rows * (dim + wide) && !(parts = cumo_cuda_runtime_malloc(rows * (dim + wide) * sizeof(T)))) return CUMO_HIP_ERROR_OUT_OF_MEMORY;
     char* const part_k = parts;
     char* const part_v = parts ? parts + rows * dim * sizeof(T) : nullptr;
     const int64_t e = sizeof(T), heads = (int64_t)d.heads, time = (int64_t)d.time;

@@ -297,6 +297,33 @@ def test_results_in_given_arrays(dt, time):
 
 
 @pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("apart", [(1 << 26) - 256, 1 << 26, (1 << 26) + 256])
+def test_steps_far_apart(dt, apart):
+    """Rows in one array, as far apart as a stretch's offsets reach and further; the last is more than 2^32 bytes from the first."""
+    import cumo_amd as m
+    cls, shape = cls_of(m, dt), (1, 70, 2, 1, 16, 16)
+    x = made(np.random.default_rng(apart), shape, dt)
+    q, k, v, a, s = on_device(m, x, ("q", "k", "v", "decay", "state"))
+    g, gl = on_device(m, x, ("g", "glast"))
+    want = [z.to_numpy() for z in m.Fused.linear_attention(q, k, v, a, s) + m.Fused.linear_attention_grad(g, q, k, v, a, s, gl)]
+    buf = cls(1, 70, apart // (16 * np.dtype(dt).itemsize), 16)
+    parts = [buf[:, :, 0:2], buf[:, :, 2:3], buf[:, :, 3:4], buf[:, :, 4:6]]
+    for part, z in zip(parts, (q, k, v, g)):
+        part.store(z)
+    q, k, v, g = parts
+    got = [z.to_numpy() for z in m.Fused.linear_attention(q, k, v, a, s) + m.Fused.linear_attention_grad(g, q, k, v, a, s, gl)]
+    (o, last), (om, lm) = reference(x)
+    close(got[0], o, om, shape, "o")
+    close(got[1], last, lm, shape, "last")
+    grads, size = reference_grad(x)
+    for n in range(4):
+        close(got[2 + n], grads[n], size[n], shape, ("gq", "gk", "gv", "gstate")[n])
+    # (the same way of working, or one step at a time)
+    if apart <= 1 << 26:
+        assert all((z == w).all() for z, w in zip(got, want))
+
+
+@pytest.mark.parametrize("dt", TYPES)
 def test_nothing_to_do(dt):
     import cumo_amd as m
     cls = cls_of(m, dt)
@@ -308,6 +335,12 @@ def test_nothing_to_do(dt):
     assert (last.to_numpy() == 0).all()
     gq, gk, gv, gs = m.Fused.linear_attention_grad(make(1, 0, 2, 4), make(1, 0, 2, 3), make(1, 0, 2, 3), make(1, 0, 2, 4), cls.cast(np.ones(2, dt)), s, s)
     assert gq.shape == (1, 0, 2, 3) and (gs.to_numpy() == s.to_numpy()).all()
+    # the same with heads that share k and v
+    s4 = cls.cast(np.arange(48, dtype=dt).reshape(1, 4, 3, 4))
+    gq, gk, gv, gs = m.Fused.linear_attention_grad(make(1, 0, 4, 4), make(1, 0, 4, 3), make(1, 0, 2, 3), make(1, 0, 2, 4), cls.cast(np.ones(4, dt)), s4, s4)
+    assert gk.shape == (1, 0, 2, 3) and (gs.to_numpy() == s4.to_numpy()).all()
+    gq, gk, gv = m.Fused.linear_attention_grad(make(1, 3, 4, 0), make(1, 3, 4, 0), make(1, 3, 2, 0), make(1, 3, 2, 0), cls.cast(np.ones(4, dt)))
+    assert gq.shape == (1, 3, 4, 0) and gk.shape == gv.shape == (1, 3, 2, 0)
     for shape in ((0, 5, 2, 3), (2, 5, 0, 3)):
         q, a = make(*shape), make(shape[2])
         o, last = m.Fused.linear_attention(q, q, q, a)
