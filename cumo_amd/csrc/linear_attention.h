@@ -205,29 +205,51 @@ __device__ __forceinline__ LaQuad<float> la_mma(float a, float b, LaQuad<float> 
 __device__ __forceinline__ LaQuad<double> la_mma(double a, double b, LaQuad<double> c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
 template <class T> __device__ __forceinline__ uint32_t la_label(uint32_t m) { return sizeof(T) == 4 ? m : 4 * (m & 3) + (m >> 2); }
 
-// a^n by squares, n >= 0; in double
-__device__ __forceinline__ double la_power(double a, uint64_t n) {
-    double p = 1.0;
+constexpr uint32_t kLaStretch = 16;
+
+// A power as the sum of two doubles where T is double: squares of squares would be off by n / 2 roundings, on one side for all of a sequence's stretches
+// (DFloat 6 x 777: states off by 4e-15 in norm).
+template <class T>
+struct LaPower {
+    double hi, lo;
+    __device__ __forceinline__ LaPower by(const LaPower& o) const {
+        const double h = hi * o.hi;
+        if (sizeof(T) == 4) return LaPower{h, 0.0};
+        double l = __builtin_fma(hi, o.lo, __builtin_fma(lo, o.hi, __builtin_fma(hi, o.hi, -h)));
+        l = h - h == 0.0 ? l : 0.0;
+        const double s = h + l;
+        return LaPower{s, l - (s - h)};
+    }
+};
+// a^n by squares, n >= 0
+template <class T>
+__device__ __forceinline__ LaPower<T> la_power(double a, uint64_t n) {
+    LaPower<T> p = {1.0, 0.0}, x = {a, 0.0};
     for (; n; n >>= 1) {
-        if (n & 1) p *= a;
-        a *= a;
+        if (n & 1) p = p.by(x);
+        x = x.by(x);
     }
     return p;
 }
-
-constexpr uint32_t kLaStretch = 16;
-
-// a^n of n up to 16 for many n
+// of n up to 16 for many n
+template <class T>
 struct LaPowers {
-    double a[5];
+    LaPower<T> a[5];
     __device__ __forceinline__ explicit LaPowers(double x) {
+        a[0] = LaPower<T>{x, 0.0};
 #pragma unroll
-        for (int k = 0; k < 5; ++k, x *= x) a[k] = x;
+        for (int k = 1; k < 5; ++k) a[k] = a[k - 1].by(a[k - 1]);
     }
-    __device__ __forceinline__ double operator()(uint32_t n) const {
-        double p = n & 1 ? a[0] : 1.0;
+    __device__ __forceinline__ LaPower<T> whole(uint32_t n) const {
+        LaPower<T> p = n & 1 ? a[0] : LaPower<T>{1.0, 0.0};
 #pragma unroll
-        for (int k = 1; k < 5; ++k) p *= n >> k & 1 ? a[k] : 1.0;
+        for (int k = 1; k < 5; ++k) p = n >> k & 1 ? p.by(a[k]) : p;
+        return p;
+    }
+    __device__ __forceinline__ double operator()(uint32_t n) const {   // (to a rounding or four)
+        double p = n & 1 ? a[0].hi : 1.0;
+#pragma unroll
+        for (int k = 1; k < 5; ++k) p *= n >> k & 1 ? a[k].hi : 1.0;
         return p;
     }
 };
@@ -348,7 +370,7 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
     const uint32_t b0 = slice * NW * 16, e0 = b0 + wave * 16;     // the block's columns, and the wave's
     const uint32_t cols = W - b0 < NW * 16 ? W - b0 : NW * 16;
     const bool column = e0 + label < W;
-    const LaPowers power((double)reinterpret_cast<const T*>(c.decay)[h]);
+    const LaPowers<T> power((double)reinterpret_cast<const T*>(c.decay)[h]);
     const bool late = w.backwards;
 
     // the state
@@ -421,23 +443,24 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
     decay_q = (T)power(m + (late ? 0 : 1));
     T o_scale = (T)w.o_scale;
     asm("" : "+v"(o_scale));   // (held: read from the arguments in every turn, it would wait for all that LDS has been asked for)
-    // S is multiplied by a^16 in every stretch. Rounded to a float, that would be off by as much each time, on one side: 1.4e-6 of a state that forgets
-    // over 2000 steps. So each factor is rounded from what makes the product of all so far the power that it stands for (5.7e-7: what the
-    // additions round). `behind`: that power by the product.
-    double behind = 1.0;
-    const double a16 = power(kLaStretch), inverse16 = 1.0 / a16;
-    const bool tracked = sizeof(T) == 4 && a16 > 0x1p-100 && a16 < 0x1p100;
-    auto next_decay = [&](double exact) {
-        const T s = (T)(exact * behind);
-        if (tracked) behind *= 2.0 - (double)s * inverse16;
+    // S is multiplied by a^16 in every stretch. Rounded to its type, that would be off by as much each time, on one side: SFloat 1.4e-6 of a state that
+    // forgets over 2000 steps. So each factor is rounded from what makes the product of all so far the power that it stands for (5.7e-7: what the
+    // additions round). `behind`: by how much of itself that product is too small.
+    double behind = 0.0;
+    const LaPower<T> a16 = power.whole(kLaStretch);
+    const double inverse16 = a16.hi > 0x1p-100 && a16.hi < 0x1p100 ? 1.0 / a16.hi : 0.0;   // (0: as they are)
+    auto rounded = [&](const LaPower<T>& exact) { return (T)(inverse16 != 0.0 ? exact.hi + __builtin_fma(exact.hi, behind, exact.lo) : exact.hi); };
+    auto next_decay = [&] {
+        const T s = rounded(a16);
+        behind = __builtin_fma((a16.hi - (double)s) + a16.lo, inverse16, behind);
         return s;
     };
     auto ends = [&](uint32_t of_all) {   // a turn of so many steps, fewer than it can have: the last
 #pragma unroll 1
         for (int sub = 0; sub < SUBS; ++sub) {
             const uint32_t n = of_all <= sub * kLaStretch ? 0 : of_all - sub * kLaStretch < kLaStretch ? of_all - sub * kLaStretch : kLaStretch;
-            T k4[4], s1 = n ? (T)(power(n) * behind) : (T)1;
-            behind = 1.0;
+            T k4[4], s1 = n ? rounded(power.whole(n)) : (T)1;
+            behind = 0.0;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const uint32_t j = 4 * g + r;
@@ -506,7 +529,7 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
                 ends(n);
             } else {
 #pragma unroll
-                for (int sub = 0; sub < SUBS; ++sub) decay_s[sub] = next_decay(a16);
+                for (int sub = 0; sub < SUBS; ++sub) decay_s[sub] = next_decay();
             }
             Quad P[EACH], all[SUBS];
             if constexpr (!ONLY) {
@@ -687,7 +710,7 @@ __global__ __launch_bounds__(256) void la_starts_kernel(LaWalks walks, LaCommon 
         const double a = (double)reinterpret_cast<const T*>(c.decay)[bh - b * c.heads];
         double s = w.state ? (double)reinterpret_cast<const T*>(w.state)[bh * size + d * w.state_row + e * w.state_col] : 0.0;
         T* p = reinterpret_cast<T*>(plan.starts[blockIdx.y]) + at;
-        const double whole = la_power(a, plan.steps);
+        const double whole = la_power<T>(a, plan.steps).hi;
         const uint32_t n_starts = plan.segments - 1;
         for (uint32_t k = 0; k < n_starts; k += U) {
             T own[U];
@@ -698,7 +721,7 @@ __global__ __launch_bounds__(256) void la_starts_kernel(LaWalks walks, LaCommon 
                 if (k + u >= n_starts) continue;
                 const uint64_t begin = (k + u) * plan.steps;
                 const uint64_t n = begin >= length ? 0 : length - begin < plan.steps ? length - begin : plan.steps;
-                s = __builtin_fma(n == plan.steps ? whole : n == 0 ? 1.0 : la_power(a, n), s, (double)own[u]);
+                s = __builtin_fma(n == plan.steps ? whole : n == 0 ? 1.0 : la_power<T>(a, n).hi, s, (double)own[u]);
                 p[(uint64_t)(k + u) * all] = (T)s;
             }
         }

@@ -446,3 +446,18 @@ def test_slow_decays_stay_powers(time):
         want = a[h].astype(np.float64) ** time * x["state"][0, h] + (x["k"][0, :, h].astype(np.float64) * by[:, None]).T @ x["v"][0, :, h].astype(np.float64)
         got = last.to_numpy()[0, h]
         assert np.linalg.norm(got - want) <= 3 * 35 * 2.0 ** -24 * np.linalg.norm(want), (h, np.linalg.norm(got - want) / np.linalg.norm(want))
+
+
+def test_slow_decays_stay_powers_in_double():
+    """The same in double: 188 stretches, 940 roundings, three times sqrt(940) half steps in norm; powers by squares in double alone would be off by seven
+    half steps a stretch on one side, over those that a decay of 1 - 10^-3.6 remembers."""
+    import cumo_amd as m
+    time = 3000
+    a = 1 - 10.0 ** -np.linspace(2.0, 3.6, 4)
+    x = made(np.random.default_rng(time), (1, time, 4, 4, 16, 16), np.float64)
+    x["decay"] = a
+    _, last = m.Fused.linear_attention(*on_device(m, x, ("q", "k", "v", "decay", "state")))
+    (_, want), _ = reference(x)
+    for h in range(4):
+        off = np.linalg.norm((last.to_numpy()[0, h] - want[0, h]).astype(float)) / np.linalg.norm(want[0, h].astype(float))
+        assert off <= 3 * 31 * 2.0 ** -53, (h, off)
