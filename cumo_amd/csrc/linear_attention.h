@@ -330,6 +330,9 @@ constexpr uint64_t kLaShared = BUFFERS * (kLaBuffer<T, DT, NW> - (ONLY ? kLaTurn
 // Waves to a SIMD that the registers are shared out for: two, so 256 of one kind, where a lane holds less (else the compiler spreads them over both
 // kinds, and moves them: also where it knows that LDS, hence told at the launch, holds one block alone).
 template <class T, int DT, int NW> constexpr int kLaWaves = sizeof(T) == 4 ? (DT <= 8 ? 2 : 1) : DT <= 4 && NW == 4 ? 2 : 1;
+// Tiles of dim that a walk of DT surely has; one behind them is left out where dim does not reach it. DFloat alone, in threes of pairs: 6 x 777 x 12 of 72
+// 158 and 148 us, of 96 159 both ways; SFloat 76 and 72, but 74 and 77, and longer rows lose as well.
+template <class T, int DT> constexpr int kLaLeast = sizeof(T) == 8 && DT == 6 ? 5 : DT;
 extern __shared__ __attribute__((aligned(16))) char la_shared[];
 
 // DT: tiles of 16 that hold dim. NW: tiles of 16 columns to a block, a wave each. QUADS: rows of dim and of wide are whole fours. ONLY: what a
@@ -370,6 +373,8 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
     const uint32_t b0 = slice * NW * 16, e0 = b0 + wave * 16;     // the block's columns, and the wave's
     const uint32_t cols = W - b0 < NW * 16 ? W - b0 : NW * 16;
     const bool column = e0 + label < W;
+    const int tiles = (int)((D + 15) / 16);
+    auto there = [&](int t) { return t < kLaLeast<T, DT> || t < tiles; };
     const LaPowers<T> power((double)reinterpret_cast<const T*>(c.decay)[h]);
     const bool late = w.backwards;
 
@@ -554,8 +559,8 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
                     for (int dt = 0; dt < DT; dt += 2) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            O = la_mma(S[dt][r], F[dt][r], O);
-                            O2 = la_mma(S[dt + 1][r], F[dt + 1][r], O2);
+                            if (there(dt)) O = la_mma(S[dt][r], F[dt][r], O);
+                            if (there(dt + 1)) O2 = la_mma(S[dt + 1][r], F[dt + 1][r], O2);
                         }
                         S[dt] *= decay_s[sub];
                         S[dt + 1] *= decay_s[sub];
@@ -607,8 +612,8 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
                 for (int dt = 0; dt < DT; dt += 2) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        S[dt] = la_mma(F[dt][r], VW[r], S[dt]);
-                        S[dt + 1] = la_mma(F[dt + 1][r], VW[r], S[dt + 1]);
+                        if (there(dt)) S[dt] = la_mma(F[dt][r], VW[r], S[dt]);
+                        if (there(dt + 1)) S[dt + 1] = la_mma(F[dt + 1][r], VW[r], S[dt + 1]);
                     }
                     if constexpr (BUFFERS == 2) {
                         read_first(last ? 0 : sub + 1, dt);
