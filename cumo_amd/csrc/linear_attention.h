@@ -6,6 +6,12 @@
 //   gk[t] = G[t] by v[t]:          backwards, v in the place of q, scale g of k, q of v, the state transposed
 //   gv[t] = G[t] by k[t]:          backwards, k in the place of q, scale q of k, g of v
 // Backwards the state decays behind a step instead of before it (`late`): what is handed on is a G.
+//
+// One step is bound by the state's bytes, many by the products: SFloat 8 x 2048 x 16 heads of 128 222 us, the matrix units busy for 60 % of them.
+// What is beside the products adds up with them, as a SIMD does not work on 32 or 64-bit products and on vector instructions at once (one
+// wave: a product of 16 x 16 x 4 floats in 39 cycles, with two vector instructions beside each 56, with four 65). Others: SFloat 1 x 65536 x 8 of 64 191 us
+// (70 for what segments leave, 12 for their starts), 64 x 1 x 16 of 128 25; DFloat 4 x 2048 x 16 of 128 355, 6 x 777 x 12 of 72 by 100 140. Gradients:
+// SFloat 4 x 2048 x 16 of 128 380, DFloat 3 x 500 x 8 of 64 53.
 #pragma once
 #include "common.h"
 
@@ -196,7 +202,8 @@ void la_step(const LaWalk& w, const LaCommon& c, char* memory, hipStream_t strea
 // them); v by columns serves as the second operand of k^T by v and the first of v^T. Nothing is moved between lanes but the products k q^T, of
 // which each of the NW waves works out a share, over its part of dim: they meet in LDS. Rows of q, k and v go through LDS too, a stretch ahead, and
 // are on their way there for a stretch before: read from memory by every wave as its lanes want them, they kept the first-level cache at
-// work for four fifths of the time (SFloat 8 x 2048 x 16 heads of 128: 266 us).
+// work for four fifths of the time (SFloat 8 x 2048 x 16 heads of 128: 266 us, and 222 so). Not kept: dim shared out over two waves of a SIMD 272, rows
+// three stretches ahead in registers 274, vector instructions spread between the products by hand 231.
 //
 // Double precision counts rows otherwise (lane (m, g) has rows g, g + 4, ...): operands are read by la_label, so that what
 // stands above holds for it too.

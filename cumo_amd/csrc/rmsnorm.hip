@@ -9,7 +9,7 @@
 // result, are in double: a square of a float is exact there, and the vector units do a hundred such operations in the time
 // that an element's bytes take. SFloat [8192,4096], with a residual, a sum and a weight: 87 us (6.2 TB/s, what an addition of two
 // large arrays reaches); in 8 bits [8192,4095] 80 us (5.4; the vector units are busy for more than half of it), and 30 us back
-// (5.5); gradients with gsum 94 + 5 us (5.7 and the weight's parts); DFloat [131072,257] gradients 200 + 5 (5.4), [8192,2047] in 8 bits 76
+// (5.5); rows as they are in 8 bits [16384,4095] 67 us (5.0), back 61 (5.5); gradients with gsum 94 + 5 us (5.7 and the weight's parts); DFloat [131072,257] gradients 200 + 5 (5.4), [8192,2047] in 8 bits 76
 // and 31 back. One row of 4096: 3.5 us, the launch's.
 #include "common.h"
 

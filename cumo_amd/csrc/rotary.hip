@@ -4,7 +4,8 @@
 //
 // Memory bounds it: an element is read and written once. The angle of a far position wants more than 32 bits (131072 * 1 radian rounded to a
 // float is off by 2^-8), so it is a double, and what is worked out from it too: the remainder of a quarter turn by two fused steps, sine
-// and cosine by their series on an eighth of a turn either way. A lane keeps them for the heads that it takes.
+// and cosine by their series on an eighth of a turn either way. A lane keeps them for the heads that it takes. SFloat 4 x 4096 x 32 heads of 96,
+// neighbours: 74 us, 5.4 TB/s; 64 x 1 x 32 of 128: 3.5, the launch's.
 #include "common.h"
 
 namespace cumo_hip {
