@@ -17,6 +17,13 @@ typedef int32_t mq_i4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ mq_i4 mq_mma(mq_i4 a, mq_i4 b, mq_i4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
+// the block's waves meet, for what LDS holds alone
+__device__ __forceinline__ void mq_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // sixteen bytes on any boundary
 __device__ __forceinline__ mq_i4 mq_read(const char* p) {
     mq_i4 v;
@@ -31,6 +38,17 @@ __device__ __forceinline__ mq_i4 mq_read_part(const char* p, int64_t n) {
 #pragma unroll
     for (int k = 0; k < 15; ++k) u.b[k] = k < n ? (int8_t)p[k] : (int8_t)0;
     return u.v;
+}
+
+// sixteen bytes of a row of which some, on the way to p, are behind its end: those before it (sixteen at least), moved down, and zeros
+__device__ __forceinline__ mq_i4 mq_read_end(const char* p, int64_t behind) {
+    if (behind <= 0) return mq_read(p);
+    unsigned __int128 u;
+    __builtin_memcpy(&u, p - behind, 16);
+    u = behind < 16 ? u >> (8 * (uint32_t)behind) : 0;
+    mq_i4 v;
+    __builtin_memcpy(&v, &u, 16);
+    return v;
 }
 
 struct MqParams : cumo_hip_matmul_q8_t {
@@ -159,11 +177,12 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_q8_tiles_kernel(MqParams 
     const uint64_t from = part * p.per, to = from + p.per < p.inner ? from + p.per : p.inner;
 
     const char* src[PIECES];
-    uint32_t dst[PIECES];
+    constexpr uint32_t STEP = THREADS / 8;   // rows from piece to piece of a lane
+    static_assert(STEP % 8 == 0, "a lane's pieces lie alike in their rows");
+    const uint32_t dst = threadIdx.x / 8 * kMqDepth + ((threadIdx.x % 8 ^ (threadIdx.x / 8 & 7)) * 16);
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
         const uint32_t id = threadIdx.x + k * THREADS, row = id / 8, piece = id % 8;
-        dst[k] = row * kMqDepth + ((piece ^ (row & 7)) * 16);
         if (row < BM) {
             const uint64_t i = i0 + row < p.rows ? i0 + row : p.rows - 1;
             src[k] = p.x + (int64_t)i * p.x_step + piece * 16;
@@ -177,6 +196,10 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_q8_tiles_kernel(MqParams 
         if (k0 + kMqDepth <= to) {
 #pragma unroll
             for (int k = 0; k < PIECES; ++k) held[k] = mq_read(src[k] + k0);
+        } else if (to >= 16) {
+            const int64_t behind = (int64_t)(k0 + (threadIdx.x % 8) * 16 + 16 - to);
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) held[k] = mq_read_end(src[k] + k0, behind);
         } else {
             const int64_t n = (int64_t)(to - k0) - (threadIdx.x % 8) * 16;
 #pragma unroll
@@ -185,7 +208,7 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_q8_tiles_kernel(MqParams 
     };
     auto place = [&](uint32_t buffer) {
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) *reinterpret_cast<mq_i4*>(&tile[buffer][dst[k]]) = held[k];
+        for (int k = 0; k < PIECES; ++k) *reinterpret_cast<mq_i4*>(&tile[buffer][dst + k * STEP * kMqDepth]) = held[k];
     };
 
     mq_i4 sum[TN][TM];
@@ -195,32 +218,60 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul_q8_tiles_kernel(MqParams 
         for (int t = 0; t < TM; ++t) sum[n][t] = mq_i4{0, 0, 0, 0};
     }
     const uint32_t x_row = (wave % WM) * (TM * 16) + m, w_row = BM + (wave / WM) * (TN * 16) + m;
+    // What LDS has is asked for ahead of the products that take it: the second half of a step's x in the first's registers as those are done with, and
+    // the next step's first half behind the middle of the second, where the waves meet.
+    mq_i4 a[2][TN], b[TM];
+    auto read_w = [&](const char* rows, int half) {
+#pragma unroll
+        for (int n = 0; n < TN; ++n) a[half][n] = *reinterpret_cast<const mq_i4*>(rows + (w_row + n * 16) * kMqDepth + ((half * 4 + g) ^ (m & 7)) * 16);
+    };
+    auto read_x = [&](const char* rows, int half, int t) { b[t] = *reinterpret_cast<const mq_i4*>(rows + (x_row + t * 16) * kMqDepth + ((half * 4 + g) ^ (m & 7)) * 16); };
+    auto multiply = [&](int half, int t) {
+#pragma unroll
+        for (int n = 0; n < TN; ++n) sum[n][t] = mq_mma(a[half][n], b[t], sum[n][t]);
+    };
     if (from < to) {
         fetch(from);
         place(0);
+        if (from + kMqDepth < to) fetch(from + kMqDepth);
     }
     __syncthreads();
     uint32_t buffer = 0;
+    if (from < to) {
+        read_w(tile[0], 0);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) read_x(tile[0], 0, t);
+    }
     for (uint64_t k0 = from; k0 < to; k0 += kMqDepth) {
         const bool more = k0 + kMqDepth < to;
-        if (more) fetch(k0 + kMqDepth);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const uint32_t swizzled = ((half * 4 + g) ^ (m & 7)) * 16;
-            mq_i4 a[TN], b[TM];
-#pragma unroll
-            for (int n = 0; n < TN; ++n) a[n] = *reinterpret_cast<const mq_i4*>(&tile[buffer][(w_row + n * 16) * kMqDepth + swizzled]);
-#pragma unroll
-            for (int t = 0; t < TM; ++t) b[t] = *reinterpret_cast<const mq_i4*>(&tile[buffer][(x_row + t * 16) * kMqDepth + swizzled]);
-#pragma unroll
-            for (int n = 0; n < TN; ++n) {
-#pragma unroll
-                for (int t = 0; t < TM; ++t) sum[n][t] = mq_mma(a[n], b[t], sum[n][t]);
-            }
-        }
         if (more) place(buffer ^ 1);
+        if (k0 + 2 * kMqDepth < to) fetch(k0 + 2 * kMqDepth);
+        const char* rows = tile[buffer];
+        read_w(rows, 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+            multiply(0, t);
+            read_x(rows, 1, t);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int t = 0; t < TM / 2; ++t) multiply(1, t);
+        mq_meet();
         buffer ^= 1;
-        __syncthreads();
+        rows = tile[buffer];
+        if (more) {
+            read_w(rows, 0);
+#pragma unroll
+            for (int t = 0; t < TM / 2; ++t) read_x(rows, 0, t);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = TM / 2; t < TM; ++t) {
+            multiply(1, t);
+            if (more) read_x(rows, 0, t);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     const uint64_t i_first = i0 + (wave % WM) * (TM * 16) + m, j_first = j0 + (wave / WM) * (TN * 16) + 4 * g;
     if (p.splits == 1) {
