@@ -5,9 +5,9 @@
 // rounded once.
 //
 // Few rows are bound by w's bytes on their way through the last-level cache: SFloat 16 x 4096 by 4096 7.5 us, 2.3 TB/s, three of them the launch's.
-// Many: 8191 x 4096 by 8192 277 to 293 us, 1.9 to 2.0 POP/s; products of 8-bit rows reach 2.1 on this card. The matrix units are busy for 45 % of the
-// waves' cycles, as a block's waves read their pieces of LDS, and multiply them, at the same time; no bank is met twice. Four waves of 128 x 128
-// read a third less, but spill: 345 us.
+// Many: 8191 x 4096 by 8192 266 us, 2.07 POP/s, where products of 8-bit rows reach 2.1 on this card. The matrix units are busy for half of the waves'
+// cycles, LDS for a third, no bank met twice: what a step waits for is its rows on their way, 64 KiB of them. With rows placed in the step in which they
+// are sent for, and LDS read just before its products, 280 us; four waves of 128 x 128 each, which spill, 345.
 #include "common.h"
 
 namespace cumo_hip {
@@ -340,14 +340,11 @@ int mq_tiles(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
     p.tiles_m = (uint32_t)((d.rows + BM - 1) / BM);
     p.tiles_n = (uint32_t)((d.cols + BN - 1) / BN);
     const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
-    // Inner is cut where tiles are few, into parts of 512 bytes or more: small tiles to two blocks a compute unit, others to one. 128 x 4096 by 4096 rows
-    // in 64 x 64: 256, 512, 1024 blocks 16.9, 15.7, 17.5 us; 256 x 4096: 21.7, 18.3, 20.6.
-    p.splits = 1;
-    if (tiles < (BM == 64 ? 300 : 192)) {
-        uint64_t most = d.inner / 512, wanted = (BM == 64 ? 512 : 256) / tiles;
-        p.splits = (uint32_t)(wanted < most ? wanted : most);
-        if (p.splits < 1) p.splits = 1;
-    }
+    // Inner is cut where tiles are few, into parts of 512 bytes or more, as many as leave a block to each compute unit. 64, 128 and 256 rows by 4096 by 4096,
+    // 256 blocks 12.2, 14.8 and 17.2 us; 512 13.3, 14.7 and 18.7; 1024 13.3, 17.3 and 20.0.
+    const uint64_t most = d.inner / 512, wanted = 256 / tiles;
+    p.splits = (uint32_t)(wanted < most ? wanted : most);
+    if (p.splits < 1) p.splits = 1;
     p.per = ((d.inner + p.splits - 1) / p.splits + kMqDepth - 1) / kMqDepth * kMqDepth;
     if (p.per == 0) p.per = kMqDepth;
     char* scratch = nullptr;
