@@ -349,6 +349,7 @@ int cumo_hip_na_rotary(const cumo_hip_narray_t* x, const cumo_hip_narray_t* posi
  * view). k and v may have fewer heads, a divisor of q's. decay: one dimension, a number a head; state
  * and last: batch x heads x dim x wide; lengths: Int32, one dimension, a number a sequence. Long sequences go in stretches of steps,
  * whose products and sums are in the arrays' type; a step's output depends on no later step, whatever that holds.
+ * (decays whose sixteenth power leaves the type, 256 and more in SFloat, may give NaN where the definition gives infinity or a number.)
  * linear_attention_grad: gq, gk, gv and gstate (NULL when state is) from g (of o) and glast (of last, or NULL). */
 int cumo_hip_na_linear_attention(const cumo_hip_narray_t* q, const cumo_hip_narray_t* k, const cumo_hip_narray_t* v, const cumo_hip_narray_t* decay,
                                  const cumo_hip_narray_t* state, const cumo_hip_narray_t* lengths, double scale, cumo_hip_narray_t* o,
