@@ -121,6 +121,20 @@ def test_matmul_matches_whole_numbers(dt, rows, inner, cols):
         check(y.to_numpy(), *product(x, xs, w, ws, b, dt))
 
 
+@pytest.mark.parametrize("rows", [70, 300, 3000])
+@pytest.mark.parametrize("inner", [1, 2, 5, 15, 16, 17, 31, 33, 47, 112, 113, 127, 143, 255, 257, 271])
+def test_matmul_of_tiles_whose_rows_end_anywhere(rows, inner):
+    """Whole arrays and windows of rows that stand among others' bytes."""
+    import cumo_amd as m
+    rng = np.random.default_rng(rows + inner)
+    x, w = (rng.integers(-127, 128, (n, inner + 20)).astype(np.int8) for n in (rows, 3100))
+    xs, ws = (rng.random((n, 1)).astype(np.float32) for n in (rows, 3100))
+    for part in (slice(0, inner), slice(9, 9 + inner)):
+        for forms in (lambda z: m.Int8.cast(np.ascontiguousarray(z[:, part])), lambda z: m.Int8.cast(z)[:, part]):
+            y = m.Fused.matmul_q8(forms(x), m.SFloat.cast(xs), forms(w), m.SFloat.cast(ws))
+            check(y.to_numpy(), *product(x[:, part], xs, w[:, part], ws, None, np.float32))
+
+
 @pytest.mark.parametrize("rows", [1, 20, 300])
 def test_matmul_sums_reach_the_ends_of_32_bits(rows):
     """131071 products of -128 by -128, of 127 by -128."""

@@ -228,3 +228,41 @@ def test_two_streams_at_once():
         L.cumo_hip_set_stream(None)
         for s in streams:
             L.cumo_hip_stream_destroy(s)
+
+
+def test_two_streams_at_once():
+    """Calls with scratch (inner cut into parts, a sequence into segments, gradients of shared heads) on two streams in turn, with no wait between
+    them: each answers what it does by itself."""
+    import cumo_amd as m
+    from cumo_amd import _lib
+    L = _lib.lib
+    ref = lambda z: C.byref(z._desc())  # noqa: E731
+    sides = []
+    for seed in (1, 2):
+        rng = np.random.default_rng(seed)
+        draw = lambda *n: m.SFloat.cast(rng.standard_normal(n).astype(np.float32))  # noqa: E731
+        x, xs = m.Fused.quantize(draw(100, 4096))
+        w, ws = m.Fused.quantize(draw(300, 4096))
+        q, k, v, g = draw(1, 3000, 4, 24), draw(1, 3000, 2, 24), draw(1, 3000, 2, 20), draw(1, 3000, 4, 20)
+        a = m.SFloat.cast(np.linspace(0.8, 0.999, 4).astype(np.float32))
+        want = [m.Fused.matmul_q8(x, xs, w, ws)] + m.Fused.linear_attention(q, k, v, a) + m.Fused.linear_attention_grad(g, q, k, v, a)
+        sides.append(([ref(z) for z in (x, xs, w, ws)], [ref(z) for z in (q, k, v, a)], ref(g), [z.to_numpy() for z in want], [m.SFloat(*z.shape) for z in want],
+                      (x, xs, w, ws, q, k, v, a, g)))
+    streams = [C.c_void_p(L.cumo_hip_stream_create()) for _ in range(2)]
+    m.synchronize()
+    try:
+        for _ in range(5):
+            for stream, (rows, heads, g, _, results, _) in zip(streams, sides):
+                L.cumo_hip_set_stream(stream)
+                z = [ref(y) for y in results]
+                _lib.call(L.cumo_hip_na_matmul_q8, *rows, None, z[0])
+                _lib.call(L.cumo_hip_na_linear_attention, *heads, None, None, 24 ** -0.5, z[1], z[2])
+                _lib.call(L.cumo_hip_na_linear_attention_grad, g, *heads, None, None, None, 24 ** -0.5, z[3], z[4], z[5], None)
+        L.cumo_hip_set_stream(None)
+        m.synchronize()
+        for _, _, _, want, results, _ in sides:
+            assert all((z.to_numpy() == y).all() for z, y in zip(results, want))
+    finally:
+        L.cumo_hip_set_stream(None)
+        for stream in streams:
+            L.cumo_hip_stream_destroy(stream)
