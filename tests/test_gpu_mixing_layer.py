@@ -230,6 +230,10 @@ def test_two_streams_at_once():
             L.cumo_hip_stream_destroy(s)
 
 
+# (under a name of its own: the next test takes this one)
+test_two_streams_with_results_from_the_pool = test_two_streams_at_once
+
+
 def test_two_streams_at_once():
     """Calls with scratch (inner cut into parts, a sequence into segments, gradients of shared heads) on two streams in turn, with no wait between
     them: each answers what it does by itself."""
