@@ -210,6 +210,13 @@ void la_step(const LaWalk& w, const LaCommon& c, char* memory, hipStream_t strea
 template <class T> using LaQuad = T __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ LaQuad<float> la_mma(float a, float b, LaQuad<float> c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ LaQuad<double> la_mma(double a, double b, LaQuad<double> c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+// four elements of a row in LDS, which starts on a boundary of 16 bytes (four doubles by themselves would be taken to start on one of 32)
+template <class T>
+__device__ __forceinline__ LaQuad<T> la_quad(const T* p) {
+    LaQuad<T> x;
+    __builtin_memcpy(&x, __builtin_assume_aligned(p, 16), sizeof(x));
+    return x;
+}
 template <class T> __device__ __forceinline__ uint32_t la_label(uint32_t m) { return sizeof(T) == 4 ? m : 4 * (m & 3) + (m >> 2); }
 
 constexpr uint32_t kLaStretch = 16;
@@ -340,7 +347,7 @@ template <class T, int DT, int NW> constexpr int kLaWaves = sizeof(T) == 4 ? (DT
 // Tiles of dim that a walk of DT surely has; one behind them is left out where dim does not reach it. DFloat alone, in threes of pairs: 6 x 777 x 12 of 72
 // 158 and 148 us, of 96 159 both ways; SFloat 76 and 72, but 74 and 77, and longer rows lose as well.
 template <class T, int DT> constexpr int kLaLeast = sizeof(T) == 8 && DT == 6 ? 5 : DT;
-extern __shared__ __attribute__((aligned(16))) char la_shared[];
+extern __shared__ __attribute__((aligned(32))) char la_shared[];
 
 // DT: tiles of 16 that hold dim. NW: tiles of 16 columns to a block, a wave each. QUADS: rows of dim and of wide are whole fours. ONLY: what a
 // segment leaves by itself.
@@ -363,6 +370,7 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
     T* const q_rows = v_rows + BUFFERS * VALUES;
     Quad* const slot = reinterpret_cast<Quad*>(q_rows + BUFFERS * KEYS);
     static_assert(sizeof(T) * (BUFFERS * (2 * KEYS + VALUES)) + kLaSlots<T, DT, NW> == kLaShared<T, DT, NW, BUFFERS, false> && kLaShared<T, DT, NW, BUFFERS, false> <= 160 * 1024, "LDS");
+    static_assert(Keys::ROW * sizeof(T) % 16 == 0 && sizeof(T) * KEYS % 32 == 0 && sizeof(T) * VALUES % 32 == 0, "rows and slots stand where they are read");
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4, label = la_label<T>(m);
     const uint64_t bh_all = c.batch * c.heads;
     uint64_t at = blockIdx.x;
@@ -510,7 +518,7 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
 #pragma unroll
             for (int r = 0; r < 4; ++r) F[dt][r] = kr[(sub * 16 + 4 * g + r) * Keys::ROW + dt * 16 + label];
         };
-        auto read_q = [&](int sub, int dt) { F[dt] = *reinterpret_cast<const Quad*>(qr + (sub * 16 + m) * Keys::ROW + dt * 16 + 4 * g); };
+        auto read_q = [&](int sub, int dt) { F[dt] = la_quad(qr + (sub * 16 + m) * Keys::ROW + dt * 16 + 4 * g); };
         auto read_first = [&](int sub, int dt) {
             if constexpr (ONLY) read_k(sub, dt);
             else read_q(sub, dt);
@@ -523,8 +531,8 @@ __global__ __launch_bounds__(64 * NW, (kLaWaves<T, DT, NW>)) void la_stretch_ker
                     const int sub = EACH > 1 ? e : (int)(wave / PARTS);
 #pragma unroll
                     for (int i = 0; i < PM; ++i) {
-                        PQ[e][i] = *reinterpret_cast<const Quad*>(qr + (sub * 16 + m) * Keys::ROW + (part * PM + i) * 16 + 4 * g);
-                        PK[e][i] = *reinterpret_cast<const Quad*>(kr + (sub * 16 + label) * Keys::ROW + (part * PM + i) * 16 + 4 * g);
+                        PQ[e][i] = la_quad(qr + (sub * 16 + m) * Keys::ROW + (part * PM + i) * 16 + 4 * g);
+                        PK[e][i] = la_quad(kr + (sub * 16 + label) * Keys::ROW + (part * PM + i) * 16 + 4 * g);
                     }
                 }
             }
