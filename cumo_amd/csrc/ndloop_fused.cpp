@@ -639,6 +639,10 @@ int cumo_hip_na_matmul_q8(const cumo_hip_narray_t* x, const cumo_hip_narray_t* x
     if (!same_shape(wscale, 2, w_scales)) return fail(CUMO_HIP_ERROR_SHAPE, "matmul_q8: wscale must have w's shape with a last dimension of 1");
     if (bias && !same_shape(bias, 1, w_scales)) return fail(CUMO_HIP_ERROR_SHAPE, "matmul_q8: bias must be one dimension, a number for each row of w");
     if (w->shape[1] >= (size_t)1 << 17) return fail(CUMO_HIP_ERROR_ARGUMENT, "matmul_q8: rows are too long for sums of 32 bits");
+    // (what the launcher refuses, before anything is held)
+    const size_t rows = total_of(xscale), cols = w->shape[0], most = (size_t)1 << 31;
+    if (rows && cols && (rows >= most || cols >= most || ((rows + 255) / 256) * ((cols + 255) / 256) >= (size_t)1 << 22))
+        return fail(CUMO_HIP_ERROR_ARGUMENT, "matmul_q8: too many rows by columns");
     want[nd - 1] = w->shape[0];
     rc = check_result(y, xscale->type, nd, want);
     if (rc) return rc;
@@ -656,9 +660,9 @@ int cumo_hip_na_matmul_q8(const cumo_hip_narray_t* x, const cumo_hip_narray_t* x
     if (!rc) rc = make(&r, y, xscale->type, nd, want, ROWS, 0, o, 5, &s), nr = 1;
     if (!rc && total_of(r.use)) {
         cumo_hip_matmul_q8_t d;
-        d.rows = total_of(xscale);
+        d.rows = rows;
         d.inner = w->shape[1];
-        d.cols = w->shape[0];
+        d.cols = cols;
         d.x = o[0].at();
         d.x_step = o[0].step[0];
         d.w = o[1].at();

@@ -1,0 +1,12 @@
+"""Limits of the operators of a layer with a matrix state, without a GPU: what is beyond them is refused before anything is held for it."""
+from test_fused_refusals import ARGUMENT, I8, L, SF, host_pool, new, refused, view  # noqa: F401
+
+
+def test_matmul_q8_of_too_many_rows_by_columns():
+    f = L.cumo_hip_na_matmul_q8
+    for rows, cols in ((1 << 30, 1), (1, 1 << 30), (1 << 31, 1), (1, 1 << 31), (1 << 20, 1 << 18)):
+        refused(ARGUMENT, f, view(I8, rows, 1), view(SF, rows, 1), view(I8, cols, 1), view(SF, cols, 1), None, new())
+    # none at all are not too many
+    for rows, cols in ((1 << 31, 0), (0, 1 << 31)):
+        z = new()
+        assert f(view(I8, rows, 1), view(SF, rows, 1), view(I8, cols, 1), view(SF, cols, 1), None, z) == 0 and list(z.shape[:2]) == [rows, cols]
