@@ -774,8 +774,10 @@ int attention_operands(const NA* q, const NA* k, const NA* v, const NA* decay, c
         if (lengths->type != CUMO_HIP_INT32) return fail(CUMO_HIP_ERROR_TYPE, kAttentionType);
         if (!same_shape(lengths, 1, q->shape)) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: lengths must be one dimension, a number for each sequence");
     }
-    // (a launch holds fewer than 2^32 lanes: 256 to a block, twelve blocks to a head at most)
-    if (q->shape[1] >= (size_t)1 << 31 || q->shape[0] * q->shape[2] >= (size_t)1 << 20) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: too many steps or heads");
+    // (a launch holds fewer than 2^32 lanes: 256 to a block, twelve blocks to a head at most; each factor by itself, as their product may pass 64 bits)
+    const size_t batch = q->shape[0], heads = q->shape[2], most = (size_t)1 << 20;
+    if (q->shape[1] >= (size_t)1 << 31 || (batch && heads && (batch >= most || heads >= most || batch * heads >= most)))
+        return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: too many steps or heads");
     return CUMO_HIP_OK;
 }
 
