@@ -753,7 +753,8 @@ int attention_operands(const NA* q, const NA* k, const NA* v, const NA* decay, c
     if (k->shape[2] != v->shape[2]) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: k and v must have the same heads");
     if (k->shape[2] ? q->shape[2] % k->shape[2] != 0 : q->shape[2] != 0) return fail(CUMO_HIP_ERROR_SHAPE, "linear_attention: heads of q must be a multiple of those of k");
     if (q->shape[3] > 256 || v->shape[3] > 256) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: heads of more than 256 elements");
-    if (!std::isfinite(scale)) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: scale must be a finite number");
+    // (it is rounded to the arrays' type)
+    if (!std::isfinite(q->type == CUMO_HIP_SFLOAT ? (double)(float)scale : scale)) return fail(CUMO_HIP_ERROR_ARGUMENT, "linear_attention: scale must be a finite number of the arrays' type");
     rc = check_float(decay, kAttentionType);
     if (rc) return rc;
     if (decay->type != q->type) return fail(CUMO_HIP_ERROR_TYPE, kAttentionType);

@@ -1,5 +1,5 @@
 """Limits of the operators of a layer with a matrix state, without a GPU: what is beyond them is refused before anything is held for it."""
-from test_fused_refusals import ARGUMENT, I8, L, SF, host_pool, new, refused, view  # noqa: F401
+from test_fused_refusals import ARGUMENT, DF, I8, L, SF, host_pool, new, refused, view  # noqa: F401
 
 
 def test_matmul_q8_of_too_many_rows_by_columns():
@@ -20,3 +20,14 @@ def test_linear_attention_of_sequences_by_heads_that_pass_64_bits():
         refused(ARGUMENT, f, q, kv, kv, a, None, None, 1.0, new(), new())
         refused(ARGUMENT, f, q, kv, kv, a, None, None, 1.0, new(), None)
         refused(ARGUMENT, grad, q, q, kv, kv, a, None, None, None, 1.0, new(), new(), new(), None)
+
+
+def test_linear_attention_by_a_scale_that_its_type_does_not_reach():
+    f, grad = L.cumo_hip_na_linear_attention, L.cumo_hip_na_linear_attention_grad
+    q, kv, a, n = view(SF, 2, 0, 4, 4), view(SF, 2, 0, 1, 4), view(SF, 4), new
+    for scale in (1e39, -1e300):
+        refused(ARGUMENT, f, q, kv, kv, a, None, None, scale, n(), None)
+        refused(ARGUMENT, grad, q, q, kv, kv, a, None, None, None, scale, n(), n(), n(), None)
+    assert f(q, kv, kv, a, None, None, 3.4e38, n(), None) == 0
+    q, kv, a = view(DF, 2, 0, 4, 4), view(DF, 2, 0, 1, 4), view(DF, 4)
+    assert f(q, kv, kv, a, None, None, -1e300, n(), None) == 0
