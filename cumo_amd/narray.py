@@ -1300,6 +1300,7 @@ class _Fused:
             pair = lambda turns: dims * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
             low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dims - 1)
             part = np.clip((np.arange(dims // 2) - low) / max(high - low, 0.001), 0.0, 1.0)
+            part[np.arange(dims // 2) >= pair(slow)] = 1.0   # (where even the first pair is one of those, high is 0 or less)
             f = f * (1 - part) + f / factor * part
             amplitude = 0.1 * math.log(factor) + 1.0
         return [DFloat.cast(f), amplitude]
