@@ -12,13 +12,20 @@ namespace cumo_hip {
 namespace {
 
 // sin x and cos x for |x| < 2^50, NaN otherwise. k quarter turns: x - k * 1.57... is exact (both are multiples of 2^-52, and nearer
-// than a turn), pi / 2 goes on with 6.1e-17. |r| <= pi / 4 and a rounding; the first term left out is r^19 / 19! and r^18 / 18!, below 3e-18,
-// for SFloat r^13 / 13! and r^14 / 14!, below 8e-12.
+// than a turn), pi / 2 goes on with 6.1e-17. k comes from a rounded product: far from 0 the quarter next to the nearest is taken at times (|r| up to
+// 1.004 pi / 4 at 2^44, 1.21 near 2^50), so from there on what is left is turned back once more. The first term left out is r^19 / 19! and
+// r^18 / 18!, below 3e-18, for SFloat r^13 / 13! and r^14 / 14!, below 8e-12.
 template <bool LONG>
 __device__ __forceinline__ void rt_sincos(double x, double* s, double* c) {
-    const double k = __builtin_rint(x * 0.63661977236758134308);
+    double k = __builtin_rint(x * 0.63661977236758134308);
     double r = __builtin_fma(-k, 1.57079632679489661923, x);
     r = __builtin_fma(-k, 6.123233995736766036e-17, r);
+    if (__builtin_fabs(x) >= 0x1p44) {
+        const double more = __builtin_rint(r * 0.63661977236758134308);
+        k += more;
+        r = __builtin_fma(-more, 1.57079632679489661923, r);
+        r = __builtin_fma(-more, 6.123233995736766036e-17, r);
+    }
     const double z = r * r;
     double ps, pc;
     if constexpr (LONG) {
