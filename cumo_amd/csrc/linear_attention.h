@@ -344,8 +344,11 @@ constexpr uint64_t kLaShared = BUFFERS * (kLaBuffer<T, DT, NW> - (ONLY ? kLaTurn
 // Waves to a SIMD that the registers are shared out for: two, so 256 of one kind, where a lane holds less (else the compiler spreads them over both
 // kinds, and moves them: also where it knows that LDS, hence told at the launch, holds one block alone).
 template <class T, int DT, int NW> constexpr int kLaWaves = sizeof(T) == 4 ? (DT <= 8 ? 2 : 1) : DT <= 4 && NW == 4 ? 2 : 1;
-// Tiles of dim that a walk of DT surely has; one behind them is left out where dim does not reach it. DFloat alone, in threes of pairs: 6 x 777 x 12 of 72
-// 158 and 148 us, of 96 159 both ways; SFloat 76 and 72, but 74 and 77, and longer rows lose as well.
+// Tiles of dim that a walk of DT surely has; one behind them is left out where dim does not reach it, which takes a branch in front of each pair of
+// products. It pays where the tile is a sixth of them and most dims of the class do without it, DFloat of 65 to 96, us with / without: of 65 to 80 a
+// twentieth and more (6 x 777 x 12 of 66 by 100 164 / 174, of 72 146 / 155, of 80 148 / 158; 4 x 2048 x 16 of 68 by 64 155 / 165; gradients 4 x 512 x 8 of 76
+// 92 / 99), of 81 to 96 up to 2 % lost (84 163 / 160, 96 158 / 158). Not so the next classes, with tiles left out from the tenth and the
+// fourteenth on: 144 270 / 278, but 160 284 / 281, 176 291 / 282, 192 297 / 278; 196 616 / 619, 240 645 / 632, 256 645 / 625. SFloat of 72 gains 5 % where 96 loses 4.
 template <class T, int DT> constexpr int kLaLeast = sizeof(T) == 8 && DT == 6 ? 5 : DT;
 extern __shared__ __attribute__((aligned(32))) char la_shared[];
 
