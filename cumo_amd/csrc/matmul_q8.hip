@@ -340,9 +340,9 @@ int mq_tiles(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
     p.tiles_m = (uint32_t)((d.rows + BM - 1) / BM);
     p.tiles_n = (uint32_t)((d.cols + BN - 1) / BN);
     const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
-    // Inner is cut where tiles are few, into parts of 512 bytes or more, as many as leave a block to each compute unit. 64, 128 and 256 rows by 4096 by 4096,
-    // 256 blocks 12.2, 14.8 and 17.2 us; 512 13.3, 14.7 and 18.7; 1024 13.3, 17.3 and 20.0.
-    const uint64_t most = d.inner / 512, wanted = 256 / tiles;
+    // Inner is cut where tiles are few, into parts of 512 bytes or more, as many as leave a block to each of 256 compute units. 64, 128 and 256 rows by 4096
+    // by 4096, 256 blocks 12.2, 14.8 and 17.2 us; 512 13.3, 14.7 and 18.7; 1024 13.3, 17.3 and 20.0.
+    const uint64_t most = d.inner / 512, wanted = (uint64_t)device_compute_units() / tiles;
     p.splits = (uint32_t)(wanted < most ? wanted : most);
     if (p.splits < 1) p.splits = 1;
     p.per = ((d.inner + p.splits - 1) / p.splits + kMqDepth - 1) / kMqDepth * kMqDepth;
@@ -385,10 +385,14 @@ int mq_launch(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
     if (d.rows <= 16 && reach) return mq_rows<T, 1>(d, stream);
     if (d.rows <= 32 && reach) return mq_rows<T, 2>(d, stream);
     if (d.rows <= 64 && d.inner <= 1024 && reach) return mq_rows<T, 4>(d, stream);
-    const uint64_t large = ((d.rows + 255) / 256) * ((d.cols + 255) / 256);
-    if (large >= 192) return mq_tiles<T, 256, 256, 2, 4>(d, stream);
+    // A larger tile reads less for each product; smaller ones leave fewer units without a block, and have others beside them on theirs. The large one from
+    // three blocks to four units on, the middle one from more than three to two. On 256 units, us for inner of 512 and of 4096, by the number of the larger
+    // tiles: large / middle 160 27 / 25 and 67 / 72, 176 28 / 26 and 68 / 74, 192 28 / 26 and 68 / 75, 200 22 / 24 and 61 / 82, 256 27 / 25 and 68 / 87; middle / small
+    // 200 12.4 / 10.5 and 35 / 32, 256 12.5 / 10.8 and 35 / 33, 320 17.1 / 13.6 and 46 / 42, 384 17.8 / 15.7 and 47 / 48, 512 17.3 / 18.5 and 48 / 62.
+    const uint64_t units = (uint64_t)device_compute_units(), large = ((d.rows + 255) / 256) * ((d.cols + 255) / 256);
+    if (large * 4 >= units * 3) return mq_tiles<T, 256, 256, 2, 4>(d, stream);
     const uint64_t middle = ((d.rows + 127) / 128) * ((d.cols + 127) / 128);
-    if (middle >= 200) return mq_tiles<T, 128, 128, 2, 2>(d, stream);
+    if (middle * 2 > units * 3) return mq_tiles<T, 128, 128, 2, 2>(d, stream);
     return mq_tiles<T, 64, 64, 2, 2>(d, stream);
 }
 

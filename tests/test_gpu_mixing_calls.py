@@ -4,6 +4,7 @@ import math
 import numpy as np
 import pytest
 
+from test_gpu_matmul_q8 import check, product
 from test_gpu_rotary import cls_of, close, reference
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +37,17 @@ def test_rotary_by_angles_up_to_the_last(dt, power):
     for inverse in (False, True):
         y = m.Fused.rotary(cls.cast(x), m.Int32.cast(p), m.DFloat.cast(f), inverse=inverse)
         close(y.to_numpy(), *reference(x, p, f, inverse=inverse))
+
+
+@pytest.mark.parametrize("dt", [np.float32, np.float64])
+@pytest.mark.parametrize("rows,inner,cols", [(1990, 136, 3097), (2041, 257, 3081), (2050, 640, 2100), (900, 1025, 4100), (3900, 33, 3200)])
+def test_matmul_in_tiles_of_each_size(dt, rows, inner, cols):
+    """Results that go through the caches, in enough tiles of 128 that they are taken, in too few, and in enough of 256 (DFloat: past the caches)."""
+    import cumo_amd as m
+    cls = cls_of(m, dt)
+    rng = np.random.default_rng(rows)
+    x, w = (rng.integers(-128, 128, s).astype(np.int8) for s in ((rows, inner), (cols, inner)))
+    xs, ws = (np.exp(rng.standard_normal((n, 1))).astype(dt) for n in (rows, cols))
+    bias = rng.standard_normal(cols).astype(dt)
+    y = m.Fused.matmul_q8(m.Int8.cast(x), cls.cast(xs), m.Int8.cast(w), cls.cast(ws), cls.cast(bias))
+    check(y.to_numpy(), *product(x, xs, w, ws, bias, dt))
