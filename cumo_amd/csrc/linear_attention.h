@@ -7,10 +7,10 @@
 //   gv[t] = G[t] by k[t]:          backwards, k in the place of q, scale q of k, g of v
 // Backwards the state decays behind a step instead of before it (`late`): what is handed on is a G.
 //
-// One step is bound by the state's bytes, many by the products: SFloat 8 x 2048 x 16 heads of 128 222 us, the matrix units busy for 60 % of them.
-// What is beside the products adds up with them, as a SIMD does not work on 32 or 64-bit products and on vector instructions at once (one
-// wave: a product of 16 x 16 x 4 floats in 39 cycles, with two vector instructions beside each 56, with four 65). Others: SFloat 1 x 65536 x 8 of 64 191 us
-// (70 for what segments leave, 12 for their starts), 64 x 1 x 16 of 128 25; DFloat 4 x 2048 x 16 of 128 355, 6 x 777 x 12 of 72 by 100 140. Gradients:
+// One step is bound by the state's bytes, many by the products: SFloat 8 x 2048 x 16 heads of 128 222 us, the matrix units busy for 60 % of them,
+// other vector instructions 11 %, LDS 6 %, waits for rows and at a turn's two meetings 14 %. What is beside the products adds up with them, as a SIMD does
+// not work on 32 or 64-bit products and on vector instructions at once (one wave: a product of 16 x 16 x 4 floats in 39 cycles, with two vector instructions beside each 56, with four 65). Others: SFloat 1 x 65536 x 8 of 64 191 us
+// (62 for what segments leave, 12 for their starts), 64 x 1 x 16 of 128 25; DFloat 4 x 2048 x 16 of 128 355, 6 x 777 x 12 of 72 by 100 140. Gradients:
 // SFloat 4 x 2048 x 16 of 128 380, DFloat 3 x 500 x 8 of 64 53.
 #pragma once
 #include "common.h"

@@ -731,7 +731,7 @@ namespace {
 
 const char kAttentionType[] = "linear_attention: operands are SFloat or DFloat, all of one type, lengths Int32";
 
-// whether an array is batch x time x heads x n, of which n is given (0: whatever it is), as are the others where they are not NULL
+// whether an array is of the type and batch x time x heads x n, with the sequences and steps of `like`, whatever its heads
 int attention_operand(const NA* a, int type, const NA* like, size_t n) {
     const int rc = check_float(a, kAttentionType);
     if (rc) return rc;

@@ -1266,7 +1266,7 @@ class _Fused:
     def matmul_q8(x, xscale, w, wscale, bias=None):
         """The rows of x by the rows of w, both Int8 with their scales as rmsnorm_q8 and quantize answer them:
         y[..., j] = sum(x[...] * w[j]) * xscale * wscale[j] (+ bias[j]), in the scales' type. The sum of products is exact (rows
-        of up to 131071), y is rounded once."""
+        of up to 131071); what follows is in double, then rounded to the type."""
         done = _native.matmul_q8(x, xscale, w, wscale, bias)  # None: the general way
         if done is not None:
             return done

@@ -748,8 +748,8 @@ void cumo_hip_quantize_kernel_launch(int type, const cumo_hip_quantize_t* d);
 
 /* The product of 8-bit rows by 8-bit rows (no counterpart in the reference):
  *   y[i][j] = (sum over k < inner of x[i][k] * w[j][k]) * xscale[i] * wscale[j] + bias[j]
- * The sum is exact in 32 bits for inner < 2^17; what follows is in double, rounded once to type
- * (0 SFloat, 1 DFloat), which the scales and bias (NULL: none) have as well, contiguous each.
+ * The sum is exact in 32 bits for inner < 2^17; what follows is in double, step by
+ * step, and then rounded to type (0 SFloat, 1 DFloat), which the scales and bias (NULL: none) have as well, contiguous each.
  * Steps from row to row in bytes. y may overlap no operand. Fewer than 2^31 rows and columns, and
  * fewer than 2^22 tiles of 256 by 256 of them. Scratch comes from the pool (left to the graph of a
  * captured call: cumo_hip_captured_free). CUMO_HIP_OK or the error reported. */
@@ -792,8 +792,8 @@ void cumo_hip_rotary_kernel_launch(int type, const cumo_hip_rotary_t* d);
  * contiguous elements, NULL for zeros; last: S behind the last step, alike, NULL where it is
  * not wanted. lengths: the steps of each sequence (between 0 and time; others are brought there),
  * NULL: time; o is 0 behind them, and last is S[length - 1]. type 0 SFloat, 1 DFloat. No result may
- * overlap an operand, but for last, which may be state where time is 1. batch x heads is less than
- * 2^20, time than 2^31. Scratch comes from the pool (left to the graph of a captured call:
+ * overlap an operand, but for last, which may be state where time is 1. scale is finite in the type.
+ * batch x heads is less than 2^20, time than 2^31. Scratch comes from the pool (left to the graph of a captured call:
  * cumo_hip_captured_free). CUMO_HIP_OK or the error reported. */
 typedef struct {
     uint64_t batch, time, heads, shared, dim, wide;

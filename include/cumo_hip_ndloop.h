@@ -349,7 +349,10 @@ int cumo_hip_na_rotary(const cumo_hip_narray_t* x, const cumo_hip_narray_t* posi
  * view). k and v may have fewer heads, a divisor of q's. decay: one dimension, a number a head; state
  * and last: batch x heads x dim x wide; lengths: Int32, one dimension, a number a sequence. Long sequences go in stretches of steps,
  * whose products and sums are in the arrays' type; a step's output depends on no later step, whatever that holds.
- * (decays whose sixteenth power leaves the type, 256 and more in SFloat, may give NaN where the definition gives infinity or a number.)
+ * (In a stretch q . k is worked out before v comes in, and the decay's powers up to the sixteenth by themselves. Where those leave the
+ * type - in SFloat q . k beyond 3.4e38 or next to 1e-38, decays of 256 and more, or below 0.0043, whose sixteenth power has not all its digits - a
+ * result may be infinite, NaN or 0 where single steps give a number; and of what an infinite q, k, v or state reaches they may differ in which is
+ * infinite and which NaN.)
  * linear_attention_grad: gq, gk, gv and gstate (NULL when state is) from g (of o) and glast (of last, or NULL). */
 int cumo_hip_na_linear_attention(const cumo_hip_narray_t* q, const cumo_hip_narray_t* k, const cumo_hip_narray_t* v, const cumo_hip_narray_t* decay,
                                  const cumo_hip_narray_t* state, const cumo_hip_narray_t* lengths, double scale, cumo_hip_narray_t* o,
