@@ -386,13 +386,15 @@ int mq_launch(const cumo_hip_matmul_q8_t& d, hipStream_t stream) {
     if (d.rows <= 32 && reach) return mq_rows<T, 2>(d, stream);
     if (d.rows <= 64 && d.inner <= 1024 && reach) return mq_rows<T, 4>(d, stream);
     // A larger tile reads less for each product; smaller ones leave fewer units without a block, and have others beside them on theirs. The large one from
-    // three blocks to four units on, the middle one from more than three to two. On 256 units, us for inner of 512 and of 4096, by the number of the larger
-    // tiles: large / middle 160 27 / 25 and 67 / 72, 176 28 / 26 and 68 / 74, 192 28 / 26 and 68 / 75, 200 22 / 24 and 61 / 82, 256 27 / 25 and 68 / 87; middle / small
-    // 200 12.4 / 10.5 and 35 / 32, 256 12.5 / 10.8 and 35 / 33, 320 17.1 / 13.6 and 46 / 42, 384 17.8 / 15.7 and 47 / 48, 512 17.3 / 18.5 and 48 / 62.
+    // three blocks to four units on, the middle one from 25 to 32 on, where small ones would come to more than three a unit. On 256 units, us by the number
+    // of the larger tiles, for inner of 512, 4096, 4095 and 16384:
+    //   large / middle   160  28 / 26, 67 / 74, 90 / 103, 219 / 251     192  29 / 26, 69 / 77, 91 / 106, 223 / 277     256  27 / 25, 70 / 92, 89 / 124, 242 / 341
+    //   middle / small   192  12.4 / 9.6, 35 / 27, 46 / 44, 112 / 92    200  12.4 / 10.6, 35 / 33, 46 / 56, 112 / 110    256  12.5 / 11.0, 35 / 35, 45 / 56, 114 / 126
+    //                    384  18 / 16, 47 / 50, 68 / 81, 160 / 194      512  17 / 19, 50 / 65, 68 / 106, 184 / 253
     const uint64_t units = (uint64_t)device_compute_units(), large = ((d.rows + 255) / 256) * ((d.cols + 255) / 256);
     if (large * 4 >= units * 3) return mq_tiles<T, 256, 256, 2, 4>(d, stream);
     const uint64_t middle = ((d.rows + 127) / 128) * ((d.cols + 127) / 128);
-    if (middle * 2 > units * 3) return mq_tiles<T, 128, 128, 2, 2>(d, stream);
+    if (middle * 32 >= units * 25) return mq_tiles<T, 128, 128, 2, 2>(d, stream);
     return mq_tiles<T, 64, 64, 2, 2>(d, stream);
 }
 
